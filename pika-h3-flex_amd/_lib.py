@@ -49,6 +49,11 @@ EXPORTS = (
     "pkh3_adaln_modulate",
     "pkh3_qkv_proj",
     "pkh3_out_proj",
+    "pkh3_paged_record_bytes",
+    "pkh3_paged_write",
+    "pkh3_paged_read",
+    "pkh3_paged_workspace_bytes",
+    "pkh3_paged_attn",
 )
 
 
@@ -113,6 +118,33 @@ class OutArgs(C.Structure):
     ]
 
 
+PAGE_KEYS = 64            # PKH3_PAGE_KEYS
+PAGED_MAX_SEQUENCES = 1024  # PKH3_PAGED_MAX_SEQUENCES
+PAGED_FP8, PAGED_CAUSAL = 1, 2
+
+
+class PagedArgs(C.Structure):
+    """Mirror of ``struct pkh3_paged_args`` (include/pkh3_paged.h)."""
+
+    _fields_ = [
+        ("pages", C.c_void_p), ("n_pages", C.c_int64),
+        ("starts", C.c_void_p), ("lengths", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p),
+        ("q_ss", C.c_int64), ("q_sh", C.c_int64), ("k_ss", C.c_int64), ("k_sh", C.c_int64),
+        ("v_ss", C.c_int64), ("v_sh", C.c_int64), ("o_ss", C.c_int64), ("o_sh", C.c_int64),
+        ("B", C.c_int32), ("table_pages", C.c_int32), ("rows", C.c_int32), ("kv_heads", C.c_int32), ("heads", C.c_int32), ("D", C.c_int32),
+        ("softmax_scale", C.c_float), ("norm_eps", C.c_float),
+        ("norm_w", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+        ("rope_mode", C.c_int32), ("flags", C.c_uint32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+# the same fields for struct.pack, in the order of PagedArgs
+PAGED_ARGS_FORMAT = struct.Struct("@Pq3Pq4P8q6i2f3PiIPN")
+assert PAGED_ARGS_FORMAT.size == C.sizeof(PagedArgs)
+
+
 class Pkh3Error(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"libpkh3attn error {code}: {message}")
@@ -159,6 +191,13 @@ def load() -> C.CDLL:
     lib.pkh3_qkv_proj.restype = C.c_int
     lib.pkh3_out_proj.argtypes = [C.POINTER(OutArgs), C.c_void_p]
     lib.pkh3_out_proj.restype = C.c_int
+    lib.pkh3_paged_record_bytes.argtypes = [C.c_uint32]
+    lib.pkh3_paged_record_bytes.restype = C.c_size_t
+    lib.pkh3_paged_workspace_bytes.argtypes = [C.POINTER(PagedArgs)]
+    lib.pkh3_paged_workspace_bytes.restype = C.c_size_t
+    for call in (lib.pkh3_paged_write, lib.pkh3_paged_read, lib.pkh3_paged_attn):
+        call.argtypes = [C.POINTER(PagedArgs), C.c_void_p]
+        call.restype = C.c_int
     lib.pkh3_version.argtypes = []
     lib.pkh3_version.restype = C.c_int
     lib.pkh3_strerror.argtypes = [C.c_int]

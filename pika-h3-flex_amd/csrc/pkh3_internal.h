@@ -211,6 +211,9 @@ hipError_t launch_attn_fwd(const FwdParams& p, hipStream_t st);
 enum AttnForm { kFormLong = 0, kFormShort = 1, kFormNarrow = 2, kFormSparse = 3, kFormRelay = 4 };
 AttnForm attn_form(const FwdParams& p, int cus);  // the form launch_attn_fwd takes on a device of `cus` CUs
 hipError_t device_cu_count(int* out);  // CUs of the current device (cached per device after the first call)
+
+// Leaves `text` as this thread's pkh3_last_error() and returns `code` (pkh3_api.hip)
+int report_error(int code, const char* text);
 hipError_t launch_sparse_plan(const SparsePlanParams& p, hipStream_t st);
 hipError_t launch_rope_tables(const double* pos, int S, const int* axis_dims, double theta, float* cos_out,
                               float* sin_out, hipStream_t st);

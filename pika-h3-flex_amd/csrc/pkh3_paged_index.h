@@ -1,0 +1,85 @@
+// The paged cache's index arithmetic, for the kernels and for host tests alike: plain C++, no HIP.  What it is given comes from arrays in
+// device memory that nobody has checked, so everything is brought into its range first.
+#pragma once
+#include <stdint.h>
+
+namespace pkh3 {
+
+constexpr int kPageKeys = 64;
+constexpr int at_most(int x, int y) { return x < y ? x : y; }
+constexpr int at_least(int x, int y) { return x > y ? x : y; }
+
+// One sequence of a batch: its rows first .. first + n - 1 of the call, its keys, the position of its first row (negative where it
+// has more rows than keys).
+struct Sequence {
+  int first, n, keys;
+  constexpr int position() const { return keys - n; }
+};
+constexpr Sequence make_sequence(int start, int end, int length, int rows, int table_pages) {
+  const int at = at_most(at_least(start, 0), rows), to = at_most(at_least(end, 0), rows);
+  return {at, at_least(to - at, 0), at_most(at_least(length, 0), table_pages * kPageKeys)};
+}
+constexpr int page_in_pool(int id, int64_t n_pages) { return id >= 0 && id < n_pages ? id : -1; }
+
+// ---- writing and reading: the tiles that a sequence's rows lie in, in front of position 0 too ----
+
+constexpr int tiles_of_rows(const Sequence& s) { return s.n > 0 ? ((s.keys - 1) >> 6) - (s.position() >> 6) + 1 : 0; }
+
+// the i-th of them, its places [p0, p1) that are rows of the call, and the call's row that place 0 would be
+struct TileRows {
+  int tile, p0, p1, row0;
+};
+constexpr TileRows tile_rows(const Sequence& s, int i) {
+  const int tile = (s.position() >> 6) + i;
+  return {tile, at_least(s.position() - tile * kPageKeys, 0), at_most(s.keys - tile * kPageKeys, kPageKeys), s.first + tile * kPageKeys - s.position()};
+}
+// Most tiles that `rows` rows of B sequences can lie in: n consecutive places touch at most floor((n + 62) / 64) + 1.
+constexpr int64_t most_tiles(int64_t rows, int64_t B) {
+  const int64_t used = B < rows ? B : rows;
+  return (rows + 62 * used) / kPageKeys + used;
+}
+
+// ---- attention: blocks of rb query rows (a token's G query heads of one kv head side by side), and the tiles they see ----
+
+constexpr int blocks_of(const Sequence& s, int G, int rb) { return (s.n * G + rb - 1) / rb; }
+// keys that query row r sees; past the last row: what that one sees
+constexpr int row_keys(const Sequence& s, int G, int causal, int r) {
+  if (!causal) return s.keys;
+  return at_most(at_least(s.position() + at_most((int)((unsigned)r / (unsigned)G), s.n - 1) + 1, 0), s.keys);
+}
+// tiles of block j: of its last row.  One at least: a block without keys writes zeros
+constexpr int block_tiles(const Sequence& s, int G, int causal, int rb, int j) {
+  return at_least((row_keys(s, G, causal, (j + 1) * rb - 1) + kPageKeys - 1) >> 6, 1);
+}
+
+// The tiles of all units end to end, in equal runs for `n` workgroups.
+constexpr int kMaxShares = 512;       // workgroups of a launch at most
+constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
+struct Shares {
+  int64_t total;
+  int n;
+  constexpr int64_t begin(int i) const { return total * i / n; }
+};
+constexpr Shares shares_of(int64_t total, int most) {
+  const int64_t worth = total / kMinShareTiles;
+  return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most)};
+}
+// The workgroup of a launch that takes run `rank`: a contiguous run of runs per XCD.  -1: none.
+constexpr int rank_of(int block, const Shares& sh) {
+  const int per_xcd = (sh.n + 7) / 8, rank = (block & 7) * per_xcd + (block >> 3);
+  return (block >> 3) < per_xcd && rank < sh.n ? rank : -1;
+}
+// A unit at [begin, end) of the tile space that several runs share: run i leaves its part in slot 2*i + 1 if its part begins the
+// unit, else in slot 2*i.
+constexpr int64_t part_slot(int run, bool begins) { return 2 * (int64_t)run + (begins ? 1 : 0); }
+// Of the boundary behind run i, inside the unit at [begin, end): whether it is the unit's first one, and then how many runs share the unit.
+// 0: not this boundary's business.
+constexpr int parts_behind(const Shares& sh, int i, int64_t unit_begin, int64_t unit_end) {
+  const int64_t pos = sh.begin(i + 1);
+  if (pos <= unit_begin || pos >= unit_end || sh.begin(i) > unit_begin) return 0;
+  int parts = 2;
+  while (i + parts < sh.n && sh.begin(i + parts) < unit_end) ++parts;
+  return parts;
+}
+
+}  // namespace pkh3

@@ -1,0 +1,464 @@
+"""The paged K/V cache on the card against a float64 restatement (oracle/paged_oracle.py).
+
+Tolerances.  bf16 rounds to half a step, 2^-8 relative; e4m3 to 2^-4, below 2^-6 of a scale to 2^-10 of it.  An attention output differs from
+the exact one by its own rounding (2^-8 |o|), by the rounding of the weights to bf16 (2^-8 of sum_j p_j |v_j|), by fp32 sums of up to some
+thousand terms (2^-14 of the same, generously) and, by the factor e^(2d) - 1, by an error d of the logits.  Without norm and rotation the
+operands are exact and d is the fp32 error of 128 products and the exponent, below 2^-14 for the logits here (|s| < 64).  With them
+the kernel rounds a query element to bf16 as the oracle does, but from an fp32 value: where that lies within 2^-20 of a border between two bf16
+numbers the two may differ by a step, 2^-7 |q|.  That happens to an element with probability 2^-12; four of a row's 128 are allowed for.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+EPS = 1e-6
+BF16 = 2.0 ** -8
+
+
+def _oracle():
+    from oracle import paged_oracle as P
+
+    return P
+
+
+def _rows(gen, n, heads, std=1.0):
+    return (torch.randn((n, heads, D), generator=gen) * std).to(torch.bfloat16)
+
+
+def _tables(gen, n):
+    angle = torch.rand((n, D // 2), generator=gen, dtype=torch.float64) * 60.0 - 30.0
+    return angle.cos().float(), angle.sin().float()
+
+
+def _dev(t):
+    if t is None:
+        return None
+    return tuple(x.cuda() for x in t) if isinstance(t, tuple) else t.cuda()
+
+
+class Held:
+    """A pool on the card and, sequence by sequence, the rows (bf16, on the host) that went into it unchanged."""
+
+    def __init__(self, lengths, heads, fp8, seed=0, poison=True, std=1.0, spare=3):
+        import pika_h3_flex_amd as pk
+
+        P = _oracle()
+        gen = torch.Generator().manual_seed(seed)
+        pages, self.lists = P.page_lists(lengths, spare, gen)
+        self.cache = pk.PagedKV(max(pages, 1), heads, fp8=fp8, device="cuda")
+        if poison:   # what no sequence holds is NaN in every reading of its bytes
+            self.cache.data.fill_(0xFF)
+        self.lengths, self.heads, self.fp8 = list(lengths), heads, fp8
+        self.k = [_rows(gen, n, heads, std) for n in lengths]
+        self.v = [_rows(gen, n, heads, std) for n in lengths]
+        if sum(lengths):
+            pk.paged_write(self.cache, self.batch(lengths), torch.cat(self.k).cuda(), torch.cat(self.v).cuda())
+
+    def batch(self, rows, lengths=None):
+        import pika_h3_flex_amd as pk
+
+        return pk.PagedBatch.build(rows, self.lengths if lengths is None else lengths, self.lists, device="cuda")
+
+    def stored(self, b):
+        P = _oracle()
+        return P.stored(self.k[b].double(), self.fp8), P.stored(self.v[b].double(), self.fp8)
+
+
+def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scale=None, std=1.0, repeat=True):
+    """New rows over a cache against the oracle, every row and head; returns the output."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    gen = torch.Generator().manual_seed(seed)
+    T = sum(rows)
+    q = _rows(gen, T, Hq, std)
+    w = (1.0 + 0.2 * torch.randn(D, generator=gen)) if norm else None
+    tables = _tables(gen, T) if rope else None
+    batch = held.batch(rows)
+    opts = dict(causal=causal, q_norm_weight=_dev(w), norm_eps=EPS, rope_mode=rope, rope_q=_dev(tables), softmax_scale=scale)
+    out = pk.paged_attention(q.cuda(), held.cache, batch, **opts)
+    torch.cuda.synchronize()
+    got = out.cpu().double()
+    assert torch.isfinite(got).all()
+    ready = P.norm_rope(q, w, EPS, tables, rope)
+    if norm or rope:
+        ready = ready.to(torch.bfloat16).double()
+    at = 0
+    for b, n in enumerate(rows):
+        k, v = held.stored(b)
+        ref, size = P.attend(ready[at:at + n], k, v, causal=causal, scale=scale)
+        d = 2.0 ** -14
+        if (norm or rope) and k.numel():
+            d = d + 4 * 2.0 ** -7 * float(ready.abs().max() * k.abs().max()) * (scale or 1 / math.sqrt(D))
+        bound = BF16 * ref.abs() + (BF16 + 2.0 ** -14 + math.expm1(2 * d)) * size * (1 + BF16)
+        off = (got[at:at + n] - ref).abs() - bound
+        assert float(off.max() if off.numel() else 0.0) <= 0.0, (b, n, float(off.max()), float((got[at:at + n] - ref).abs().max()))
+        # the sum over all elements leaves less room than the largest of them
+        if ref.numel() and float(ref.norm()) > 0:
+            assert float((got[at:at + n] - ref).norm() / ref.norm()) < 2 * BF16, (b, n)
+        at += n
+    if repeat:
+        again = pk.paged_attention(q.cuda(), held.cache, batch, **opts)
+        assert torch.equal(again, out)
+    return out
+
+
+# ---- writing and reading ----
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths,heads", [([1], 1), ([64], 2), ([65, 1, 130], 3), ([0, 63, 200, 0, 7], 8), ([1000, 321], 24)])
+def test_rows_come_back_as_they_are_held(lengths, heads, fp8):
+    import pika_h3_flex_amd as pk
+
+    held = Held(lengths, heads, fp8, seed=len(lengths) + heads)
+    k, v = pk.paged_read(held.cache, held.batch(lengths))
+    want = [held.stored(b) for b in range(len(lengths))]
+    assert torch.equal(k.cpu().double(), torch.cat([w[0] for w in want]))
+    assert torch.equal(v.cpu().double(), torch.cat([w[1] for w in want]))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_rows_arrive_in_pieces_and_nothing_else_is_touched(fp8):
+    """Chunks of 1 to 100 rows, page by page, equal one write of everything; the pool outside of the written places keeps its bytes."""
+    import pika_h3_flex_amd as pk
+
+    lengths, heads = [150, 37, 64, 0], 3
+    whole = Held(lengths, heads, fp8, seed=5, poison=False)
+    whole.cache.data.fill_(0x5A)
+    pk.paged_write(whole.cache, whole.batch(lengths), torch.cat(whole.k).cuda(), torch.cat(whole.v).cuda())
+    pieces = pk.PagedKV(whole.cache.pages, heads, fp8=fp8, device="cuda")
+    pieces.data.fill_(0x5A)
+    have = [0] * 4
+    for step in ([1, 1, 5, 0], [3, 0, 59, 0], [60, 20, 0, 0], [1, 16, 0, 0], [85, 0, 0, 0]):
+        have = [h + n for h, n in zip(have, step)]
+        cut = lambda rows: torch.cat([x[h - n:h] for x, h, n in zip(rows, have, step)]).cuda()   # noqa: E731
+        pk.paged_write(pieces, whole.batch(step, have), cut(whole.k), cut(whole.v))
+    assert have == lengths
+    assert torch.equal(pieces.data, whole.cache.data)
+    untouched = sorted(set(range(whole.cache.pages)) - {p for x in whole.lists for p in x})
+    assert untouched and bool((pieces.data[untouched] == 0x5A).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("norm,rope", [(True, 0), (False, 1), (True, 2), (True, 1)])
+def test_norm_and_rotation_of_the_keys(norm, rope, fp8):
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    lengths, rows, heads = [100, 333], [70, 129], 5
+    held = Held(lengths, heads, fp8, seed=9)
+    gen = torch.Generator().manual_seed(2)
+    T = sum(rows)
+    wide = torch.randn((T, heads + 2, 3 * D), generator=gen).to(torch.bfloat16)
+    wide_dev = wide.cuda()
+    k, v = wide[:, 1:1 + heads, D:2 * D], wide[:, :heads, 2 * D:]        # strided rows
+    w = (1.0 + 0.2 * torch.randn(D, generator=gen)) if norm else None
+    tables = _tables(gen, T) if rope else None
+    batch = held.batch(rows)
+    pk.paged_write(held.cache, batch, wide_dev[:, 1:1 + heads, D:2 * D], wide_dev[:, :heads, 2 * D:], k_norm_weight=_dev(w), norm_eps=EPS,
+                   rope_mode=rope, rope_k=_dev(tables))
+    got_k, got_v = (t.cpu().double() for t in pk.paged_read(held.cache, batch))
+    assert torch.equal(got_v, P.stored(v.double(), fp8))
+    exact = P.norm_rope(k, w, EPS, tables, rope)
+    slack = 2.0 ** -20 * exact.abs().amax(-1, keepdim=True)               # fp32 norm, weights and rotation
+    if fp8:
+        # a scale at a power of two may fall on either side of it: twice its share of the smallest step
+        bound = 2.0 ** -4 * exact.abs() + 2 * 2.0 ** -10 * P.key_scales(exact) + slack
+    else:
+        bound = BF16 * exact.abs() + slack
+    assert bool(((got_k - exact).abs() <= bound).all())
+    want = P.stored(exact, fp8)
+    assert float((got_k != want).double().mean()) < 2.0 ** -9              # nearly all round the same way
+
+
+def test_eight_bit_rows_of_every_size():
+    """Scales from the smallest to the largest that a bf16 row can need, rows of zeros, single values, magnitudes that are a power of two times 448."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    gen = torch.Generator().manual_seed(3)
+    n = 256
+    x = torch.randn((n, 1, D), generator=gen) * torch.exp2(torch.linspace(-100, 110, n))[:, None, None]
+    x[5] = 0.0
+    x[6] = 0.0
+    x[6, 0, 77] = 448.0
+    x[7, 0] = 448.0 * 2.0 ** -3
+    x[8, 0, :] = 0.0
+    x[8, 0, 3] = -450.0
+    x[9] = 1.0
+    x = x.to(torch.bfloat16)
+    held = Held([n], 1, True)
+    batch = held.batch([n])
+    pk.paged_write(held.cache, batch, x.cuda(), x.flip(0).contiguous().cuda())
+    k, v = (t.cpu().double() for t in pk.paged_read(held.cache, batch))
+    assert torch.equal(k, P.stored(x.double(), True)) and torch.equal(v, P.stored(x.flip(0).double(), True))
+
+
+def test_what_is_not_finite_is_stored_as_nan():
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    held = Held([5], 2, True)
+    x = _rows(torch.Generator().manual_seed(1), 5, 2)
+    bad = x.clone()
+    bad[1, 0, 3], bad[1, 0, 100], bad[2, 1, 0] = float("inf"), float("nan"), float("-inf")
+    pk.paged_write(held.cache, held.batch([5]), bad.cuda(), bad.cuda())
+    ref = x.double()
+    ref[1, 0, 3] = ref[1, 0, 100] = ref[2, 1, 0] = 0.0
+    want = P.stored(ref, True)
+    want[1, 0, 3] = want[1, 0, 100] = want[2, 1, 0] = float("nan")
+    for got in pk.paged_read(held.cache, held.batch([5])):
+        assert torch.equal(got.cpu().double().nan_to_num(1e9), want.nan_to_num(1e9))
+
+
+# ---- attention ----
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths,kv,Hq", [([1], 1, 1), ([2, 63, 64, 65], 1, 3), ([33, 700, 1, 129], 2, 2), ([500, 0, 3000], 4, 24), ([40] * 70, 3, 6)])
+def test_single_tokens(lengths, kv, Hq, fp8):
+    held = Held(lengths, kv, fp8, seed=kv)
+    _check_attention(held, [1] * len(lengths), Hq, causal=True)
+    _check_attention(held, [1] * len(lengths), Hq, causal=False, norm=True, rope=1)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,lengths,kv,Hq", [
+    ([2, 17], [2, 100], 2, 2), ([16, 0, 33, 1], [16, 64, 64, 300], 1, 5), ([65, 5], [200, 4], 2, 6), ([200, 31], [777, 31], 3, 3),
+    ([1, 300], [1500, 900], 2, 16), ([20, 20, 20], [0, 3, 500], 2, 2), ([700], [700], 1, 4)])
+def test_chunks(rows, lengths, kv, Hq, causal, fp8):
+    """Ragged chunks, more rows than keys, sequences without rows or keys, lengths at and around the ends of pages."""
+    held = Held(lengths, kv, fp8, seed=sum(rows))
+    _check_attention(held, rows, Hq, causal=causal)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("norm,rope,scale", [(True, 0, None), (False, 2, None), (True, 1, 0.05), (False, 0, 0.2)])
+def test_queries_through_norm_and_rotation(norm, rope, scale, fp8):
+    held = Held([300, 40, 129], 2, fp8, seed=4)
+    for rows in ([1, 1, 1], [40, 7, 100]):
+        _check_attention(held, rows, 4, causal=True, norm=norm, rope=rope, scale=scale)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows", [[1, 1], [50, 130]])
+def test_large_logits_raise_the_running_maximum(rows, fp8):
+    """Logits up to +-60, larger ones towards the end of the keys: the maximum is raised over and over."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([900, 400], 2, fp8, seed=8, std=1.0)
+    for b in range(2):
+        held.k[b] = (held.k[b].float() * torch.linspace(0.1, 1.5, held.lengths[b])[:, None, None]).to(torch.bfloat16)
+    pk.paged_write(held.cache, held.batch(held.lengths), torch.cat(held.k).cuda(), torch.cat(held.v).cuda())
+    _check_attention(held, rows, 4, causal=False, std=8.0)
+
+
+def test_long_contexts_are_shared_out():
+    """Few units of many tiles: every workgroup has a part of one, and the parts are joined."""
+    held = Held([9000, 20000], 2, False, seed=3)
+    _check_attention(held, [1, 1], 2, causal=True)
+    _check_attention(held, [3, 20], 4, causal=True)
+    _check_attention(Held([20000], 1, True, seed=3), [2], 8, causal=True)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_pages_that_are_not_there(fp8):
+    """Table entries outside of the pool: their keys are seen by nobody, writes to them dropped, reads of them zero; the rest as without them."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    lengths, kv = [200, 70], 2
+    held = Held(lengths, kv, fp8, seed=6)
+    rows = [5, 3]
+    batch = held.batch(rows)
+    table = batch.table.clone()
+    table[0, 1], table[1, 0] = held.cache.pages, -5
+    batch = pk.PagedBatch(batch.starts, batch.lengths, table, batch.rows)
+    q = _rows(torch.Generator().manual_seed(1), 8, 4)
+    got = pk.paged_attention(q.cuda(), held.cache, batch).cpu().double()
+    k0, v0 = held.stored(0)
+    k1, v1 = held.stored(1)
+    here = [i for i in range(200) if not 64 <= i < 128]
+    ref = torch.cat([P.attend(q[:5], k0[here], v0[here], causal=False)[0], P.attend(q[5:], k1[64:], v1[64:], causal=False)[0]])
+    size = torch.cat([P.attend(q[:5], k0[here], v0[here], causal=False)[1], P.attend(q[5:], k1[64:], v1[64:], causal=False)[1]])
+    assert bool(((got - ref).abs() <= BF16 * ref.abs() + (BF16 + 2.0 ** -12) * size).all())
+    everything = pk.PagedBatch.build(lengths, lengths, held.lists, device="cuda")
+    everything.table.copy_(table)
+    k, v = pk.paged_read(held.cache, everything)
+    want = torch.cat([k0, k1])
+    want[64:128] = 0
+    want[200:264] = 0
+    assert torch.equal(k.cpu().double(), want) and bool((v[64:128] == 0).all()) and bool((v[200:264] == 0).all())
+    before = held.cache.data.clone()
+    table.fill_(2 ** 31 - 1)
+    nowhere = pk.PagedBatch(everything.starts, everything.lengths, table, everything.rows)
+    pk.paged_write(held.cache, nowhere, torch.cat(held.k).cuda(), torch.cat(held.v).cuda())
+    assert torch.equal(held.cache.data, before)
+    assert bool((pk.paged_attention(q.cuda(), held.cache, pk.PagedBatch(batch.starts, batch.lengths, table, 8)) == 0).all())
+
+
+def test_arrays_out_of_range_are_brought_into_it():
+    """starts beyond the rows, lengths beyond the table: as the header says, and rows of no sequence keep what they held."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([128, 64], 2, False, seed=6)
+    q = _rows(torch.Generator().manual_seed(1), 6, 2).cuda()
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    table = held.batch([0, 0]).table
+    wild = pk.PagedBatch(as_int([1, 4, 99]), as_int([10 ** 9, -3]), table)
+    tame = pk.PagedBatch(as_int([1, 4, 6]), as_int([128, 0]), table)
+    a, b = (torch.full_like(q, 7.0) for _ in range(2))
+    pk.paged_attention(q, held.cache, wild, out=a)
+    pk.paged_attention(q, held.cache, tame, out=b)
+    assert torch.equal(a, b) and bool((a[0] == 7.0).all()) and bool((a[4:] == 0).all())
+    ka, va = (torch.full((6, 2, D), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pk.paged_read(held.cache, wild, out=(ka, va))
+    assert bool((ka[0] == 7.0).all()) and bool((ka[4:] == 0).all()) and torch.equal(ka[1:4].cpu(), held.k[0][125:128])
+    backwards = pk.PagedBatch(as_int([4, 1, 1]), as_int([128, 64]), table)
+    c = torch.full_like(q, 7.0)
+    pk.paged_attention(q, held.cache, backwards, out=c)
+    assert bool((c == 7.0).all())
+
+
+def test_strides_order_and_the_output_in_the_queries_place():
+    import pika_h3_flex_amd as pk
+
+    held = Held([300, 90], 2, False, seed=7)
+    batch = held.batch([40, 3])
+    gen = torch.Generator().manual_seed(5)
+    q = _rows(gen, 43, 6).cuda()
+    want = pk.paged_attention(q, held.cache, batch, causal=True)
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)           # [rows, heads, 128] with the heads outermost in memory
+    wide = torch.full((43, 6, 2 * D), 3.0, dtype=torch.bfloat16, device="cuda")
+    got = pk.paged_attention(heads_first, held.cache, batch, causal=True, out=wide[..., D:])
+    assert torch.equal(got, want) and bool((wide[..., :D] == 3.0).all())
+    same = q.clone()
+    assert torch.equal(pk.paged_attention(same, held.cache, batch, causal=True, out=same), want)
+    table = torch.full((2, 40), -1, dtype=torch.int32, device="cuda")[:, ::1]
+    table[:, :batch.table.shape[1]] = batch.table
+    assert torch.equal(pk.paged_attention(q, held.cache, pk.PagedBatch(batch.starts, batch.lengths, table[:, :batch.table.shape[1] + 3]), causal=True), want)
+
+
+def test_one_page_in_two_sequences():
+    """A prefix that two sequences share is read by both."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    held = Held([64 + 20, 64 + 50], 1, False, seed=2)
+    lists = [list(x) for x in held.lists]
+    lists[1][0] = lists[0][0]
+    batch = pk.PagedBatch.build([1, 1], held.lengths, lists, device="cuda")
+    q = _rows(torch.Generator().manual_seed(1), 2, 1)
+    got = pk.paged_attention(q.cuda(), held.cache, batch).cpu().double()
+    (k0, v0), (k1, v1) = held.stored(0), held.stored(1)
+    ref, size = P.attend(q[1:], torch.cat([k0[:64], k1[64:]]), torch.cat([v0[:64], v1[64:]]), causal=False)
+    assert bool(((got[1:] - ref).abs() <= BF16 * ref.abs() + (BF16 + 2.0 ** -12) * size).all())
+
+
+def test_a_captured_step_replays_with_changed_batches():
+    """A token step in a graph: rows, lengths, pages and inputs change in place between the replays, and every replay equals the eager calls."""
+    import pika_h3_flex_amd as pk
+
+    for fp8 in (False, True):
+        held = Held([100, 63, 5], 2, fp8, seed=1, spare=9)
+        used = [list(x) for x in held.lists]
+        free = [p for p in range(held.cache.pages) if p not in {y for x in used for y in x}]
+        table = torch.full((3, 4), -1, dtype=torch.int32)
+        for b, x in enumerate(used):
+            x += [free.pop() for _ in range(4 - len(x))]
+            table[b] = torch.tensor(x, dtype=torch.int32)
+        as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+        batch = pk.PagedBatch(as_int([0, 1, 2, 3]), as_int([100, 63, 5]), table.cuda())
+        gen = torch.Generator().manual_seed(4)
+        q, k, v = (torch.zeros((3, h, D), dtype=torch.bfloat16, device="cuda") for h in (4, 2, 2))
+        out = torch.empty_like(q)
+
+        def step(cache, out):
+            pk.paged_write(cache, batch, k, v)
+            pk.paged_attention(q, cache, batch, causal=True, out=out)
+
+        twin = pk.PagedKV(held.cache.pages, 2, fp8=fp8, data=held.cache.data.clone())
+        pk.paged_attention(q, held.cache, batch, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(held.cache, out)
+        for turn in range(4):
+            batch.lengths.add_(as_int([1, 2, 60]) if turn == 2 else 1)
+            for t, h in ((q, 4), (k, 2), (v, 2)):
+                t.copy_(_rows(gen, 3, h))
+            eager = torch.empty_like(q)
+            step(twin, eager)
+            graph.replay()
+            torch.cuda.synchronize()
+            # (bits: the jump of turn 2 brings keys into two of the sequences that nobody wrote, and those hold NaN)
+            assert torch.equal(out.view(torch.int16), eager.view(torch.int16)) and bool(torch.isfinite(out[0 if turn >= 2 else slice(None)]).all()), turn
+            assert torch.equal(held.cache.data, twin.data)
+
+
+def test_two_streams_with_a_workspace_each():
+    import pika_h3_flex_amd as pk
+
+    held = Held([5000, 3000], 4, True, seed=2)
+    batch = held.batch([1, 20])
+    gen = torch.Generator().manual_seed(3)
+    qs = [_rows(gen, 21, 8).cuda() for _ in range(2)]
+    want = [pk.paged_attention(q, held.cache, batch, causal=True) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(pk.paged_attention(qs[i], held.cache, batch, causal=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_a_given_workspace_may_hold_anything():
+    import pika_h3_flex_amd as pk
+
+    held = Held([4000], 2, False, seed=2)
+    batch = held.batch([3])
+    q = _rows(torch.Generator().manual_seed(3), 3, 2).cuda()
+    want = pk.paged_attention(q, held.cache, batch)
+    seen = []
+
+    def scratch(device, nbytes):
+        seen.append(nbytes)
+        return torch.full((nbytes,), 0xFF, dtype=torch.uint8, device=device)
+
+    assert torch.equal(pk.paged_attention(q, held.cache, batch, workspace=scratch), want) and seen
+    small = torch.empty(16, dtype=torch.uint8, device="cuda")              # too small: the call takes one of its own
+    assert torch.equal(pk.paged_attention(q, held.cache, batch, workspace=small), want)
+
+
+def test_empty_calls():
+    import pika_h3_flex_amd as pk
+
+    held = Held([70], 2, False)
+    batch = held.batch([0])
+    none = torch.empty((0, 2, D), dtype=torch.bfloat16, device="cuda")
+    assert pk.paged_attention(none, held.cache, batch).shape == (0, 2, D)
+    pk.paged_write(held.cache, batch, none, none)
+    assert pk.paged_read(held.cache, batch)[0].shape == (0, 2, D)
+
+
+def test_agrees_with_attention_over_the_same_rows():
+    """The paged call against the dense one of this library on the rows that paged_read gives back."""
+    import pika_h3_flex_amd as pk
+
+    for fp8 in (False, True):
+        held = Held([640], 4, fp8, seed=12)
+        q = _rows(torch.Generator().manual_seed(3), 200, 4).cuda()
+        got = pk.paged_attention(q, held.cache, held.batch([200]))
+        k, v = pk.paged_read(held.cache, held.batch([640]))
+        dense = pk.attention(q[None], k[None], v[None])[0]
+        # both round their weights and outputs to bf16, the dense call its queries too (after the softmax scale): logits off by at most 2^-8 |q| |k| / sqrt(D)
+        size = pk.attention(q[None], k[None], v[None].abs())[0].float()
+        d = 2.0 ** -8 * float(q.float().norm(dim=-1).max() * k.float().norm(dim=-1).max()) / math.sqrt(D)
+        assert bool(((got.float() - dense.float()).abs() <= (4 * BF16 + math.expm1(2 * d)) * size).all())

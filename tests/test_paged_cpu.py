@@ -1,0 +1,271 @@
+"""The paged K/V cache without a GPU: refusals of the C entries and of the Python front end, and the index arithmetic of the kernels in a
+host build -- batches whose arrays hold anything, and every tile of every unit done once."""
+import ctypes as C
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import pika_h3_flex_amd as pk
+from pika_h3_flex_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "pika-h3-flex_amd", "csrc")
+
+
+def test_struct_layout_matches_header():
+    header = open(os.path.join(ROOT, "include", "pkh3_paged.h")).read()
+    body = header[header.index("typedef struct pkh3_paged_args {"): header.index("} pkh3_paged_args;")]
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S).split("{", 1)[1]
+    names = [re.findall(r"[A-Za-z_][A-Za-z_0-9]*", part)[-1] for decl in body.split(";") if decl.strip() for part in decl.split(",")]
+    assert names == [f[0] for f in _lib.PagedArgs._fields_]
+
+
+def _args():
+    a = _lib.PagedArgs()
+    buf = 0x10000   # made-up, aligned addresses: refusals come before anything looks at them
+    for n in ("pages", "starts", "lengths", "table", "q", "k", "v", "o", "workspace"):
+        setattr(a, n, buf)
+    for n in ("q", "k", "v", "o"):
+        setattr(a, n + "_ss", 4 * 128)
+        setattr(a, n + "_sh", 128)
+    a.n_pages, a.table_stride, a.B, a.table_pages, a.rows, a.kv_heads, a.heads, a.D = 9, 4, 2, 4, 5, 2, 4, 128
+    a.norm_eps = 1e-6
+    a.workspace_bytes = 1 << 30
+    return a
+
+
+def test_sizes_on_the_host(lib):
+    assert lib.pkh3_paged_record_bytes(0) == 32768 and lib.pkh3_paged_record_bytes(_lib.PAGED_FP8) == 16384 + 128
+    assert lib.pkh3_paged_record_bytes(8) == 0
+    a = _args()
+    n = lib.pkh3_paged_workspace_bytes(C.byref(a))
+    assert n > 0 and n % 256 == 0
+    a.rows = 0
+    assert lib.pkh3_paged_workspace_bytes(C.byref(a)) > 0
+    a.heads = 3
+    assert lib.pkh3_paged_workspace_bytes(C.byref(a)) == 0
+
+
+def _set(**kw):
+    return lambda a: [setattr(a, k, v) for k, v in kw.items()]
+
+
+COMMON = [
+    (_set(pages=0), _lib.PKH3_ENULL), (_set(pages=0x10010), _lib.PKH3_EALIGN), (_set(starts=0), _lib.PKH3_ENULL),
+    (_set(lengths=0), _lib.PKH3_ENULL), (_set(table=0), _lib.PKH3_ENULL), (_set(starts=0x10002), _lib.PKH3_EALIGN),
+    (_set(D=64), _lib.PKH3_EHEADDIM), (_set(flags=4), _lib.PKH3_EARG), (_set(B=0), _lib.PKH3_ESHAPE), (_set(B=1025), _lib.PKH3_ESHAPE),
+    (_set(rows=-1), _lib.PKH3_ESHAPE), (_set(rows=(1 << 24) + 1), _lib.PKH3_ESHAPE), (_set(kv_heads=0), _lib.PKH3_ESHAPE),
+    (_set(table_pages=0), _lib.PKH3_ESHAPE), (_set(table_pages=(1 << 24) + 1), _lib.PKH3_ESHAPE), (_set(table_stride=-4), _lib.PKH3_ESTRIDE),
+    (_set(n_pages=0), _lib.PKH3_ESHAPE), (_set(n_pages=1 << 31), _lib.PKH3_ESHAPE), (_set(rows=1 << 24, heads=65534), _lib.PKH3_ESHAPE),
+]
+ROWS_IN = [(_set(rope_mode=3), _lib.PKH3_EARG), (_set(rope_mode=1), _lib.PKH3_ENULL), (_set(rope_mode=1, rope_cos=0x10008, rope_sin=0x10000), _lib.PKH3_EALIGN),
+           (_set(norm_w=0x10004), _lib.PKH3_EALIGN), (_set(norm_w=0x10000, norm_eps=-1.0), _lib.PKH3_EARG),
+           (_set(norm_w=0x10000, norm_eps=float("nan")), _lib.PKH3_EARG)]
+
+
+def _refuses(lib, entry, mutate, code):
+    a = _args()
+    mutate(a)
+    assert getattr(lib, entry)(C.byref(a), None) == code
+    assert lib.pkh3_last_error() != b""
+
+
+@pytest.mark.parametrize("mutate,code", COMMON + ROWS_IN + [
+    (_set(q=0), _lib.PKH3_ENULL), (_set(o=0), _lib.PKH3_ENULL), (_set(q=0x10008), _lib.PKH3_EALIGN), (_set(q_ss=132), _lib.PKH3_ESTRIDE),
+    (_set(q_sh=-128), _lib.PKH3_ESTRIDE), (_set(o_sh=0), _lib.PKH3_ESTRIDE), (_set(o_ss=0), _lib.PKH3_ESTRIDE), (_set(heads=3), _lib.PKH3_ESHAPE),
+    (_set(heads=0), _lib.PKH3_ESHAPE), (_set(softmax_scale=float("nan")), _lib.PKH3_EARG), (_set(softmax_scale=float("inf")), _lib.PKH3_EARG),
+    (_set(workspace=0), _lib.PKH3_EWORKSPACE), (_set(workspace=0x10010), _lib.PKH3_EWORKSPACE), (_set(workspace_bytes=1024), _lib.PKH3_EWORKSPACE)])
+def test_attention_refuses(lib, mutate, code):
+    _refuses(lib, "pkh3_paged_attn", mutate, code)
+
+
+@pytest.mark.parametrize("mutate,code", [c for c in COMMON[:-1]] + ROWS_IN + [
+    (_set(k=0), _lib.PKH3_ENULL), (_set(v=0x10008), _lib.PKH3_EALIGN), (_set(k_ss=100), _lib.PKH3_ESTRIDE), (_set(flags=2), _lib.PKH3_EARG)])
+def test_write_refuses(lib, mutate, code):
+    _refuses(lib, "pkh3_paged_write", mutate, code)
+
+
+@pytest.mark.parametrize("mutate,code", [c for c in COMMON[:-1]] + [
+    (_set(k=0), _lib.PKH3_ENULL), (_set(v=0), _lib.PKH3_ENULL), (_set(v_sh=64), _lib.PKH3_ESTRIDE), (_set(k_sh=0), _lib.PKH3_ESTRIDE), (_set(flags=2), _lib.PKH3_EARG)])
+def test_read_refuses(lib, mutate, code):
+    _refuses(lib, "pkh3_paged_read", mutate, code)
+
+
+def test_no_rows_is_no_launch(lib):
+    a = _args()
+    a.rows = 0
+    for entry in ("pkh3_paged_write", "pkh3_paged_read", "pkh3_paged_attn"):
+        assert getattr(lib, entry)(C.byref(a), None) == 0 and lib.pkh3_last_error() == b""
+    assert lib.pkh3_paged_attn(None, None) == _lib.PKH3_ENULL
+
+
+def test_batches_are_checked_where_they_are_built():
+    build = lambda *a: pk.PagedBatch.build(*a, device="cpu")   # noqa: E731
+    b = build([1, 0, 3], [70, 0, 3], [[4, 2], [], [0]])
+    assert b.starts.tolist() == [0, 1, 1, 4] and b.lengths.tolist() == [70, 0, 3] and b.table.tolist() == [[4, 2], [-1, -1], [0, -1]] and b.rows == 4
+    assert build([2], [0], [[]]).table.tolist() == [[-1]]
+    for bad in (([], [], []), ([1], [1, 2], [[0]]), ([1], [65], [[0]]), ([-1], [1], [[0]]), ([1], [-1], [[0]]), ([1], [1], [[-2]]),
+                ([1] * 1025, [1] * 1025, [[0]] * 1025)):
+        with pytest.raises(ValueError):
+            build(*bad)
+
+
+def test_the_front_end_refuses_what_the_kernels_cannot_take():
+    """Tensors of the host, wrong types, shapes and strides are errors before any call."""
+    cache = pk.PagedKV(3, 2, device="cpu")
+    batch = pk.PagedBatch.build([1], [1], [[0]], device="cpu")
+    rows = torch.zeros((1, 2, 128), dtype=torch.bfloat16)
+    for call in (lambda: pk.paged_write(cache, batch, rows, rows), lambda: pk.paged_attention(rows, cache, batch), lambda: pk.paged_read(cache, batch)):
+        with pytest.raises(ValueError, match="device memory"):
+            call()
+    with pytest.raises(TypeError):
+        pk.paged_attention(rows.float(), cache, batch)
+    with pytest.raises(ValueError):
+        pk.paged_attention(rows[..., :64], cache, batch)
+    with pytest.raises(ValueError):
+        pk.paged_write(cache, batch, rows[:, :1], rows)
+    with pytest.raises(ValueError):
+        pk.PagedKV(0, 2, device="cpu")
+    with pytest.raises(ValueError):
+        pk.PagedKV(3, 2, device="cpu", data=torch.zeros((3, 2, 5), dtype=torch.uint8))
+    with pytest.raises(ValueError, match="say how many"):
+        pk.paged_read(cache, pk.PagedBatch(batch.starts, batch.lengths, batch.table))
+
+
+# ---- index arithmetic ----
+
+def _run(tmp_path, body):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no C++ compiler")
+    src, exe = tmp_path / "host.cc", tmp_path / "host"
+    src.write_text('#include "pkh3_paged_index.h"\n#include <stdio.h>\n#include <stdlib.h>\n#include <vector>\n#include <algorithm>\nusing namespace pkh3;\n'
+                   '#define CHECK(x, ...) do { if (!(x)) { printf(#x ": " __VA_ARGS__); return 1; } } while (0)\n'
+                   "[[maybe_unused]] static int any(int lo, int hi) { return lo + (int)(rand() % (hi - lo + 1)); }\n"
+                   "int main() {\n  srand(1);\n" + body + "\n  return 0;\n}\n")
+    subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", CSRC, str(src), "-o", str(exe)],
+                   check=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_rows_and_pages_stay_in_range_whatever_the_arrays_hold(tmp_path):
+    _run(tmp_path, """
+  const int wild[] = {0, 1, 5, 63, 64, 65, 1000, -1, -7, 2147483647, -2147483647 - 1, 16777216, 1 << 30};
+  const int n_wild = sizeof(wild) / sizeof(int);
+  for (int a = 0; a < n_wild; ++a) for (int b = 0; b < n_wild; ++b) for (int c = 0; c < n_wild; ++c)
+    for (int rows : {0, 1, 70, 16777216}) for (int pages : {1, 3, 16777216}) {
+      const Sequence s = make_sequence(wild[a], wild[b], wild[c], rows, pages);
+      CHECK(s.first >= 0 && s.n >= 0 && s.first + s.n <= rows && s.keys >= 0 && s.keys <= pages * 64, "%d %d %d", wild[a], wild[b], wild[c]);
+      const int tiles = tiles_of_rows(s);
+      CHECK((tiles > 0) == (s.n > 0) && tiles <= s.n / 64 + 2, "%d tiles of %d rows", tiles, s.n);
+      for (int i : {0, 1, tiles / 2, tiles - 1}) {
+        if (i < 0 || i >= tiles) continue;
+        const TileRows t = tile_rows(s, i);
+        CHECK(t.p0 >= 0 && t.p0 < t.p1 && t.p1 <= 64 && t.row0 + t.p0 >= s.first && t.row0 + t.p1 <= s.first + s.n, "tile %d", i);
+      }
+      for (int G : {1, 6}) for (int causal : {0, 1}) for (int rb : {16, 32, 128, 384}) {
+        if (s.n == 0 || (int64_t)rows * G > (1 << 30)) continue;
+        const int blocks = blocks_of(s, G, rb);
+        for (int j : {0, blocks / 2, blocks - 1}) {
+          const int t = block_tiles(s, G, causal, rb, j);
+          CHECK(t >= 1 && t <= (pages > 1 ? pages : 1), "%d tiles", t);
+          for (int r = j * rb; r < std::min((j + 1) * rb, s.n * G); ++r) {
+            const int k = row_keys(s, G, causal, r);
+            CHECK(k >= 0 && k <= s.keys && k <= 64 * t, "row %d sees %d", r, k);
+            CHECK(k == (causal ? std::max(0, std::min(s.keys, s.keys - s.n + r / G + 1)) : s.keys), "row %d sees %d", r, k);
+            CHECK(k >= row_keys(s, G, causal, j * rb), "the first row of a block sees least");
+          }
+        }
+      }
+    }
+  for (int id : {-1, 0, 4, 5, 2147483647}) CHECK(page_in_pool(id, 5) == (id >= 0 && id < 5 ? id : -1), "%d", id);""")
+
+
+def test_every_row_lies_in_one_tile_of_the_launch(tmp_path):
+    _run(tmp_path, """
+  for (int go = 0; go < 3000; ++go) {
+    const int B = any(1, 9);
+    std::vector<int> starts(1, any(0, 2)), keys;
+    for (int b = 0; b < B; ++b) {
+      starts.push_back(starts.back() + (any(0, 3) ? any(0, 3) ? any(0, 5) : any(0, 300) : 0));
+      keys.push_back(any(0, 3) ? any(0, 400) : any(0, 3));
+    }
+    const int rows = starts.back() + any(0, 2);
+    std::vector<int> times(rows, 0);
+    int64_t tiles = 0;
+    for (int b = 0; b < B; ++b) {
+      const Sequence s = make_sequence(starts[b], starts[b + 1], keys[b], rows, 10);
+      tiles += tiles_of_rows(s);
+      for (int i = 0; i < tiles_of_rows(s); ++i) {
+        const TileRows t = tile_rows(s, i);
+        for (int at = t.p0; at < t.p1; ++at) {
+          ++times[t.row0 + at];
+          CHECK(t.tile * 64 + at == s.position() + (t.row0 + at - s.first), "place");
+        }
+      }
+    }
+    CHECK(tiles <= most_tiles(rows, B), "%lld tiles, the launch has %lld", (long long)tiles, (long long)most_tiles(rows, B));
+    for (int r = 0; r < rows; ++r) CHECK(times[r] == (r >= starts[0] && r < starts[B] ? 1 : 0), "row %d: %d times", r, times[r]);
+  }""")
+
+
+def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
+    """The walk of the attention kernels, all workgroups of a launch: every tile of every unit in one run, a unit's parts in slots of their own, and
+    every cut unit joined at one boundary, in the order of the runs."""
+    _run(tmp_path, """
+  for (int go = 0; go < 4000; ++go) {
+    const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 4 == 0 ? 384 : go % 4 == 1 ? 32 : 16;
+    const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 512;
+    std::vector<Sequence> seq;
+    struct Unit { int64_t begin, end; };
+    std::vector<Unit> units;
+    int64_t total = 0;
+    for (int b = 0; b < B; ++b) {
+      const int n = any(0, 2) ? any(0, 40) : any(0, 900), keys = any(0, 3) ? any(0, 2000) : any(0, 64);
+      seq.push_back(make_sequence(0, n, keys, 1000, 100));
+      for (int h = 0; h < H; ++h)
+        for (int j = 0; j < blocks_of(seq[b], G, rb); ++j) {
+          const int t = block_tiles(seq[b], G, causal, rb, j);
+          units.push_back({total, total + t});
+          total += t;
+        }
+    }
+    const Shares sh = shares_of(total, grid);
+    CHECK(sh.n >= 1 && sh.n <= grid && sh.begin(0) == 0 && sh.begin(sh.n) == total, "%d runs", sh.n);
+    std::vector<int> who(sh.n, 0);
+    for (int block = 0; block < grid; ++block) {
+      const int r = rank_of(block, sh);
+      CHECK(r >= -1 && r < sh.n, "rank %d", r);
+      if (r >= 0) ++who[r];
+    }
+    for (int r = 0; r < sh.n; ++r) CHECK(who[r] == 1, "run %d of %d taken %d times", r, sh.n, who[r]);
+    if (total == 0) continue;
+    std::vector<int> left(2 * sh.n, -1);                    // the unit whose part lies in a slot
+    for (int r = 0; r < sh.n; ++r) {
+      CHECK(sh.begin(r) < sh.begin(r + 1), "run %d is empty", r);
+      for (size_t u = 0; u < units.size(); ++u) {
+        const int64_t from = std::max(units[u].begin, sh.begin(r)), to = std::min(units[u].end, sh.begin(r + 1));
+        if (from >= to || (from == units[u].begin && to == units[u].end)) continue;
+        const int64_t slot = part_slot(r, from == units[u].begin);
+        CHECK(slot >= 0 && slot < 2 * sh.n && left[slot] < 0, "slot %lld twice", (long long)slot);
+        left[slot] = (int)u;
+      }
+    }
+    for (size_t u = 0; u < units.size(); ++u) {
+      int joined = 0, cuts = 0;
+      for (int i = 0; i + 1 < sh.n; ++i) {
+        if (sh.begin(i + 1) > units[u].begin && sh.begin(i + 1) < units[u].end) ++cuts;
+        const int parts = parts_behind(sh, i, units[u].begin, units[u].end);
+        if (!parts) continue;
+        ++joined;
+        for (int k = 0; k < parts; ++k) CHECK(left[part_slot(i + k, k == 0)] == (int)u, "part %d", k);
+        CHECK(parts == 1 + (int)std::count(left.begin() + 2 * i + 2, left.end(), (int)u), "%d parts", parts);
+      }
+      CHECK(joined == (cuts > 0), "unit cut %d times, joined %d", cuts, joined);
+    }
+  }""")
