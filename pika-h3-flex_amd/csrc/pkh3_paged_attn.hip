@@ -13,19 +13,25 @@
 // from one to the other in its lane, running maximum raised when exceeded by 2^8.  Q' is rounded to bf16 after norm and rotation and not
 // before: the softmax scale multiplies S^T (in fp32, in the subtraction of the maximum), so that queries without norm and rotation are exact.
 // e4m3 keys times their power of two are exact in bf16; the scale of a value's key goes to P instead, exact there as well.
-#include <float.h>
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pkh3_paged.h"
 #include "pkh3_internal.h"
+#include "pkh3_wave.h"
 
 namespace pkh3 {
 
-constexpr float kNoMax = -FLT_MAX;       // the running max before the first key: finite, so that rows without a key add up to nothing
-constexpr float kRescaleSlack = 8.0f;    // the running max is raised only when exceeded by 2^8
 constexpr int kSplitWaves = 4;
+
+// The lane's number, made where it is used
+__device__ __forceinline__ int lane_here() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
 
 // ---- the tile space ----
 
@@ -103,6 +109,24 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t*
     rest -= __shfl(x, 63);
   }
 }
+
+// On to the next unit of a run with `left` tiles to go.  False where there is none.
+__device__ __forceinline__ bool next_unit(const PagedParams& p, Place& at, Sequence& s, int& blocks, int rb, int64_t left) {
+  if (left <= 0) return false;
+  if (++at.j < blocks) return true;
+  at.j = 0;
+  if (++at.h < p.H) return true;
+  at.h = 0;
+  do {
+    if (++at.b >= p.B) return false;
+    s = uniform_sequence(p, at.b);
+  } while (s.n == 0);
+  blocks = blocks_of(p, s, rb);
+  return true;
+}
+
+// 1 / l; rows without a key: 0.  (A sum that is not a number stays one.)
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
 // A part of a unit in the scratch: RB rows of 128, then their maxima, then their sums
 __host__ __device__ constexpr int part_floats(int rb) { return rb * (kD + 2); }
@@ -406,7 +430,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
         }
       }
       if (finished) {
-        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a sum that is not a number stays one)
+        const float inv = inverse_sum(l);
         bf16x8 out;
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] = (__bf16)(sum[i >> 2][i & 3] * inv);
@@ -423,17 +447,332 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
     }
     left -= take;
     at.t = 0;
-    if (++at.j == blocks) {
-      at.j = 0;
-      if (++at.h == p.H) {
-        at.h = 0;
-        do {                                                   // (a run that goes on does so in a sequence with rows)
-          if (++at.b >= p.B) return;
-          s = uniform_sequence(p, at.b);
-        } while (s.n == 0);
-        blocks = blocks_of(p, s, RB);
+    if (!next_unit(p, at, s, blocks, RB, left)) return;
+  }
+}
+
+// ---- the tile form: many query rows, all waves of a workgroup share every key tile ----
+//
+// A unit is 32 query rows a wave: 384 rows in 12 waves (three a SIMD, one workgroup a CU), or 128 in 4 (three workgroups a CU) where 384 would
+// leave most of a workgroup without rows.  The loop is that of the dense calls: K/V steps (a tile of 64 keys, half of one in the small
+// form) in an LDS ring of three, two steps ahead of the products, one barrier a step.  The page of a step is looked up a step before its copy.
+// Eight-bit pages come to LDS as they are, one step further ahead, and are expanded there to the bf16 images of the loop, a share of
+// them by every wave, under the products of the step before: once for all waves, and the loop has no conversions.
+//
+// The running maximum costs little here: only whether any logit of the wave exceeds its query's maximum by 2^8 is asked for in every step, the exchange
+// between lanes and the rescale happen when one does.
+
+template <int WAVES>
+struct TileForm {
+  static constexpr int kStep = WAVES == 4 ? 32 : 64;                     // keys
+  static constexpr int kBytes = kStep * 2 * kD * 2;                      // of a step's bf16 images: K, then V
+  static constexpr int kRaw = kStep * 2 * kD;                            // of its e4m3 values
+  static constexpr int kRawSlot = kRaw + kPageScales;
+  // bf16: a ring of three steps.  e4m3: two steps of images, two as they come
+  template <bool FP8>
+  static constexpr int ring_bytes() { return FP8 ? 2 * kBytes + 2 * kRawSlot : 3 * kBytes; }
+  static constexpr int kStage = 32 * kD * 2;                             // a wave's output rows
+  template <bool FP8>
+  static constexpr int lds_bytes() {
+    // before the loop the queries are turned around where the third step goes (e4m3: the second step's images) and behind it
+    const int before = (FP8 ? 1 : 2) * kBytes + WAVES * 4096, after = WAVES * kStage, sums = (kMaxSequences + 1) * (int)sizeof(int64_t);
+    int most = ring_bytes<FP8>() > before ? ring_bytes<FP8>() : before;
+    most = most > after ? most : after;
+    return most > sums ? most : sums;
+  }
+};
+
+// The weights of NKB blocks of 16 keys, as operands of P.V (see softmax_blocks of the dense calls).  MASKED: lim[qb] keys of these exist for the
+// lane's query.
+template <int NKB, bool MASKED>
+__device__ __forceinline__ void tile_softmax(WaveState<false>& w, bf16x8 (&pf)[NKB / 2][2], float c, const int (&lim)[2], int lane) {
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const int mine = lim[qb] - 4 * (lane >> 4);                         // (against constants from here on)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.s[kb][qb][i] = 16 * kb + i >= mine ? -INFINITY : w.s[kb][qb][i];
+    }
+  }
+  float mx[2];
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    mx[qb] = w.s[0][qb][0];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[qb] = fmaxf(mx[qb], w.s[kb][qb][i]);
+    mx[qb] *= c;
+  }
+  if (__any(mx[0] > w.m[0] + kRescaleSlack || mx[1] > w.m[1] + kRescaleSlack)) {
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const float top = max_across_groups(mx[qb]);
+      const float m_new = top > w.m[qb] + kRescaleSlack ? top : w.m[qb];
+      const float alpha = __builtin_amdgcn_exp2f(w.m[qb] - m_new);
+      w.m[qb] = m_new;
+      w.l[qb] *= alpha;
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.o[db][qb][i] *= alpha;
+    }
+  }
+  const bf16x2 one2 = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+  for (int half = 0; half < NKB / 2; ++half)
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      bf16x8 pk;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pk[j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(w.s[2 * half + (j >> 2)][qb][j & 3], c, -w.m[qb]));
+      // row sum over the rounded weights, the same numbers P.V takes
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const bf16x2 pr = {pk[j], pk[j + 1]};
+        w.l[qb] = __builtin_amdgcn_fdot2_f32_bf16(pr, one2, w.l[qb], false);
+      }
+      pf[half][qb] = pk;
+    }
+}
+
+// O^T += V^T P^T of a step, V images read four ahead of their products
+template <int NKB>
+__device__ __forceinline__ void tile_pv(WaveState<false>& w, const bf16x8 (&pf)[NKB / 2][2], const char* vbuf, int lane) {
+  constexpr int kImages = 4 * NKB;
+  bf16x8 vg[kImages];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) vg[i] = *(const bf16x8*)(vbuf + (i * 64 + lane) * 16);
+#pragma unroll
+  for (int i = 0; i < kImages; ++i) {
+#pragma unroll
+    for (int q = 0, qb = i & 1; q < 2; ++q, qb ^= 1) w.o[i & 7][qb] = PKH3_MFMA16(vg[i], pf[i >> 3][qb], w.o[i & 7][qb]);
+    if (i + 4 < kImages) vg[i + 4] = *(const bf16x8*)(vbuf + ((i + 4) * 64 + lane) * 16);
+  }
+}
+
+// A wave's share of a step's e4m3 values to bf16 images.  1 KiB of them, 16 values a lane, are two images.  A key's values have one scale: of K that is
+// one per lane, of V one per value of the eight, applied as the value is converted (the conversion takes a power of two along).
+template <int WAVES>
+__device__ __forceinline__ void expand_step(const char* raw, char* images, int half_of_page, int wave, int lane) {
+  using F = TileForm<WAVES>;
+  constexpr int kPieces = F::kRaw / 1024, kOfK = kPieces / 2;
+  const int g = lane >> 4, c = lane & 15;
+  const char* scales = raw + F::kRaw + (F::kStep == 32 ? 32 * half_of_page : 0);
+#pragma unroll
+  for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
+    const int piece = n * WAVES + wave;
+    if ((n + 1) * WAVES > kPieces && piece >= kPieces) break;
+    const i32x4 v = *(const i32x4*)(raw + (piece * 64 + lane) * 16);
+    if (piece < kOfK) {                                                   // key block kb, images ks = 2*c2, 2*c2 + 1
+      const int kb = piece >> 1, c2 = piece & 1;
+      const float scale = exponent_scale((unsigned char)scales[16 * kb + c]);
+      char* to = images + ((((kb >> 1) * 4 + 2 * c2) * 2 + (kb & 1)) * 64 + lane) * 16;
+      *(bf16x8*)to = expand_fp8(v[0], v[1], scale);
+      *(bf16x8*)(to + 2048) = expand_fp8(v[2], v[3], scale);
+    } else {                                                              // (half, dbp), images db = 2*dbp, 2*dbp + 1
+      const int at = piece - kOfK, half = at >> 2, dbp = at & 3;
+      unsigned e[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) e[kb] = *(const unsigned*)(scales + 64 + 32 * half + 16 * kb + 4 * g);
+      char* to = images + F::kBytes / 2 + ((half * 8 + 2 * dbp) * 64 + lane) * 16;
+#pragma unroll
+      for (int par = 0; par < 2; ++par) {
+        bf16x8 out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned src = v[2 * par + (j >> 2)];
+          const float scale = exponent_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
+          const bf16x2 both = (j & 2) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, false);
+          out[j] = both[j & 1];
+        }
+        *(bf16x8*)(to + par * 1024) = out;
       }
     }
+  }
+}
+
+// Values of keys that do not exist are zero (see clear_missing), in the V images of a step in LDS
+template <int WAVES>
+__device__ __forceinline__ void clear_missing_images(char* v, int there, int wave) {
+  constexpr int kPieces = TileForm<WAVES>::kBytes / 2 / 16;
+#pragma unroll 1
+  for (int n = wave; n < kPieces / 64; n += WAVES) {                      // images: of a half 8
+    const int lane = lane_here(), i = n * 64 + lane, half = n >> 3, g = lane >> 4;
+    i32x4 piece[1] = {*(const i32x4*)(v + i * 16)};
+    clear_missing<false>(piece, there - 32 * half, g);
+    *(i32x4*)(v + i * 16) = piece[0];
+  }
+}
+
+template <bool FP8, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_kernel(PagedParams p) {
+  using F = TileForm<WAVES>;
+  constexpr int RB = 32 * WAVES, kStep = F::kStep, NKB = kStep / 16, kPerTile = kTileKeys / kStep;
+  constexpr int kRecord = FP8 ? kPageRecord8 : kPageRecord16;
+  constexpr int kCopy = FP8 ? F::kRaw : F::kBytes;                        // bytes of a step as they come, half of them K
+  constexpr int kSlotBytes = FP8 ? F::kRawSlot : F::kBytes;
+  __shared__ __attribute__((aligned(1024))) char lds[F::template lds_bytes<FP8>()];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  int64_t* cum = (int64_t*)lds;
+  sum_tiles(p, cum, RB);
+  const Shares sh = shares_of(cum[p.B], gridDim.x);
+  const int rank = rank_of(blockIdx.x, sh);
+  if (rank < 0 || sh.total == 0) return;
+  const int64_t begin = sh.begin(rank);
+  int64_t left = sh.begin(rank + 1) - begin;
+  Place at = find_place(p, cum, RB, begin);
+  Sequence s = uniform_sequence(p, at.b);
+  int blocks = blocks_of(p, s, RB);
+  char* copies = lds + (FP8 ? 2 * F::kBytes : 0);                         // the ring that pages are copied to
+
+#pragma unroll 1
+  while (left > 0) {
+    // what is made of the lane's number is made where it is used: kept from unit to unit, or from the queries to the output, it does not fit the registers
+    const int lane = lane_here();
+    const unsigned lane_off = lane * 16;
+    const int nt = block_tiles(p, s, RB, at.j), take = (int)min((int64_t)(nt - at.t), left);
+    const int first = at.t * kPerTile, end = (at.t + take) * kPerTile;    // steps
+    __syncthreads();                                                      // the sums, or the output of the unit before, are read
+    const char* head = p.pages + (int64_t)at.h * kRecord;
+    auto page = [&](int step) { return uniform_page(p, at.b, min(step, end - 1) / kPerTile); };
+    auto copy = [&](int id, int step, int slot) {
+      const char* r = head + (int64_t)max(id, 0) * p.page_stride + (kPerTile == 2 ? (step & 1) * (kCopy / 2) : 0);
+      char* d = copies + slot * kSlotBytes;
+      constexpr int kPieces = kCopy / 1024;
+#pragma unroll
+      for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
+        const int piece = n * WAVES + wave;
+        // a step's K, then its V: of half a page the two do not lie side by side
+        const char* g = r + piece * 1024 + (kPerTile == 2 && piece >= kPieces / 2 ? kCopy / 2 : 0);
+        if ((n + 1) * WAVES <= kPieces || piece < kPieces) lds_dma16(g, lane_off, d + piece * 1024);
+      }
+      if constexpr (FP8) {
+        if (wave == WAVES - 1 && lane < kPageScales / 16)
+          lds_dma16(head + (int64_t)max(id, 0) * p.page_stride + kRecord - kPageScales, lane_off, d + F::kRaw);
+      }
+    };
+    int id[3];                                                            // pages of this step, the next and the one after it
+#pragma unroll
+    for (int i = 0; i < 3; ++i) id[i] = page(first + i);
+    copy(id[0], first, 0);
+    copy(id[1], min(first + 1, end - 1), 1);
+
+    WaveState<false> w;
+    const int r0 = at.j * RB + 32 * wave;
+    char* turn = lds + (FP8 ? F::kBytes : 2 * F::kBytes) + wave * 4096;
+    if constexpr (FP8) {
+      // the copies lie behind the images here: the queries take the images' place
+      static_assert(2 * F::kBytes >= WAVES * 4096, "the images' place");
+      turn = lds + wave * 4096;
+    }
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) query_rows(p, s, at.h, r0 + 16 * qb, turn, lane_here(), w.qf[qb]);
+    const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) w.o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) w.m[qb] = kNoMax, w.l[qb] = 0.f;
+
+    int slot = 0, slot_prev = 2;
+    if constexpr (FP8) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      expand_step<WAVES>(copies, lds, first & 1, wave, lane);
+    }
+    // One step.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
+    auto step = [&](int i, auto masked) {
+      constexpr bool MASKED = decltype(masked)::value;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      char* images = lds + slot * F::kBytes;
+      int there = 0;
+      if constexpr (MASKED) {
+        there = id[0] < 0 ? 0 : s.keys - kStep * i;
+        if (there < kStep) {
+          clear_missing_images<WAVES>(images + F::kBytes / 2, there, wave);
+          __syncthreads();
+        }
+      }
+      if constexpr (NKB == 4) qk_tile<false, true, MASKED ? 2 : 4>(w, images, images, lane);
+      else qk_half<false, true>(w, images, images, lane);
+      if constexpr (!FP8) {
+        if (i + 2 < end) copy(id[2], i + 2, slot_prev);
+        slot_prev = slot;
+        slot = slot == 2 ? 0 : slot + 1;
+      } else {
+        if (i + 2 < end) copy(id[2], i + 2, slot);
+        if (i + 1 < end) expand_step<WAVES>(copies + (slot ^ 1) * kSlotBytes, lds + (slot ^ 1) * F::kBytes, (i + 1) & 1, wave, lane_here());
+        slot ^= 1;
+      }
+      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3);
+      int lim[2] = {};                                                    // (made here: kept from step to step, it does not fit the registers)
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kStep * i);
+      }
+      bf16x8 pf[NKB / 2][2];
+      tile_softmax<NKB, MASKED>(w, pf, p.c, lim, lane);
+      tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane);
+    };
+    // Whether a step is masked differs from wave to wave, how many barriers it has does not: a step with keys that do not exist, or a page that does not,
+    // is masked for all.
+    const int whole = min(all_see / kStep, end);                         // steps in front of this one are seen whole by all rows
+    int i = first;
+#pragma unroll 1
+    while (i < end) {
+#pragma unroll 1
+      for (; i < whole && id[0] >= 0; ++i) step(i, std::false_type{});
+#pragma unroll 1
+      for (; i < end && (i >= whole || id[0] < 0); ++i) step(i, std::true_type{});
+    }
+    PKH3_MFMA_DRAIN(w);
+
+    __syncthreads();                                                      // every wave is done reading: the LDS becomes staging space
+    float l[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) l[qb] = wave_sum_groups(w.l[qb]);
+    const int last = s.n * p.G - 1, out_lane = lane_here(), c16 = out_lane & 15, g4 = out_lane >> 4;
+    if (at.t == 0 && take == nt) {
+      char* stage = lds + wave * F::kStage;
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const float inv = inverse_sum(l[qb]);
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          bf16x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = (__bf16)(w.o[db][qb][e] * inv);
+          *(bf16x4*)(stage + (16 * qb + c16) * 256 + (((2 * db + (g4 >> 1)) ^ c16) * 16) + 8 * (g4 & 1)) = v;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const int row = 4 * n + g4;
+        const bf16x8 v = *(const bf16x8*)(stage + row * 256 + ((c16 ^ (row & 15)) * 16));
+        int token;
+        const int64_t to = row_offset(p, s, at.h, min(r0 + row, last), p.o_ss, p.o_sh, token);
+        if (r0 + row <= last) *(bf16x8*)(p.o + to + c16 * 16) = v;
+      }
+    } else {
+      float* part = p.partials + part_slot(rank, at.t == 0) * part_floats(RB);
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        const int row = 32 * wave + 16 * qb + c16;
+        if (at.j * RB + row > last) continue;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
+        if (g4 == 0) part[RB * kD + row] = w.m[qb], part[RB * (kD + 1) + row] = l[qb];
+      }
+    }
+    left -= take;
+    at.t = 0;
+    if (!next_unit(p, at, s, blocks, RB, left)) return;
   }
 }
 
@@ -470,7 +809,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int gri
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
   }
-  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  const float inv = inverse_sum(l);
   bf16x4 out;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (__bf16)(sum[e] * inv);
@@ -480,20 +819,30 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int gri
 
 // ---- host ----
 
-static int split_blocks(int rows, int B, int G) {   // 16-row blocks of a unit
-  return (int64_t)rows * G > 16 * (int64_t)std::min(rows, B) ? 2 : 1;
+// The form of a call, from what the host knows of it: the query rows of a (sequence, kv head) on the average.
+enum PagedForm { kSplit16, kSplit32, kTile128, kTile384 };
+static PagedForm form_of(int rows, int B, int G) {
+  const int64_t per = (int64_t)rows * G / std::max(1, std::min(rows, B));
+  return per <= 16 ? kSplit16 : per <= 48 ? kSplit32 : per <= 256 ? kTile128 : kTile384;
+}
+static int rows_of(PagedForm f) { return f == kSplit16 ? 16 : f == kSplit32 ? 32 : f == kTile128 ? 128 : 384; }
+static int most_workgroups(PagedForm f) { return f == kTile384 ? kMaxShares / 3 : f == kTile128 ? kMaxShares : kMaxShares / 3 * 2; }
+static int workgroups_of(PagedForm f, int cus) {
+  const int per_cu = f == kTile384 ? 1 : f == kTile128 ? 3 : 2;
+  return std::min(most_workgroups(f), std::max(8, per_cu * cus / 8 * 8));
 }
 
 size_t paged_attn_scratch(int rows, int B, int H, int G, int table_pages) {
-  return (size_t)2 * kMaxShares * part_floats(16 * split_blocks(rows, B, G));
+  const PagedForm f = form_of(rows, B, G);
+  return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f));
 }
 
-template <bool FP8, int QB>
-static hipError_t launch_split(const PagedParams& p, int grid, hipStream_t st) {
-  hipLaunchKernelGGL((paged_split_kernel<FP8, QB>), dim3(grid), dim3(64 * kSplitWaves), 0, st, p);
-  hipError_t e = hipGetLastError();
+template <int RB, class Kernel>
+static hipError_t launch_form(Kernel kernel, int threads, int grid, const PagedParams& p, hipStream_t st) {
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, p);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<16 * QB>), dim3(grid, 2 * QB), dim3(256), 0, st, p, grid);
+  hipLaunchKernelGGL(paged_merge_kernel<RB>, dim3(grid, RB / 8), dim3(256), 0, st, p, grid);
   return hipGetLastError();
 }
 
@@ -501,9 +850,14 @@ hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
   if (e != hipSuccess) return e;
-  const int grid = std::min(kMaxShares, std::max(8, 2 * cus / 8 * 8));
-  if (split_blocks(p.rows, p.B, p.G) == 1) return fp8 ? launch_split<true, 1>(p, grid, st) : launch_split<false, 1>(p, grid, st);
-  return fp8 ? launch_split<true, 2>(p, grid, st) : launch_split<false, 2>(p, grid, st);
+  const PagedForm f = form_of(p.rows, p.B, p.G);
+  const int grid = workgroups_of(f, cus);
+  switch (f) {
+    case kSplit16: return launch_form<16>(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 256, grid, p, st);
+    case kSplit32: return launch_form<32>(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 256, grid, p, st);
+    case kTile128: return launch_form<128>(fp8 ? paged_tile_kernel<true, 4> : paged_tile_kernel<false, 4>, 256, grid, p, st);
+    default: return launch_form<384>(fp8 ? paged_tile_kernel<true, 12> : paged_tile_kernel<false, 12>, 768, grid, p, st);
+  }
 }
 
 }  // namespace pkh3

@@ -53,7 +53,7 @@ constexpr int block_tiles(const Sequence& s, int G, int causal, int rb, int j) {
 }
 
 // The tiles of all units end to end, in equal runs for `n` workgroups.
-constexpr int kMaxShares = 512;       // workgroups of a launch at most
+constexpr int kMaxShares = 768;       // workgroups of a launch at most
 constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
 struct Shares {
   int64_t total;

@@ -220,7 +220,7 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     _run(tmp_path, """
   for (int go = 0; go < 4000; ++go) {
     const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 4 == 0 ? 384 : go % 4 == 1 ? 32 : 16;
-    const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 512;
+    const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 768;
     std::vector<Sequence> seq;
     struct Unit { int64_t begin, end; };
     std::vector<Unit> units;
