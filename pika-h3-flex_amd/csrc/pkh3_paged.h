@@ -39,7 +39,8 @@ struct PagedParams {
   int G;                             // attn: query heads of one of the cache's
   float c;                           // attn: softmax scale * log2(e)
   int causal;
-  float* partials;                   // attn: see pkh3_paged_attn.hip
+  i32x4* cuts;                       // attn: where runs begin inside a unit, and ...
+  float* partials;                   // ... the parts of units (see pkh3_paged_attn.hip)
 };
 
 __device__ __forceinline__ Sequence sequence(const PagedParams& p, int b) {

@@ -149,7 +149,8 @@ int pkh3_paged_attn(const pkh3_paged_args* a, void* stream) {
   PagedParams p = params(a);
   p.G = a->heads / a->kv_heads;
   p.c = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)kD)) * kLog2e;
-  p.partials = (float*)a->workspace;
+  p.cuts = (i32x4*)a->workspace;
+  p.partials = (float*)a->workspace + 4 * kMaxShares;
   return done(launch_paged_attn(p, a->flags & PKH3_PAGED_FP8, (hipStream_t)stream), "paged attention");
 }
 

@@ -38,10 +38,15 @@ __device__ __forceinline__ int lane_here() {
 __device__ __forceinline__ int blocks_of(const PagedParams& p, const Sequence& s, int rb) { return blocks_of(s, p.G, rb); }
 __device__ __forceinline__ int block_tiles(const PagedParams& p, const Sequence& s, int rb, int j) { return block_tiles(s, p.G, p.causal, rb, j); }
 __device__ __forceinline__ int row_keys(const PagedParams& p, const Sequence& s, int r) { return row_keys(s, p.G, p.causal, r); }
+__device__ __forceinline__ int block_cost(const PagedParams& p, const Sequence& s, int rb, int j) { return block_cost(s, p.G, rb, j); }
+__device__ __forceinline__ int64_t unit_cost(const PagedParams& p, const Sequence& s, int rb, int j) {
+  return (int64_t)block_tiles(p, s, rb, j) * block_cost(p, s, rb, j);
+}
 
-// Where a run begins: sequence, head, block and tile.
+// Where a run begins: sequence, head, block and tile, and how far in the space of all tiles the unit and the tile begin.
 struct Place {
   int b, h, j, t;
+  int64_t unit, pos;
 };
 
 // The sums of the tiles of all sequences in `cum`, by the whole workgroup.  Blocks of a causal sequence differ in length: where
@@ -57,16 +62,16 @@ __device__ __forceinline__ void sum_tiles(const PagedParams& p, int64_t* cum, in
       const Sequence s = sequence(p, b);
       const int blocks = blocks_of(p, s, rb);
       many = p.causal && blocks > kAlone;
-      if (!p.causal) mine = blocks ? (int64_t)blocks * block_tiles(p, s, rb, 0) : 0;
+      if (!p.causal) mine = blocks ? (blocks - 1) * unit_cost(p, s, rb, 0) + unit_cost(p, s, rb, blocks - 1) : 0;
       else if (!many)
-        for (int j = 0; j < blocks; ++j) mine += block_tiles(p, s, rb, j);
+        for (int j = 0; j < blocks; ++j) mine += unit_cost(p, s, rb, j);
     }
     for (unsigned long long left = __ballot(many); left; left &= left - 1) {
       const int l = __ffsll((unsigned long long)left) - 1;
       const Sequence s = uniform_sequence(p, __builtin_amdgcn_readfirstlane(at + l));
       const int blocks = blocks_of(p, s, rb);
       int64_t sum = 0;
-      for (int j = lane; j < blocks; j += 64) sum += block_tiles(p, s, rb, j);
+      for (int j = lane; j < blocks; j += 64) sum += unit_cost(p, s, rb, j);
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
       if (lane == l) mine = sum;
@@ -76,41 +81,68 @@ __device__ __forceinline__ void sum_tiles(const PagedParams& p, int64_t* cum, in
   prefix_sums(cum, p.B);
 }
 
-__device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t* cum, int rb, int64_t pos) {
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x), hi = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The boundary at `pos`, brought to a tile (see boundary_tile); 0 <= pos < cum[B]
+__device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t* cum, int rb, const Shares& sh, int64_t pos) {
   Place at;
   at.b = find_sequence(cum, p.B, pos);
   const Sequence s = uniform_sequence(p, at.b);
-  const int64_t per_head = (cum[at.b + 1] - cum[at.b]) / p.H;
-  const int64_t in = pos - cum[at.b];
-  at.h = __builtin_amdgcn_readfirstlane((int)(in / per_head));
-  int64_t rest = in - at.h * per_head;
+  const int blocks = blocks_of(p, s, rb);
+  const int64_t per_head = divided(cum[at.b + 1] - cum[at.b], p.H);
+  int64_t rest = pos - cum[at.b];
+  at.h = __builtin_amdgcn_readfirstlane((int)divided(rest, per_head));
+  rest -= at.h * per_head;
   if (!p.causal) {
-    const int nt = block_tiles(p, s, rb, 0);
-    at.j = __builtin_amdgcn_readfirstlane((int)(rest / nt));
-    at.t = __builtin_amdgcn_readfirstlane((int)(rest - (int64_t)at.j * nt));
-    return at;
-  }
-  const int lane = threadIdx.x & 63, blocks = blocks_of(p, s, rb);
-  for (int first = 0;; first += 64) {
-    int64_t x = first + lane < blocks ? block_tiles(p, s, rb, first + lane) : 0;
-    const int64_t own = x;
+    at.j = __builtin_amdgcn_readfirstlane(min((int)divided(rest, unit_cost(p, s, rb, 0)), blocks - 1));
+    rest -= at.j * unit_cost(p, s, rb, 0);
+  } else {
+    const int lane = threadIdx.x & 63;
+    for (int first = 0;; first += 64) {
+      int64_t x = first + lane < blocks ? unit_cost(p, s, rb, first + lane) : 0;
+      const int64_t own = x;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(x, d);
-      if (lane >= d) x += y;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+      }
+      const unsigned long long past = __ballot(x > rest);
+      if (past || first + 64 >= blocks) {
+        const int l = past ? __ffsll((unsigned long long)past) - 1 : blocks - 1 - first;
+        at.j = __builtin_amdgcn_readfirstlane(first + l);
+        rest -= __shfl(x - own, l);
+        break;
+      }
+      rest -= __shfl(x, 63);
     }
-    const unsigned long long past = __ballot(x > rest);
-    if (past || first + 64 >= blocks) {
-      const int l = past ? __ffsll((unsigned long long)past) - 1 : 63;
-      at.j = __builtin_amdgcn_readfirstlane(first + l);
-      at.t = __builtin_amdgcn_readfirstlane((int)(rest - __shfl(x - own, l)));
-      return at;
-    }
-    rest -= __shfl(x, 63);
   }
+  const int nt = block_tiles(p, s, rb, at.j), cost = block_cost(p, s, rb, at.j);
+  at.unit = uniform64(pos - rest);
+  at.t = __builtin_amdgcn_readfirstlane(boundary_tile(sh, rest, nt, cost));
+  at.pos = at.unit + (int64_t)at.t * cost;
+  return at;
 }
 
-// On to the next unit of a run with `left` tiles to go.  False where there is none.
+// The run of this workgroup: which one, what it costs, the unit and tile it begins at.  False: none.  Leaves what the second launch has to know of the
+// run's beginning.
+__device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int rb, int& rank, int64_t& left, Place& at) {
+  const Shares sh = shares_of(cum[p.B], gridDim.x, rb);
+  rank = rank_of(blockIdx.x, sh);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.cuts[0] = i32x4{sh.n, 0, 0, 0};
+  if (rank < 0 || sh.total == 0) return false;
+  at = find_place(p, cum, rb, sh, sh.begin(rank));
+  left = (rank + 1 < sh.n ? find_place(p, cum, rb, sh, sh.begin(rank + 1)).pos : uniform64(sh.total)) - at.pos;
+  const Sequence s = uniform_sequence(p, at.b);
+  const int nt = block_tiles(p, s, rb, at.j);
+  if (rank > 0 && threadIdx.x == 0)
+    p.cuts[rank] = i32x4{at.b, at.h, at.j, parts_at(sh, rank, at.unit, at.t, nt, block_cost(p, s, rb, at.j))};
+  return left > 0;
+}
+
+// On to the next unit of a run with `left` to go.  False where there is none.
 __device__ __forceinline__ bool next_unit(const PagedParams& p, Place& at, Sequence& s, int& blocks, int rb, int64_t left) {
   if (left <= 0) return false;
   if (++at.j < blocks) return true;
@@ -129,6 +161,7 @@ __device__ __forceinline__ bool next_unit(const PagedParams& p, Place& at, Seque
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
 // A part of a unit in the scratch: RB rows of 128, then their maxima, then their sums
+constexpr int kCutFloats = 4 * kMaxShares;   // of the records in front of the parts
 __host__ __device__ constexpr int part_floats(int rb) { return rb * (kD + 2); }
 
 // ---- the split form: few query rows, the waves of a workgroup share the keys out ----
@@ -208,23 +241,26 @@ __device__ __forceinline__ int64_t row_offset(const PagedParams& p, const Sequen
   return (int64_t)(s.first + token) * ss + (int64_t)(h * p.G + r - token * p.G) * sh;
 }
 
-// Sixteen query rows from r on (those past the last are the last one again) through norm and rotation, in the lane order of the B images.
-__device__ __forceinline__ void query_rows(const PagedParams& p, const Sequence& s, int h, int r0, char* turn, int lane, bf16x8 (&out)[4]) {
+// Sixteen query rows from r0 on (those past the last are the last one again), as they lie in memory ..
+__device__ __forceinline__ void ask_queries(const PagedParams& p, const Sequence& s, int h, int r0, Rows16& q, int lane) {
   const int last = s.n * p.G - 1;
-  Rows16 q, cos, sin;
-  int token[4];
+  int token;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t at = row_offset(p, s, h, min(r0 + 4 * i + (lane >> 4), last), p.q_ss, p.q_sh, token[i]);
-    q.v[i] = *(const i32x4*)(p.q + at + (lane & 15) * 16);
-  }
+  for (int i = 0; i < 4; ++i)
+    q.v[i] = *(const i32x4*)(p.q + row_offset(p, s, h, min(r0 + 4 * i + (lane >> 4), last), p.q_ss, p.q_sh, token) + (lane & 15) * 16);
+}
+// .. and through norm and rotation, in the lane order of the B images, by way of 4 KiB of LDS of the wave's own
+__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, char* turn, int lane, bf16x8 (&out)[4]) {
+  Rows16 cos, sin;
   NormLanes norm;
   load_norm_lanes(norm, p.norm_w, lane);
   RopeQuarter rope;
   if (p.rope_mode != 0) {
+    const int last = s.n * p.G - 1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t at = (int64_t)(s.first + token[i]) * (kD / 2 * (int)sizeof(float)) + (lane & 15) * 16;
+      const int token = (int)((unsigned)min(r0 + 4 * i + (lane >> 4), last) / (unsigned)p.G);
+      const int64_t at = (int64_t)(s.first + token) * (kD / 2 * (int)sizeof(float)) + (lane & 15) * 16;
       cos.v[i] = *(const i32x4*)((const char*)p.cos_t + at);
       sin.v[i] = *(const i32x4*)((const char*)p.sin_t + at);
     }
@@ -261,14 +297,16 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 
   int64_t* cum = (int64_t*)part;
   sum_tiles(p, cum, RB);
-  const Shares sh = shares_of(cum[p.B], gridDim.x);
-  const int rank = rank_of(blockIdx.x, sh);
-  if (rank < 0 || sh.total == 0) return;
-  const int64_t begin = sh.begin(rank);
-  int64_t left = sh.begin(rank + 1) - begin;
-  Place at = find_place(p, cum, RB, begin);
+  int rank;
+  int64_t left;
+  Place at;
+  if (!find_run(p, cum, RB, rank, left, at)) return;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
+  if (at.t == block_tiles(p, s, RB, at.j)) {
+    at.t = 0;
+    if (!next_unit(p, at, s, blocks, RB, left)) return;
+  }
 
 #pragma unroll 1
   while (left > 0) {
@@ -277,7 +315,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
     SplitState<FP8, QB> w;
     if (wave < QB) {
       bf16x8 img[4];
-      query_rows(p, s, at.h, at.j * RB + 16 * wave, part + wave * 4096, lane, img);
+      Rows16 q;
+      ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
+      queries_ready(p, s, at.j * RB + 16 * wave, q, part + wave * 4096, lane, img);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
     }
@@ -471,13 +511,11 @@ struct TileForm {
   // bf16: a ring of three steps.  e4m3: two steps of images, two as they come
   template <bool FP8>
   static constexpr int ring_bytes() { return FP8 ? 2 * kBytes + 2 * kRawSlot : 3 * kBytes; }
-  static constexpr int kStage = 32 * kD * 2;                             // a wave's output rows
   template <bool FP8>
   static constexpr int lds_bytes() {
-    // before the loop the queries are turned around where the third step goes (e4m3: the second step's images) and behind it
-    const int before = (FP8 ? 1 : 2) * kBytes + WAVES * 4096, after = WAVES * kStage, sums = (kMaxSequences + 1) * (int)sizeof(int64_t);
-    int most = ring_bytes<FP8>() > before ? ring_bytes<FP8>() : before;
-    most = most > after ? most : after;
+    // queries and outputs are turned around where the third step goes (e4m3: the images) and behind it
+    const int turned = (FP8 ? 0 : 2) * kBytes + WAVES * 4096, sums = (kMaxSequences + 1) * (int)sizeof(int64_t);
+    const int most = ring_bytes<FP8>() > turned ? ring_bytes<FP8>() : turned;
     return most > sums ? most : sums;
   }
 };
@@ -619,58 +657,69 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
 
   int64_t* cum = (int64_t*)lds;
   sum_tiles(p, cum, RB);
-  const Shares sh = shares_of(cum[p.B], gridDim.x);
-  const int rank = rank_of(blockIdx.x, sh);
-  if (rank < 0 || sh.total == 0) return;
-  const int64_t begin = sh.begin(rank);
-  int64_t left = sh.begin(rank + 1) - begin;
-  Place at = find_place(p, cum, RB, begin);
+  int rank;
+  int64_t left;
+  Place at;
+  if (!find_run(p, cum, RB, rank, left, at)) return;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
+  if (at.t == block_tiles(p, s, RB, at.j)) {
+    at.t = 0;
+    if (!next_unit(p, at, s, blocks, RB, left)) return;
+  }
   char* copies = lds + (FP8 ? 2 * F::kBytes : 0);                         // the ring that pages are copied to
+  // 4 KiB of the wave's own, for queries on their way in and outputs on their way out, that no copy ahead of the loop goes to
+  char* turn = lds + (FP8 ? 0 : 2 * F::kBytes) + wave * 4096;
+  static_assert(2 * F::kBytes >= WAVES * 4096, "the images' place");
 
-#pragma unroll 1
-  while (left > 0) {
-    // what is made of the lane's number is made where it is used: kept from unit to unit, or from the queries to the output, it does not fit the registers
-    const int lane = lane_here();
-    const unsigned lane_off = lane * 16;
-    const int nt = block_tiles(p, s, RB, at.j), take = (int)min((int64_t)(nt - at.t), left);
-    const int first = at.t * kPerTile, end = (at.t + take) * kPerTile;    // steps
-    __syncthreads();                                                      // the sums, or the output of the unit before, are read
-    const char* head = p.pages + (int64_t)at.h * kRecord;
-    auto page = [&](int step) { return uniform_page(p, at.b, min(step, end - 1) / kPerTile); };
-    auto copy = [&](int id, int step, int slot) {
-      const char* r = head + (int64_t)max(id, 0) * p.page_stride + (kPerTile == 2 ? (step & 1) * (kCopy / 2) : 0);
-      char* d = copies + slot * kSlotBytes;
-      constexpr int kPieces = kCopy / 1024;
+  // The copies of a unit's steps.  (What they need of the unit is uniform; `end`: the step behind the last of this run.)
+  auto page = [&](int step, int end) { return uniform_page(p, at.b, min(step, end - 1) / kPerTile); };
+  auto copy = [&](int id, int step, int slot) {
+    const char* record = p.pages + (int64_t)max(id, 0) * p.page_stride + (int64_t)at.h * kRecord;
+    const char* r = record + (kPerTile == 2 ? (step & 1) * (kCopy / 2) : 0);
+    const unsigned lane_off = lane_here() * 16;
+    char* d = copies + slot * kSlotBytes;
+    constexpr int kPieces = kCopy / 1024;
 #pragma unroll
-      for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
-        const int piece = n * WAVES + wave;
-        // a step's K, then its V: of half a page the two do not lie side by side
-        const char* g = r + piece * 1024 + (kPerTile == 2 && piece >= kPieces / 2 ? kCopy / 2 : 0);
-        if ((n + 1) * WAVES <= kPieces || piece < kPieces) lds_dma16(g, lane_off, d + piece * 1024);
-      }
-      if constexpr (FP8) {
-        if (wave == WAVES - 1 && lane < kPageScales / 16)
-          lds_dma16(head + (int64_t)max(id, 0) * p.page_stride + kRecord - kPageScales, lane_off, d + F::kRaw);
-      }
-    };
-    int id[3];                                                            // pages of this step, the next and the one after it
+    for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
+      const int piece = n * WAVES + wave;
+      // a step's K, then its V: of half a page the two do not lie side by side
+      const char* g = r + piece * 1024 + (kPerTile == 2 && piece >= kPieces / 2 ? kCopy / 2 : 0);
+      if ((n + 1) * WAVES <= kPieces || piece < kPieces) lds_dma16(g, lane_off, d + piece * 1024);
+    }
+    if constexpr (FP8) {
+      if (wave == WAVES - 1 && lane_off < kPageScales) lds_dma16(record + kRecord - kPageScales, lane_off, d + F::kRaw);
+    }
+  };
+  int id[3];                                                              // pages of this step, the next and the one after it
+  int nt, take, first, end;
+  Rows16 ahead[2];
+  auto begin_unit = [&]() {                                               // asks for everything the unit's loop begins with
+    nt = block_tiles(p, s, RB, at.j);
+    const int cost = block_cost(p, s, RB, at.j);
+    take = (int)min((int64_t)(nt - at.t), divided(left, cost));
+    left -= (int64_t)take * cost;
+    first = at.t * kPerTile, end = (at.t + take) * kPerTile;              // steps
 #pragma unroll
-    for (int i = 0; i < 3; ++i) id[i] = page(first + i);
+    for (int i = 0; i < 3; ++i) id[i] = page(first + i, end);
     copy(id[0], first, 0);
     copy(id[1], min(first + 1, end - 1), 1);
-
+  };
+  auto ask = [&](int qb) { ask_queries(p, s, at.h, at.j * RB + 32 * wave + 16 * qb, ahead[qb], lane_here()); };
+  __syncthreads();                                                        // the sums are read
+  begin_unit();
+  ask(0), ask(1);
+#pragma unroll 1
+  for (;;) {
+    // what is made of the lane's number is made where it is used: kept from unit to unit, or from the queries to the output, it does not fit the registers
+    const int r0 = at.j * RB + 32 * wave, last = s.n * p.G - 1;
+    const bool idle = r0 > last;                                          // a wave without rows: copies and barriers alone
     WaveState<false> w;
-    const int r0 = at.j * RB + 32 * wave;
-    char* turn = lds + (FP8 ? F::kBytes : 2 * F::kBytes) + wave * 4096;
-    if constexpr (FP8) {
-      // the copies lie behind the images here: the queries take the images' place
-      static_assert(2 * F::kBytes >= WAVES * 4096, "the images' place");
-      turn = lds + wave * 4096;
-    }
+    if (!idle) {
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) query_rows(p, s, at.h, r0 + 16 * qb, turn, lane_here(), w.qf[qb]);
+      for (int qb = 0; qb < 2; ++qb) queries_ready(p, s, r0 + 16 * qb, ahead[qb], turn, lane_here(), w.qf[qb]);
+    }
+    const int lane = lane_here();
     const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
 #pragma unroll
     for (int db = 0; db < 8; ++db)
@@ -686,8 +735,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
       expand_step<WAVES>(copies, lds, first & 1, wave, lane);
     }
     // One step.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
-    auto step = [&](int i, auto masked) {
-      constexpr bool MASKED = decltype(masked)::value;
+    auto step = [&](int i, auto masked, auto works) {
+      constexpr bool MASKED = decltype(masked)::value, WORKS = decltype(works)::value;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       char* images = lds + slot * F::kBytes;
@@ -699,8 +748,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
           __syncthreads();
         }
       }
-      if constexpr (NKB == 4) qk_tile<false, true, MASKED ? 2 : 4>(w, images, images, lane);
-      else qk_half<false, true>(w, images, images, lane);
+      if constexpr (WORKS) {
+        if constexpr (NKB == 4) qk_tile<false, true, MASKED ? 2 : 4>(w, images, images, lane);
+        else qk_half<false, true>(w, images, images, lane);
+      }
       if constexpr (!FP8) {
         if (i + 2 < end) copy(id[2], i + 2, slot_prev);
         slot_prev = slot;
@@ -710,111 +761,144 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
         if (i + 1 < end) expand_step<WAVES>(copies + (slot ^ 1) * kSlotBytes, lds + (slot ^ 1) * F::kBytes, (i + 1) & 1, wave, lane_here());
         slot ^= 1;
       }
-      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3);
-      int lim[2] = {};                                                    // (made here: kept from step to step, it does not fit the registers)
-      if constexpr (MASKED) {
+      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3, end);
+      if constexpr (WORKS) {
+        int lim[2] = {};                                                  // (made here: kept from step to step, it does not fit the registers)
+        if constexpr (MASKED) {
 #pragma unroll
-        for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kStep * i);
+          for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kStep * i);
+        }
+        bf16x8 pf[NKB / 2][2];
+        tile_softmax<NKB, MASKED>(w, pf, p.c, lim, lane);
+        tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane);
       }
-      bf16x8 pf[NKB / 2][2];
-      tile_softmax<NKB, MASKED>(w, pf, p.c, lim, lane);
-      tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane);
     };
     // Whether a step is masked differs from wave to wave, how many barriers it has does not: a step with keys that do not exist, or a page that does not,
     // is masked for all.
     const int whole = min(all_see / kStep, end);                         // steps in front of this one are seen whole by all rows
     int i = first;
+    if (idle) {
+#pragma unroll 1
+      for (; i < end; ++i) step(i, std::true_type{}, std::false_type{});
+    }
 #pragma unroll 1
     while (i < end) {
 #pragma unroll 1
-      for (; i < whole && id[0] >= 0; ++i) step(i, std::false_type{});
+      for (; i < whole && id[0] >= 0; ++i) step(i, std::false_type{}, std::true_type{});
 #pragma unroll 1
-      for (; i < end && (i >= whole || id[0] < 0); ++i) step(i, std::true_type{});
+      for (; i < end && (i >= whole || id[0] < 0); ++i) step(i, std::true_type{}, std::true_type{});
     }
     PKH3_MFMA_DRAIN(w);
 
-    __syncthreads();                                                      // every wave is done reading: the LDS becomes staging space
-    float l[2];
+    __syncthreads();                                                      // every wave is done reading: the ring is free
+    // the next unit's first steps and queries are on their way while this one's rows go out
+    const Sequence out_s = s;
+    const int out_h = at.h;
+    const bool finished = at.t == 0 && take == nt, begins = at.t == 0;
+    at.t = 0;
+    const bool more = next_unit(p, at, s, blocks, RB, left);
+    if (more) begin_unit();
+    float* part = p.partials + part_slot(rank, begins) * part_floats(RB);
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) l[qb] = wave_sum_groups(w.l[qb]);
-    const int last = s.n * p.G - 1, out_lane = lane_here(), c16 = out_lane & 15, g4 = out_lane >> 4;
-    if (at.t == 0 && take == nt) {
-      char* stage = lds + wave * F::kStage;
+    for (int qb = 0; qb < 2; ++qb) {
+      ask(qb);                                                            // (without a next unit: rows of this one, which nobody takes)
+      asm volatile("" ::: "memory");                                      // (one block after the other: both at once do not fit the registers)
+      if (!idle) {
+        const int out_lane = lane_here(), c16 = out_lane & 15, g4 = out_lane >> 4;
+        const float l = wave_sum_groups(w.l[qb]);
+        if (finished) {
+          const float inv = inverse_sum(l);
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        const float inv = inverse_sum(l[qb]);
+          for (int db = 0; db < 8; ++db) {
+            bf16x4 v;
 #pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          bf16x4 v;
+            for (int e = 0; e < 4; ++e) v[e] = (__bf16)(w.o[db][qb][e] * inv);
+            *(bf16x4*)(turn + c16 * 256 + (((2 * db + (g4 >> 1)) ^ c16) * 16) + 8 * (g4 & 1)) = v;
+          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (__bf16)(w.o[db][qb][e] * inv);
-          *(bf16x4*)(stage + (16 * qb + c16) * 256 + (((2 * db + (g4 >> 1)) ^ c16) * 16) + 8 * (g4 & 1)) = v;
+          for (int n = 0; n < 4; ++n) {
+            const int row = 4 * n + g4, r = r0 + 16 * qb + row;
+            const bf16x8 v = *(const bf16x8*)(turn + row * 256 + ((c16 ^ row) * 16));
+            int token;
+            const int64_t to = row_offset(p, out_s, out_h, min(r, last), p.o_ss, p.o_sh, token);
+            if (r <= last) *(bf16x8*)(p.o + to + c16 * 16) = v;
+          }
+        } else {
+          const int row = 32 * wave + 16 * qb + c16;
+          if (r0 + 16 * qb + c16 <= last) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
+            if (g4 == 0) part[RB * kD + row] = w.m[qb], part[RB * (kD + 1) + row] = l;
+          }
         }
       }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int row = 4 * n + g4;
-        const bf16x8 v = *(const bf16x8*)(stage + row * 256 + ((c16 ^ (row & 15)) * 16));
-        int token;
-        const int64_t to = row_offset(p, s, at.h, min(r0 + row, last), p.o_ss, p.o_sh, token);
-        if (r0 + row <= last) *(bf16x8*)(p.o + to + c16 * 16) = v;
-      }
-    } else {
-      float* part = p.partials + part_slot(rank, at.t == 0) * part_floats(RB);
-#pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        const int row = 32 * wave + 16 * qb + c16;
-        if (at.j * RB + row > last) continue;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
-        if (g4 == 0) part[RB * kD + row] = w.m[qb], part[RB * (kD + 1) + row] = l[qb];
-      }
     }
-    left -= take;
-    at.t = 0;
-    if (!next_unit(p, at, s, blocks, RB, left)) return;
+    if (!more) return;
   }
 }
 
 // ---- the parts of units that more than one workgroup worked on ----
 //
-// Boundary i between the runs of workgroups i - 1 and i, where it is the first inside its unit, does the unit: its parts are slot 1 of
-// workgroup i - 1 and slot 0 of i, i + 1, .., in that order.  blockIdx.y: 8 of its rows.
+// Workgroup i of the launch in front, if its run begins inside a unit and is the first that does, has left in cut[i] which unit that is and how many
+// runs share it: its parts are slot 1 of run i - 1 and slot 0 of i, i + 1, .., in that order.  Eight rows a workgroup (blockIdx.y); 32 threads
+// have a row, four columns each, and where there are fewer rows than that takes, its parts are dealt out to several such groups.  (Found by
+// every workgroup for itself, from the sums of the whole batch, the units were most of this launch: 41 to 52 us of 256 x 48 workgroups.)
 template <int RB>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p, int grid) {
-  __shared__ int64_t cum[kMaxSequences + 1];
-  sum_tiles(p, cum, RB);
-  const Shares sh = shares_of(cum[p.B], grid);
-  const int first = (int)blockIdx.x;                             // the workgroup in front of the boundary
-  if (first + 1 >= sh.n) return;
-  const int64_t pos = sh.begin(first + 1);
-  const Place at = find_place(p, cum, RB, pos);
-  const Sequence s = uniform_sequence(p, at.b);
-  const int parts = parts_behind(sh, first, pos - at.t, pos - at.t + block_tiles(p, s, RB, at.j));
-  if (parts == 0) return;
-  const int row = (int)blockIdx.y * 8 + (threadIdx.x >> 5), col = (threadIdx.x & 31) * 4;
-  const int r = at.j * RB + row;
-  if (r >= s.n * p.G) return;
-  auto slot = [&](int i) { return p.partials + part_slot(first + i, i == 0) * part_floats(RB); };
-  float top = kNoMax;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, slot(i)[RB * kD + row]);
-  float l = 0.f;
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
+  __shared__ f32x4 part_sum[256];
+  __shared__ float part_m[8], part_l[8];
+  const int run = (int)blockIdx.x + 1;
+  const i32x4 cut = p.cuts[run];
+  if (run >= p.cuts[0][0] || cut[3] == 0) return;
+  const Sequence s = uniform_sequence(p, cut[0]);
+  const int rows = min(RB, s.n * p.G - cut[2] * RB), row0 = (int)blockIdx.y * 8;
+  if (row0 >= rows) return;
+  const int here = min(8, rows - row0), groups = here == 1 ? 8 : here == 2 ? 4 : here <= 4 ? 2 : 1;   // groups of 32 threads a row
+  const int mine = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
+  const int row = row0 + mine / groups, sub = mine % groups;
+  const bool live = mine / groups < here;
+  auto slot = [&](int i) { return p.partials + part_slot(run - 1 + i, i == 0) * part_floats(RB); };
+  float top = kNoMax, l = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
 #pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float* t = slot(i);
-    const float a = __builtin_amdgcn_exp2f(t[RB * kD + row] - top);
-    l += a * t[RB * (kD + 1) + row];
-    const f32x4 o = *(const f32x4*)(t + row * kD + col);
+    for (int i = sub; i < cut[3]; i += groups) top = fmaxf(top, slot(i)[RB * kD + row]);
+#pragma unroll 4
+    for (int i = sub; i < cut[3]; i += groups) {
+      const float* t = slot(i);
+      const float a = __builtin_amdgcn_exp2f(t[RB * kD + row] - top);
+      l += a * t[RB * (kD + 1) + row];
+      const f32x4 o = *(const f32x4*)(t + row * kD + col);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
+      for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
+    }
   }
+  if (groups > 1) {                                                        // (the same for the whole workgroup)
+    part_sum[threadIdx.x] = sum;
+    if ((threadIdx.x & 31) == 0) part_m[mine] = top, part_l[mine] = l;
+    __syncthreads();
+    if (sub != 0) return;
+    const float own = top;
+    for (int g = 1; g < groups; ++g) top = fmaxf(top, part_m[mine + g]);
+    const float a0 = __builtin_amdgcn_exp2f(own - top);
+    l *= a0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] *= a0;
+    for (int g = 1; g < groups; ++g) {
+      const float a = __builtin_amdgcn_exp2f(part_m[mine + g] - top);
+      l += a * part_l[mine + g];
+      const f32x4 o = part_sum[threadIdx.x + 32 * g];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
+    }
+  }
+  if (!live) return;
   const float inv = inverse_sum(l);
   bf16x4 out;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (__bf16)(sum[e] * inv);
   int token;
-  *(bf16x4*)(p.o + row_offset(p, s, at.h, r, p.o_ss, p.o_sh, token) + col * 2) = out;
+  *(bf16x4*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row, p.o_ss, p.o_sh, token) + col * 2) = out;
 }
 
 // ---- host ----
@@ -834,7 +918,7 @@ static int workgroups_of(PagedForm f, int cus) {
 
 size_t paged_attn_scratch(int rows, int B, int H, int G, int table_pages) {
   const PagedForm f = form_of(rows, B, G);
-  return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f));
+  return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f)) + kCutFloats;
 }
 
 template <int RB, class Kernel>
@@ -842,7 +926,7 @@ static hipError_t launch_form(Kernel kernel, int threads, int grid, const PagedP
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(paged_merge_kernel<RB>, dim3(grid, RB / 8), dim3(256), 0, st, p, grid);
+  hipLaunchKernelGGL(paged_merge_kernel<RB>, dim3(grid - 1, RB / 8), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 

@@ -52,16 +52,28 @@ constexpr int block_tiles(const Sequence& s, int G, int causal, int rb, int j) {
   return at_least((row_keys(s, G, causal, (j + 1) * rb - 1) + kPageKeys - 1) >> 6, 1);
 }
 
-// The tiles of all units end to end, in equal runs for `n` workgroups.
+// What a tile of block j costs, by the waves of a workgroup that have rows of it: in the form of 384 rows (12 waves, three a SIMD) 4, or where there
+// are rows for two a SIMD or one, 3 or 2 (the waves without rows leave the products out); 1 in the other forms.
+constexpr int most_cost(int rb) { return rb == 384 ? 4 : 1; }
+constexpr int block_cost(const Sequence& s, int G, int rb, int j) {
+  if (rb != 384) return 1;
+  const int rows = s.n * G - j * rb;
+  return rows > 256 ? 4 : rows > 128 ? 3 : 2;
+}
+
+// The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
+constexpr int64_t divided(int64_t x, int64_t by) { return (uint64_t)(x | by) >> 32 ? x / by : (int64_t)((uint32_t)x / (uint32_t)by); }
 constexpr int kMaxShares = 768;       // workgroups of a launch at most
 constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
+constexpr int kWholeTiles = 16;       // a unit of at most so many, and no dearer than a run, is not cut
 struct Shares {
   int64_t total;
   int n;
-  constexpr int64_t begin(int i) const { return total * i / n; }
+  constexpr int64_t begin(int i) const { return divided(total * i, n); }
+  constexpr int64_t run() const { return divided(total, n); }
 };
-constexpr Shares shares_of(int64_t total, int most) {
-  const int64_t worth = total / kMinShareTiles;
+constexpr Shares shares_of(int64_t total, int most, int rb) {
+  const int64_t worth = total / (kMinShareTiles * most_cost(rb));
   return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most)};
 }
 // The workgroup of a launch that takes run `rank`: a contiguous run of runs per XCD.  -1: none.
@@ -69,16 +81,20 @@ constexpr int rank_of(int block, const Shares& sh) {
   const int per_xcd = (sh.n + 7) / 8, rank = (block & 7) * per_xcd + (block >> 3);
   return (block >> 3) < per_xcd && rank < sh.n ? rank : -1;
 }
-// A unit at [begin, end) of the tile space that several runs share: run i leaves its part in slot 2*i + 1 if its part begins the
-// unit, else in slot 2*i.
+// A run boundary that lies `in` behind the beginning of a unit of nt tiles at this cost goes to the tile there, or to the nearer end of a unit that is not
+// cut.  The result may be nt: the next unit's beginning.
+constexpr int boundary_tile(const Shares& sh, int64_t in, int nt, int cost) {
+  const int t = (int)divided(in, cost);
+  return nt <= kWholeTiles && (int64_t)nt * cost <= sh.run() ? (2 * t >= nt ? nt : 0) : t;
+}
+// A unit that several runs share: run i leaves its part in slot 2*i + 1 if its part begins the unit, else in slot 2*i.
 constexpr int64_t part_slot(int run, bool begins) { return 2 * (int64_t)run + (begins ? 1 : 0); }
-// Of the boundary behind run i, inside the unit at [begin, end): whether it is the unit's first one, and then how many runs share the unit.
-// 0: not this boundary's business.
-constexpr int parts_behind(const Shares& sh, int i, int64_t unit_begin, int64_t unit_end) {
-  const int64_t pos = sh.begin(i + 1);
-  if (pos <= unit_begin || pos >= unit_end || sh.begin(i) > unit_begin) return 0;
+// Of boundary i, at tile t of the unit at [begin, begin + nt*cost): if it cuts the unit and is the first that does, how many runs share the unit (the
+// one in front of the boundary, the one behind it, ..).  0: not this boundary's business.
+constexpr int parts_at(const Shares& sh, int i, int64_t begin, int t, int nt, int cost) {
+  if (t <= 0 || t >= nt || sh.begin(i - 1) >= begin + cost) return 0;
   int parts = 2;
-  while (i + parts < sh.n && sh.begin(i + parts) < unit_end) ++parts;
+  while (i + parts - 1 < sh.n && sh.begin(i + parts - 1) < begin + (int64_t)nt * cost) ++parts;
   return parts;
 }
 

@@ -218,24 +218,24 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     """The walk of the attention kernels, all workgroups of a launch: every tile of every unit in one run, a unit's parts in slots of their own, and
     every cut unit joined at one boundary, in the order of the runs."""
     _run(tmp_path, """
-  for (int go = 0; go < 4000; ++go) {
-    const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 4 == 0 ? 384 : go % 4 == 1 ? 32 : 16;
+  for (int go = 0; go < 6000; ++go) {
+    const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 5 <= 1 ? 384 : go % 5 == 2 ? 128 : go % 5 == 3 ? 32 : 16;
     const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 768;
-    std::vector<Sequence> seq;
-    struct Unit { int64_t begin, end; };
+    struct Unit { int64_t begin; int nt, cost; };
     std::vector<Unit> units;
     int64_t total = 0;
     for (int b = 0; b < B; ++b) {
       const int n = any(0, 2) ? any(0, 40) : any(0, 900), keys = any(0, 3) ? any(0, 2000) : any(0, 64);
-      seq.push_back(make_sequence(0, n, keys, 1000, 100));
+      const Sequence s = make_sequence(0, n, keys, 1000, 100);
       for (int h = 0; h < H; ++h)
-        for (int j = 0; j < blocks_of(seq[b], G, rb); ++j) {
-          const int t = block_tiles(seq[b], G, causal, rb, j);
-          units.push_back({total, total + t});
-          total += t;
+        for (int j = 0; j < blocks_of(s, G, rb); ++j) {
+          const int t = block_tiles(s, G, causal, rb, j), cost = block_cost(s, G, rb, j);
+          CHECK(cost >= 1 && cost <= most_cost(rb), "cost %d", cost);
+          units.push_back({total, t, cost});
+          total += (int64_t)t * cost;
         }
     }
-    const Shares sh = shares_of(total, grid);
+    const Shares sh = shares_of(total, grid, rb);
     CHECK(sh.n >= 1 && sh.n <= grid && sh.begin(0) == 0 && sh.begin(sh.n) == total, "%d runs", sh.n);
     std::vector<int> who(sh.n, 0);
     for (int block = 0; block < grid; ++block) {
@@ -245,27 +245,52 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     }
     for (int r = 0; r < sh.n; ++r) CHECK(who[r] == 1, "run %d of %d taken %d times", r, sh.n, who[r]);
     if (total == 0) continue;
-    std::vector<int> left(2 * sh.n, -1);                    // the unit whose part lies in a slot
+    // where every run begins: unit and tile, and the same as a place in the space of all tiles; parts as its workgroup leaves them
+    std::vector<int> unit_of(sh.n), tile_of(sh.n), parts(sh.n);
+    std::vector<int64_t> pos(sh.n + 1, total);
+    for (int r = 0, u = 0; r < sh.n; ++r) {
+      while (sh.begin(r) >= units[u].begin + (int64_t)units[u].nt * units[u].cost) ++u;
+      const int t = boundary_tile(sh, sh.begin(r) - units[u].begin, units[u].nt, units[u].cost);
+      CHECK(t >= 0 && t <= units[u].nt, "tile %d", t);
+      unit_of[r] = u, tile_of[r] = t, pos[r] = units[u].begin + (int64_t)t * units[u].cost;
+      parts[r] = r == 0 ? 0 : parts_at(sh, r, units[u].begin, t, units[u].nt, units[u].cost);
+    }
+    CHECK(pos[0] == 0, "the first run begins at %lld", (long long)pos[0]);
+    for (int r = 0; r < sh.n; ++r) CHECK(pos[r] <= pos[r + 1], "run %d is negative", r);
+    // the walk
+    std::vector<std::vector<int>> done(units.size()), shared(units.size());
+    std::vector<int> slot(2 * sh.n, -1);
+    for (size_t u = 0; u < units.size(); ++u) done[u].assign(units[u].nt, 0);
     for (int r = 0; r < sh.n; ++r) {
-      CHECK(sh.begin(r) < sh.begin(r + 1), "run %d is empty", r);
-      for (size_t u = 0; u < units.size(); ++u) {
-        const int64_t from = std::max(units[u].begin, sh.begin(r)), to = std::min(units[u].end, sh.begin(r + 1));
-        if (from >= to || (from == units[u].begin && to == units[u].end)) continue;
-        const int64_t slot = part_slot(r, from == units[u].begin);
-        CHECK(slot >= 0 && slot < 2 * sh.n && left[slot] < 0, "slot %lld twice", (long long)slot);
-        left[slot] = (int)u;
+      int64_t left = pos[r + 1] - pos[r];
+      int u = unit_of[r], t = tile_of[r];
+      if (left > 0 && t == units[u].nt) ++u, t = 0;
+      while (left > 0) {
+        const int take = (int)std::min<int64_t>(units[u].nt - t, divided(left, units[u].cost));
+        CHECK(take >= 1, "run %d stands still", r);
+        for (int i = 0; i < take; ++i) ++done[u][t + i];
+        if (!(t == 0 && take == units[u].nt)) {
+          const int64_t at = part_slot(r, t == 0);
+          CHECK(at >= 0 && at < 2 * sh.n && slot[at] < 0, "slot %lld twice", (long long)at);
+          slot[at] = u;
+          shared[u].push_back(r);
+        }
+        left -= (int64_t)take * units[u].cost;
+        ++u, t = 0;
       }
+      CHECK(left == 0, "run %d ends inside a tile", r);
     }
-    for (size_t u = 0; u < units.size(); ++u) {
-      int joined = 0, cuts = 0;
-      for (int i = 0; i + 1 < sh.n; ++i) {
-        if (sh.begin(i + 1) > units[u].begin && sh.begin(i + 1) < units[u].end) ++cuts;
-        const int parts = parts_behind(sh, i, units[u].begin, units[u].end);
-        if (!parts) continue;
-        ++joined;
-        for (int k = 0; k < parts; ++k) CHECK(left[part_slot(i + k, k == 0)] == (int)u, "part %d", k);
-        CHECK(parts == 1 + (int)std::count(left.begin() + 2 * i + 2, left.end(), (int)u), "%d parts", parts);
-      }
-      CHECK(joined == (cuts > 0), "unit cut %d times, joined %d", cuts, joined);
+    for (size_t u = 0; u < units.size(); ++u)
+      for (int t = 0; t < units[u].nt; ++t) CHECK(done[u][t] == 1, "tile %d of unit %d done %d times", t, (int)u, done[u][t]);
+    // the second launch
+    std::vector<int> joined(units.size(), 0);
+    for (int r = 1; r < sh.n; ++r) {
+      if (!parts[r]) continue;
+      const int u = unit_of[r];
+      ++joined[u];
+      CHECK(parts[r] == (int)shared[u].size(), "%d parts of %d", parts[r], (int)shared[u].size());
+      for (int k = 0; k < parts[r]; ++k) CHECK(slot[part_slot(r - 1 + k, k == 0)] == u && shared[u][k] == r - 1 + k, "part %d", k);
     }
-  }""")
+    for (size_t u = 0; u < units.size(); ++u) CHECK(joined[u] == (shared[u].empty() ? 0 : 1), "unit of %d parts joined %d times", (int)shared[u].size(), joined[u]);
+  }
+  CHECK(divided(7, 2) == 3 && divided(1ll << 40, 3) == (1ll << 40) / 3 && divided(5, 1ll << 33) == 0 && divided(4294967295ll, 7) == 4294967295ll / 7, "division");""")
