@@ -40,7 +40,7 @@ __device__ __forceinline__ int block_tiles(const PagedParams& p, const Sequence&
 __device__ __forceinline__ int row_keys(const PagedParams& p, const Sequence& s, int r) { return row_keys(s, p.G, p.causal, r); }
 __device__ __forceinline__ int block_cost(const PagedParams& p, const Sequence& s, int rb, int j) { return block_cost(s, p.G, rb, j); }
 __device__ __forceinline__ int64_t unit_cost(const PagedParams& p, const Sequence& s, int rb, int j) {
-  return (int64_t)block_tiles(p, s, rb, j) * block_cost(p, s, rb, j);
+  return unit_length(block_tiles(p, s, rb, j), block_cost(p, s, rb, j));
 }
 
 // Where a run begins: sequence, head, block and tile, and how far in the space of all tiles the unit and the tile begin.
@@ -122,7 +122,7 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t*
   const int nt = block_tiles(p, s, rb, at.j), cost = block_cost(p, s, rb, at.j);
   at.unit = uniform64(pos - rest);
   at.t = __builtin_amdgcn_readfirstlane(boundary_tile(sh, rest, nt, cost));
-  at.pos = at.unit + (int64_t)at.t * cost;
+  at.pos = at.unit + tile_place(at.t, cost);
   return at;
 }
 
@@ -250,7 +250,8 @@ __device__ __forceinline__ void ask_queries(const PagedParams& p, const Sequence
     q.v[i] = *(const i32x4*)(p.q + row_offset(p, s, h, min(r0 + 4 * i + (lane >> 4), last), p.q_ss, p.q_sh, token) + (lane & 15) * 16);
 }
 // .. and through norm and rotation, in the lane order of the B images, by way of 4 KiB of LDS of the wave's own
-__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, char* turn, int lane, bf16x8 (&out)[4]) {
+__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, char* turn, int lane, float factor,
+                                              bf16x8 (&out)[4]) {
   Rows16 cos, sin;
   NormLanes norm;
   load_norm_lanes(norm, p.norm_w, lane);
@@ -272,7 +273,7 @@ __device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequen
     turn_table(sin, rope.s, p.rope_mode, turn, lane);
   }
   float x[32];
-  norm_row(x, raw, p.norm_w != nullptr, p.eps, norm, 1.0f);
+  norm_row(x, raw, p.norm_w != nullptr, p.eps, norm, factor);
   rope_row(x, p.rope_mode, rope);
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks)
@@ -310,14 +311,14 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 
 #pragma unroll 1
   while (left > 0) {
-    const int nt = block_tiles(p, s, RB, at.j), take = (int)min((int64_t)(nt - at.t), left);
+    const int nt = block_tiles(p, s, RB, at.j), take = tiles_left(left, at.t, nt, 1);
     __syncthreads();                                           // the sums, or the results of the unit before, are read
     SplitState<FP8, QB> w;
     if (wave < QB) {
       bf16x8 img[4];
       Rows16 q;
       ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
-      queries_ready(p, s, at.j * RB + 16 * wave, q, part + wave * 4096, lane, img);
+      queries_ready(p, s, at.j * RB + 16 * wave, q, part + wave * 4096, lane, 1.0f, img);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
     }
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
         }
       }
     }
-    left -= take;
+    left -= take + (at.t == 0 ? kUnitTiles : 0);
     at.t = 0;
     if (!next_unit(p, at, s, blocks, RB, left)) return;
   }
@@ -520,10 +521,54 @@ struct TileForm {
   }
 };
 
+// A query's running maximum in the log2 domain.  FOLD: the softmax scale and log2 e ride in Q', which norm or rotation has rounded to bf16 anyway, and the sums of
+// S^T begin with the negative maximum (a quad, as the MFMA takes it), so that they are the exponents of the weights as they come out.  Otherwise Q' is the
+// query as it is, and the scale multiplies in the subtraction.
+template <bool FOLD>
+struct Running;
+template <>
+struct Running<true> {
+  f32x4 neg[2];
+  __device__ __forceinline__ void start() { neg[0] = neg[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
+  __device__ __forceinline__ float of(int qb) const { return -neg[qb][0]; }
+  __device__ __forceinline__ f32x4 first(int qb) const { return neg[qb]; }
+};
+template <>
+struct Running<false> {
+  float m[2];
+  __device__ __forceinline__ void start() { m[0] = m[1] = kNoMax; }
+  __device__ __forceinline__ float of(int qb) const { return m[qb]; }
+  __device__ __forceinline__ f32x4 first(int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+};
+
+// S^T of a step (see qk_tile: images read AHEAD of their products)
+template <int NKB, int AHEAD, bool FOLD>
+__device__ __forceinline__ void tile_qk(WaveState<false>& w, const Running<FOLD>& run, const char* kbuf, int lane) {
+  constexpr int kImages = 4 * NKB;                                        // (half, ks, kb2)
+  bf16x8 kf[kImages];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) kf[i] = *(const bf16x8*)(kbuf + (i * 64 + lane) * 16);
+#pragma unroll
+  for (int i = 0; i < kImages; ++i) {
+    const int ks = (i >> 1) & 3, kb = 2 * (i >> 3) + (i & 1);
+#pragma unroll
+    for (int q = 0, qb = i & 1; q < 2; ++q, qb ^= 1) w.s[kb][qb] = PKH3_MFMA16(kf[i], w.qf[qb][ks], ks == 0 ? run.first(qb) : w.s[kb][qb]);
+    if (i + AHEAD < kImages) kf[i + AHEAD] = *(const bf16x8*)(kbuf + ((i + AHEAD) * 64 + lane) * 16);
+  }
+  if constexpr (AHEAD > 2) {                                              // (the copies of the loop that run once or twice a unit fit the registers without)
+    PKH3_SGB(kSgDsRead, AHEAD);
+#pragma unroll
+    for (int i = 0; i < kImages; ++i) {
+      PKH3_SGB(kSgMfma, 2);
+      if (i + AHEAD < kImages) PKH3_SGB(kSgDsRead, 1);
+    }
+  }
+}
+
 // The weights of NKB blocks of 16 keys, as operands of P.V (see softmax_blocks of the dense calls).  MASKED: lim[qb] keys of these exist for the
 // lane's query.
-template <int NKB, bool MASKED>
-__device__ __forceinline__ void tile_softmax(WaveState<false>& w, bf16x8 (&pf)[NKB / 2][2], float c, const int (&lim)[2], int lane) {
+template <int NKB, bool MASKED, bool FOLD>
+__device__ __forceinline__ void tile_softmax(WaveState<false>& w, Running<FOLD>& run, bf16x8 (&pf)[NKB / 2][2], float c, const int (&lim)[2], int lane) {
   if constexpr (MASKED) {
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -542,15 +587,35 @@ __device__ __forceinline__ void tile_softmax(WaveState<false>& w, bf16x8 (&pf)[N
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx[qb] = fmaxf(mx[qb], w.s[kb][qb][i]);
-    mx[qb] *= c;
+    if constexpr (!FOLD) mx[qb] *= c;
   }
-  if (__any(mx[0] > w.m[0] + kRescaleSlack || mx[1] > w.m[1] + kRescaleSlack)) {
+  bool raise = false;
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    // FOLD: what is there is over the maximum so far, which a query without a weight so far does not have
+    if constexpr (FOLD) raise |= mx[qb] > kRescaleSlack || (w.l[qb] == 0.f && mx[qb] > -INFINITY);
+    else raise |= mx[qb] > run.m[qb] + kRescaleSlack;
+  }
+  if (__any(raise)) {
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       const float top = max_across_groups(mx[qb]);
-      const float m_new = top > w.m[qb] + kRescaleSlack ? top : w.m[qb];
-      const float alpha = __builtin_amdgcn_exp2f(w.m[qb] - m_new);
-      w.m[qb] = m_new;
+      float alpha;
+      if constexpr (FOLD) {
+        const bool none = wave_sum_groups(w.l[qb]) == 0.f && top > -INFINITY;
+        const float up = none || top > kRescaleSlack ? top : 0.f;
+        alpha = none ? 0.f : __builtin_amdgcn_exp2f(-up);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) run.neg[qb][i] -= up;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.s[kb][qb][i] -= up;
+      } else {
+        const float m_new = top > run.m[qb] + kRescaleSlack ? top : run.m[qb];
+        alpha = __builtin_amdgcn_exp2f(run.m[qb] - m_new);
+        run.m[qb] = m_new;
+      }
       w.l[qb] *= alpha;
 #pragma unroll
       for (int db = 0; db < 8; ++db)
@@ -565,7 +630,10 @@ __device__ __forceinline__ void tile_softmax(WaveState<false>& w, bf16x8 (&pf)[N
     for (int qb = 0; qb < 2; ++qb) {
       bf16x8 pk;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pk[j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(w.s[2 * half + (j >> 2)][qb][j & 3], c, -w.m[qb]));
+      for (int j = 0; j < 8; ++j) {
+        const float s = w.s[2 * half + (j >> 2)][qb][j & 3];
+        pk[j] = (__bf16)__builtin_amdgcn_exp2f(FOLD ? s : fmaf(s, c, -run.of(qb)));
+      }
       // row sum over the rounded weights, the same numbers P.V takes
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
@@ -599,10 +667,8 @@ __device__ __forceinline__ void expand_step(const char* raw, char* images, int h
   constexpr int kPieces = F::kRaw / 1024, kOfK = kPieces / 2;
   const int g = lane >> 4, c = lane & 15;
   const char* scales = raw + F::kRaw + (F::kStep == 32 ? 32 * half_of_page : 0);
-#pragma unroll
-  for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
-    const int piece = n * WAVES + wave;
-    if ((n + 1) * WAVES > kPieces && piece >= kPieces) break;
+#pragma unroll 1
+  for (int piece = wave; piece < kPieces; piece += WAVES) {
     const i32x4 v = *(const i32x4*)(raw + (piece * 64 + lane) * 16);
     if (piece < kOfK) {                                                   // key block kb, images ks = 2*c2, 2*c2 + 1
       const int kb = piece >> 1, c2 = piece & 1;
@@ -645,7 +711,7 @@ __device__ __forceinline__ void clear_missing_images(char* v, int there, int wav
   }
 }
 
-template <bool FP8, int WAVES>
+template <bool FP8, int WAVES, bool FOLD>
 __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_kernel(PagedParams p) {
   using F = TileForm<WAVES>;
   constexpr int RB = 32 * WAVES, kStep = F::kStep, NKB = kStep / 16, kPerTile = kTileKeys / kStep;
@@ -697,8 +763,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
   auto begin_unit = [&]() {                                               // asks for everything the unit's loop begins with
     nt = block_tiles(p, s, RB, at.j);
     const int cost = block_cost(p, s, RB, at.j);
-    take = (int)min((int64_t)(nt - at.t), divided(left, cost));
-    left -= (int64_t)take * cost;
+    take = tiles_left(left, at.t, nt, cost);
+    left -= (int64_t)(take + (at.t == 0 ? kUnitTiles : 0)) * cost;
     first = at.t * kPerTile, end = (at.t + take) * kPerTile;              // steps
 #pragma unroll
     for (int i = 0; i < 3; ++i) id[i] = page(first + i, end);
@@ -717,22 +783,23 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
     WaveState<false> w;
     if (!idle) {
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) queries_ready(p, s, r0 + 16 * qb, ahead[qb], turn, lane_here(), w.qf[qb]);
+      for (int qb = 0; qb < 2; ++qb) queries_ready(p, s, r0 + 16 * qb, ahead[qb], turn, lane_here(), FOLD ? p.c : 1.0f, w.qf[qb]);
     }
-    const int lane = lane_here();
     const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
 #pragma unroll
     for (int db = 0; db < 8; ++db)
 #pragma unroll
       for (int qb = 0; qb < 2; ++qb) w.o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) w.m[qb] = kNoMax, w.l[qb] = 0.f;
+    for (int qb = 0; qb < 2; ++qb) w.l[qb] = 0.f;
+    Running<FOLD> run;
+    run.start();
 
     int slot = 0, slot_prev = 2;
     if constexpr (FP8) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      expand_step<WAVES>(copies, lds, first & 1, wave, lane);
+      expand_step<WAVES>(copies, lds, first & 1, wave, lane_here());
     }
     // One step.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
     auto step = [&](int i, auto masked, auto works) {
@@ -749,8 +816,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
         }
       }
       if constexpr (WORKS) {
-        if constexpr (NKB == 4) qk_tile<false, true, MASKED ? 2 : 4>(w, images, images, lane);
-        else qk_half<false, true>(w, images, images, lane);
+        tile_qk<NKB, MASKED ? 2 : FOLD ? 3 : 4, FOLD>(w, run, images, lane_here());
       }
       if constexpr (!FP8) {
         if (i + 2 < end) copy(id[2], i + 2, slot_prev);
@@ -769,8 +835,8 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
           for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kStep * i);
         }
         bf16x8 pf[NKB / 2][2];
-        tile_softmax<NKB, MASKED>(w, pf, p.c, lim, lane);
-        tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane);
+        tile_softmax<NKB, MASKED, FOLD>(w, run, pf, p.c, lim, lane_here());
+        tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane_here());
       }
     };
     // Whether a step is masked differs from wave to wave, how many barriers it has does not: a step with keys that do not exist, or a page that does not,
@@ -828,7 +894,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
           if (r0 + 16 * qb + c16 <= last) {
 #pragma unroll
             for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
-            if (g4 == 0) part[RB * kD + row] = w.m[qb], part[RB * (kD + 1) + row] = l;
+            if (g4 == 0) part[RB * kD + row] = l == 0.f ? kNoMax : run.of(qb), part[RB * (kD + 1) + row] = l;
           }
         }
       }
@@ -930,17 +996,25 @@ static hipError_t launch_form(Kernel kernel, int threads, int grid, const PagedP
   return hipGetLastError();
 }
 
+template <int WAVES>
+static hipError_t launch_tile(bool fp8, bool fold, int grid, const PagedParams& p, hipStream_t st) {
+  auto* kernel = fp8 ? (fold ? paged_tile_kernel<true, WAVES, true> : paged_tile_kernel<true, WAVES, false>)
+                     : (fold ? paged_tile_kernel<false, WAVES, true> : paged_tile_kernel<false, WAVES, false>);
+  return launch_form<32 * WAVES>(kernel, 64 * WAVES, grid, p, st);
+}
+
 hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
   if (e != hipSuccess) return e;
   const PagedForm f = form_of(p.rows, p.B, p.G);
   const int grid = workgroups_of(f, cus);
+  const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {
     case kSplit16: return launch_form<16>(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 256, grid, p, st);
     case kSplit32: return launch_form<32>(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 256, grid, p, st);
-    case kTile128: return launch_form<128>(fp8 ? paged_tile_kernel<true, 4> : paged_tile_kernel<false, 4>, 256, grid, p, st);
-    default: return launch_form<384>(fp8 ? paged_tile_kernel<true, 12> : paged_tile_kernel<false, 12>, 768, grid, p, st);
+    case kTile128: return launch_tile<4>(fp8, fold, grid, p, st);
+    default: return launch_tile<12>(fp8, fold, grid, p, st);
   }
 }
 

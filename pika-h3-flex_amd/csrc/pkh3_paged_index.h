@@ -61,8 +61,20 @@ constexpr int block_cost(const Sequence& s, int G, int rb, int j) {
   return rows > 256 ? 4 : rows > 128 ? 3 : 2;
 }
 
-// The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
+// What a unit costs besides its tiles, in tiles: queries in and out, the first keys' way.  Units of 384 rows against 2, 5 and 8 tiles took 8 us and 2.7 a
+// tile; shared out by their tiles alone, the last workgroup of such a call was done at 320 us and the first at 102.
+constexpr int kUnitTiles = 3;
+constexpr int64_t unit_length(int nt, int cost) { return (int64_t)(nt + kUnitTiles) * cost; }
+// where tile t of a unit begins
+constexpr int64_t tile_place(int t, int cost) { return t == 0 ? 0 : (int64_t)(t + kUnitTiles) * cost; }
+// tiles that `left` of a run is worth from tile t of a unit on (boundaries lie at tiles: nothing is left over)
 constexpr int64_t divided(int64_t x, int64_t by) { return (uint64_t)(x | by) >> 32 ? x / by : (int64_t)((uint32_t)x / (uint32_t)by); }
+constexpr int tiles_left(int64_t left, int t, int nt, int cost) {
+  const int64_t all = divided(left, cost) - (t == 0 ? kUnitTiles : 0);
+  return all < nt - t ? (int)all : nt - t;
+}
+
+// The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
 constexpr int kMaxShares = 768;       // workgroups of a launch at most
 constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
 constexpr int kWholeTiles = 16;       // a unit of at most so many, and no dearer than a run, is not cut
@@ -73,7 +85,7 @@ struct Shares {
   constexpr int64_t run() const { return divided(total, n); }
 };
 constexpr Shares shares_of(int64_t total, int most, int rb) {
-  const int64_t worth = total / (kMinShareTiles * most_cost(rb));
+  const int64_t worth = total / ((kMinShareTiles + kUnitTiles) * most_cost(rb));
   return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most)};
 }
 // The workgroup of a launch that takes run `rank`: a contiguous run of runs per XCD.  -1: none.
@@ -84,17 +96,17 @@ constexpr int rank_of(int block, const Shares& sh) {
 // A run boundary that lies `in` behind the beginning of a unit of nt tiles at this cost goes to the tile there, or to the nearer end of a unit that is not
 // cut.  The result may be nt: the next unit's beginning.
 constexpr int boundary_tile(const Shares& sh, int64_t in, int nt, int cost) {
-  const int t = (int)divided(in, cost);
-  return nt <= kWholeTiles && (int64_t)nt * cost <= sh.run() ? (2 * t >= nt ? nt : 0) : t;
+  const int t = at_least((int)divided(in, cost) - kUnitTiles, 0);
+  return nt <= kWholeTiles && unit_length(nt, cost) <= sh.run() ? (2 * in >= unit_length(nt, cost) ? nt : 0) : t;
 }
 // A unit that several runs share: run i leaves its part in slot 2*i + 1 if its part begins the unit, else in slot 2*i.
 constexpr int64_t part_slot(int run, bool begins) { return 2 * (int64_t)run + (begins ? 1 : 0); }
-// Of boundary i, at tile t of the unit at [begin, begin + nt*cost): if it cuts the unit and is the first that does, how many runs share the unit (the
+// Of boundary i, at tile t of the unit of nt tiles that begins at `begin`: if it cuts the unit and is the first that does, how many runs share the unit (the
 // one in front of the boundary, the one behind it, ..).  0: not this boundary's business.
 constexpr int parts_at(const Shares& sh, int i, int64_t begin, int t, int nt, int cost) {
-  if (t <= 0 || t >= nt || sh.begin(i - 1) >= begin + cost) return 0;
+  if (t <= 0 || t >= nt || sh.begin(i - 1) >= begin + tile_place(1, cost)) return 0;
   int parts = 2;
-  while (i + parts - 1 < sh.n && sh.begin(i + parts - 1) < begin + (int64_t)nt * cost) ++parts;
+  while (i + parts - 1 < sh.n && sh.begin(i + parts - 1) < begin + unit_length(nt, cost)) ++parts;
   return parts;
 }
 

@@ -232,7 +232,7 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
           const int t = block_tiles(s, G, causal, rb, j), cost = block_cost(s, G, rb, j);
           CHECK(cost >= 1 && cost <= most_cost(rb), "cost %d", cost);
           units.push_back({total, t, cost});
-          total += (int64_t)t * cost;
+          total += unit_length(t, cost);
         }
     }
     const Shares sh = shares_of(total, grid, rb);
@@ -249,10 +249,10 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     std::vector<int> unit_of(sh.n), tile_of(sh.n), parts(sh.n);
     std::vector<int64_t> pos(sh.n + 1, total);
     for (int r = 0, u = 0; r < sh.n; ++r) {
-      while (sh.begin(r) >= units[u].begin + (int64_t)units[u].nt * units[u].cost) ++u;
+      while (sh.begin(r) >= units[u].begin + unit_length(units[u].nt, units[u].cost)) ++u;
       const int t = boundary_tile(sh, sh.begin(r) - units[u].begin, units[u].nt, units[u].cost);
       CHECK(t >= 0 && t <= units[u].nt, "tile %d", t);
-      unit_of[r] = u, tile_of[r] = t, pos[r] = units[u].begin + (int64_t)t * units[u].cost;
+      unit_of[r] = u, tile_of[r] = t, pos[r] = units[u].begin + tile_place(t, units[u].cost);
       parts[r] = r == 0 ? 0 : parts_at(sh, r, units[u].begin, t, units[u].nt, units[u].cost);
     }
     CHECK(pos[0] == 0, "the first run begins at %lld", (long long)pos[0]);
@@ -266,7 +266,7 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
       int u = unit_of[r], t = tile_of[r];
       if (left > 0 && t == units[u].nt) ++u, t = 0;
       while (left > 0) {
-        const int take = (int)std::min<int64_t>(units[u].nt - t, divided(left, units[u].cost));
+        const int take = tiles_left(left, t, units[u].nt, units[u].cost);
         CHECK(take >= 1, "run %d stands still", r);
         for (int i = 0; i < take; ++i) ++done[u][t + i];
         if (!(t == 0 && take == units[u].nt)) {
@@ -275,7 +275,7 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
           slot[at] = u;
           shared[u].push_back(r);
         }
-        left -= (int64_t)take * units[u].cost;
+        left -= (int64_t)(take + (t == 0 ? kUnitTiles : 0)) * units[u].cost;
         ++u, t = 0;
       }
       CHECK(left == 0, "run %d ends inside a tile", r);
