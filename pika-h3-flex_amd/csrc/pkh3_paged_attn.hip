@@ -494,129 +494,124 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 
 // ---- the tile form: many query rows, all waves of a workgroup share every key tile ----
 //
-// A unit is 32 query rows a wave: 384 rows in 12 waves (three a SIMD, one workgroup a CU), or 128 in 4 (three workgroups a CU) where 384 would
-// leave most of a workgroup without rows.  The loop is that of the dense calls: K/V steps (a tile of 64 keys, half of one in the small
-// form) in an LDS ring of three, two steps ahead of the products, one barrier a step.  The page of a step is looked up a step before its copy.
+// A unit is 384 query rows, 32 a wave; twelve waves are three a SIMD, one workgroup a CU.  The loop is that of the dense calls: K/V tiles in an LDS ring
+// of three, two tiles ahead of the products, one barrier a tile.  The page of a tile is looked up a step before its copy.  (Units of 128 rows
+// in four waves, three workgroups a CU, in halves of tiles, were behind on all but some calls of a few dozen rows, and there by 2 %: 1,560 rows over
+// 48,360 keys 881 us here, 1,355 there; 120 rows over 20,000 keys 58 and 72; three requests against 77 to 512 keys 212 and 218.)
 // Eight-bit pages come to LDS as they are, one step further ahead, and are expanded there to the bf16 images of the loop, a share of
 // them by every wave, under the products of the step before: once for all waves, and the loop has no conversions.
 //
-// The running maximum costs little here: only whether any logit of the wave exceeds its query's maximum by 2^8 is asked for in every step, the exchange
-// between lanes and the rescale happen when one does.
 
-template <int WAVES>
-struct TileForm {
-  static constexpr int kStep = WAVES == 4 ? 32 : 64;                     // keys
-  static constexpr int kBytes = kStep * 2 * kD * 2;                      // of a step's bf16 images: K, then V
-  static constexpr int kRaw = kStep * 2 * kD;                            // of its e4m3 values
-  static constexpr int kRawSlot = kRaw + kPageScales;
-  // bf16: a ring of three steps.  e4m3: two steps of images, two as they come
-  template <bool FP8>
-  static constexpr int ring_bytes() { return FP8 ? 2 * kBytes + 2 * kRawSlot : 3 * kBytes; }
-  template <bool FP8>
-  static constexpr int lds_bytes() {
-    // queries and outputs are turned around where the third step goes (e4m3: the images) and behind it
-    const int turned = (FP8 ? 0 : 2) * kBytes + WAVES * 4096, sums = (kMaxSequences + 1) * (int)sizeof(int64_t);
-    const int most = ring_bytes<FP8>() > turned ? ring_bytes<FP8>() : turned;
-    return most > sums ? most : sums;
+// The kernel's arguments, read again where they are used: those of the queries and outputs, kept through the loop, take the scalar registers that its copies need.
+__device__ __forceinline__ PagedParams arguments_here() {
+  PagedParams args;
+  auto* a = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  __builtin_memcpy(&args, (const char*)a, sizeof(args));
+  return args;
+}
+
+constexpr int kTileWaves = 12, kTileRows = 32 * kTileWaves;
+constexpr int kImageBytes = kKTileBytes + kVTileBytes;                    // of a tile's bf16 images
+constexpr int kRawBytes = kPageRecord8;                                   // of a tile's e4m3 values and scales, as they come
+constexpr int kTurnBytes12 = kTileWaves * 4096;                           // where queries and outputs are turned around
+// bf16: a ring of three tiles, the turning place where the third goes and behind it.  e4m3: two tiles of images (the turning place), two as they come
+template <bool FP8>
+constexpr int tile_lds_bytes() {
+  static_assert(2 * kImageBytes >= kTurnBytes12 && kTurnBytes12 > kImageBytes, "the places");
+  return FP8 ? 2 * kImageBytes + 2 * kRawBytes : 2 * kImageBytes + kTurnBytes12;
+}
+
+// A query's running maximum in the log2 domain, negative.  FOLD: the softmax scale and log2 e ride in Q', which norm or rotation has rounded to bf16 anyway,
+// and the sums of S^T begin with it (a quad, as the MFMA takes it), so that they are the exponents of the weights as they come out.  Otherwise Q' is the
+// query as it is, and the scale multiplies in the subtraction.
+template <bool FOLD>
+struct Running {
+  f32x4 neg[FOLD ? 2 : 1];
+  float m[FOLD ? 1 : 2];
+  __device__ __forceinline__ float negative(int qb) const {
+    if constexpr (FOLD) return neg[qb][0];
+    else return m[qb];
+  }
+  __device__ __forceinline__ f32x4 first(int qb) const {
+    if constexpr (FOLD) return neg[qb];
+    else return f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void set(int qb, float x) {
+    if constexpr (FOLD) neg[qb] = f32x4{x, x, x, x};
+    else m[qb] = x;
   }
 };
 
-// A query's running maximum in the log2 domain.  FOLD: the softmax scale and log2 e ride in Q', which norm or rotation has rounded to bf16 anyway, and the sums of
-// S^T begin with the negative maximum (a quad, as the MFMA takes it), so that they are the exponents of the weights as they come out.  Otherwise Q' is the
-// query as it is, and the scale multiplies in the subtraction.
-template <bool FOLD>
-struct Running;
-template <>
-struct Running<true> {
-  f32x4 neg[2];
-  __device__ __forceinline__ void start() { neg[0] = neg[1] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-  __device__ __forceinline__ float of(int qb) const { return -neg[qb][0]; }
-  __device__ __forceinline__ f32x4 first(int qb) const { return neg[qb]; }
-};
-template <>
-struct Running<false> {
-  float m[2];
-  __device__ __forceinline__ void start() { m[0] = m[1] = kNoMax; }
-  __device__ __forceinline__ float of(int qb) const { return m[qb]; }
-  __device__ __forceinline__ f32x4 first(int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
-};
-
-// S^T of a step (see qk_tile: images read AHEAD of their products)
-template <int NKB, int AHEAD, bool FOLD>
+// S^T of a tile (see qk_tile: images read AHEAD of their products)
+template <int AHEAD, bool FOLD>
 __device__ __forceinline__ void tile_qk(WaveState<false>& w, const Running<FOLD>& run, const char* kbuf, int lane) {
-  constexpr int kImages = 4 * NKB;                                        // (half, ks, kb2)
-  bf16x8 kf[kImages];
+  bf16x8 kf[16];                                                          // (half, ks, kb2)
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) kf[i] = *(const bf16x8*)(kbuf + (i * 64 + lane) * 16);
 #pragma unroll
-  for (int i = 0; i < kImages; ++i) {
+  for (int i = 0; i < 16; ++i) {
     const int ks = (i >> 1) & 3, kb = 2 * (i >> 3) + (i & 1);
 #pragma unroll
     for (int q = 0, qb = i & 1; q < 2; ++q, qb ^= 1) w.s[kb][qb] = PKH3_MFMA16(kf[i], w.qf[qb][ks], ks == 0 ? run.first(qb) : w.s[kb][qb]);
-    if (i + AHEAD < kImages) kf[i + AHEAD] = *(const bf16x8*)(kbuf + ((i + AHEAD) * 64 + lane) * 16);
+    if (i + AHEAD < 16) kf[i + AHEAD] = *(const bf16x8*)(kbuf + ((i + AHEAD) * 64 + lane) * 16);
   }
-  if constexpr (AHEAD > 2) {                                              // (the copies of the loop that run once or twice a unit fit the registers without)
-    PKH3_SGB(kSgDsRead, AHEAD);
+  PKH3_SGB(kSgDsRead, AHEAD);
 #pragma unroll
-    for (int i = 0; i < kImages; ++i) {
-      PKH3_SGB(kSgMfma, 2);
-      if (i + AHEAD < kImages) PKH3_SGB(kSgDsRead, 1);
-    }
+  for (int i = 0; i < 16; ++i) {
+    PKH3_SGB(kSgMfma, 2);
+    if (i + AHEAD < 16) PKH3_SGB(kSgDsRead, 1);
   }
 }
 
-// The weights of NKB blocks of 16 keys, as operands of P.V (see softmax_blocks of the dense calls).  MASKED: lim[qb] keys of these exist for the
-// lane's query.
-template <int NKB, bool MASKED, bool FOLD>
-__device__ __forceinline__ void tile_softmax(WaveState<false>& w, Running<FOLD>& run, bf16x8 (&pf)[NKB / 2][2], float c, const int (&lim)[2], int lane) {
-  if constexpr (MASKED) {
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      const int mine = lim[qb] - 4 * (lane >> 4);                         // (against constants from here on)
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w.s[kb][qb][i] = 16 * kb + i >= mine ? -INFINITY : w.s[kb][qb][i];
-    }
-  }
-  float mx[2];
+// see tile_softmax: beside weights that began at 1 or more and go down by 2^-126 at most before they are gone themselves
+constexpr float kSomeWeight = 0x1p-100f;
+
+// The weights of a tile, as operands of P.V (see softmax_blocks of the dense calls).  MASKED: lim[qb] keys of it exist for the lane's query.
+// The maximum of a query is that of its first tile with keys, and is raised when exceeded by 2^8.  Whether any is, the largest exponent tells as an integer (any
+// positive float is a larger one than any negative, and NaN than all): no order among the negative ones is needed.  A lane that has no weight yet looks.
+template <bool MASKED, bool FOLD>
+__device__ __forceinline__ void tile_softmax(WaveState<false>& w, Running<FOLD>& run, bf16x8 (&pf)[2][2], float c, const int (&lim)[2], int lane) {
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    mx[qb] = w.s[0][qb][0];
+    const int mine = lim[qb] - 4 * (lane >> 4);                           // (against constants from here on)
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb)
+    for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx[qb] = fmaxf(mx[qb], w.s[kb][qb][i]);
-    if constexpr (!FOLD) mx[qb] *= c;
-  }
-  bool raise = false;
-#pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
-    // FOLD: what is there is over the maximum so far, which a query without a weight so far does not have
-    if constexpr (FOLD) raise |= mx[qb] > kRescaleSlack || (w.l[qb] == 0.f && mx[qb] > -INFINITY);
-    else raise |= mx[qb] > run.m[qb] + kRescaleSlack;
-  }
-  if (__any(raise)) {
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      const float top = max_across_groups(mx[qb]);
-      float alpha;
-      if constexpr (FOLD) {
-        const bool none = wave_sum_groups(w.l[qb]) == 0.f && top > -INFINITY;
-        const float up = none || top > kRescaleSlack ? top : 0.f;
-        alpha = none ? 0.f : __builtin_amdgcn_exp2f(-up);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) run.neg[qb][i] -= up;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w.s[kb][qb][i] -= up;
-      } else {
-        const float m_new = top > run.m[qb] + kRescaleSlack ? top : run.m[qb];
-        alpha = __builtin_amdgcn_exp2f(run.m[qb] - m_new);
-        run.m[qb] = m_new;
+      for (int i = 0; i < 4; ++i) {
+        float x = w.s[kb][qb][i];
+        if constexpr (!FOLD) x = fmaf(x, c, run.negative(qb));
+        if constexpr (MASKED) x = 16 * kb + i >= mine ? -INFINITY : x;
+        w.s[kb][qb][i] = x;
       }
-      w.l[qb] *= alpha;
+  }
+  int most = __float_as_int(w.s[0][0][0]);
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = max(most, __float_as_int(w.s[kb][qb][i]));
+  if (__any(most > __float_as_int(kRescaleSlack) || w.l[0] == 0.f || w.l[1] == 0.f)) {
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      float top = w.s[0][qb][0];
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, w.s[kb][qb][i]);
+      top = max_across_groups(top);
+      const float before = wave_sum_groups(w.l[qb]);
+      const bool none = before == 0.f;                                    // no maximum yet
+      const float up = none ? (top > -INFINITY ? top : 0.f) : top > kRescaleSlack ? top : 0.f;
+      const float alpha = none ? 0.f : __builtin_amdgcn_exp2f(-up);
+      run.set(qb, run.negative(qb) - up);
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.s[kb][qb][i] -= up;
+      // a lane without a weight whose query has some in others need not look again: it gets one that is nothing beside those
+      w.l[qb] = none ? 0.f : fmaxf(w.l[qb] * alpha, kSomeWeight);
 #pragma unroll
       for (int db = 0; db < 8; ++db)
 #pragma unroll
@@ -625,15 +620,12 @@ __device__ __forceinline__ void tile_softmax(WaveState<false>& w, Running<FOLD>&
   }
   const bf16x2 one2 = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
-  for (int half = 0; half < NKB / 2; ++half)
+  for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       bf16x8 pk;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float s = w.s[2 * half + (j >> 2)][qb][j & 3];
-        pk[j] = (__bf16)__builtin_amdgcn_exp2f(FOLD ? s : fmaf(s, c, -run.of(qb)));
-      }
+      for (int j = 0; j < 8; ++j) pk[j] = (__bf16)__builtin_amdgcn_exp2f(w.s[2 * half + (j >> 2)][qb][j & 3]);
       // row sum over the rounded weights, the same numbers P.V takes
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
@@ -644,44 +636,39 @@ __device__ __forceinline__ void tile_softmax(WaveState<false>& w, Running<FOLD>&
     }
 }
 
-// O^T += V^T P^T of a step, V images read four ahead of their products
-template <int NKB>
-__device__ __forceinline__ void tile_pv(WaveState<false>& w, const bf16x8 (&pf)[NKB / 2][2], const char* vbuf, int lane) {
-  constexpr int kImages = 4 * NKB;
-  bf16x8 vg[kImages];
+// O^T += V^T P^T of a tile, V images read four ahead of their products
+__device__ __forceinline__ void tile_pv(WaveState<false>& w, const bf16x8 (&pf)[2][2], const char* vbuf, int lane) {
+  bf16x8 vg[16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) vg[i] = *(const bf16x8*)(vbuf + (i * 64 + lane) * 16);
 #pragma unroll
-  for (int i = 0; i < kImages; ++i) {
+  for (int i = 0; i < 16; ++i) {
 #pragma unroll
     for (int q = 0, qb = i & 1; q < 2; ++q, qb ^= 1) w.o[i & 7][qb] = PKH3_MFMA16(vg[i], pf[i >> 3][qb], w.o[i & 7][qb]);
-    if (i + 4 < kImages) vg[i + 4] = *(const bf16x8*)(vbuf + ((i + 4) * 64 + lane) * 16);
+    if (i + 4 < 16) vg[i + 4] = *(const bf16x8*)(vbuf + ((i + 4) * 64 + lane) * 16);
   }
 }
 
-// A wave's share of a step's e4m3 values to bf16 images.  1 KiB of them, 16 values a lane, are two images.  A key's values have one scale: of K that is
+// A wave's share of a tile's e4m3 values to bf16 images.  1 KiB of them, 16 values a lane, are two images.  A key's values have one scale: of K that is
 // one per lane, of V one per value of the eight, applied as the value is converted (the conversion takes a power of two along).
-template <int WAVES>
-__device__ __forceinline__ void expand_step(const char* raw, char* images, int half_of_page, int wave, int lane) {
-  using F = TileForm<WAVES>;
-  constexpr int kPieces = F::kRaw / 1024, kOfK = kPieces / 2;
+__device__ __forceinline__ void expand_tile(const char* raw, char* images, int wave, int lane) {
   const int g = lane >> 4, c = lane & 15;
-  const char* scales = raw + F::kRaw + (F::kStep == 32 ? 32 * half_of_page : 0);
+  const char* scales = raw + kRawBytes - kPageScales;
 #pragma unroll 1
-  for (int piece = wave; piece < kPieces; piece += WAVES) {
+  for (int piece = wave; piece < 16; piece += kTileWaves) {
     const i32x4 v = *(const i32x4*)(raw + (piece * 64 + lane) * 16);
-    if (piece < kOfK) {                                                   // key block kb, images ks = 2*c2, 2*c2 + 1
+    if (piece < 8) {                                                      // key block kb, images ks = 2*c2, 2*c2 + 1
       const int kb = piece >> 1, c2 = piece & 1;
       const float scale = exponent_scale((unsigned char)scales[16 * kb + c]);
       char* to = images + ((((kb >> 1) * 4 + 2 * c2) * 2 + (kb & 1)) * 64 + lane) * 16;
       *(bf16x8*)to = expand_fp8(v[0], v[1], scale);
       *(bf16x8*)(to + 2048) = expand_fp8(v[2], v[3], scale);
     } else {                                                              // (half, dbp), images db = 2*dbp, 2*dbp + 1
-      const int at = piece - kOfK, half = at >> 2, dbp = at & 3;
+      const int half = (piece - 8) >> 2, dbp = piece & 3;
       unsigned e[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) e[kb] = *(const unsigned*)(scales + 64 + 32 * half + 16 * kb + 4 * g);
-      char* to = images + F::kBytes / 2 + ((half * 8 + 2 * dbp) * 64 + lane) * 16;
+      char* to = images + kKTileBytes + ((half * 8 + 2 * dbp) * 64 + lane) * 16;
 #pragma unroll
       for (int par = 0; par < 2; ++par) {
         bf16x8 out;
@@ -698,27 +685,24 @@ __device__ __forceinline__ void expand_step(const char* raw, char* images, int h
   }
 }
 
-// Values of keys that do not exist are zero (see clear_missing), in the V images of a step in LDS
-template <int WAVES>
+// Values of keys that do not exist are zero (see clear_missing), in the V images of a tile in LDS
 __device__ __forceinline__ void clear_missing_images(char* v, int there, int wave) {
-  constexpr int kPieces = TileForm<WAVES>::kBytes / 2 / 16;
 #pragma unroll 1
-  for (int n = wave; n < kPieces / 64; n += WAVES) {                      // images: of a half 8
-    const int lane = lane_here(), i = n * 64 + lane, half = n >> 3, g = lane >> 4;
-    i32x4 piece[1] = {*(const i32x4*)(v + i * 16)};
-    clear_missing<false>(piece, there - 32 * half, g);
-    *(i32x4*)(v + i * 16) = piece[0];
+  for (int n = wave; n < 16; n += kTileWaves) {                           // images: of a half 8
+    const int lane = lane_here(), half = n >> 3;
+    char* at = v + (n * 64 + lane) * 16;
+    i32x4 piece[1] = {*(const i32x4*)at};
+    clear_missing<false>(piece, there - 32 * half, lane >> 4);
+    *(i32x4*)at = piece[0];
   }
 }
 
-template <bool FP8, int WAVES, bool FOLD>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_kernel(PagedParams p) {
-  using F = TileForm<WAVES>;
-  constexpr int RB = 32 * WAVES, kStep = F::kStep, NKB = kStep / 16, kPerTile = kTileKeys / kStep;
-  constexpr int kRecord = FP8 ? kPageRecord8 : kPageRecord16;
-  constexpr int kCopy = FP8 ? F::kRaw : F::kBytes;                        // bytes of a step as they come, half of them K
-  constexpr int kSlotBytes = FP8 ? F::kRawSlot : F::kBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[F::template lds_bytes<FP8>()];
+template <bool FP8, bool FOLD>
+__global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedParams p) {
+  constexpr int RB = kTileRows, kRecord = FP8 ? kPageRecord8 : kPageRecord16;   // (a record is what a tile takes in the ring that pages are copied to)
+  constexpr int kPieces = kRecord / 1024;                                 // whole KiB of it
+  __shared__ __attribute__((aligned(1024))) char lds[tile_lds_bytes<FP8>()];
+  static_assert((kMaxSequences + 1) * sizeof(int64_t) <= sizeof(lds), "the sums");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   int64_t* cum = (int64_t*)lds;
@@ -733,45 +717,51 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
     at.t = 0;
     if (!next_unit(p, at, s, blocks, RB, left)) return;
   }
-  char* copies = lds + (FP8 ? 2 * F::kBytes : 0);                         // the ring that pages are copied to
+  char* copies = lds + (FP8 ? 2 * kImageBytes : 0);                       // the ring that pages are copied to
   // 4 KiB of the wave's own, for queries on their way in and outputs on their way out, that no copy ahead of the loop goes to
-  char* turn = lds + (FP8 ? 0 : 2 * F::kBytes) + wave * 4096;
-  static_assert(2 * F::kBytes >= WAVES * 4096, "the images' place");
+  char* turn = lds + (FP8 ? 0 : 2 * kImageBytes) + wave * 4096;
 
-  // The copies of a unit's steps.  (What they need of the unit is uniform; `end`: the step behind the last of this run.)
-  auto page = [&](int step, int end) { return uniform_page(p, at.b, min(step, end - 1) / kPerTile); };
-  auto copy = [&](int id, int step, int slot) {
+  // Pages of the tiles [64*n, 64*n + 64) of the sequence, one a lane.  (A scalar load in every step would have every wait for an LDS read behind it wait for
+  // all of them: the two come back in no order.)
+  int ids, ids_of = -1, ids_from = 0;
+  auto ask_pages = [&](int tile) {
+    ids_of = at.b, ids_from = tile & ~63;
+    const int t = ids_from + lane_here();
+    ids = t < p.table_pages ? page_in_pool(p.table[(int64_t)at.b * p.table_stride + t], p.n_pages) : -1;
+  };
+  auto page = [&](int tile) { return __builtin_amdgcn_readlane(ids, tile & 63); };
+  auto copy = [&](int id, int slot) {
     const char* record = p.pages + (int64_t)max(id, 0) * p.page_stride + (int64_t)at.h * kRecord;
-    const char* r = record + (kPerTile == 2 ? (step & 1) * (kCopy / 2) : 0);
     const unsigned lane_off = lane_here() * 16;
-    char* d = copies + slot * kSlotBytes;
-    constexpr int kPieces = kCopy / 1024;
+    char* d = copies + slot * kRecord;
 #pragma unroll
-    for (int n = 0; n < (kPieces + WAVES - 1) / WAVES; ++n) {
-      const int piece = n * WAVES + wave;
-      // a step's K, then its V: of half a page the two do not lie side by side
-      const char* g = r + piece * 1024 + (kPerTile == 2 && piece >= kPieces / 2 ? kCopy / 2 : 0);
-      if ((n + 1) * WAVES <= kPieces || piece < kPieces) lds_dma16(g, lane_off, d + piece * 1024);
+    for (int n = 0; n < (kPieces + kTileWaves - 1) / kTileWaves; ++n) {
+      const int piece = n * kTileWaves + wave;
+      if ((n + 1) * kTileWaves <= kPieces || piece < kPieces) lds_dma16(record + piece * 1024, lane_off, d + piece * 1024);
     }
     if constexpr (FP8) {
-      if (wave == WAVES - 1 && lane_off < kPageScales) lds_dma16(record + kRecord - kPageScales, lane_off, d + F::kRaw);
+      if (wave == kTileWaves - 1 && lane_off < kPageScales) lds_dma16(record + kPieces * 1024, lane_off, d + kPieces * 1024);
     }
   };
-  int id[3];                                                              // pages of this step, the next and the one after it
-  int nt, take, first, end;
+  int id[3];                                                              // pages of this tile, the next and the one after it
+  int nt, take, first, end;                                               // of the unit: its tiles, those of this run, [first, end)
   Rows16 ahead[2];
   auto begin_unit = [&]() {                                               // asks for everything the unit's loop begins with
     nt = block_tiles(p, s, RB, at.j);
     const int cost = block_cost(p, s, RB, at.j);
     take = tiles_left(left, at.t, nt, cost);
     left -= (int64_t)(take + (at.t == 0 ? kUnitTiles : 0)) * cost;
-    first = at.t * kPerTile, end = (at.t + take) * kPerTile;              // steps
+    first = at.t, end = at.t + take;
+    if (at.b != ids_of || (first & ~63) != ids_from) ask_pages(first);    // (mostly those of the unit before)
 #pragma unroll
-    for (int i = 0; i < 3; ++i) id[i] = page(first + i, end);
-    copy(id[0], first, 0);
-    copy(id[1], min(first + 1, end - 1), 1);
+    for (int i = 0; i < 3; ++i) {
+      if (i > 0 && ((first + i) & 63) == 0) ask_pages(first + i);
+      id[i] = page(first + i);                                            // (past the end: a page, or none, that is not used)
+    }
+    copy(id[0], 0);
+    copy(id[take > 1 ? 1 : 0], 1);                                        // (of a single tile: once more)
   };
-  auto ask = [&](int qb) { ask_queries(p, s, at.h, at.j * RB + 32 * wave + 16 * qb, ahead[qb], lane_here()); };
+  auto ask = [&](int qb) { ask_queries(arguments_here(), s, at.h, at.j * RB + 32 * wave + 16 * qb, ahead[qb], lane_here()); };
   __syncthreads();                                                        // the sums are read
   begin_unit();
   ask(0), ask(1);
@@ -783,7 +773,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
     WaveState<false> w;
     if (!idle) {
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) queries_ready(p, s, r0 + 16 * qb, ahead[qb], turn, lane_here(), FOLD ? p.c : 1.0f, w.qf[qb]);
+      for (int qb = 0; qb < 2; ++qb) queries_ready(arguments_here(), s, r0 + 16 * qb, ahead[qb], turn, lane_here(), FOLD ? p.c : 1.0f, w.qf[qb]);
     }
     const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
 #pragma unroll
@@ -793,55 +783,56 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) w.l[qb] = 0.f;
     Running<FOLD> run;
-    run.start();
+    run.set(0, 0.f), run.set(1, 0.f);
 
     int slot = 0, slot_prev = 2;
     if constexpr (FP8) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      expand_step<WAVES>(copies, lds, first & 1, wave, lane_here());
+      expand_tile(copies, lds, wave, lane_here());
     }
-    // One step.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
+    // One tile.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
     auto step = [&](int i, auto masked, auto works) {
       constexpr bool MASKED = decltype(masked)::value, WORKS = decltype(works)::value;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      char* images = lds + slot * F::kBytes;
+      char* images = lds + slot * kImageBytes;
       int there = 0;
       if constexpr (MASKED) {
-        there = id[0] < 0 ? 0 : s.keys - kStep * i;
-        if (there < kStep) {
-          clear_missing_images<WAVES>(images + F::kBytes / 2, there, wave);
+        there = id[0] < 0 ? 0 : s.keys - kTileKeys * i;
+        if (there < kTileKeys) {
+          clear_missing_images(images + kKTileBytes, there, wave);
           __syncthreads();
         }
       }
       if constexpr (WORKS) {
-        tile_qk<NKB, MASKED ? 2 : FOLD ? 3 : 4, FOLD>(w, run, images, lane_here());
+        tile_qk<MASKED || FOLD ? 3 : 4, FOLD>(w, run, images, lane_here());
       }
       if constexpr (!FP8) {
-        if (i + 2 < end) copy(id[2], i + 2, slot_prev);
+        if (i + 2 < end) copy(id[2], slot_prev);
         slot_prev = slot;
         slot = slot == 2 ? 0 : slot + 1;
       } else {
-        if (i + 2 < end) copy(id[2], i + 2, slot);
-        if (i + 1 < end) expand_step<WAVES>(copies + (slot ^ 1) * kSlotBytes, lds + (slot ^ 1) * F::kBytes, (i + 1) & 1, wave, lane_here());
+        if (i + 2 < end) copy(id[2], slot);
+        if (i + 1 < end) expand_tile(copies + (slot ^ 1) * kRecord, lds + (slot ^ 1) * kImageBytes, wave, lane_here());
         slot ^= 1;
       }
-      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3, end);
+      if (((i + 3) & 63) == 0) ask_pages(i + 3);
+      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3);
       if constexpr (WORKS) {
         int lim[2] = {};                                                  // (made here: kept from step to step, it does not fit the registers)
         if constexpr (MASKED) {
 #pragma unroll
-          for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kStep * i);
+          for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kTileKeys * i);
         }
-        bf16x8 pf[NKB / 2][2];
-        tile_softmax<NKB, MASKED, FOLD>(w, run, pf, p.c, lim, lane_here());
-        tile_pv<NKB>(w, pf, images + F::kBytes / 2, lane_here());
+        bf16x8 pf[2][2];
+        tile_softmax<MASKED, FOLD>(w, run, pf, p.c, lim, lane_here());
+        tile_pv(w, pf, images + kKTileBytes, lane_here());
       }
     };
-    // Whether a step is masked differs from wave to wave, how many barriers it has does not: a step with keys that do not exist, or a page that does not,
+    // Whether a tile is masked differs from wave to wave, how many barriers it has does not: a tile with keys that do not exist, or a page that does not,
     // is masked for all.
-    const int whole = min(all_see / kStep, end);                         // steps in front of this one are seen whole by all rows
+    const int whole = min(all_see / kTileKeys, end);                     // tiles in front of this one are seen whole by all rows
     int i = first;
     if (idle) {
 #pragma unroll 1
@@ -864,13 +855,13 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
     at.t = 0;
     const bool more = next_unit(p, at, s, blocks, RB, left);
     if (more) begin_unit();
-    float* part = p.partials + part_slot(rank, begins) * part_floats(RB);
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       ask(qb);                                                            // (without a next unit: rows of this one, which nobody takes)
       asm volatile("" ::: "memory");                                      // (one block after the other: both at once do not fit the registers)
       if (!idle) {
         const int out_lane = lane_here(), c16 = out_lane & 15, g4 = out_lane >> 4;
+        const PagedParams args = arguments_here();
         const float l = wave_sum_groups(w.l[qb]);
         if (finished) {
           const float inv = inverse_sum(l);
@@ -886,15 +877,16 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? 3 : 1) void paged_tile_ker
             const int row = 4 * n + g4, r = r0 + 16 * qb + row;
             const bf16x8 v = *(const bf16x8*)(turn + row * 256 + ((c16 ^ row) * 16));
             int token;
-            const int64_t to = row_offset(p, out_s, out_h, min(r, last), p.o_ss, p.o_sh, token);
-            if (r <= last) *(bf16x8*)(p.o + to + c16 * 16) = v;
+            const int64_t to = row_offset(args, out_s, out_h, min(r, last), args.o_ss, args.o_sh, token);
+            if (r <= last) *(bf16x8*)(args.o + to + c16 * 16) = v;
           }
         } else {
+          float* part = args.partials + part_slot(rank, begins) * part_floats(RB);
           const int row = 32 * wave + 16 * qb + c16;
           if (r0 + 16 * qb + c16 <= last) {
 #pragma unroll
             for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
-            if (g4 == 0) part[RB * kD + row] = l == 0.f ? kNoMax : run.of(qb), part[RB * (kD + 1) + row] = l;
+            if (g4 == 0) part[RB * kD + row] = l == 0.f ? kNoMax : -run.negative(qb), part[RB * (kD + 1) + row] = l;
           }
         }
       }
@@ -970,19 +962,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
 // ---- host ----
 
 // The form of a call, from what the host knows of it: the query rows of a (sequence, kv head) on the average.
-enum PagedForm { kSplit16, kSplit32, kTile128, kTile384 };
+enum PagedForm { kSplit16, kSplit32, kTile };
 static PagedForm form_of(int rows, int B, int G) {
   const int64_t per = (int64_t)rows * G / std::max(1, std::min(rows, B));
-  return per <= 16 ? kSplit16 : per <= 48 ? kSplit32 : per <= 256 ? kTile128 : kTile384;
+  return per <= 16 ? kSplit16 : per <= 32 ? kSplit32 : kTile;
 }
-static int rows_of(PagedForm f) { return f == kSplit16 ? 16 : f == kSplit32 ? 32 : f == kTile128 ? 128 : 384; }
-static int most_workgroups(PagedForm f) { return f == kTile384 ? kMaxShares / 3 : f == kTile128 ? kMaxShares : kMaxShares / 3 * 2; }
-static int workgroups_of(PagedForm f, int cus) {
-  const int per_cu = f == kTile384 ? 1 : f == kTile128 ? 3 : 2;
-  return std::min(most_workgroups(f), std::max(8, per_cu * cus / 8 * 8));
-}
+static int rows_of(PagedForm f) { return f == kSplit16 ? 16 : f == kSplit32 ? 32 : kTileRows; }
+static int most_workgroups(PagedForm f) { return f == kTile ? kMaxShares / 2 : kMaxShares; }
+static int workgroups_of(PagedForm f, int cus) { return std::min(most_workgroups(f), std::max(8, (f == kTile ? 1 : 2) * cus / 8 * 8)); }
 
-size_t paged_attn_scratch(int rows, int B, int H, int G, int table_pages) {
+size_t paged_attn_scratch(int rows, int B, int G) {
   const PagedForm f = form_of(rows, B, G);
   return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f)) + kCutFloats;
 }
@@ -996,13 +985,6 @@ static hipError_t launch_form(Kernel kernel, int threads, int grid, const PagedP
   return hipGetLastError();
 }
 
-template <int WAVES>
-static hipError_t launch_tile(bool fp8, bool fold, int grid, const PagedParams& p, hipStream_t st) {
-  auto* kernel = fp8 ? (fold ? paged_tile_kernel<true, WAVES, true> : paged_tile_kernel<true, WAVES, false>)
-                     : (fold ? paged_tile_kernel<false, WAVES, true> : paged_tile_kernel<false, WAVES, false>);
-  return launch_form<32 * WAVES>(kernel, 64 * WAVES, grid, p, st);
-}
-
 hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
@@ -1013,8 +995,8 @@ hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   switch (f) {
     case kSplit16: return launch_form<16>(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 256, grid, p, st);
     case kSplit32: return launch_form<32>(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 256, grid, p, st);
-    case kTile128: return launch_tile<4>(fp8, fold, grid, p, st);
-    default: return launch_tile<12>(fp8, fold, grid, p, st);
+    default: return launch_form<kTileRows>(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
+                                               : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>), 64 * kTileWaves, grid, p, st);
   }
 }
 

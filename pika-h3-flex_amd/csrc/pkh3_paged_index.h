@@ -75,7 +75,7 @@ constexpr int tiles_left(int64_t left, int t, int nt, int cost) {
 }
 
 // The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
-constexpr int kMaxShares = 768;       // workgroups of a launch at most
+constexpr int kMaxShares = 512;       // workgroups of a launch at most
 constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
 constexpr int kWholeTiles = 16;       // a unit of at most so many, and no dearer than a run, is not cut
 struct Shares {

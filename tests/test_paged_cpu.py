@@ -220,7 +220,7 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     _run(tmp_path, """
   for (int go = 0; go < 6000; ++go) {
     const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 5 <= 1 ? 384 : go % 5 == 2 ? 128 : go % 5 == 3 ? 32 : 16;
-    const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 768;
+    const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 512;
     struct Unit { int64_t begin; int nt, cost; };
     std::vector<Unit> units;
     int64_t total = 0;
