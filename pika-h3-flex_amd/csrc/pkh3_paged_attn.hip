@@ -128,11 +128,12 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t*
 
 // The run of this workgroup: which one, what it costs, the unit and tile it begins at.  False: none.  Leaves what the second launch has to know of the
 // run's beginning.
-__device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int rb, int& rank, int64_t& left, Place& at) {
+__device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int rb, int& rank, int64_t& left, Place& at, int64_t& run) {
   const Shares sh = shares_of(cum[p.B], gridDim.x, rb);
   rank = rank_of(blockIdx.x, sh);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.cuts[0] = i32x4{sh.n, 0, 0, 0};
   if (rank < 0 || sh.total == 0) return false;
+  run = uniform64(sh.run());
   at = find_place(p, cum, rb, sh, sh.begin(rank));
   left = (rank + 1 < sh.n ? find_place(p, cum, rb, sh, sh.begin(rank + 1)).pos : uniform64(sh.total)) - at.pos;
   const Sequence s = uniform_sequence(p, at.b);
@@ -160,7 +161,7 @@ __device__ __forceinline__ bool next_unit(const PagedParams& p, Place& at, Seque
 // 1 / l; rows without a key: 0.  (A sum that is not a number stays one.)
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
-// A part of a unit in the scratch: RB rows of 128, then their maxima, then their sums
+// A part of a unit in the scratch: RB rows of 128 (in the tile form blocks of 16 rows, as the lanes hold them), then the rows' maxima, then their sums
 constexpr int kCutFloats = 4 * kMaxShares;   // of the records in front of the parts
 __host__ __device__ constexpr int part_floats(int rb) { return rb * (kD + 2); }
 
@@ -299,9 +300,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
   int64_t* cum = (int64_t*)part;
   sum_tiles(p, cum, RB);
   int rank;
-  int64_t left;
+  int64_t left, run;
   Place at;
-  if (!find_run(p, cum, RB, rank, left, at)) return;
+  if (!find_run(p, cum, RB, rank, left, at, run)) return;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
@@ -708,9 +709,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
   int64_t* cum = (int64_t*)lds;
   sum_tiles(p, cum, RB);
   int rank;
-  int64_t left;
+  int64_t left, run;
   Place at;
-  if (!find_run(p, cum, RB, rank, left, at)) return;
+  if (!find_run(p, cum, RB, rank, left, at, run)) return;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
@@ -723,13 +724,15 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
 
   // Pages of the tiles [64*n, 64*n + 64) of the sequence, one a lane.  (A scalar load in every step would have every wait for an LDS read behind it wait for
   // all of them: the two come back in no order.)
-  int ids, ids_of = -1, ids_from = 0;
-  auto ask_pages = [&](int tile) {
-    ids_of = at.b, ids_from = tile & ~63;
-    const int t = ids_from + lane_here();
-    ids = t < p.table_pages ? page_in_pool(p.table[(int64_t)at.b * p.table_stride + t], p.n_pages) : -1;
+  int ids, ids_of = -1, ids_from = -1;
+  auto page = [&](int tile) {
+    if ((tile & ~63) != ids_from) {
+      ids_of = at.b, ids_from = tile & ~63;
+      const int t = ids_from + lane_here();
+      ids = t < p.table_pages ? page_in_pool(p.table[(int64_t)at.b * p.table_stride + t], p.n_pages) : -1;
+    }
+    return __builtin_amdgcn_readlane(ids, tile & 63);
   };
-  auto page = [&](int tile) { return __builtin_amdgcn_readlane(ids, tile & 63); };
   auto copy = [&](int id, int slot) {
     const char* record = p.pages + (int64_t)max(id, 0) * p.page_stride + (int64_t)at.h * kRecord;
     const unsigned lane_off = lane_here() * 16;
@@ -743,21 +746,59 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
       if (wave == kTileWaves - 1 && lane_off < kPageScales) lds_dma16(record + kPieces * 1024, lane_off, d + kPieces * 1024);
     }
   };
+  // Workgroups that walk the same keys at the same time find them in their L2.  So they start where their neighbours are: with R tiles a run, every run inside a
+  // unit begins at the multiple of R in it and goes on from its own first tile when it is through; a run over the end of one unit does the beginning of
+  // the next first.  At any time all of a head are then at one of a few places, R apart, whatever block of rows they have.
+  struct {
+    int b, h, j, t;
+    int64_t left;
+  } later = {-1, 0, 0, 0, 0};                                             // the end of a unit that is done after the beginning of the next
+  if (at.t > 0) {
+    const int nt = block_tiles(p, s, RB, at.j), cost = block_cost(p, s, RB, at.j);
+    const int64_t behind = left - (int64_t)(nt - at.t) * cost;
+    Place next = at;
+    Sequence next_s = s;
+    int next_blocks = blocks;
+    next.t = 0;
+    if (next_unit(p, next, next_s, next_blocks, RB, behind)) {
+      const int next_nt = block_tiles(p, next_s, RB, next.j);
+      if (tiles_left(behind, 0, next_nt, block_cost(p, next_s, RB, next.j)) < next_nt) {
+        later = {at.b, at.h, at.j, at.t, left - behind};
+        at = next, s = next_s, blocks = next_blocks, left = behind;
+      }
+    }
+  }
+  auto advance = [&]() {
+    if (next_unit(p, at, s, blocks, RB, left)) return true;
+    if (later.b < 0) return false;
+    at.b = later.b, at.h = later.h, at.j = later.j, at.t = later.t, left = later.left;
+    s = uniform_sequence(p, at.b);
+    blocks = blocks_of(p, s, RB);
+    later.b = -1;
+    return true;
+  };
+
   int id[3];                                                              // pages of this tile, the next and the one after it
-  int nt, take, first, end;                                               // of the unit: its tiles, those of this run, [first, end)
+  int nt, take, first, start;                                             // of the unit: its tiles, those of this run, its first one and where it starts
+  auto tile_at = [&](int n) {                                             // the run's n-th tile
+    const int i = start + n;
+    return i < first + take ? i : i - take;
+  };
   Rows16 ahead[2];
   auto begin_unit = [&]() {                                               // asks for everything the unit's loop begins with
     nt = block_tiles(p, s, RB, at.j);
     const int cost = block_cost(p, s, RB, at.j);
     take = tiles_left(left, at.t, nt, cost);
     left -= (int64_t)(take + (at.t == 0 ? kUnitTiles : 0)) * cost;
-    first = at.t, end = at.t + take;
-    if (at.b != ids_of || (first & ~63) != ids_from) ask_pages(first);    // (mostly those of the unit before)
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      if (i > 0 && ((first + i) & 63) == 0) ask_pages(first + i);
-      id[i] = page(first + i);                                            // (past the end: a page, or none, that is not used)
+    first = start = at.t;
+    if (first > 0 && first + take < nt) {
+      const int apart = max((int)divided(run, cost), 1);
+      const int place = (first + apart - 1) / apart * apart;
+      start = __builtin_amdgcn_readfirstlane(place < first + take ? place : first);
     }
+    if (at.b != ids_of) ids_from = -1;                                    // (mostly those of the unit before)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) id[i] = page(tile_at(i));                 // (past the end: a page, or none, that is not used)
     copy(id[0], 0);
     copy(id[take > 1 ? 1 : 0], 1);                                        // (of a single tile: once more)
   };
@@ -782,8 +823,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
       for (int qb = 0; qb < 2; ++qb) w.o[db][qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) w.l[qb] = 0.f;
-    Running<FOLD> run;
-    run.set(0, 0.f), run.set(1, 0.f);
+    Running<FOLD> run_max;
+    run_max.set(0, 0.f), run_max.set(1, 0.f);
 
     int slot = 0, slot_prev = 2;
     if constexpr (FP8) {
@@ -792,7 +833,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
       expand_tile(copies, lds, wave, lane_here());
     }
     // One tile.  MASKED: some rows of the wave do not see all of its keys, or its page is not there.
-    auto step = [&](int i, auto masked, auto works) {
+    auto step = [&](int n, int i, auto masked, auto works) {
       constexpr bool MASKED = decltype(masked)::value, WORKS = decltype(works)::value;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
@@ -806,19 +847,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
         }
       }
       if constexpr (WORKS) {
-        tile_qk<MASKED || FOLD ? 3 : 4, FOLD>(w, run, images, lane_here());
+        tile_qk<MASKED || FOLD ? 3 : 4, FOLD>(w, run_max, images, lane_here());
       }
       if constexpr (!FP8) {
-        if (i + 2 < end) copy(id[2], slot_prev);
+        if (n + 2 < take) copy(id[2], slot_prev);
         slot_prev = slot;
         slot = slot == 2 ? 0 : slot + 1;
       } else {
-        if (i + 2 < end) copy(id[2], slot);
-        if (i + 1 < end) expand_tile(copies + (slot ^ 1) * kRecord, lds + (slot ^ 1) * kImageBytes, wave, lane_here());
+        if (n + 2 < take) copy(id[2], slot);
+        if (n + 1 < take) expand_tile(copies + (slot ^ 1) * kRecord, lds + (slot ^ 1) * kImageBytes, wave, lane_here());
         slot ^= 1;
       }
-      if (((i + 3) & 63) == 0) ask_pages(i + 3);
-      id[0] = id[1], id[1] = id[2], id[2] = page(i + 3);
+      id[0] = id[1], id[1] = id[2], id[2] = page(tile_at(n + 3));
       if constexpr (WORKS) {
         int lim[2] = {};                                                  // (made here: kept from step to step, it does not fit the registers)
         if constexpr (MASKED) {
@@ -826,24 +866,33 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
           for (int qb = 0; qb < 2; ++qb) lim[qb] = min(there, row_keys(p, s, r0 + 16 * qb + (lane_here() & 15)) - kTileKeys * i);
         }
         bf16x8 pf[2][2];
-        tile_softmax<MASKED, FOLD>(w, run, pf, p.c, lim, lane_here());
+        tile_softmax<MASKED, FOLD>(w, run_max, pf, p.c, lim, lane_here());
         tile_pv(w, pf, images + kKTileBytes, lane_here());
       }
     };
     // Whether a tile is masked differs from wave to wave, how many barriers it has does not: a tile with keys that do not exist, or a page that does not,
     // is masked for all.
-    const int whole = min(all_see / kTileKeys, end);                     // tiles in front of this one are seen whole by all rows
-    int i = first;
+    const int whole = all_see / kTileKeys;                               // tiles in front of this one are seen whole by all rows
+    int n = 0, i = start;
     if (idle) {
 #pragma unroll 1
-      for (; i < end; ++i) step(i, std::true_type{}, std::false_type{});
+      for (; n < take; i = tile_at(++n)) step(n, i, std::true_type{}, std::false_type{});
     }
+    bool plain = i < whole && id[0] >= 0;
 #pragma unroll 1
-    while (i < end) {
+    while (n < take) {
 #pragma unroll 1
-      for (; i < whole && id[0] >= 0; ++i) step(i, std::false_type{}, std::true_type{});
+      while (plain) {
+        step(n, i, std::false_type{}, std::true_type{});
+        i = tile_at(++n);
+        plain = n < take && i < whole && id[0] >= 0;
+      }
 #pragma unroll 1
-      for (; i < end && (i >= whole || id[0] < 0); ++i) step(i, std::true_type{}, std::true_type{});
+      while (n < take && !plain) {
+        step(n, i, std::true_type{}, std::true_type{});
+        i = tile_at(++n);
+        plain = n < take && i < whole && id[0] >= 0;
+      }
     }
     PKH3_MFMA_DRAIN(w);
 
@@ -853,7 +902,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
     const int out_h = at.h;
     const bool finished = at.t == 0 && take == nt, begins = at.t == 0;
     at.t = 0;
-    const bool more = next_unit(p, at, s, blocks, RB, left);
+    const bool more = advance();
     if (more) begin_unit();
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -881,12 +930,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
             if (r <= last) *(bf16x8*)(args.o + to + c16 * 16) = v;
           }
         } else {
+          // as the lanes hold it, whole KiB a store: by rows, 64 bytes of 16 of them a store, a workgroup's part took 12 us
           float* part = args.partials + part_slot(rank, begins) * part_floats(RB);
-          const int row = 32 * wave + 16 * qb + c16;
+          float* to = part + (2 * wave + qb) * (16 * kD) + out_lane * 4;
           if (r0 + 16 * qb + c16 <= last) {
 #pragma unroll
-            for (int db = 0; db < 8; ++db) *(f32x4*)(part + row * kD + 16 * db + 4 * g4) = w.o[db][qb];
-            if (g4 == 0) part[RB * kD + row] = l == 0.f ? kNoMax : -run.negative(qb), part[RB * (kD + 1) + row] = l;
+            for (int db = 0; db < 8; ++db) *(f32x4*)(to + db * 256) = w.o[db][qb];
+            const int row = 32 * wave + 16 * qb + c16;
+            if (g4 == 0) part[RB * kD + row] = l == 0.f ? kNoMax : -run_max.negative(qb), part[RB * (kD + 1) + row] = l;
           }
         }
       }
@@ -959,6 +1010,55 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   *(bf16x4*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row, p.o_ss, p.o_sh, token) + col * 2) = out;
 }
 
+// The same for the tile form, whose parts lie as its lanes hold them: blockIdx.y is a block of 16 rows, thread t has the columns 16*db + 4*g .. +3 of row c
+// (t % 64 = 16*g + c) for two db, and the rows go out by way of LDS.
+__global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
+  constexpr int RB = kTileRows;
+  __shared__ __attribute__((aligned(16))) char turn[4096];
+  const int run = (int)blockIdx.x + 1;
+  const i32x4 cut = p.cuts[run];
+  if (run >= p.cuts[0][0] || cut[3] == 0) return;
+  const Sequence s = uniform_sequence(p, cut[0]);
+  const int rows = min(RB, s.n * p.G - cut[2] * RB), row0 = (int)blockIdx.y * 16;
+  if (row0 >= rows) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+  const int row = min(row0 + c, rows - 1);                       // (rows that are not there: another's maximum and sum, and nothing is stored)
+  auto slot = [&](int i) { return p.partials + part_slot(run - 1 + i, i == 0) * part_floats(RB); };
+  float top = kNoMax, l = 0.f;
+  for (int i = 0; i < cut[3]; ++i) top = fmaxf(top, slot(i)[RB * kD + row]);
+  f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  const bool live = row0 + c < rows;
+#pragma unroll 2
+  for (int i = 0; i < cut[3]; ++i) {
+    const float* t = slot(i);
+    const float a = __builtin_amdgcn_exp2f(t[RB * kD + row] - top);
+    l += a * t[RB * (kD + 1) + row];
+    if (live) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 o = *(const f32x4*)(t + row0 * kD + (2 * wave + e) * 256 + lane * 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[e][k] += a * o[k];
+      }
+    }
+  }
+  const float inv = inverse_sum(l);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    bf16x4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (__bf16)(sum[e][k] * inv);
+    const int db = 2 * wave + e;
+    *(bf16x4*)(turn + c * 256 + (((2 * db + (g >> 1)) ^ c) * 16) + 8 * (g & 1)) = v;
+  }
+  __syncthreads();
+  const int out = threadIdx.x >> 4, chunk = threadIdx.x & 15;
+  if (row0 + out >= rows) return;
+  int token;
+  *(bf16x8*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row0 + out, p.o_ss, p.o_sh, token) + chunk * 16) =
+      *(const bf16x8*)(turn + out * 256 + ((chunk ^ out) * 16));
+}
+
 // ---- host ----
 
 // The form of a call, from what the host knows of it: the query rows of a (sequence, kv head) on the average.
@@ -976,12 +1076,12 @@ size_t paged_attn_scratch(int rows, int B, int G) {
   return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f)) + kCutFloats;
 }
 
-template <int RB, class Kernel>
-static hipError_t launch_form(Kernel kernel, int threads, int grid, const PagedParams& p, hipStream_t st) {
+template <class Kernel, class Merge>
+static hipError_t launch_form(Kernel kernel, int threads, Merge merge, int blocks, int grid, const PagedParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(paged_merge_kernel<RB>, dim3(grid - 1, RB / 8), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(merge, dim3(grid - 1, blocks), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
@@ -993,10 +1093,14 @@ hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   const int grid = workgroups_of(f, cus);
   const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {
-    case kSplit16: return launch_form<16>(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 256, grid, p, st);
-    case kSplit32: return launch_form<32>(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 256, grid, p, st);
-    default: return launch_form<kTileRows>(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
-                                               : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>), 64 * kTileWaves, grid, p, st);
+    case kSplit16:
+      return launch_form(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 64 * kSplitWaves, paged_merge_kernel<16>, 2, grid, p, st);
+    case kSplit32:
+      return launch_form(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 64 * kSplitWaves, paged_merge_kernel<32>, 4, grid, p, st);
+    default:
+      return launch_form(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
+                             : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>),
+                         64 * kTileWaves, paged_merge_tile_kernel, kTileRows / 16, grid, p, st);
   }
 }
 
