@@ -36,7 +36,7 @@ struct PagedParams {
   const float* cos_t;
   const float* sin_t;
   int heads_per_wg, groups;          // write, read
-  int G;                             // attn: query heads of one of the cache's
+  Group G;                           // attn: query heads of one of the cache's
   float c;                           // attn: softmax scale * log2(e)
   int causal;
   i32x4* cuts;                       // attn: where runs begin inside a unit, and ...
@@ -65,8 +65,7 @@ __device__ __forceinline__ void prefix_sums(int64_t* cum, int B) {
     for (int at = 0; at < B; at += 64) {
       const int b = at + lane;
       int64_t x = b < B ? cum[b + 1] : 0;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
+      for (int d = 1; d < 64 && d < B; d <<= 1) {
         const int64_t y = __shfl_up(x, d);
         if (lane >= d) x += y;
       }

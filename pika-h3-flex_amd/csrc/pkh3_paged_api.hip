@@ -147,7 +147,7 @@ int pkh3_paged_attn(const pkh3_paged_args* a, void* stream) {
   if (a->workspace_bytes < scratch(a)) return fail(PKH3_EWORKSPACE, "workspace too small: %zu < %zu bytes", a->workspace_bytes, scratch(a));
   if (a->rows == 0) return report_error(PKH3_OK, "");
   PagedParams p = params(a);
-  p.G = a->heads / a->kv_heads;
+  p.G = make_group(a->heads / a->kv_heads);
   p.c = (a->softmax_scale > 0.f ? a->softmax_scale : 1.0f / sqrtf((float)kD)) * kLog2e;
   p.cuts = (i32x4*)a->workspace;
   p.partials = (float*)a->workspace + 4 * kMaxShares;

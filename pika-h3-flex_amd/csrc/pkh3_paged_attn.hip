@@ -52,7 +52,7 @@ struct Place {
 // The sums of the tiles of all sequences in `cum`, by the whole workgroup.  Blocks of a causal sequence differ in length: where
 // there are more than a few, a wave adds them up together.
 __device__ __forceinline__ void sum_tiles(const PagedParams& p, int64_t* cum, int rb) {
-  constexpr int kAlone = 16;
+  constexpr int kAlone = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   for (int at = 64 * wave; at < p.B; at += 64 * waves) {
     const int b = at + lane;
@@ -126,21 +126,39 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t*
   return at;
 }
 
-// The run of this workgroup: which one, what it costs, the unit and tile it begins at.  False: none.  Leaves what the second launch has to know of the
-// run's beginning.
-__device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int rb, int& rank, int64_t& left, Place& at, int64_t& run) {
+// The run of this workgroup: which one, what it costs, the unit and tile it begins at, and how long runs are.  False: none.  The first wave finds its beginning, the
+// second its end, `found` (LDS) tells the others.  Leaves what the second launch has to know of the run's beginning.
+struct Run {
+  int rank;
+  int64_t left, length;
+};
+__device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int64_t* found, int rb, Run& run, Place& at) {
   const Shares sh = shares_of(cum[p.B], gridDim.x, rb);
-  rank = rank_of(blockIdx.x, sh);
+  run.rank = rank_of(blockIdx.x, sh);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.cuts[0] = i32x4{sh.n, 0, 0, 0};
-  if (rank < 0 || sh.total == 0) return false;
-  run = uniform64(sh.run());
-  at = find_place(p, cum, rb, sh, sh.begin(rank));
-  left = (rank + 1 < sh.n ? find_place(p, cum, rb, sh, sh.begin(rank + 1)).pos : uniform64(sh.total)) - at.pos;
-  const Sequence s = uniform_sequence(p, at.b);
-  const int nt = block_tiles(p, s, rb, at.j);
-  if (rank > 0 && threadIdx.x == 0)
-    p.cuts[rank] = i32x4{at.b, at.h, at.j, parts_at(sh, rank, at.unit, at.t, nt, block_cost(p, s, rb, at.j))};
-  return left > 0;
+  if (run.rank < 0 || sh.total == 0) return false;
+  if (threadIdx.x < 64) {
+    const Place x = find_place(p, cum, rb, sh, sh.begin(run.rank));
+    if (threadIdx.x == 0) {
+      found[0] = (int64_t)(uint32_t)x.b << 32 | (uint32_t)x.h;
+      found[1] = (int64_t)(uint32_t)x.j << 32 | (uint32_t)x.t;
+      found[2] = x.pos;
+      if (run.rank > 0) {
+        const Sequence s = uniform_sequence(p, x.b);
+        const int nt = block_tiles(p, s, rb, x.j);
+        p.cuts[run.rank] = i32x4{x.b, x.h, x.j, parts_at(sh, run.rank, x.unit, x.t, nt, block_cost(p, s, rb, x.j))};
+      }
+    }
+  } else if (threadIdx.x < 128) {
+    const int64_t end = run.rank + 1 < sh.n ? find_place(p, cum, rb, sh, sh.begin(run.rank + 1)).pos : sh.total;
+    if (threadIdx.x == 64) found[3] = end;
+  }
+  run.length = uniform64(sh.run());
+  __syncthreads();
+  const int64_t bh = uniform64(found[0]), jt = uniform64(found[1]);
+  at.b = (int)(bh >> 32), at.h = (int)bh, at.j = (int)(jt >> 32), at.t = (int)jt;
+  run.left = uniform64(found[3] - found[2]);
+  return run.left > 0;
 }
 
 // On to the next unit of a run with `left` to go.  False where there is none.
@@ -238,30 +256,28 @@ __device__ __forceinline__ void clear_missing(i32x4 (&v)[N], int there, int g) {
 
 // The address of query row r of (sequence, kv head) in a [rows, heads, 128] tensor, and its token
 __device__ __forceinline__ int64_t row_offset(const PagedParams& p, const Sequence& s, int h, int r, int64_t ss, int64_t sh, int& token) {
-  token = (int)((unsigned)r / (unsigned)p.G);
-  return (int64_t)(s.first + token) * ss + (int64_t)(h * p.G + r - token * p.G) * sh;
+  token = p.G.token(r);
+  return (int64_t)(s.first + token) * ss + (int64_t)(h * p.G.n + r - token * p.G.n) * sh;
 }
 
 // Sixteen query rows from r0 on (those past the last are the last one again), as they lie in memory ..
 __device__ __forceinline__ void ask_queries(const PagedParams& p, const Sequence& s, int h, int r0, Rows16& q, int lane) {
-  const int last = s.n * p.G - 1;
+  const int last = s.n * p.G.n - 1;
   int token;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     q.v[i] = *(const i32x4*)(p.q + row_offset(p, s, h, min(r0 + 4 * i + (lane >> 4), last), p.q_ss, p.q_sh, token) + (lane & 15) * 16);
 }
 // .. and through norm and rotation, in the lane order of the B images, by way of 4 KiB of LDS of the wave's own
-__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, char* turn, int lane, float factor,
-                                              bf16x8 (&out)[4]) {
+__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, const NormLanes& norm, char* turn, int lane,
+                                              float factor, bf16x8 (&out)[4]) {
   Rows16 cos, sin;
-  NormLanes norm;
-  load_norm_lanes(norm, p.norm_w, lane);
   RopeQuarter rope;
   if (p.rope_mode != 0) {
-    const int last = s.n * p.G - 1;
+    const int last = s.n * p.G.n - 1;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int token = (int)((unsigned)min(r0 + 4 * i + (lane >> 4), last) / (unsigned)p.G);
+      const int token = p.G.token(min(r0 + 4 * i + (lane >> 4), last));
       const int64_t at = (int64_t)(s.first + token) * (kD / 2 * (int)sizeof(float)) + (lane & 15) * 16;
       cos.v[i] = *(const i32x4*)((const char*)p.cos_t + at);
       sin.v[i] = *(const i32x4*)((const char*)p.sin_t + at);
@@ -299,10 +315,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 
   int64_t* cum = (int64_t*)part;
   sum_tiles(p, cum, RB);
-  int rank;
-  int64_t left, run;
+  __shared__ int64_t found[4];
+  Run run;
   Place at;
-  if (!find_run(p, cum, RB, rank, left, at, run)) return;
+  if (!find_run(p, cum, found, RB, run, at)) return;
+  int64_t left = run.left;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
@@ -319,7 +336,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
       bf16x8 img[4];
       Rows16 q;
       ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
-      queries_ready(p, s, at.j * RB + 16 * wave, q, part + wave * 4096, lane, 1.0f, img);
+      NormLanes norm;
+      load_norm_lanes(norm, p.norm_w, lane);
+      queries_ready(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, img);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
     }
@@ -445,12 +464,12 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
     }
     __syncthreads();
     const bool finished = at.t == 0 && take == nt;
-    float* slot = p.partials + part_slot(rank, at.t == 0) * part_floats(RB);
+    float* slot = p.partials + part_slot(run.rank, at.t == 0) * part_floats(RB);
     const int row = threadIdx.x >> 4, chunk = threadIdx.x & 15;   // 8 columns of one of 16 rows
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int r = at.j * RB + 16 * qb + row;
-      if (r >= s.n * p.G) continue;
+      if (r >= s.n * p.G.n) continue;
       float top = kNoMax, l = 0.f, a[NW];
 #pragma unroll
       for (int j = 0; j < NW; ++j) top = fmaxf(top, part_m[j][qb][row]);
@@ -703,15 +722,17 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
   constexpr int RB = kTileRows, kRecord = FP8 ? kPageRecord8 : kPageRecord16;   // (a record is what a tile takes in the ring that pages are copied to)
   constexpr int kPieces = kRecord / 1024;                                 // whole KiB of it
   __shared__ __attribute__((aligned(1024))) char lds[tile_lds_bytes<FP8>()];
+  __shared__ float norm_w[kD];                                            // from here a unit has them at once
   static_assert((kMaxSequences + 1) * sizeof(int64_t) <= sizeof(lds), "the sums");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   int64_t* cum = (int64_t*)lds;
   sum_tiles(p, cum, RB);
-  int rank;
-  int64_t left, run;
+  __shared__ int64_t found[4];
+  Run run;
   Place at;
-  if (!find_run(p, cum, RB, rank, left, at, run)) return;
+  if (!find_run(p, cum, found, RB, run, at)) return;
+  int64_t left = run.left;
   Sequence s = uniform_sequence(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
@@ -792,7 +813,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
     left -= (int64_t)(take + (at.t == 0 ? kUnitTiles : 0)) * cost;
     first = start = at.t;
     if (first > 0 && first + take < nt) {
-      const int apart = max((int)divided(run, cost), 1);
+      const int apart = max((int)divided(run.length, cost), 1);
       const int place = (first + apart - 1) / apart * apart;
       start = __builtin_amdgcn_readfirstlane(place < first + take ? place : first);
     }
@@ -803,18 +824,24 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
     copy(id[take > 1 ? 1 : 0], 1);                                        // (of a single tile: once more)
   };
   auto ask = [&](int qb) { ask_queries(arguments_here(), s, at.h, at.j * RB + 32 * wave + 16 * qb, ahead[qb], lane_here()); };
+  if (threadIdx.x < kD) norm_w[threadIdx.x] = p.norm_w ? p.norm_w[threadIdx.x] : 1.0f;
   __syncthreads();                                                        // the sums are read
   begin_unit();
   ask(0), ask(1);
 #pragma unroll 1
   for (;;) {
     // what is made of the lane's number is made where it is used: kept from unit to unit, or from the queries to the output, it does not fit the registers
-    const int r0 = at.j * RB + 32 * wave, last = s.n * p.G - 1;
+    const int r0 = at.j * RB + 32 * wave, last = s.n * p.G.n - 1;
     const bool idle = r0 > last;                                          // a wave without rows: copies and barriers alone
     WaveState<false> w;
     if (!idle) {
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) queries_ready(arguments_here(), s, r0 + 16 * qb, ahead[qb], turn, lane_here(), FOLD ? p.c : 1.0f, w.qf[qb]);
+      for (int qb = 0; qb < 2; ++qb) {
+        const int l = lane_here();
+        NormLanes norm;
+        load_norm_lanes(norm, norm_w, l);
+        queries_ready(arguments_here(), s, r0 + 16 * qb, ahead[qb], norm, turn, l, FOLD ? p.c : 1.0f, w.qf[qb]);
+      }
     }
     const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
 #pragma unroll
@@ -931,7 +958,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
           }
         } else {
           // as the lanes hold it, whole KiB a store: by rows, 64 bytes of 16 of them a store, a workgroup's part took 12 us
-          float* part = args.partials + part_slot(rank, begins) * part_floats(RB);
+          float* part = args.partials + part_slot(run.rank, begins) * part_floats(RB);
           float* to = part + (2 * wave + qb) * (16 * kD) + out_lane * 4;
           if (r0 + 16 * qb + c16 <= last) {
 #pragma unroll
@@ -960,7 +987,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   const i32x4 cut = p.cuts[run];
   if (run >= p.cuts[0][0] || cut[3] == 0) return;
   const Sequence s = uniform_sequence(p, cut[0]);
-  const int rows = min(RB, s.n * p.G - cut[2] * RB), row0 = (int)blockIdx.y * 8;
+  const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)blockIdx.y * 8;
   if (row0 >= rows) return;
   const int here = min(8, rows - row0), groups = here == 1 ? 8 : here == 2 ? 4 : here <= 4 ? 2 : 1;   // groups of 32 threads a row
   const int mine = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
@@ -1010,53 +1037,63 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   *(bf16x4*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row, p.o_ss, p.o_sh, token) + col * 2) = out;
 }
 
-// The same for the tile form, whose parts lie as its lanes hold them: blockIdx.y is a block of 16 rows, thread t has the columns 16*db + 4*g .. +3 of row c
-// (t % 64 = 16*g + c) for two db, and the rows go out by way of LDS.
+// The same for the tile form, whose parts lie as its lanes hold them: blockIdx.y / 2 is a block of 16 rows, and wave w has the columns 16*db .. +15 of it for
+// db = 4 * (blockIdx.y % 2) + w, four of row c a lane (16*g + c).  Eight parts are on their way at once.  The rows go out by way of LDS.
 __global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
-  constexpr int RB = kTileRows;
-  __shared__ __attribute__((aligned(16))) char turn[4096];
+  constexpr int RB = kTileRows, kAtOnce = 8;
+  __shared__ __attribute__((aligned(16))) char turn[2048];
   const int run = (int)blockIdx.x + 1;
   const i32x4 cut = p.cuts[run];
   if (run >= p.cuts[0][0] || cut[3] == 0) return;
   const Sequence s = uniform_sequence(p, cut[0]);
-  const int rows = min(RB, s.n * p.G - cut[2] * RB), row0 = (int)blockIdx.y * 16;
+  const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)(blockIdx.y >> 1) * 16, half = blockIdx.y & 1;
   if (row0 >= rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int row = min(row0 + c, rows - 1);                       // (rows that are not there: another's maximum and sum, and nothing is stored)
-  auto slot = [&](int i) { return p.partials + part_slot(run - 1 + i, i == 0) * part_floats(RB); };
+  const int at = min(row0 + c, rows - 1);                        // (rows that are not there: another's, and nothing is stored)
+  const int col = row0 * kD + (4 * half + wave) * 256 + (16 * g + at - row0) * 4;
   float top = kNoMax, l = 0.f;
-  for (int i = 0; i < cut[3]; ++i) top = fmaxf(top, slot(i)[RB * kD + row]);
-  f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  const bool live = row0 + c < rows;
-#pragma unroll 2
-  for (int i = 0; i < cut[3]; ++i) {
-    const float* t = slot(i);
-    const float a = __builtin_amdgcn_exp2f(t[RB * kD + row] - top);
-    l += a * t[RB * (kD + 1) + row];
-    if (live) {
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int i0 = 0; i0 < cut[3]; i0 += kAtOnce) {
+    float m[kAtOnce], w[kAtOnce];
+    f32x4 o[kAtOnce];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const f32x4 o = *(const f32x4*)(t + row0 * kD + (2 * wave + e) * 256 + lane * 4);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int part = min(i0 + i, cut[3] - 1);
+      const float* t = p.partials + part_slot(run - 1 + part, part == 0) * part_floats(RB);
+      m[i] = t[RB * kD + at];
+      w[i] = t[RB * (kD + 1) + at];
+      o[i] = *(const f32x4*)(t + col);
+    }
+    float most = top;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[e][k] += a * o[k];
+    for (int i = 0; i < kAtOnce; ++i) most = i0 + i < cut[3] ? fmaxf(most, m[i]) : most;
+    const float a0 = __builtin_amdgcn_exp2f(top - most);
+    top = most;
+    l *= a0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] *= a0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (i0 + i < cut[3]) {
+        const float a = __builtin_amdgcn_exp2f(m[i] - top);
+        l += a * w[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += a * o[i][k];
       }
     }
   }
   const float inv = inverse_sum(l);
+  bf16x4 v;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    bf16x4 v;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (__bf16)(sum[e][k] * inv);
-    const int db = 2 * wave + e;
-    *(bf16x4*)(turn + c * 256 + (((2 * db + (g >> 1)) ^ c) * 16) + 8 * (g & 1)) = v;
-  }
+  for (int k = 0; k < 4; ++k) v[k] = (__bf16)(sum[k] * inv);
+  *(bf16x4*)(turn + c * 128 + (((2 * wave + (g >> 1)) ^ (c & 7)) * 16) + 8 * (g & 1)) = v;
   __syncthreads();
-  const int out = threadIdx.x >> 4, chunk = threadIdx.x & 15;
-  if (row0 + out >= rows) return;
+  const int out = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  if (out >= 16 || row0 + out >= rows) return;
   int token;
-  *(bf16x8*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row0 + out, p.o_ss, p.o_sh, token) + chunk * 16) =
-      *(const bf16x8*)(turn + out * 256 + ((chunk ^ out) * 16));
+  *(bf16x8*)(p.o + row_offset(p, s, cut[1], cut[2] * RB + row0 + out, p.o_ss, p.o_sh, token) + half * 128 + chunk * 16) =
+      *(const bf16x8*)(turn + out * 128 + ((chunk ^ (out & 7)) * 16));
 }
 
 // ---- host ----
@@ -1089,7 +1126,7 @@ hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
   if (e != hipSuccess) return e;
-  const PagedForm f = form_of(p.rows, p.B, p.G);
+  const PagedForm f = form_of(p.rows, p.B, p.G.n);
   const int grid = workgroups_of(f, cus);
   const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {
@@ -1100,7 +1137,7 @@ hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
     default:
       return launch_form(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
                              : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>),
-                         64 * kTileWaves, paged_merge_tile_kernel, kTileRows / 16, grid, p, st);
+                         64 * kTileWaves, paged_merge_tile_kernel, kTileRows / 8, grid, p, st);
   }
 }
 

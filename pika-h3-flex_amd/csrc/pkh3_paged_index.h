@@ -39,25 +39,39 @@ constexpr int64_t most_tiles(int64_t rows, int64_t B) {
   return (rows + 62 * used) / kPageKeys + used;
 }
 
-// ---- attention: blocks of rb query rows (a token's G query heads of one kv head side by side), and the tiles they see ----
+// ---- attention: blocks of rb query rows (a token's query heads of one kv head side by side), and the tiles they see ----
 
-constexpr int blocks_of(const Sequence& s, int G, int rb) { return (s.n * G + rb - 1) / rb; }
+// The query heads of one kv head, and the token of a query row r, 0 <= r < 2^30: r / n by a multiplication.  With s the first power 2^s >= n and
+// mul = ceil(2^(30+s) / n) (at most 2^31), r * mul / 2^(30+s) is over r / n by less than r / 2^30 / n, too little to reach the next whole number.
+struct Group {
+  int n;
+  uint32_t mul;
+  int shift;
+  constexpr int token(int r) const { return (int)(uint32_t)(((uint64_t)((uint32_t)r << 2) * mul >> 32) >> shift); }
+};
+constexpr Group make_group(int n) {
+  int s = 0;
+  while ((1 << s) < n) ++s;
+  return {n, (uint32_t)((((uint64_t)1 << (30 + s)) + n - 1) / n), s};
+}
+
+constexpr int blocks_of(const Sequence& s, const Group& G, int rb) { return (s.n * G.n + rb - 1) / rb; }
 // keys that query row r sees; past the last row: what that one sees
-constexpr int row_keys(const Sequence& s, int G, int causal, int r) {
+constexpr int row_keys(const Sequence& s, const Group& G, int causal, int r) {
   if (!causal) return s.keys;
-  return at_most(at_least(s.position() + at_most((int)((unsigned)r / (unsigned)G), s.n - 1) + 1, 0), s.keys);
+  return at_most(at_least(s.position() + G.token(at_most(r, s.n * G.n - 1)) + 1, 0), s.keys);
 }
 // tiles of block j: of its last row.  One at least: a block without keys writes zeros
-constexpr int block_tiles(const Sequence& s, int G, int causal, int rb, int j) {
+constexpr int block_tiles(const Sequence& s, const Group& G, int causal, int rb, int j) {
   return at_least((row_keys(s, G, causal, (j + 1) * rb - 1) + kPageKeys - 1) >> 6, 1);
 }
 
 // What a tile of block j costs, by the waves of a workgroup that have rows of it: in the form of 384 rows (12 waves, three a SIMD) 4, or where there
 // are rows for two a SIMD or one, 3 or 2 (the waves without rows leave the products out); 1 in the other forms.
 constexpr int most_cost(int rb) { return rb == 384 ? 4 : 1; }
-constexpr int block_cost(const Sequence& s, int G, int rb, int j) {
+constexpr int block_cost(const Sequence& s, const Group& G, int rb, int j) {
   if (rb != 384) return 1;
-  const int rows = s.n * G - j * rb;
+  const int rows = s.n * G.n - j * rb;
   return rows > 256 ? 4 : rows > 128 ? 3 : 2;
 }
 
@@ -94,19 +108,21 @@ constexpr int rank_of(int block, const Shares& sh) {
   return (block >> 3) < per_xcd && rank < sh.n ? rank : -1;
 }
 // A run boundary that lies `in` behind the beginning of a unit of nt tiles at this cost goes to the tile there, or to the nearer end of a unit that is not
-// cut.  The result may be nt: the next unit's beginning.
+// cut, or to an end that is so near that a part of its own costs more than it gives.  The result may be nt: the next unit's beginning.
+constexpr int kNearTiles = 3;
 constexpr int boundary_tile(const Shares& sh, int64_t in, int nt, int cost) {
-  const int t = at_least((int)divided(in, cost) - kUnitTiles, 0);
-  return nt <= kWholeTiles && unit_length(nt, cost) <= sh.run() ? (2 * in >= unit_length(nt, cost) ? nt : 0) : t;
+  if (nt <= kWholeTiles && unit_length(nt, cost) <= sh.run()) return 2 * in >= unit_length(nt, cost) ? nt : 0;
+  const int t = (int)divided(in, cost) - kUnitTiles;
+  return t > kNearTiles ? (t < nt - kNearTiles ? t : nt) : 2 * t < nt ? 0 : nt;
 }
 // A unit that several runs share: run i leaves its part in slot 2*i + 1 if its part begins the unit, else in slot 2*i.
 constexpr int64_t part_slot(int run, bool begins) { return 2 * (int64_t)run + (begins ? 1 : 0); }
 // Of boundary i, at tile t of the unit of nt tiles that begins at `begin`: if it cuts the unit and is the first that does, how many runs share the unit (the
 // one in front of the boundary, the one behind it, ..).  0: not this boundary's business.
 constexpr int parts_at(const Shares& sh, int i, int64_t begin, int t, int nt, int cost) {
-  if (t <= 0 || t >= nt || sh.begin(i - 1) >= begin + tile_place(1, cost)) return 0;
+  if (t <= 0 || t >= nt || sh.begin(i - 1) >= begin + tile_place(kNearTiles + 1, cost)) return 0;
   int parts = 2;
-  while (i + parts - 1 < sh.n && sh.begin(i + parts - 1) < begin + unit_length(nt, cost)) ++parts;
+  while (i + parts - 1 < sh.n && sh.begin(i + parts - 1) < begin + tile_place(nt - kNearTiles, cost)) ++parts;
   return parts;
 }
 

@@ -168,21 +168,29 @@ def test_rows_and_pages_stay_in_range_whatever_the_arrays_hold(tmp_path):
         const TileRows t = tile_rows(s, i);
         CHECK(t.p0 >= 0 && t.p0 < t.p1 && t.p1 <= 64 && t.row0 + t.p0 >= s.first && t.row0 + t.p1 <= s.first + s.n, "tile %d", i);
       }
-      for (int G : {1, 6}) for (int causal : {0, 1}) for (int rb : {16, 32, 128, 384}) {
-        if (s.n == 0 || (int64_t)rows * G > (1 << 30)) continue;
+      for (int g : {1, 6}) for (int causal : {0, 1}) for (int rb : {16, 32, 128, 384}) {
+        const Group G = make_group(g);
+        if (s.n == 0 || (int64_t)rows * g > (1 << 30)) continue;
         const int blocks = blocks_of(s, G, rb);
         for (int j : {0, blocks / 2, blocks - 1}) {
           const int t = block_tiles(s, G, causal, rb, j);
           CHECK(t >= 1 && t <= (pages > 1 ? pages : 1), "%d tiles", t);
-          for (int r = j * rb; r < std::min((j + 1) * rb, s.n * G); ++r) {
+          for (int r = j * rb; r < std::min((j + 1) * rb, s.n * g); ++r) {
             const int k = row_keys(s, G, causal, r);
             CHECK(k >= 0 && k <= s.keys && k <= 64 * t, "row %d sees %d", r, k);
-            CHECK(k == (causal ? std::max(0, std::min(s.keys, s.keys - s.n + r / G + 1)) : s.keys), "row %d sees %d", r, k);
+            CHECK(k == (causal ? std::max(0, std::min(s.keys, s.keys - s.n + r / g + 1)) : s.keys), "row %d sees %d", r, k);
             CHECK(k >= row_keys(s, G, causal, j * rb), "the first row of a block sees least");
           }
         }
       }
     }
+  for (int g = 1; g <= 65535; g = g < 70 ? g + 1 : g + any(1, 999)) {
+    const Group G = make_group(g);
+    for (int k = 0; k < 300; ++k) {
+      const int r = k < 40 ? k : k < 80 ? (1 << 30) - k + 39 : k < 200 ? any(0, (1 << 30) - 1) : std::min(any(0, (1 << 30) / g) * g + any(-1, 1) + (k == 200), (1 << 30) - 1);
+      if (r >= 0) CHECK(G.token(r) == r / g, "%d / %d is %d", r, g, G.token(r));
+    }
+  }
   for (int id : {-1, 0, 4, 5, 2147483647}) CHECK(page_in_pool(id, 5) == (id >= 0 && id < 5 ? id : -1), "%d", id);""")
 
 
@@ -219,8 +227,9 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     every cut unit joined at one boundary, in the order of the runs."""
     _run(tmp_path, """
   for (int go = 0; go < 6000; ++go) {
-    const int B = any(1, 6), H = any(1, 4), G = any(1, 4), causal = any(0, 1), rb = go % 5 <= 1 ? 384 : go % 5 == 2 ? 128 : go % 5 == 3 ? 32 : 16;
+    const int B = any(1, 6), H = any(1, 4), causal = any(0, 1), rb = go % 5 <= 1 ? 384 : go % 5 == 2 ? 128 : go % 5 == 3 ? 32 : 16;
     const int grid = go % 3 == 0 ? 8 : go % 3 == 1 ? 24 : 512;
+    const Group G = make_group(any(1, 4));
     struct Unit { int64_t begin; int nt, cost; };
     std::vector<Unit> units;
     int64_t total = 0;
