@@ -36,6 +36,7 @@ struct PagedParams {
   const float* cos_t;
   const float* sin_t;
   int heads_per_wg, groups;          // write, read
+  int whole;                         // attn: no unit is cut (short tables), and there is no second launch
   Group G;                           // attn: query heads of one of the cache's
   float c;                           // attn: softmax scale * log2(e)
   int causal;
@@ -101,6 +102,18 @@ __device__ __forceinline__ bf16x8 expand_fp8(int lo, int hi, float scale) {
   return out;
 }
 __device__ __forceinline__ float exponent_scale(unsigned byte) { return __uint_as_float(byte << 23); }
+// the same of eight keys' values, each times its own scale (exponent bytes e[0], e[1])
+__device__ __forceinline__ bf16x8 expand_fp8_keys(int lo, int hi, const unsigned (&e)[2]) {
+  bf16x8 out;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned src = j < 4 ? lo : hi;
+    const float scale = exponent_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
+    const bf16x2 both = (j & 2) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, false);
+    out[j] = both[j & 1];
+  }
+  return out;
+}
 
 hipError_t launch_paged_write(const PagedParams& p, bool fp8, hipStream_t st);
 hipError_t launch_paged_read(const PagedParams& p, bool fp8, hipStream_t st);

@@ -133,7 +133,7 @@ struct Run {
   int64_t left, length;
 };
 __device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cum, int64_t* found, int rb, Run& run, Place& at) {
-  const Shares sh = shares_of(cum[p.B], gridDim.x, rb);
+  const Shares sh = shares_of(cum[p.B], gridDim.x, rb, p.whole != 0);
   run.rank = rank_of(blockIdx.x, sh);
   if (blockIdx.x == 0 && threadIdx.x == 0) p.cuts[0] = i32x4{sh.n, 0, 0, 0};
   if (run.rank < 0 || sh.total == 0) return false;
@@ -332,16 +332,6 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
     const int nt = block_tiles(p, s, RB, at.j), take = tiles_left(left, at.t, nt, 1);
     __syncthreads();                                           // the sums, or the results of the unit before, are read
     SplitState<FP8, QB> w;
-    if (wave < QB) {
-      bf16x8 img[4];
-      Rows16 q;
-      ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
-      NormLanes norm;
-      load_norm_lanes(norm, p.norm_w, lane);
-      queries_ready(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, img);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
-    }
     int sees[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) sees[qb] = row_keys(p, s, at.j * RB + 16 * qb + c16);
@@ -371,6 +361,16 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
     if (first < end) {
       id = uniform_page(p, at.b, first >> 1);
       ask_k(id, first & 1);
+    }
+    if (wave < QB) {
+      bf16x8 img[4];
+      Rows16 q;
+      ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
+      NormLanes norm;
+      load_norm_lanes(norm, p.norm_w, lane);
+      queries_ready(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, img);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
     }
     __syncthreads();
 #pragma unroll
@@ -691,15 +691,7 @@ __device__ __forceinline__ void expand_tile(const char* raw, char* images, int w
       char* to = images + kKTileBytes + ((half * 8 + 2 * dbp) * 64 + lane) * 16;
 #pragma unroll
       for (int par = 0; par < 2; ++par) {
-        bf16x8 out;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned src = v[2 * par + (j >> 2)];
-          const float scale = exponent_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
-          const bf16x2 both = (j & 2) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(src, scale, false);
-          out[j] = both[j & 1];
-        }
-        *(bf16x8*)(to + par * 1024) = out;
+        *(bf16x8*)(to + par * 1024) = expand_fp8_keys(v[2 * par], v[2 * par + 1], e);
       }
     }
   }
@@ -1113,16 +1105,21 @@ size_t paged_attn_scratch(int rows, int B, int G) {
   return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f)) + kCutFloats;
 }
 
+// Tables of so few pages that whole units are no longer than cutting them and putting them together again: one launch.
+static bool short_table(int table_pages) { return table_pages <= kWholeTiles; }
+
 template <class Kernel, class Merge>
 static hipError_t launch_form(Kernel kernel, int threads, Merge merge, int blocks, int grid, const PagedParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || p.whole) return e;
   hipLaunchKernelGGL(merge, dim3(grid - 1, blocks), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 
-hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st) {
+hipError_t launch_paged_attn(const PagedParams& given, bool fp8, hipStream_t st) {
+  PagedParams p = given;
+  p.whole = short_table(p.table_pages);
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
   if (e != hipSuccess) return e;

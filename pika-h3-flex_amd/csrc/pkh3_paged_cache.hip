@@ -30,7 +30,8 @@ __device__ __forceinline__ float row_max16(float x) {   // over the 16 lanes of 
   x = max_with<0x141>(x);
   return max_with<0x140>(x);
 }
-// Largest magnitude of a row's values as the scale rule takes it: what is not finite counts as nothing (it is stored as NaN whatever the scale).
+// What is not finite is stored as NaN and counts as nothing for the scale.  The conversion does that with NaN, and the largest magnitude passes over it; a
+// largest magnitude of infinity says that the careful way is needed.
 __device__ __forceinline__ float finite_magnitude(float x) {
   const float a = fabsf(x);
   return a < INFINITY ? a : 0.f;
@@ -81,14 +82,20 @@ __device__ __forceinline__ void write_k(const PagedParams& p, const TileRows& t,
     } else {
       float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, finite_magnitude(x[i]));
+      for (int i = 0; i < 32; ++i) amax = fmaxf(amax, fabsf(x[i]));
+      if (__any(!(amax < INFINITY))) {
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          amax = fmaxf(amax, finite_magnitude(x[i]));
+          x[i] = to_quantise(x[i], 1.0f);
+        }
+      }
       const float scale = key_scale(max_across_groups(amax));
       const float inv = 1.0f / scale;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) x[i] = to_quantise(x[i], inv);
-#pragma unroll
       for (int c2 = 0; c2 < 2; ++c2) {
-        const i32x2 q0 = quant_fp8_piece(x + 16 * c2, 1.0f), q1 = quant_fp8_piece(x + 16 * c2 + 8, 1.0f);
+        const i32x2 q0 = quant_fp8_piece(x + 16 * c2, inv), q1 = quant_fp8_piece(x + 16 * c2 + 8, inv);
         if (mine) *(i32x4*)(record + ((kb * 2 + c2) * 64 + lane) * 16) = i32x4{q0[0], q0[1], q1[0], q1[1]};
       }
       if (mine && g == 0) record[kK8TileBytes + kVTileBytes / 2 + place] = (char)e8m0_of(scale);
@@ -125,7 +132,15 @@ __device__ __forceinline__ void write_v(const PagedParams& p, const TileRows& t,
       for (int i = 0; i < 8; ++i) {
         float amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_magnitude((float)next[i][j]));
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf((float)next[i][j]));
+        if (__any(!(amax < INFINITY))) {
+          amax = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            amax = fmaxf(amax, finite_magnitude((float)next[i][j]));
+            next[i][j] = (__bf16)to_quantise((float)next[i][j], 1.0f);
+          }
+        }
         const float scale = key_scale(row_max16(amax));
         const int place = half * 32 + 4 * i + g;
         if (c == 0) {
@@ -171,7 +186,7 @@ __device__ __forceinline__ void write_v(const PagedParams& p, const TileRows& t,
       } else {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = to_quantise((float)img[j], inv[j]);
+        for (int j = 0; j < 8; ++j) x[j] = (float)img[j] * inv[j];
         bytes[db & 1] = quant_fp8_piece(x, 1.0f);
         if (db & 1) {
           char* to = record + kK8TileBytes + ((half * 4 + (db >> 1)) * 64 + lane) * 16;
@@ -283,11 +298,7 @@ __device__ __forceinline__ void read_v(const PagedParams& p, const TileRows& t, 
       for (int dbp = 0; dbp < 4; ++dbp) {
         const i32x4 w = *(const i32x4*)(record + ((half * 4 + dbp) * 64 + lane) * 16);
 #pragma unroll
-        for (int par = 0; par < 2; ++par) {
-          const bf16x8 v = expand_fp8(w[2 * par], w[2 * par + 1], 1.0f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) img[2 * dbp + par][j] = (__bf16)((float)v[j] * exponent_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu));
-        }
+        for (int par = 0; par < 2; ++par) img[2 * dbp + par] = expand_fp8_keys(w[2 * par], w[2 * par + 1], e);
       }
     }
 #pragma unroll

@@ -77,7 +77,7 @@ constexpr int block_cost(const Sequence& s, const Group& G, int rb, int j) {
 
 // What a unit costs besides its tiles, in tiles: queries in and out, the first keys' way.  Units of 384 rows against 2, 5 and 8 tiles took 8 us and 2.7 a
 // tile; shared out by their tiles alone, the last workgroup of such a call was done at 320 us and the first at 102.
-constexpr int kUnitTiles = 3;
+constexpr int kUnitTiles = 4;
 constexpr int64_t unit_length(int nt, int cost) { return (int64_t)(nt + kUnitTiles) * cost; }
 // where tile t of a unit begins
 constexpr int64_t tile_place(int t, int cost) { return t == 0 ? 0 : (int64_t)(t + kUnitTiles) * cost; }
@@ -95,12 +95,13 @@ constexpr int kWholeTiles = 16;       // a unit of at most so many, and no deare
 struct Shares {
   int64_t total;
   int n;
+  bool whole;                         // no unit is cut
   constexpr int64_t begin(int i) const { return divided(total * i, n); }
   constexpr int64_t run() const { return divided(total, n); }
 };
-constexpr Shares shares_of(int64_t total, int most, int rb) {
-  const int64_t worth = total / ((kMinShareTiles + kUnitTiles) * most_cost(rb));
-  return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most)};
+constexpr Shares shares_of(int64_t total, int most, int rb, bool whole) {
+  const int64_t worth = total / (((whole ? 1 : kMinShareTiles) + kUnitTiles) * (whole ? 1 : most_cost(rb)));
+  return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most), whole};
 }
 // The workgroup of a launch that takes run `rank`: a contiguous run of runs per XCD.  -1: none.
 constexpr int rank_of(int block, const Shares& sh) {
@@ -111,7 +112,7 @@ constexpr int rank_of(int block, const Shares& sh) {
 // cut, or to an end that is so near that a part of its own costs more than it gives.  The result may be nt: the next unit's beginning.
 constexpr int kNearTiles = 3;
 constexpr int boundary_tile(const Shares& sh, int64_t in, int nt, int cost) {
-  if (nt <= kWholeTiles && unit_length(nt, cost) <= sh.run()) return 2 * in >= unit_length(nt, cost) ? nt : 0;
+  if (sh.whole || (nt <= kWholeTiles && unit_length(nt, cost) <= sh.run())) return 2 * in >= unit_length(nt, cost) ? nt : 0;
   const int t = (int)divided(in, cost) - kUnitTiles;
   return t > kNearTiles ? (t < nt - kNearTiles ? t : nt) : 2 * t < nt ? 0 : nt;
 }

@@ -9,15 +9,17 @@ the rows are those of its attention module (src/pika_h3/core/loader.py:9).
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .ops import HEAD_DIM, _f32, _on_device, _raw_stream
+from .ops import HEAD_DIM, _raw_stream
 
 PAGE_KEYS = _lib.PAGE_KEYS
+_F32 = C.c_float
 
 
 class PagedKV:
@@ -29,30 +31,55 @@ class PagedKV:
         self.pages, self.heads, self.fp8 = int(pages), int(heads), bool(fp8)
         if self.pages < 1 or self.heads < 1:
             raise ValueError(f"a pool has at least one page and one head, got {pages} and {heads}")
-        self.record_bytes = int(_lib.load().pkh3_paged_record_bytes(_lib.PAGED_FP8 if self.fp8 else 0))
+        self.flags = _lib.PAGED_FP8 if self.fp8 else 0
+        self.record_bytes = int(_lib.load().pkh3_paged_record_bytes(self.flags))
         shape = (self.pages, self.heads, self.record_bytes)
         if data is None:
             data = torch.empty(shape, dtype=torch.uint8, device=device if device is not None else "cuda")
         elif data.dtype != torch.uint8 or not data.is_contiguous() or data.shape != shape:
             raise ValueError(f"data must be contiguous uint8 {shape}, got {data.dtype} {tuple(data.shape)}")
-        self.data = data
+        self._data = data
+        self._head = (data.data_ptr(), self.pages)
+        self._index = data.get_device()
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
 
     @property
     def device(self):
-        return self.data.device
+        return self._data.device
 
 
-@dataclass
+@dataclass(frozen=True)
 class PagedBatch:
     """The sequences of a call: int32 device tensors ``starts [B + 1]`` (sequence b owns the call's rows ``starts[b] ..
     starts[b+1]-1``, its newest), ``lengths [B]`` (its keys, these rows among them where they are written) and ``table [B, P]``
-    (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows them.  The tensors may be changed in
-    place between calls, replays of a captured graph among them; include/pkh3_paged.h says what out-of-range values do."""
+    (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows them.  What the tensors hold may be
+    changed in place between calls, replays of a captured graph among them; include/pkh3_paged.h says what out-of-range values do."""
 
     starts: torch.Tensor
     lengths: torch.Tensor
     table: torch.Tensor
     rows: Optional[int] = None
+    _arrays: tuple = field(init=False, repr=False, compare=False)
+    _sizes: tuple = field(init=False, repr=False, compare=False)
+    _index: int = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self):
+        # checked once: small calls wait for the host, and a batch is the handle of many
+        index = self.table.get_device()
+        for name, t, dim in (("starts", self.starts, 1), ("lengths", self.lengths, 1), ("table", self.table, 2)):
+            if t.dtype != torch.int32 or t.dim() != dim or (t.stride(dim - 1) != 1 and t.shape[dim - 1] > 1):
+                raise ValueError(f"batch {name} must be int32 with {dim} dimension(s) and unit stride, got {t.dtype} {tuple(t.shape)}")
+            if t.get_device() != index:
+                raise ValueError(f"batch {name} must live with the table on {self.table.device} (got {t.device})")
+        B = self.lengths.shape[0]
+        if self.starts.shape[0] != B + 1 or self.table.shape[0] != B:
+            raise ValueError(f"batch of {B} lengths has {self.starts.shape[0]} starts (need {B + 1}) and {self.table.shape[0]} rows of pages")
+        object.__setattr__(self, "_arrays", (self.starts.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), self.table.stride(0)))
+        object.__setattr__(self, "_sizes", (B, self.table.shape[1]))
+        object.__setattr__(self, "_index", index)
 
     @staticmethod
     def build(new_rows: Sequence[int], lengths: Sequence[int], pages: Sequence[Sequence[int]], *, device=None) -> "PagedBatch":
@@ -78,87 +105,118 @@ class PagedBatch:
         return PagedBatch(as_int(starts), as_int([int(n) for n in lengths]), as_int(table), starts[-1])
 
 
-def _rows_of(name: str, t: torch.Tensor, heads: Optional[int], device) -> Tuple[int, int]:
-    """Raises unless the kernels can read (or write) ``t`` as [rows, heads, 128]; its strides."""
-    if t.dim() != 3 or t.shape[2] != HEAD_DIM or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {HEAD_DIM}], got {tuple(t.shape)}")
-    if t.dtype != torch.bfloat16:
+def _rows_of(name: str, t: torch.Tensor, heads: int, index: int) -> Tuple[int, int, int]:
+    """Raises unless the kernels can read (or write) ``t`` as [rows, heads, 128] on device ``index``; its strides and rows.  ``heads`` 0: any."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or (heads and shape[1] != heads):
+        raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {HEAD_DIM}], got {tuple(shape)}")
+    if t.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}: head-dim stride must be 1, got {t.stride(2)}")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must live in device memory (got {t.device}); the HIP library is the only compute path")
-    _on_device(name, t, device)
-    return t.stride(0), t.stride(1)
+    strides = t.stride()
+    if strides[2] != 1:
+        raise ValueError(f"{name}: head-dim stride must be 1, got {strides[2]}")
+    on = t.get_device()
+    if on != index or on < 0:
+        raise ValueError(f"{name} must live in device memory, with the cache (got {t.device}); the HIP library is the only compute path")
+    return strides[0], strides[1], shape[0]
 
 
-def _args(cache: PagedKV, batch: PagedBatch, rows: int, *, q=None, k=None, v=None, o=None, strides=(0,) * 8, heads=0, softmax_scale=None,
-          norm_w=None, norm_eps=1e-6, rope_mode=_lib.ROPE_NONE, rope=None, flags=0) -> _lib.PagedArgs:
-    dev = cache.data.device
-    for name, t, dim in (("starts", batch.starts, 1), ("lengths", batch.lengths, 1), ("table", batch.table, 2)):
-        if t.dtype != torch.int32 or t.dim() != dim or (t.stride(dim - 1) != 1 and t.shape[dim - 1] > 1):
-            raise ValueError(f"batch {name} must be int32 with {dim} dimension(s) and unit stride, got {t.dtype} {tuple(t.shape)}")
-        _on_device(f"batch {name}", t, dev)
-    B = batch.lengths.shape[0]
-    if batch.starts.shape[0] != B + 1 or batch.table.shape[0] != B:
-        raise ValueError(f"batch of {B} lengths has {batch.starts.shape[0]} starts (need {B + 1}) and {batch.table.shape[0]} rows of pages")
+def _f32(name: str, t: torch.Tensor, shape: tuple, index: int) -> int:
+    if t.dtype is not torch.float32 or not t.is_contiguous() or t.shape != shape:
+        raise ValueError(f"{name} must be contiguous float32 {shape}, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must live in device memory, with the cache (got {t.device})")
+    return t.data_ptr()
+
+
+def _norm_rope(norm_w, rope_mode, rope, rows: int, index: int) -> tuple:
+    """The fields norm_w, rope_cos, rope_sin, rope_mode."""
+    w = 0 if norm_w is None else _f32("norm weight", norm_w, (HEAD_DIM,), index)
+    rope_mode = int(rope_mode)
+    if rope_mode == _lib.ROPE_NONE:
+        return w, 0, 0, rope_mode
+    if rope is None:
+        raise ValueError("rope_mode set but its tables are missing")
+    shape = (rows, HEAD_DIM // 2)
+    return w, _f32("rope cos", rope[0], shape, index), _f32("rope sin", rope[1], shape, index), rope_mode
+
+
+def _check_batch(cache: PagedKV, batch: PagedBatch, rows: int) -> None:
+    if batch._index != cache._index:
+        raise ValueError(f"the batch must live with the cache on {cache.device} (got {batch.table.device})")
     if batch.rows is not None and batch.rows != rows:
         raise ValueError(f"the batch has {batch.rows} rows, the call {rows}")
-    norm_w = _f32("norm weight", norm_w, (HEAD_DIM,), dev)
-    rope_mode = int(rope_mode)
-    cos = sin = None
-    if rope_mode != _lib.ROPE_NONE:
-        if rope is None:
-            raise ValueError("rope_mode set but its tables are missing")
-        cos, sin = (_f32(f"rope {n}", t, (rows, HEAD_DIM // 2), dev) for n, t in zip(("cos", "sin"), rope))
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    return _lib.PagedArgs.from_buffer_copy(_lib.PAGED_ARGS_FORMAT.pack(
-        cache.data.data_ptr(), cache.pages, batch.starts.data_ptr(), batch.lengths.data_ptr(), batch.table.data_ptr(), batch.table.stride(0),
-        ptr(q), ptr(k), ptr(v), ptr(o), *strides, B, batch.table.shape[1], rows, cache.heads, heads, HEAD_DIM,
-        0.0 if softmax_scale is None else C.c_float(softmax_scale).value, C.c_float(norm_eps).value, ptr(norm_w), ptr(cos), ptr(sin), rope_mode,
-        flags | (_lib.PAGED_FP8 if cache.fp8 else 0), 0, 0))
 
 
-def _call(entry, args: _lib.PagedArgs, device) -> None:
-    if device.index == torch.cuda.current_device():
-        _lib.check(entry(C.byref(args), _raw_stream(device.index)))
+_pack = _lib.PAGED_ARGS_FORMAT.pack
+
+
+@lru_cache(maxsize=None)
+def _entry(name: str):
+    """A C entry that takes the packed bytes of its arguments."""
+    call = _lib.load()[name]
+    call.argtypes = [C.c_char_p, C.c_void_p]
+    call.restype = C.c_int
+    return call
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, B: int, table_pages: int, kv_heads: int, heads: int) -> int:
+    """Scratch of an attention call: a matter of its sizes alone."""
+    args = _lib.PagedArgs(n_pages=1, B=B, table_pages=table_pages, rows=rows, kv_heads=kv_heads, heads=heads, D=HEAD_DIM)
+    lib = _lib.load()
+    n = int(lib.pkh3_paged_workspace_bytes(C.byref(args)))
+    if n == 0:
+        raise _lib.Pkh3Error(_lib.PKH3_EARG, lib.pkh3_last_error().decode())
+    return n
+
+
+def _call(name: str, args: bytes, index: int) -> None:
+    if index == torch.cuda.current_device():
+        rc = _entry(name)(args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(entry(C.byref(args), _raw_stream(device.index)))
+        with torch.cuda.device(index):
+            rc = _entry(name)(args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def paged_write(cache: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, *, k_norm_weight: Optional[torch.Tensor] = None,
                 norm_eps: float = 1e-6, rope_mode: int = _lib.ROPE_NONE, rope_k=None) -> None:
     """Keys (through RMSNorm and rotation, as given) and values of the call's rows, bf16 ``[rows, heads, 128]``, into their pages.
     ``rope_k``: cos/sin tables ``[rows, 64]``, a row per row of the call.  Runs asynchronously on the current stream."""
-    dev = cache.data.device
-    strides = _rows_of("k", k, cache.heads, dev) + _rows_of("v", v, cache.heads, dev)
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-    args = _args(cache, batch, k.shape[0], k=k, v=v, strides=(0, 0) + strides + (0, 0), norm_w=k_norm_weight, norm_eps=norm_eps,
-                 rope_mode=rope_mode, rope=rope_k)
-    if k.shape[0]:
-        _call(_lib.load().pkh3_paged_write, args, dev)
+    index, H = cache._index, cache.heads
+    k_ss, k_sh, rows = _rows_of("k", k, H, index)
+    v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
+    if rows != v_rows:
+        raise ValueError(f"k has {rows} rows, v {v_rows}")
+    _check_batch(cache, batch, rows)
+    prep = _norm_rope(k_norm_weight, rope_mode, rope_k, rows, index)
+    if rows:
+        _call("pkh3_paged_write", _pack(*cache._head, *batch._arrays, 0, k.data_ptr(), v.data_ptr(), 0, 0, 0, k_ss, k_sh, v_ss, v_sh, 0, 0,
+                                        *batch._sizes, rows, H, 0, HEAD_DIM, 0.0, _F32(norm_eps).value, *prep, cache.flags, 0, 0), index)
 
 
 def paged_read(cache: PagedKV, batch: PagedBatch, rows: Optional[int] = None, *, out=None) -> List[torch.Tensor]:
     """Keys and values of the call's rows as the cache holds them: ``[k, v]``, bf16 ``[rows, heads, 128]`` (``out``: two tensors
     to put them in).  ``rows``: as ``batch.rows`` where the batch does not know.  Rows of no sequence, in given tensors, stay as they are;
     in new ones they hold anything."""
-    dev = cache.data.device
+    index, H = cache._index, cache.heads
     if rows is None:
         rows = batch.rows if out is None else out[0].shape[0]
     if rows is None:
         raise ValueError("the batch does not know its rows: say how many")
     if out is None:
-        out = [torch.empty((rows, cache.heads, HEAD_DIM), dtype=torch.bfloat16, device=dev) for _ in range(2)]
+        out = torch.empty((2, rows, H, HEAD_DIM), dtype=torch.bfloat16, device=cache.device).unbind(0)
     k, v = out
-    strides = _rows_of("k", k, cache.heads, dev) + _rows_of("v", v, cache.heads, dev)
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError(f"out has {k.shape[0]} and {v.shape[0]} rows, the call {rows}")
-    args = _args(cache, batch, rows, k=k, v=v, strides=(0, 0) + strides + (0, 0))
+    k_ss, k_sh, k_rows = _rows_of("k", k, H, index)
+    v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
+    if k_rows != rows or v_rows != rows:
+        raise ValueError(f"out has {k_rows} and {v_rows} rows, the call {rows}")
+    _check_batch(cache, batch, rows)
     if rows:
-        _call(_lib.load().pkh3_paged_read, args, dev)
+        _call("pkh3_paged_read", _pack(*cache._head, *batch._arrays, 0, k.data_ptr(), v.data_ptr(), 0, 0, 0, k_ss, k_sh, v_ss, v_sh, 0, 0,
+                                       *batch._sizes, rows, H, 0, HEAD_DIM, 0.0, 0.0, 0, 0, 0, 0, cache.flags, 0, 0), index)
     return [k, v]
 
 
@@ -169,33 +227,32 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     cache's, over all keys of their sequence, or with ``causal`` over those up to their own position.  A row that sees no key gets
     zeros.  ``workspace``: a uint8 device tensor, or a callable ``(device, nbytes) -> tensor``, as :func:`.ops.attention` takes it; two calls
     that may overlap need one each.  Returns ``out`` (may be ``q``)."""
-    dev = cache.data.device
-    lib = _lib.load()
-    q_strides = _rows_of("q", q, None, dev)
+    index = cache._index
+    q_ss, q_sh, rows = _rows_of("q", q, 0, index)
     heads = q.shape[1]
     if heads == 0 or heads % cache.heads:
         raise ValueError(f"{heads} query heads are no multiple of the cache's {cache.heads}")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
-    o_strides = _rows_of("out", out, heads, dev)
-    if out.shape[0] != q.shape[0]:
-        raise ValueError(f"out has {out.shape[0]} rows, q {q.shape[0]}")
-    args = _args(cache, batch, q.shape[0], q=q, o=out, strides=q_strides + (0,) * 4 + o_strides, heads=heads, softmax_scale=softmax_scale,
-                 norm_w=q_norm_weight, norm_eps=norm_eps, rope_mode=rope_mode, rope=rope_q, flags=_lib.PAGED_CAUSAL if causal else 0)
-    if not q.shape[0]:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=cache.device)
+    o_ss, o_sh, o_rows = _rows_of("out", out, heads, index)
+    if o_rows != rows:
+        raise ValueError(f"out has {o_rows} rows, q {rows}")
+    _check_batch(cache, batch, rows)
+    prep = _norm_rope(q_norm_weight, rope_mode, rope_q, rows, index)
+    if not rows:
         return out
-    need = int(lib.pkh3_paged_workspace_bytes(C.byref(args)))
-    if need == 0:
-        raise _lib.Pkh3Error(_lib.PKH3_EARG, lib.pkh3_last_error().decode())
+    need = _workspace_bytes(rows, *batch._sizes, cache.heads, heads)
     if callable(workspace):
-        workspace = workspace(dev, need)
+        workspace = workspace(cache.device, need)
     own = workspace is None or workspace.numel() * workspace.element_size() < need
     if own:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev:
-        raise ValueError(f"workspace must live on {dev} (got {workspace.device})")
-    args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(lib.pkh3_paged_attn, args, dev)
+        workspace = torch.empty(need, dtype=torch.uint8, device=cache.device)
+    elif workspace.get_device() != index:
+        raise ValueError(f"workspace must live on {cache.device} (got {workspace.device})")
+    _call("pkh3_paged_attn", _pack(*cache._head, *batch._arrays, q.data_ptr(), 0, 0, out.data_ptr(), q_ss, q_sh, 0, 0, 0, 0, o_ss, o_sh,
+                                   *batch._sizes, rows, cache.heads, heads, HEAD_DIM, 0.0 if softmax_scale is None else _F32(softmax_scale).value,
+                                   _F32(norm_eps).value, *prep, cache.flags | (_lib.PAGED_CAUSAL if causal else 0), workspace.data_ptr(),
+                                   workspace.numel() * workspace.element_size()), index)
     if not own:
-        workspace.record_stream(torch.cuda.current_stream(dev))
+        workspace.record_stream(torch.cuda.current_stream(index))
     return out
