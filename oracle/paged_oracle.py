@@ -2,7 +2,7 @@
 from __future__ import annotations
 
 import math
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -39,20 +39,23 @@ def stored(x: torch.Tensor, fp8: bool) -> torch.Tensor:
     return torch.round(y / step) * step * scale                                    # (torch.round: ties to even)
 
 
-def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool, scale: Optional[float] = None
-           ) -> Tuple[torch.Tensor, torch.Tensor]:
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool, scale: Optional[float] = None,
+           gone: Sequence[int] = ()) -> Tuple[torch.Tensor, torch.Tensor]:
     """One sequence in float64: queries ``[n, Hq, 128]``, its keys and values ``[m, H, 128]``.  Returns the output and sum_j p_j |v_j|, what an
-    error of the weights is measured by; rows without a key give zeros in both."""
+    error of the weights is measured by; rows without a key give zeros in both.  ``gone``: pages whose keys nobody sees."""
     n, Hq, D = q.shape
     m, H, _ = k.shape
-    out = torch.zeros((n, Hq, D), dtype=torch.float64)
+    out = torch.zeros((n, Hq, D), dtype=torch.float64, device=q.device)
     size = torch.zeros_like(out)
     if n == 0 or m == 0:
         return out, size
     scale = 1.0 / math.sqrt(D) if scale is None else scale
-    seen = torch.ones((n, m), dtype=torch.bool)
+    seen = torch.ones((n, m), dtype=torch.bool, device=q.device)
     if causal:
-        seen = torch.arange(m)[None] <= (m - n + torch.arange(n))[:, None]
+        seen = torch.arange(m, device=q.device)[None] <= (m - n + torch.arange(n, device=q.device))[:, None]
+    for page in gone:
+        seen = seen.clone()
+        seen[:, PAGE * page:PAGE * (page + 1)] = False
     for h in range(Hq):
         s = q[:, h].double() @ k[:, h * H // Hq].double().t() * scale
         s = torch.where(seen, s, torch.full_like(s, -math.inf))

@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from .ops import BlockMask, PreparedKV, attention, attention_prepared, fp8_mode, prepare_kv, rope_tables
+from .paged import PagedBatch, PagedKV, paged_attention, paged_write
 from .projections import PackedLinear, adaln_modulate, out_proj, pack_rows, qkv_attention
 
 
@@ -212,6 +213,49 @@ class PikaH3AttnProcessor:
             total -= self._cross_kv.pop(oldest)[1].workspace.numel()
         return kv
 
+    def write_paged(self, attn, states: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, position_ids: Optional[torch.Tensor] = None,
+                    rope_cos_sin: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, rope_key: Optional[Hashable] = None) -> None:
+        """Keys and values of ``states [1, T, C]`` (``attn``'s ``to_k`` / ``to_v``, K-side norm, rotation where positions are given) into the
+        pages of ``batch``: the rows of a continued document, or the text states of several requests, whose keys the denoising
+        steps then find in place (``paged_write=False``)."""
+        if states.dim() != 3 or states.shape[0] != 1:
+            raise ValueError(f"paged rows come packed, [1, T, C], got {tuple(states.shape)}")
+        T, H = states.shape[1], cache.heads
+        k, v = attn.to_k(states).view(T, H, -1), attn.to_v(states).view(T, H, -1)
+        if k.dtype != torch.bfloat16:
+            k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        qn, kn = getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
+        eps = getattr(qn, "eps", None)
+        opts = dict(k_norm_weight=_norm_weight(kn, k.shape[-1], k.device), norm_eps=self.norm_eps if eps is None else float(eps))
+        if rope_cos_sin is None and position_ids is not None:
+            rope_cos_sin = self._tables(position_ids, rope_key)
+        if rope_cos_sin is not None:
+            opts.update(rope_mode=self.rope_mode, rope_k=rope_cos_sin)
+        paged_write(cache, batch, k, v, **opts)
+
+    def _paged(self, attn, hidden_states, cache: PagedKV, batch: PagedBatch, *, write: bool, causal: bool, position_ids, rope_cos_sin,
+               rope_key) -> torch.Tensor:
+        if hidden_states.shape[0] != 1:
+            raise ValueError(f"paged rows come packed, [1, T, C], got {tuple(hidden_states.shape)}")
+        T, H = hidden_states.shape[1], int(attn.heads)
+        if rope_cos_sin is None and position_ids is not None:
+            rope_cos_sin = self._tables(position_ids, rope_key)
+        if write:
+            self.write_paged(attn, hidden_states, cache, batch, rope_cos_sin=rope_cos_sin)
+        q = attn.to_q(hidden_states).view(T, H, -1)
+        if q.dtype != torch.bfloat16:
+            q = q.to(torch.bfloat16)
+        qn = getattr(attn, "norm_q", None)
+        eps = getattr(qn, "eps", None)
+        scale = getattr(attn, "scale", None)
+        opts = dict(causal=causal, q_norm_weight=_norm_weight(qn, q.shape[-1], q.device), norm_eps=self.norm_eps if eps is None else float(eps),
+                    softmax_scale=None if scale is None else float(scale), workspace=self._workspace)
+        if rope_cos_sin is not None:
+            opts.update(rope_mode=self.rope_mode, rope_q=rope_cos_sin)
+        out = paged_attention(q, cache, batch, **opts).view(1, T, -1).to(hidden_states.dtype)
+        out = attn.to_out[0](out)
+        return attn.to_out[1](out) if len(attn.to_out) > 1 else out
+
     def __call__(
         self,
         attn,
@@ -229,6 +273,10 @@ class PikaH3AttnProcessor:
         gate_index: Optional[torch.Tensor] = None,
         residual: Optional[torch.Tensor] = None,
         cross_kv_key: Optional[Hashable] = None,
+        paged_kv: Optional[PagedKV] = None,
+        paged_batch: Optional[PagedBatch] = None,
+        paged_write: bool = True,
+        paged_causal: bool = False,
     ) -> torch.Tensor:
         """``hidden_states [B, S, H*D]`` -> ``[B, S, H*D]``.
 
@@ -249,9 +297,23 @@ class PikaH3AttnProcessor:
         ``cross_kv_key`` (with ``cache_cross_kv``): the caller's name for the prompt whose text states this call
         carries; prepared keys are then found by (module, key) instead of by tensor identity, see
         :meth:`_prepared_cross_kv`.
+
+        ``paged_kv`` and ``paged_batch``: ``hidden_states [1, T, C]`` holds the new rows of several sequences one behind the other, and
+        attention is over the keys that the pool (one per module; its heads may be fewer than the module's, in groups) holds of each of
+        them.  The rows' own keys are written first, unless ``paged_write`` is False: cross-attention to states whose keys
+        :meth:`write_paged` has put there.  ``paged_causal``: a row sees the keys up to its own.  Positions are those of the rows
+        (``position_ids [T, 3]``).  Masks, block maps, fp8 QK^T and the fused block do not go with it.
         """
         if hidden_states.dim() != 3:
             raise ValueError(f"hidden_states must be [B, S, C], got {tuple(hidden_states.shape)}")
+        if paged_kv is not None or paged_batch is not None:
+            if paged_kv is None or paged_batch is None:
+                raise ValueError("paged_kv and paged_batch go together")
+            if any(x is not None for x in (encoder_hidden_states, attention_mask, block_mask, adaln, gate, gate_index, residual, cross_kv_key)) or fp8_qk:
+                raise ValueError("paged attention takes rows, positions and a batch; masks, block maps, fp8 QK^T, encoder states (write_paged) and the "
+                                 "fused block's arguments do not go with it")
+            return self._paged(attn, hidden_states, paged_kv, paged_batch, write=bool(paged_write), causal=bool(paged_causal),
+                               position_ids=position_ids, rope_cos_sin=rope_cos_sin, rope_key=rope_key)
         B, S, _ = hidden_states.shape
         H = int(attn.heads)
         mask_given = attention_mask  # the caller's tensor: what the cross-attention key cache recognises

@@ -68,8 +68,9 @@ class Held:
         return P.stored(self.k[b].double(), self.fp8), P.stored(self.v[b].double(), self.fp8)
 
 
-def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scale=None, std=1.0, repeat=True):
-    """New rows over a cache against the oracle, every row and head; returns the output."""
+def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scale=None, std=1.0, repeat=True, on="cpu", missing=()):
+    """New rows over a cache against the oracle (run on device ``on``), every row and head; returns the output.  ``missing``: pages (sequence, which of
+    its pages) that are taken out of the table."""
     import pika_h3_flex_amd as pk
 
     P = _oracle()
@@ -79,10 +80,12 @@ def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scal
     w = (1.0 + 0.2 * torch.randn(D, generator=gen)) if norm else None
     tables = _tables(gen, T) if rope else None
     batch = held.batch(rows)
+    for b, page in missing:
+        batch.table[b, page] = -1
     opts = dict(causal=causal, q_norm_weight=_dev(w), norm_eps=EPS, rope_mode=rope, rope_q=_dev(tables), softmax_scale=scale)
     out = pk.paged_attention(q.cuda(), held.cache, batch, **opts)
     torch.cuda.synchronize()
-    got = out.cpu().double()
+    got = out.to(on).double()
     assert torch.isfinite(got).all()
     ready = P.norm_rope(q, w, EPS, tables, rope)
     if norm or rope:
@@ -90,7 +93,8 @@ def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scal
     at = 0
     for b, n in enumerate(rows):
         k, v = held.stored(b)
-        ref, size = P.attend(ready[at:at + n], k, v, causal=causal, scale=scale)
+        gone = [page for which, page in missing if which == b]
+        ref, size = P.attend(ready[at:at + n].to(on), k.to(on), v.to(on), causal=causal, scale=scale, gone=gone)
         d = 2.0 ** -14
         if (norm or rope) and k.numel():
             d = d + 4 * 2.0 ** -7 * float(ready.abs().max() * k.abs().max()) * (scale or 1 / math.sqrt(D))
@@ -257,12 +261,73 @@ def test_large_logits_raise_the_running_maximum(rows, fp8):
     _check_attention(held, rows, 4, causal=False, std=8.0)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows,Hq", [(1, 1), (20, 1), (60, 2), (450, 1)])
+@pytest.mark.parametrize("order", [1, -1])
+def test_logits_that_run_over_hundreds(rows, Hq, order, fp8):
+    """Keys along the queries, their logits from -200 to 200 (in powers of two: +-290) or the other way round: weights of whole tiles vanish beside those
+    of others, before or after them; all queries see their last or first keys alone in the end."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    n = 1000
+    held = Held([n], 1, fp8, seed=3)
+    gen = torch.Generator().manual_seed(1)
+    direction = torch.where(torch.rand(D, generator=gen) < 0.5, -1.0, 1.0)
+    ramp = torch.linspace(-200.0, 200.0, n)[::1] if order == 1 else torch.linspace(200.0, -200.0, n)
+    # q k / sqrt(D) = 8 * D * x / sqrt(D) with x = ramp / (8 sqrt(D)); every component of a key has the same size, so its e4m3 value is that of x
+    held.k[0] = ((ramp / (8 * math.sqrt(D)))[:, None, None] * direction).to(torch.bfloat16)
+    pk.paged_write(held.cache, held.batch([n]), held.k[0].cuda(), held.v[0].cuda())
+    q = (8.0 * direction).expand(rows, Hq, D).to(torch.bfloat16)
+    got = pk.paged_attention(q.cuda(), held.cache, held.batch([rows])).cpu().double()
+    k, v = held.stored(0)
+    ref, size = P.attend(q, k, v, causal=False)
+    # products are exact (q is a power of two), sums and exponents are fp32 of up to 290: 2^-23 * 290 * a few
+    bound = BF16 * ref.abs() + (BF16 + math.expm1(2 * 2.0 ** -10)) * size
+    assert torch.isfinite(got).all() and bool(((got - ref).abs() <= bound).all()), float((got - ref).abs().max())
+
+
+def _sweep(seed):
+    gen = torch.Generator().manual_seed(seed)
+    pick = lambda *x: x[int(torch.randint(len(x), (1,), generator=gen))]   # noqa: E731
+    size = lambda lo, hi: int(round(math.exp(float(torch.rand(1, generator=gen)) * math.log(hi / lo)) * lo))   # noqa: E731
+    B, kv = pick(1, 1, 2, 3, 7), pick(1, 2, 3, 4)
+    Hq = kv * pick(1, 1, 2, 5, 8)
+    top = pick(1, 40, 400, 1500)
+    lengths = [pick(0, size(1, 300), size(1, 9000)) if B > 1 else size(1, 20000) for _ in range(B)]
+    rows = [pick(0, size(1, top), size(1, top)) if B > 1 else size(1, top) for _ in range(B)]
+    missing = []
+    if pick(0, 0, 1):
+        missing = [(b, int(torch.randint(n // 64 + 1, (1,), generator=gen)) % ((n + 63) // 64)) for b, n in enumerate(lengths) if n for _ in range(3)]
+    if not any(rows):
+        rows[0] = 3
+    return dict(lengths=lengths, rows=rows, kv=kv, Hq=Hq, causal=bool(pick(0, 1)), norm=bool(pick(0, 1)), rope=pick(0, 1, 2), fp8=bool(pick(0, 1)), missing=missing)
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_random_batches(seed):
+    """Seeded: ragged batches of one to seven sequences, every form of the kernel, pages taken out of the table, against the oracle on the card."""
+    c = _sweep(seed)
+    held = Held(c["lengths"], c["kv"], c["fp8"], seed=seed)
+    _check_attention(held, c["rows"], c["Hq"], causal=c["causal"], seed=seed + 100, norm=c["norm"], rope=c["rope"], on="cuda", missing=c["missing"])
+
+
 def test_long_contexts_are_shared_out():
     """Few units of many tiles: every workgroup has a part of one, and the parts are joined."""
     held = Held([9000, 20000], 2, False, seed=3)
     _check_attention(held, [1, 1], 2, causal=True)
     _check_attention(held, [3, 20], 4, causal=True)
     _check_attention(Held([20000], 1, True, seed=3), [2], 8, causal=True)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_long_units_of_many_rows_are_shared_out(fp8):
+    """Units many times as long as a workgroup's run: runs inside a unit start in their middle, runs over a unit's end do the next one first; blocks with
+    rows for one, two and three waves a SIMD."""
+    held = Held([30000, 9000], 3, fp8, seed=3)
+    for rows in ([770, 130], [300, 0]):
+        _check_attention(held, rows, 3, causal=False, on="cuda", norm=True, rope=1)
+    _check_attention(held, [400, 200], 6, causal=True, on="cuda")
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -462,3 +527,88 @@ def test_agrees_with_attention_over_the_same_rows():
         size = pk.attention(q[None], k[None], v[None].abs())[0].float()
         d = 2.0 ** -8 * float(q.float().norm(dim=-1).max() * k.float().norm(dim=-1).max()) / math.sqrt(D)
         assert bool(((got.float() - dense.float()).abs() <= (4 * BF16 + math.expm1(2 * d)) * size).all())
+
+
+# ---- through the attention processor ----
+
+class _Norm(torch.nn.Module):
+    def __init__(self, gen):
+        super().__init__()
+        self.weight = torch.nn.Parameter(1.0 + 0.1 * torch.randn(D, generator=gen))
+        self.eps = EPS
+
+
+class _Module(torch.nn.Module):
+    """An attention module as the processor finds it: ``kv`` heads of keys and values, ``heads`` of queries."""
+
+    def __init__(self, heads, kv, width, seed):
+        super().__init__()
+        gen = torch.Generator().manual_seed(seed)
+        linear = lambda i, o: torch.nn.Linear(i, o, bias=False)   # noqa: E731
+        self.heads = heads
+        self.to_q, self.to_k, self.to_v = linear(width, heads * D), linear(width, kv * D), linear(width, kv * D)
+        self.to_out = torch.nn.ModuleList([linear(heads * D, width)])
+        for m in (self.to_q, self.to_k, self.to_v, self.to_out[0]):
+            m.weight.data = torch.randn(m.weight.shape, generator=gen) / math.sqrt(m.weight.shape[1])
+        self.to(torch.bfloat16)
+        self.norm_q, self.norm_k = _Norm(gen), _Norm(gen)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_document_continued_by_the_processor(fp8):
+    """Frames of two documents arrive chunk by chunk through the processor; every chunk's output is that of the library's calls on the rows that the
+    projections give, and without the cache's rounding the last one is that of the dense processor over the whole document."""
+    import pika_h3_flex_amd as pk
+
+    heads, kv, width = 4, 4, 256
+    mod = _Module(heads, kv, width, 3).cuda()
+    proc = pk.PikaH3AttnProcessor(rope_mode=pk.ROPE_INTERLEAVED)
+    lists = [[3, 0, 7, 5], [1, 4, 2, 6]]
+    cache, twin = pk.PagedKV(8, kv, fp8=fp8, device="cuda"), pk.PagedKV(8, kv, fp8=fp8, device="cuda")
+    gen = torch.Generator().manual_seed(8)
+    docs = [torch.randn((200, width), generator=gen).to(torch.bfloat16).cuda() for _ in range(2)]
+    where = torch.rand((2, 200, 3), generator=gen, dtype=torch.float64).cuda() * 30.0
+    have = [0, 0]
+    last = None
+    with torch.no_grad():
+        for step in ([100, 64], [1, 1], [99, 0], [0, 135]):
+            have = [h + n for h, n in zip(have, step)]
+            rows = torch.cat([docs[b][have[b] - step[b]:have[b]] for b in range(2)])
+            pos = torch.cat([where[b][have[b] - step[b]:have[b]] for b in range(2)])
+            batch = pk.PagedBatch.build(step, have, lists, device="cuda")
+            got = proc(mod, rows[None], position_ids=pos, paged_kv=cache, paged_batch=batch)
+            tabs = pk.rope_tables(pos)
+            heads_of = lambda x, h: x.view(len(rows), h, D)   # noqa: E731
+            pk.paged_write(twin, batch, heads_of(mod.to_k(rows), kv), heads_of(mod.to_v(rows), kv), k_norm_weight=mod.norm_k.weight.detach(), norm_eps=EPS,
+                           rope_mode=1, rope_k=tabs)
+            o = pk.paged_attention(heads_of(mod.to_q(rows), heads), twin, batch, q_norm_weight=mod.norm_q.weight.detach(), norm_eps=EPS, rope_mode=1, rope_q=tabs)
+            assert torch.equal(got[0], mod.to_out[0](o.view(len(rows), -1)))
+            last = (step, got)
+        if not fp8:
+            b = 1
+            dense = proc(mod, docs[b][None], position_ids=where[b])[0, 200 - last[0][b]:]
+            # both round weights, operands and outputs to bf16 on the way: differences of bf16 size
+            assert float((last[1][0].float() - dense.float()).norm() / dense.float().norm()) < 4 * BF16
+
+
+def test_text_keys_of_several_requests_through_the_processor():
+    """Cross-attention: text states of three requests of other lengths go into the pages once, and later steps find their keys there."""
+    import pika_h3_flex_amd as pk
+
+    heads, width = 4, 256
+    mod = _Module(heads, heads, width, 5).cuda()
+    proc = pk.PikaH3AttnProcessor()
+    text = [77, 302, 5]
+    rows = [130, 40, 64]
+    gen = torch.Generator().manual_seed(2)
+    states = [torch.randn((n, width), generator=gen).to(torch.bfloat16).cuda() for n in text]
+    cache = pk.PagedKV(9, heads, device="cuda")
+    lists = [[8, 1], [0, 3, 5, 7, 2], [6]]
+    with torch.no_grad():
+        proc.write_paged(mod, torch.cat(states)[None], cache, pk.PagedBatch.build(text, text, lists, device="cuda"))
+        batch = pk.PagedBatch.build(rows, text, lists, device="cuda")
+        for step in range(2):
+            x = [torch.randn((n, width), generator=gen).to(torch.bfloat16).cuda() for n in rows]
+            got = proc(mod, torch.cat(x)[None], paged_kv=cache, paged_batch=batch, paged_write=False)[0]
+            want = torch.cat([proc(mod, xs[None], encoder_hidden_states=t[None])[0] for xs, t in zip(x, states)])
+            assert float((got.float() - want.float()).norm() / want.float().norm()) < 4 * BF16

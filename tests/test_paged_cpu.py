@@ -304,3 +304,23 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
     for (size_t u = 0; u < units.size(); ++u) CHECK(joined[u] == (shared[u].empty() ? 0 : 1), "unit of %d parts joined %d times", (int)shared[u].size(), joined[u]);
   }
   CHECK(divided(7, 2) == 3 && divided(1ll << 40, 3) == (1ll << 40) / 3 && divided(5, 1ll << 33) == 0 && divided(4294967295ll, 7) == 4294967295ll / 7, "division");""")
+
+
+def test_the_processor_refuses_what_does_not_go_with_pages():
+    proc = pk.PikaH3AttnProcessor()
+    cache = pk.PagedKV(2, 1, device="cpu")
+    batch = pk.PagedBatch.build([3], [3], [[0]], device="cpu")
+    x = torch.zeros((1, 3, 128), dtype=torch.bfloat16)
+
+    class Attn:
+        heads = 1
+
+    with pytest.raises(ValueError, match="together"):
+        proc(Attn(), x, paged_kv=cache)
+    for bad in (dict(encoder_hidden_states=x), dict(attention_mask=torch.ones((1, 3), dtype=torch.bool)), dict(fp8_qk=True), dict(residual=x)):
+        with pytest.raises(ValueError, match="do not go with it"):
+            proc(Attn(), x, paged_kv=cache, paged_batch=batch, **bad)
+    with pytest.raises(ValueError, match="packed"):
+        proc(Attn(), x.expand(2, 3, 128), paged_kv=cache, paged_batch=batch)
+    with pytest.raises(ValueError, match="packed"):
+        proc.write_paged(Attn(), x[0], cache, batch)
