@@ -19,8 +19,11 @@
  * of scales.  A pool needs no clearing: what lies behind a sequence's last key is never part of a result, whatever it is.
  * With PKH3_PAGED_FP8 every key has two scales per head, one for K and one for V: the smallest power of two that is at least
  * max|x| / 448 (formed in float32, 2^-126 at least; 1 for a row of zeros), and x / scale is rounded to the nearest
- * e4m3 value.  (Stored values below 2^-126 may come back as 0.)  A row's values do not depend on the rows around it, so what is written once stays as it is.  What is not
- * finite is stored as NaN; it reaches the results of those rows that see its key.
+ * e4m3 value.  (Stored values below 2^-126 may come back as 0.)  A row's values do not depend on the rows around it, so
+ * what is written once stays as it is.  What is not finite is stored as NaN there, and as it is in bf16.  A NaN in a key makes
+ * the results of the rows that see the key NaN; a value that is not finite reaches the results of those rows too and, under
+ * PKH3_PAGED_CAUSAL, may reach those of rows of the same sequence and call in front of it (their weight of 0 times it is NaN).
+ * Keys that the batch does not hold (behind a length, on a page that is not there) reach nothing, whatever their memory holds.
  *
  * The batch.  B sequences share the pool.  Sequence b owns the rows starts[b] .. starts[b+1]-1 of the call (n of them) and has
  * lengths[b] keys, those of the call's rows among them where they are written; its i-th row stands at position
