@@ -119,6 +119,6 @@ hipError_t launch_paged_write(const PagedParams& p, bool fp8, hipStream_t st);
 hipError_t launch_paged_read(const PagedParams& p, bool fp8, hipStream_t st);
 hipError_t launch_paged_attn(const PagedParams& p, bool fp8, hipStream_t st);
 // scratch of the attention call in floats, from the sizes that the host knows
-size_t paged_attn_scratch(int rows, int B, int G);
+size_t paged_attn_scratch(int rows, int B, int H, int G, int table_pages, bool fp8);
 
 }  // namespace pkh3

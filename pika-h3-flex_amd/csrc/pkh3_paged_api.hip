@@ -105,7 +105,7 @@ PagedParams params(const pkh3_paged_args* a) {
 }
 
 size_t scratch(const pkh3_paged_args* a) {
-  return (paged_attn_scratch(a->rows, a->B, a->heads / a->kv_heads) * sizeof(float) + 255) / 256 * 256;
+  return (paged_attn_scratch(a->rows, a->B, a->kv_heads, a->heads / a->kv_heads, a->table_pages, a->flags & PKH3_PAGED_FP8) * sizeof(float) + 255) / 256 * 256;
 }
 
 }  // namespace

@@ -1090,18 +1090,29 @@ __global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
 
 // ---- host ----
 
-// The form of a call, from what the host knows of it: the query rows of a (sequence, kv head) on the average.
+// The form of a call, from what the host knows of it; the table's width stands for the lengths.  Where the query rows of a (sequence, kv head) are 32 or fewer on
+// the average, the split form.  Where they are more, it is still ahead while there is little to do: its blocks of 32 rows are twelve times as many, so that
+// all CUs have some, and a tile of one takes 0.4 us against 2.6.  The tile form takes about as long as one of its units of up to 16 tiles (longer ones are
+// cut), the split form as its tiles and kUnitTiles more a block: it goes as far as 900 blocks of 16 tiles.  (us, split / tile, bf16: 768 blocks over 128, 256,
+// 512 and 1,024 keys 19 / 22, 21 / 26, 26 / 34, 36 / 50; 1,152 blocks over 256 keys 30 / 26; 8 heads over 4,096 keys, 384 rows 29 / 44, 768 rows 38 / 48, three
+// such batches 55 / 55.)  It reads a key once for 32 rows: out of L2 that is well, but where a head's keys do not fit the 4 MB of one, or all
+// of them the 32 MB of all, it falls behind sooner (8 heads over 16,384 keys: 96 rows 38 / 40, 192 rows 63 / 46; 64 heads over 4,096: 96 rows 69 / 41).
 enum PagedForm { kSplit16, kSplit32, kTile };
-static PagedForm form_of(int rows, int B, int G) {
-  const int64_t per = (int64_t)rows * G / std::max(1, std::min(rows, B));
-  return per <= 16 ? kSplit16 : per <= 32 ? kSplit32 : kTile;
+static PagedForm form_of(int rows, int B, int H, int G, int table_pages, bool fp8) {
+  const int64_t all = (int64_t)rows * G, used = std::max(1, std::min(rows, B));
+  if (all <= 16 * used) return kSplit16;
+  if (all <= 32 * used) return kSplit32;
+  const int64_t tiles = (all / 32 + used) * H * (table_pages + kUnitTiles);
+  const int64_t keys = (int64_t)table_pages * (fp8 ? 1 : 2) * 16384;      // bytes of a head's
+  const bool cached = keys <= 4 << 20 && keys * H * used <= 32 << 20;
+  return tiles <= (cached ? 900 * (std::min(table_pages, kWholeTiles) + kUnitTiles) : 8192) ? kSplit32 : kTile;
 }
 static int rows_of(PagedForm f) { return f == kSplit16 ? 16 : f == kSplit32 ? 32 : kTileRows; }
 static int most_workgroups(PagedForm f) { return f == kTile ? kMaxShares / 2 : kMaxShares; }
 static int workgroups_of(PagedForm f, int cus) { return std::min(most_workgroups(f), std::max(8, (f == kTile ? 1 : 2) * cus / 8 * 8)); }
 
-size_t paged_attn_scratch(int rows, int B, int G) {
-  const PagedForm f = form_of(rows, B, G);
+size_t paged_attn_scratch(int rows, int B, int H, int G, int table_pages, bool fp8) {
+  const PagedForm f = form_of(rows, B, H, G, table_pages, fp8);
   return (size_t)2 * most_workgroups(f) * part_floats(rows_of(f)) + kCutFloats;
 }
 
@@ -1123,7 +1134,7 @@ hipError_t launch_paged_attn(const PagedParams& given, bool fp8, hipStream_t st)
   int cus = 0;
   const hipError_t e = device_cu_count(&cus);
   if (e != hipSuccess) return e;
-  const PagedForm f = form_of(p.rows, p.B, p.G.n);
+  const PagedForm f = form_of(p.rows, p.B, p.H, p.G.n, p.table_pages, fp8);
   const int grid = workgroups_of(f, cus);
   const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {

@@ -161,9 +161,9 @@ def _entry(name: str):
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(rows: int, B: int, table_pages: int, kv_heads: int, heads: int) -> int:
+def _workspace_bytes(rows: int, B: int, table_pages: int, kv_heads: int, heads: int, flags: int) -> int:
     """Scratch of an attention call: a matter of its sizes alone."""
-    args = _lib.PagedArgs(n_pages=1, B=B, table_pages=table_pages, rows=rows, kv_heads=kv_heads, heads=heads, D=HEAD_DIM)
+    args = _lib.PagedArgs(n_pages=1, B=B, table_pages=table_pages, rows=rows, kv_heads=kv_heads, heads=heads, D=HEAD_DIM, flags=flags)
     lib = _lib.load()
     n = int(lib.pkh3_paged_workspace_bytes(C.byref(args)))
     if n == 0:
@@ -241,7 +241,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     prep = _norm_rope(q_norm_weight, rope_mode, rope_q, rows, index)
     if not rows:
         return out
-    need = _workspace_bytes(rows, *batch._sizes, cache.heads, heads)
+    need = _workspace_bytes(rows, *batch._sizes, cache.heads, heads, cache.flags)
     if callable(workspace):
         workspace = workspace(cache.device, need)
     own = workspace is None or workspace.numel() * workspace.element_size() < need

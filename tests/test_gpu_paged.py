@@ -43,6 +43,8 @@ def _dev(t):
 class Held:
     """A pool on the card and, sequence by sequence, the rows (bf16, on the host) that went into it unchanged."""
 
+    width = 0   # least width of the tables of its batches, in pages (behind a sequence's own: none)
+
     def __init__(self, lengths, heads, fp8, seed=0, poison=True, std=1.0, spare=3):
         import pika_h3_flex_amd as pk
 
@@ -61,7 +63,10 @@ class Held:
     def batch(self, rows, lengths=None):
         import pika_h3_flex_amd as pk
 
-        return pk.PagedBatch.build(rows, self.lengths if lengths is None else lengths, self.lists, device="cuda")
+        lists = [own + [-1] * (Held.width - len(own)) for own in self.lists]
+        made = pk.PagedBatch.build(rows, self.lengths if lengths is None else lengths, self.lists, device="cuda")
+        table = torch.tensor([x + [-1] * (max(1, max(map(len, lists))) - len(x)) for x in lists], dtype=torch.int32, device="cuda")
+        return pk.PagedBatch(made.starts, made.lengths, table, made.rows)
 
     def stored(self, b):
         P = _oracle()
@@ -109,6 +114,14 @@ def _check_attention(held, rows, Hq, *, causal, seed=1, norm=False, rope=0, scal
         again = pk.paged_attention(q.cuda(), held.cache, batch, **opts)
         assert torch.equal(again, out)
     return out
+
+
+@pytest.fixture(params=["narrow", "wide"])
+def table_width(request):
+    """A call's form goes by the width of its table, which stands for the lengths: over a wide one chunks take the form of many rows, however few there are."""
+    Held.width = 0 if request.param == "narrow" else 8300
+    yield
+    Held.width = 0
 
 
 # ---- writing and reading ----
@@ -229,6 +242,7 @@ def test_single_tokens(lengths, kv, Hq, fp8):
     _check_attention(held, [1] * len(lengths), Hq, causal=False, norm=True, rope=1)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("rows,lengths,kv,Hq", [
@@ -240,6 +254,7 @@ def test_chunks(rows, lengths, kv, Hq, causal, fp8):
     _check_attention(held, rows, Hq, causal=causal)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("norm,rope,scale", [(True, 0, None), (False, 2, None), (True, 1, 0.05), (False, 0, 0.2)])
 def test_queries_through_norm_and_rotation(norm, rope, scale, fp8):
@@ -248,6 +263,7 @@ def test_queries_through_norm_and_rotation(norm, rope, scale, fp8):
         _check_attention(held, rows, 4, causal=True, norm=norm, rope=rope, scale=scale)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("rows", [[1, 1], [50, 130]])
 def test_large_logits_raise_the_running_maximum(rows, fp8):
@@ -261,6 +277,7 @@ def test_large_logits_raise_the_running_maximum(rows, fp8):
     _check_attention(held, rows, 4, causal=False, std=8.0)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("rows,Hq", [(1, 1), (20, 1), (60, 2), (450, 1)])
 @pytest.mark.parametrize("order", [1, -1])
@@ -304,12 +321,21 @@ def _sweep(seed):
     return dict(lengths=lengths, rows=rows, kv=kv, Hq=Hq, causal=bool(pick(0, 1)), norm=bool(pick(0, 1)), rope=pick(0, 1, 2), fp8=bool(pick(0, 1)), missing=missing)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("seed", range(60))
 def test_random_batches(seed):
     """Seeded: ragged batches of one to seven sequences, every form of the kernel, pages taken out of the table, against the oracle on the card."""
     c = _sweep(seed)
     held = Held(c["lengths"], c["kv"], c["fp8"], seed=seed)
     _check_attention(held, c["rows"], c["Hq"], causal=c["causal"], seed=seed + 100, norm=c["norm"], rope=c["rope"], on="cuda", missing=c["missing"])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_short_tables_under_many_rows(fp8):
+    """Tables of a few pages and rows enough for every workgroup: units are not cut, and there is no second launch."""
+    held = Held([70, 300, 1000, 512, 0], 8, fp8, seed=6)
+    _check_attention(held, [450, 900, 1400, 30, 2], 8, causal=False, on="cuda", norm=True, rope=2)
+    _check_attention(held, [90, 200, 640, 512, 70], 16, causal=True, on="cuda")
 
 
 def test_long_contexts_are_shared_out():
@@ -320,6 +346,7 @@ def test_long_contexts_are_shared_out():
     _check_attention(Held([20000], 1, True, seed=3), [2], 8, causal=True)
 
 
+@pytest.mark.usefixtures("table_width")
 @pytest.mark.parametrize("fp8", [False, True])
 def test_long_units_of_many_rows_are_shared_out(fp8):
     """Units many times as long as a workgroup's run: runs inside a unit start in their middle, runs over a unit's end do the next one first; blocks with
