@@ -968,59 +968,83 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
 // ---- the parts of units that more than one workgroup worked on ----
 //
 // Workgroup i of the launch in front, if its run begins inside a unit and is the first that does, has left in cut[i] which unit that is and how many
-// runs share it: its parts are slot 1 of run i - 1 and slot 0 of i, i + 1, .., in that order.  Eight rows a workgroup (blockIdx.y); 32 threads
-// have a row, four columns each, and where there are fewer rows than that takes, its parts are dealt out to several such groups.  (Found by
-// every workgroup for itself, from the sums of the whole batch, the units were most of this launch: 41 to 52 us of 256 x 48 workgroups.)
+// runs share it: its parts are slot 1 of run i - 1 and slot 0 of i, i + 1, .., in that order.  This launch takes as long as what hangs together in it: eight
+// parts are asked for at once.  (Found by every workgroup for itself, from the sums of the whole batch, the units were most of it:
+// 41 to 52 us of 256 x 48 workgroups.)
+constexpr int kPartsAtOnce = 8;
+
+// `n` of eight parts (all of them in registers) to what is there of those in front
+__device__ __forceinline__ void add_parts(float& top, float& l, f32x4& sum, const float (&m)[kPartsAtOnce], const float (&w)[kPartsAtOnce],
+                                          const f32x4 (&o)[kPartsAtOnce], int n) {
+  float most = top;
+#pragma unroll
+  for (int i = 0; i < kPartsAtOnce; ++i) most = i < n ? fmaxf(most, m[i]) : most;
+  const float a0 = __builtin_amdgcn_exp2f(top - most);
+  top = most;
+  l *= a0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sum[k] *= a0;
+#pragma unroll
+  for (int i = 0; i < kPartsAtOnce; ++i) {
+    if (i < n) {
+      const float a = __builtin_amdgcn_exp2f(m[i] - top);
+      l += a * w[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] += a * o[i][k];
+    }
+  }
+}
+
+// An eighth of a unit's rows a workgroup (blockIdx.y), 32 threads a row and part, four columns each: a row's parts are dealt out to four such groups (of
+// units of 16 rows) or two, a single row's to eight.  (Eight rows a workgroup, a group each, their parts one after the other: 768 rows over 16,384 keys
+// 60 us where it is 58 now, single tokens of 32 query heads over 8,192 keys 31.5 and 29.5.)
 template <int RB>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
+  constexpr int kRows = RB / 8;
   __shared__ f32x4 part_sum[256];
   __shared__ float part_m[8], part_l[8];
   const int run = (int)blockIdx.x + 1;
   const i32x4 cut = p.cuts[run];
   if (run >= p.cuts[0][0] || cut[3] == 0) return;
   const Sequence s = uniform_sequence(p, cut[0]);
-  const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)blockIdx.y * 8;
+  const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)blockIdx.y * kRows;
   if (row0 >= rows) return;
-  const int here = min(8, rows - row0), groups = here == 1 ? 8 : here == 2 ? 4 : here <= 4 ? 2 : 1;   // groups of 32 threads a row
+  const int here = min(kRows, rows - row0), groups = here > 2 ? 2 : 8 / here;   // groups of 32 threads a row
   const int mine = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
-  const int row = row0 + mine / groups, sub = mine % groups;
-  const bool live = mine / groups < here;
-  auto slot = [&](int i) { return p.partials + part_slot(run - 1 + i, i == 0) * part_floats(RB); };
+  const int row = min(row0 + mine / groups, rows - 1), sub = mine % groups;   // (those past the last: as the last, not stored)
   float top = kNoMax, l = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-#pragma unroll 4
-    for (int i = sub; i < cut[3]; i += groups) top = fmaxf(top, slot(i)[RB * kD + row]);
-#pragma unroll 4
-    for (int i = sub; i < cut[3]; i += groups) {
-      const float* t = slot(i);
-      const float a = __builtin_amdgcn_exp2f(t[RB * kD + row] - top);
-      l += a * t[RB * (kD + 1) + row];
-      const f32x4 o = *(const f32x4*)(t + row * kD + col);
+#pragma unroll 1
+  for (int i0 = sub; i0 < cut[3]; i0 += kPartsAtOnce * groups) {
+    float m[kPartsAtOnce], w[kPartsAtOnce];
+    f32x4 o[kPartsAtOnce];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
+    for (int i = 0; i < kPartsAtOnce; ++i) {
+      const int part = min(i0 + i * groups, cut[3] - 1);
+      const float* t = p.partials + part_slot(run - 1 + part, part == 0) * part_floats(RB);
+      m[i] = t[RB * kD + row];
+      w[i] = t[RB * (kD + 1) + row];
+      o[i] = *(const f32x4*)(t + row * kD + col);
     }
+    add_parts(top, l, sum, m, w, o, (cut[3] - i0 + groups - 1) / groups);
   }
-  if (groups > 1) {                                                        // (the same for the whole workgroup)
-    part_sum[threadIdx.x] = sum;
-    if ((threadIdx.x & 31) == 0) part_m[mine] = top, part_l[mine] = l;
-    __syncthreads();
-    if (sub != 0) return;
-    const float own = top;
-    for (int g = 1; g < groups; ++g) top = fmaxf(top, part_m[mine + g]);
-    const float a0 = __builtin_amdgcn_exp2f(own - top);
-    l *= a0;
+  part_sum[threadIdx.x] = sum;
+  if ((threadIdx.x & 31) == 0) part_m[mine] = top, part_l[mine] = l;
+  __syncthreads();
+  if (sub != 0 || mine / groups >= here) return;
+  const float own = top;
+  for (int g = 1; g < groups; ++g) top = fmaxf(top, part_m[mine + g]);
+  const float a0 = __builtin_amdgcn_exp2f(own - top);
+  l *= a0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] *= a0;
-    for (int g = 1; g < groups; ++g) {
-      const float a = __builtin_amdgcn_exp2f(part_m[mine + g] - top);
-      l += a * part_l[mine + g];
-      const f32x4 o = part_sum[threadIdx.x + 32 * g];
+  for (int e = 0; e < 4; ++e) sum[e] *= a0;
+  for (int g = 1; g < groups; ++g) {
+    const float a = __builtin_amdgcn_exp2f(part_m[mine + g] - top);
+    l += a * part_l[mine + g];
+    const f32x4 o = part_sum[threadIdx.x + 32 * g];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
-    }
+    for (int e = 0; e < 4; ++e) sum[e] += a * o[e];
   }
-  if (!live) return;
   const float inv = inverse_sum(l);
   bf16x4 out;
 #pragma unroll
@@ -1030,9 +1054,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
 }
 
 // The same for the tile form, whose parts lie as its lanes hold them: blockIdx.y / 2 is a block of 16 rows, and wave w has the columns 16*db .. +15 of it for
-// db = 4 * (blockIdx.y % 2) + w, four of row c a lane (16*g + c).  Eight parts are on their way at once.  The rows go out by way of LDS.
+// db = 4 * (blockIdx.y % 2) + w, four of row c a lane (16*g + c).  The rows go out by way of LDS.
 __global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
-  constexpr int RB = kTileRows, kAtOnce = 8;
+  constexpr int RB = kTileRows;
   __shared__ __attribute__((aligned(16))) char turn[2048];
   const int run = (int)blockIdx.x + 1;
   const i32x4 cut = p.cuts[run];
@@ -1046,34 +1070,18 @@ __global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
   float top = kNoMax, l = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-  for (int i0 = 0; i0 < cut[3]; i0 += kAtOnce) {
-    float m[kAtOnce], w[kAtOnce];
-    f32x4 o[kAtOnce];
+  for (int i0 = 0; i0 < cut[3]; i0 += kPartsAtOnce) {
+    float m[kPartsAtOnce], w[kPartsAtOnce];
+    f32x4 o[kPartsAtOnce];
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
+    for (int i = 0; i < kPartsAtOnce; ++i) {
       const int part = min(i0 + i, cut[3] - 1);
       const float* t = p.partials + part_slot(run - 1 + part, part == 0) * part_floats(RB);
       m[i] = t[RB * kD + at];
       w[i] = t[RB * (kD + 1) + at];
       o[i] = *(const f32x4*)(t + col);
     }
-    float most = top;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) most = i0 + i < cut[3] ? fmaxf(most, m[i]) : most;
-    const float a0 = __builtin_amdgcn_exp2f(top - most);
-    top = most;
-    l *= a0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] *= a0;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      if (i0 + i < cut[3]) {
-        const float a = __builtin_amdgcn_exp2f(m[i] - top);
-        l += a * w[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] += a * o[i][k];
-      }
-    }
+    add_parts(top, l, sum, m, w, o, cut[3] - i0);
   }
   const float inv = inverse_sum(l);
   bf16x4 v;
@@ -1139,9 +1147,9 @@ hipError_t launch_paged_attn(const PagedParams& given, bool fp8, hipStream_t st)
   const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {
     case kSplit16:
-      return launch_form(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 64 * kSplitWaves, paged_merge_kernel<16>, 2, grid, p, st);
+      return launch_form(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 64 * kSplitWaves, paged_merge_kernel<16>, 8, grid, p, st);
     case kSplit32:
-      return launch_form(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 64 * kSplitWaves, paged_merge_kernel<32>, 4, grid, p, st);
+      return launch_form(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 64 * kSplitWaves, paged_merge_kernel<32>, 8, grid, p, st);
     default:
       return launch_form(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
                              : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>),

@@ -90,7 +90,7 @@ constexpr int tiles_left(int64_t left, int t, int nt, int cost) {
 
 // The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
 constexpr int kMaxShares = 512;       // workgroups of a launch at most
-constexpr int kMinShareTiles = 4;     // fewest tiles a workgroup is started for
+constexpr int least_tiles(int rb) { return rb == 384 ? 1 : 2; }   // fewest tiles a workgroup is started for (units that are cut)
 constexpr int kWholeTiles = 16;       // a unit of at most so many, and no dearer than a run, is not cut
 struct Shares {
   int64_t total;
@@ -100,7 +100,7 @@ struct Shares {
   constexpr int64_t run() const { return divided(total, n); }
 };
 constexpr Shares shares_of(int64_t total, int most, int rb, bool whole) {
-  const int64_t worth = total / (((whole ? 1 : kMinShareTiles) + kUnitTiles) * (whole ? 1 : most_cost(rb)));
+  const int64_t worth = total / (((whole ? 1 : least_tiles(rb)) + kUnitTiles) * (whole ? 1 : most_cost(rb)));
   return {total, (int)(worth < 1 ? 1 : worth < most ? worth : most), whole};
 }
 // The workgroup of a launch that takes run `rank`: a contiguous run of runs per XCD.  -1: none.
