@@ -529,6 +529,46 @@ def test_a_given_workspace_may_hold_anything():
     assert torch.equal(pk.paged_attention(q, held.cache, batch, workspace=small), want)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_past_32_bits(new, fp8):
+    """Pages behind the pool's first 4 GiB, and rows more than 4 GiB apart in their tensors: written, read back and attended to as the same rows close together are."""
+    import pika_h3_flex_amd as pk
+
+    P, H = _oracle(), 24
+    pages = -(-(5 << 30) // (H * int(pk._lib.load().pkh3_paged_record_bytes(pk._lib.PAGED_FP8 if fp8 else 0))))
+    cache = pk.PagedKV(pages, H, fp8=fp8, device="cuda")
+    lists, lengths = [[pages - 1, 0, pages - 3], [pages - 2]], [150, 64]
+    gen = torch.Generator().manual_seed(4)
+    k, v = (_rows(gen, sum(lengths), H) for _ in range(2))
+    pk.paged_write(cache, pk.PagedBatch.build(lengths, lengths, lists, device="cuda"), k.cuda(), v.cuda())
+    sk, sv = (P.stored(t.double(), fp8) for t in (k, v))
+    back = pk.paged_read(cache, pk.PagedBatch.build(lengths, lengths, lists, device="cuda"))
+    assert torch.equal(back[0].cpu().double(), sk) and torch.equal(back[1].cpu().double(), sv)
+    q = _rows(gen, 2 * new, H)
+    batch = pk.PagedBatch.build([new, new], lengths, lists, device="cuda")
+    got = pk.paged_attention(q.cuda(), cache, batch)
+    for b, (lo, hi) in enumerate(((0, 150), (150, 214))):
+        ref, size = P.attend(q[b * new:(b + 1) * new], sk[lo:hi], sv[lo:hi], causal=False)
+        off = (got[b * new:(b + 1) * new].cpu().double() - ref).abs() - (BF16 * ref.abs() + (BF16 + 2.0 ** -12) * size)
+        assert float(off.max()) <= 0.0
+    if new == 1:   # two rows, 2^31 + 64 elements from one to the other
+        step = 2 ** 31 + 64
+        far = torch.empty(step + H * D, dtype=torch.bfloat16, device="cuda").as_strided((2, H, D), (step, D, 1))
+        far.copy_(q.cuda())
+        assert torch.equal(pk.paged_attention(far, cache, batch), got)
+        pk.paged_attention(q.cuda(), cache, batch, out=far)
+        assert torch.equal(far, got)
+        far.copy_(k[:2].cuda())
+        ends = pk.PagedBatch.build([1, 1], lengths, lists, device="cuda")
+        pk.paged_write(cache, ends, far, far)
+        near = pk.paged_read(cache, ends)
+        assert torch.equal(near[0].cpu().double(), sk[:2])
+        far.zero_()
+        pk.paged_read(cache, ends, out=(near[1], far))
+        assert torch.equal(far.cpu().double(), P.stored(k[:2].double(), fp8))
+
+
 def test_empty_calls():
     import pika_h3_flex_amd as pk
 
