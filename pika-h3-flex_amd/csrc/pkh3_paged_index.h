@@ -91,7 +91,7 @@ constexpr int tiles_left(int64_t left, int t, int nt, int cost) {
 // The tiles of all units end to end, at their cost, in equal runs for `n` workgroups.  (The division is the 32-bit one where that does.)
 constexpr int kMaxShares = 512;       // workgroups of a launch at most
 constexpr int least_tiles(int rb) { return rb == 384 ? 1 : 2; }   // fewest tiles a workgroup is started for (units that are cut)
-constexpr int kWholeTiles = 16;       // a unit of at most so many, and no dearer than a run, is not cut
+constexpr int kWholeTiles = 16;       // pages of a table under which no unit is cut
 struct Shares {
   int64_t total;
   int n;
@@ -108,11 +108,12 @@ constexpr int rank_of(int block, const Shares& sh) {
   const int per_xcd = (sh.n + 7) / 8, rank = (block & 7) * per_xcd + (block >> 3);
   return (block >> 3) < per_xcd && rank < sh.n ? rank : -1;
 }
-// A run boundary that lies `in` behind the beginning of a unit of nt tiles at this cost goes to the tile there, or to the nearer end of a unit that is not
-// cut, or to an end that is so near that a part of its own costs more than it gives.  The result may be nt: the next unit's beginning.
-constexpr int kNearTiles = 3;
+// A run boundary that lies `in` behind the beginning of a unit of nt tiles at this cost goes to the tile there, or to an end that is so near that a part
+// of its own costs more than it gives, or where no unit is cut to the nearer end.  The result may be nt: the next unit's beginning.  (Three tiles for
+// near, and units of up to 16 tiles and a run uncut: five ragged prompts 83 us where they are 74 now, nine of up to 2,930 rows 83 and 75.)
+constexpr int kNearTiles = 2;
 constexpr int boundary_tile(const Shares& sh, int64_t in, int nt, int cost) {
-  if (sh.whole || (nt <= kWholeTiles && unit_length(nt, cost) <= sh.run())) return 2 * in >= unit_length(nt, cost) ? nt : 0;
+  if (sh.whole) return 2 * in >= unit_length(nt, cost) ? nt : 0;
   const int t = (int)divided(in, cost) - kUnitTiles;
   return t > kNearTiles ? (t < nt - kNearTiles ? t : nt) : 2 * t < nt ? 0 : nt;
 }
