@@ -10,8 +10,9 @@
 // do not depend on who is first.  (At most two parts a workgroup: the unit its run begins in and the one it ends in.)
 //
 // The arithmetic is that of the dense calls (see pkh3_attn_fwd.hip): S^T = K Q'^T and O^T += V^T P^T on the 16x16x32 MFMA, P
-// from one to the other in its lane, running maximum raised when exceeded by 2^8.  Q' is rounded to bf16 after norm and rotation and not
-// before: the softmax scale multiplies S^T (in fp32, in the subtraction of the maximum), so that queries without norm and rotation are exact.
+// from one to the other in its lane, running maximum raised when exceeded by 2^8.  Queries without norm and rotation are taken as they are, and the softmax
+// scale multiplies S^T (in fp32, in the subtraction of the maximum).  After norm or rotation Q' is rounded to bf16, as in the dense calls: to
+// keep what that leaves would be half as many products of S^T again, and registers that the tile form does not have.  Blocks of 16 rows keep it.
 // e4m3 keys times their power of two are exact in bf16; the scale of a value's key goes to P instead, exact there as well.
 #include <math.h>
 
@@ -187,7 +188,10 @@ __host__ __device__ constexpr int part_floats(int rb) { return rb * (kD + 2); }
 //
 // A unit is one or two blocks of 16 query rows, and each of the four waves walks a quarter of the run's part of it in 32-key halves.  No two
 // waves read the same images, so these go straight from memory into the registers of the MFMAs: no LDS and no barrier in the loop, the
-// next keys asked for under the softmax, the values under S^T.  The waves' results meet in LDS.  Bound by the bytes of K and V.
+// next keys asked for under the softmax, the values under S^T.  The waves' results meet in LDS.  Bound by the bytes of K and V: one token of 24 heads
+// over 124,992 keys 261 us, 5.9 TB/s; eight over up to 48,360 in e4m3 214, 5.7 TB/s.  REST: what the rounding of Q' to bf16 leaves is kept, in
+// bf16 as well, and its products with K are added to S^T; under the bytes of 16 rows that is free (the error of a result against 64 bits falls from 0.0029 of
+// it to 0.0024, where the rounding of P and of the result is left), with 32 rows, whose keys come out of L2, calls took up to 1.8 times as long.
 
 template <bool FP8, int QB>
 struct SplitState {
@@ -269,8 +273,8 @@ __device__ __forceinline__ void ask_queries(const PagedParams& p, const Sequence
     q.v[i] = *(const i32x4*)(p.q + row_offset(p, s, h, min(r0 + 4 * i + (lane >> 4), last), p.q_ss, p.q_sh, token) + (lane & 15) * 16);
 }
 // .. and through norm and rotation, in the lane order of the B images, by way of 4 KiB of LDS of the wave's own
-__device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, const NormLanes& norm, char* turn, int lane,
-                                              float factor, bf16x8 (&out)[4]) {
+__device__ __forceinline__ void queries_moved(const PagedParams& p, const Sequence& s, int r0, const Rows16& q, const NormLanes& norm, char* turn, int lane,
+                                              float factor, float (&x)[32]) {
   Rows16 cos, sin;
   RopeQuarter rope;
   if (p.rope_mode != 0) {
@@ -289,16 +293,11 @@ __device__ __forceinline__ void queries_ready(const PagedParams& p, const Sequen
     turn_table(cos, rope.c, p.rope_mode, turn, lane);
     turn_table(sin, rope.s, p.rope_mode, turn, lane);
   }
-  float x[32];
   norm_row(x, raw, p.norm_w != nullptr, p.eps, norm, factor);
   rope_row(x, p.rope_mode, rope);
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) out[ks][j] = (__bf16)x[8 * ks + j];
 }
 
-template <bool FP8, int QB>
+template <bool FP8, int QB, bool REST>
 __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedParams p) {
   constexpr int RB = 16 * QB, NW = kSplitWaves;
   constexpr int kSlot = QB * 8 * 64 * 16;                      // one wave's O^T in fp32
@@ -307,7 +306,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
   constexpr int kVOff = FP8 ? kK8TileBytes : kKTileBytes;
   constexpr int kScaleOff = kK8TileBytes + kVTileBytes / 2;
   __shared__ __attribute__((aligned(1024))) char part[NW * kSlot];
-  __shared__ __attribute__((aligned(1024))) char rows[QB * 4096];
+  static_assert(!REST || QB == 1, "see above");
+  __shared__ __attribute__((aligned(1024))) char rows[(REST ? 2 : 1) * QB * 4096];   // Q' in bf16, and what that leaves
   __shared__ float part_m[NW][QB][16], part_l[NW][QB][16];
   static_assert((kMaxSequences + 1) * sizeof(int64_t) <= sizeof(part), "the sums lie where the waves' results meet afterwards");
   const int lane = threadIdx.x & 63, c16 = lane & 15, g4 = lane >> 4;
@@ -363,14 +363,24 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
       ask_k(id, first & 1);
     }
     if (wave < QB) {
-      bf16x8 img[4];
       Rows16 q;
       ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
       NormLanes norm;
       load_norm_lanes(norm, p.norm_w, lane);
-      queries_ready(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, img);
+      float x[32];
+      queries_moved(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, x);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) *(bf16x8*)(rows + ((wave * 4 + ks) * 64 + lane) * 16) = img[ks];
+      for (int ks = 0; ks < 4; ++ks) {
+        bf16x8 img, rest;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          img[j] = (__bf16)x[8 * ks + j];
+          rest[j] = (__bf16)(x[8 * ks + j] - (float)img[j]);
+        }
+        char* to = rows + ((wave * 4 + ks) * 64 + lane) * 16;
+        *(bf16x8*)to = img;
+        if constexpr (REST) *(bf16x8*)(to + QB * 4096) = rest;
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -378,6 +388,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) w.qf[qb][ks] = *(const bf16x8*)(rows + ((qb * 4 + ks) * 64 + lane) * 16);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    auto rest = [&](int qb, int ks) { return *(const bf16x8*)(rows + QB * 4096 + ((qb * 4 + ks) * 64 + lane) * 16); };
 #pragma unroll 1
     for (int i = first; i < end; ++i) {
       const int next = min(i + 1, end - 1);
@@ -396,10 +407,15 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
       f32x4 sT[2][QB];
       if constexpr (!FP8) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)                            // image (ks, kb) = (j / 2, j % 2)
+        for (int j = 0; j < 8; ++j) {                          // image (ks, kb) = (j / 2, j % 2)
+          if constexpr (REST) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) sT[j & 1][qb] = PKH3_MFMA16(__builtin_bit_cast(bf16x8, kf[j]), rest(qb, j >> 1), j < 2 ? zero : sT[j & 1][qb]);
+          }
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb)
-            sT[j & 1][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[j]), w.qf[qb][j >> 1], j < 2 ? zero : sT[j & 1][qb], 0, 0, 0);
+            sT[j & 1][qb] = PKH3_MFMA16(__builtin_bit_cast(bf16x8, kf[j]), w.qf[qb][j >> 1], !REST && j < 2 ? zero : sT[j & 1][qb]);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {                          // chunk (kb, c2) = (j / 2, j % 2): images ks = 2*c2, 2*c2 + 1
@@ -407,9 +423,13 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const bf16x8 a = expand_fp8(kf[j][2 * e], kf[j][2 * e + 1], scale);
+            const int ks = 2 * (j & 1) + e;
+            if constexpr (REST) {
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-              sT[j >> 1][qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w.qf[qb][2 * (j & 1) + e], (j & 1) + e == 0 ? zero : sT[j >> 1][qb], 0, 0, 0);
+              for (int qb = 0; qb < QB; ++qb) sT[j >> 1][qb] = PKH3_MFMA16(a, rest(qb, ks), ks == 0 ? zero : sT[j >> 1][qb]);
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) sT[j >> 1][qb] = PKH3_MFMA16(a, w.qf[qb][ks], !REST && ks == 0 ? zero : sT[j >> 1][qb]);
           }
         }
       }
@@ -832,7 +852,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
         const int l = lane_here();
         NormLanes norm;
         load_norm_lanes(norm, norm_w, l);
-        queries_ready(arguments_here(), s, r0 + 16 * qb, ahead[qb], norm, turn, l, FOLD ? p.c : 1.0f, w.qf[qb]);
+        float x[32];
+        queries_moved(arguments_here(), s, r0 + 16 * qb, ahead[qb], norm, turn, l, FOLD ? p.c : 1.0f, x);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w.qf[qb][ks][j] = (__bf16)x[8 * ks + j];
       }
     }
     const int all_see = __builtin_amdgcn_readfirstlane(row_keys(p, s, r0));   // keys that every row of the wave sees
@@ -1152,15 +1177,16 @@ hipError_t launch_paged_attn(const PagedParams& given, bool fp8, hipStream_t st)
   if (e != hipSuccess) return e;
   const PagedForm f = form_of(p.rows, p.B, p.H, p.G.n, p.table_pages, fp8);
   const int grid = workgroups_of(f, p, cus);
-  const bool fold = p.norm_w != nullptr || p.rope_mode != 0;
+  const bool moved = p.norm_w != nullptr || p.rope_mode != 0;
   switch (f) {
     case kSplit16:
-      return launch_form(fp8 ? paged_split_kernel<true, 1> : paged_split_kernel<false, 1>, 64 * kSplitWaves, paged_merge_kernel<16>, 8, grid, p, st);
+      return launch_form(fp8 ? (moved ? paged_split_kernel<true, 1, true> : paged_split_kernel<true, 1, false>)
+                             : (moved ? paged_split_kernel<false, 1, true> : paged_split_kernel<false, 1, false>), 64 * kSplitWaves, paged_merge_kernel<16>, 8, grid, p, st);
     case kSplit32:
-      return launch_form(fp8 ? paged_split_kernel<true, 2> : paged_split_kernel<false, 2>, 64 * kSplitWaves, paged_merge_kernel<32>, 8, grid, p, st);
+      return launch_form(fp8 ? paged_split_kernel<true, 2, false> : paged_split_kernel<false, 2, false>, 64 * kSplitWaves, paged_merge_kernel<32>, 8, grid, p, st);
     default:
-      return launch_form(fp8 ? (fold ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
-                             : (fold ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>),
+      return launch_form(fp8 ? (moved ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>)
+                             : (moved ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>),
                          64 * kTileWaves, paged_merge_tile_kernel, kTileRows / 8, grid, p, st);
   }
 }

@@ -1,4 +1,6 @@
-// Writing the paged K/V cache and reading it back.  Both are one pass over rows and pages, bound by HBM.
+// Writing the paged K/V cache and reading it back.  Both are one pass over rows and pages, bound by HBM: 15,342 rows of 24 heads in e4m3 are
+// written in 59 to 67 us (norm, rotation, rounding; 288 MB, 4.3 to 4.9 TB/s) and read back in 47 to 48 (284 MB, 5.9 TB/s).  A few rows are a launch:
+// 4.4 and 3.7 us.
 //
 // A workgroup takes one 64-key tile of one sequence for `heads_per_wg` heads, its K or its V (by the parity of blockIdx.x), as the
 // K/V pass of the dense calls does: rows as they lie in memory, turned around in LDS into the lane order of the operand images.

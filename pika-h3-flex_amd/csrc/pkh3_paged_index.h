@@ -75,8 +75,8 @@ constexpr int block_cost(const Sequence& s, const Group& G, int rb, int j) {
   return rows > 256 ? 4 : rows > 128 ? 3 : 2;
 }
 
-// What a unit costs besides its tiles, in tiles: queries in and out, the first keys' way.  Units of 384 rows against 2, 5 and 8 tiles took 8 us and 2.7 a
-// tile; shared out by their tiles alone, the last workgroup of such a call was done at 320 us and the first at 102.
+// What a unit costs besides its tiles, in tiles: queries in and out, the first keys' way.  Units of 384 rows against 2 and 8 tiles take 10 us and 3.0 a
+// tile, longer ones 7 and 2.4 to 2.9; shared out by their tiles alone, the last workgroup of such a call was done at 320 us and the first at 102.
 constexpr int kUnitTiles = 4;
 constexpr int64_t unit_length(int nt, int cost) { return (int64_t)(nt + kUnitTiles) * cost; }
 // where tile t of a unit begins
