@@ -42,6 +42,10 @@ class PagedKV:
         self._head = (data.data_ptr(), self.pages)
         self._index = data.get_device()
 
+    def __reduce__(self):
+        # copies and pickles are made anew: what is kept beside the tensor holds its address
+        return _pool_of, (self.pages, self.heads, self.fp8, self._data)
+
     @property
     def data(self) -> torch.Tensor:
         return self._data
@@ -51,12 +55,17 @@ class PagedKV:
         return self._data.device
 
 
+def _pool_of(pages: int, heads: int, fp8: bool, data: torch.Tensor) -> PagedKV:
+    return PagedKV(pages, heads, fp8=fp8, data=data)
+
+
 @dataclass(frozen=True)
 class PagedBatch:
     """The sequences of a call: int32 device tensors ``starts [B + 1]`` (sequence b owns the call's rows ``starts[b] ..
     starts[b+1]-1``, its newest), ``lengths [B]`` (its keys, these rows among them where they are written) and ``table [B, P]``
     (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows them.  What the tensors hold may be
-    changed in place between calls, replays of a captured graph among them; include/pkh3_paged.h says what out-of-range values do."""
+    changed in place between calls, replays of a captured graph among them, the tensors themselves stay where they are;
+    include/pkh3_paged.h says what out-of-range values do."""
 
     starts: torch.Tensor
     lengths: torch.Tensor
@@ -80,6 +89,9 @@ class PagedBatch:
         object.__setattr__(self, "_arrays", (self.starts.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), self.table.stride(0)))
         object.__setattr__(self, "_sizes", (B, self.table.shape[1]))
         object.__setattr__(self, "_index", index)
+
+    def __reduce__(self):
+        return PagedBatch, (self.starts, self.lengths, self.table, self.rows)
 
     @staticmethod
     def build(new_rows: Sequence[int], lengths: Sequence[int], pages: Sequence[Sequence[int]], *, device=None) -> "PagedBatch":

@@ -224,8 +224,8 @@ class PikaH3AttnProcessor:
         k, v = attn.to_k(states).view(T, H, -1), attn.to_v(states).view(T, H, -1)
         if k.dtype != torch.bfloat16:
             k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
-        qn, kn = getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
-        eps = getattr(qn, "eps", None)
+        kn = getattr(attn, "norm_k", None)
+        eps = getattr(kn, "eps", None)
         opts = dict(k_norm_weight=_norm_weight(kn, k.shape[-1], k.device), norm_eps=self.norm_eps if eps is None else float(eps))
         if rope_cos_sin is None and position_ids is not None:
             rope_cos_sin = self._tables(position_ids, rope_key)

@@ -691,3 +691,22 @@ def test_text_keys_of_several_requests_through_the_processor():
             got = proc(mod, torch.cat(x)[None], paged_kv=cache, paged_batch=batch, paged_write=False)[0]
             want = torch.cat([proc(mod, xs[None], encoder_hidden_states=t[None])[0] for xs, t in zip(x, states)])
             assert float((got.float() - want.float()).norm() / want.float().norm()) < 4 * BF16
+
+
+def test_keys_written_by_the_processor_take_their_own_norm():
+    """norm_k's weight and epsilon, whatever norm_q's are."""
+    import pika_h3_flex_amd as pk
+
+    mod = _Module(2, 2, 64, 5).cuda()
+    mod.norm_k.eps = 0.5
+    cache, twin = (pk.PagedKV(1, 2, device="cuda") for _ in range(2))
+    batch = pk.PagedBatch.build([20], [20], [[0]], device="cuda")
+    x = _rows(torch.Generator().manual_seed(1), 20, 1)[:, 0, :64].contiguous().cuda()
+    with torch.no_grad():
+        pk.PikaH3AttnProcessor().write_paged(mod, x[None], cache, batch)
+        k, v = mod.to_k(x).view(20, 2, D), mod.to_v(x).view(20, 2, D)
+        pk.paged_write(twin, batch, k, v, k_norm_weight=mod.norm_k.weight.detach(), norm_eps=0.5)
+        assert all(torch.equal(a, b) for a, b in zip(pk.paged_read(cache, batch), pk.paged_read(twin, batch)))
+        mod.norm_k.eps = EPS
+        pk.PikaH3AttnProcessor().write_paged(mod, x[None], cache, batch)
+        assert not torch.equal(pk.paged_read(cache, batch)[0], pk.paged_read(twin, batch)[0])

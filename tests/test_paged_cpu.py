@@ -324,3 +324,22 @@ def test_the_processor_refuses_what_does_not_go_with_pages():
         proc(Attn(), x.expand(2, 3, 128), paged_kv=cache, paged_batch=batch)
     with pytest.raises(ValueError, match="packed"):
         proc.write_paged(Attn(), x[0], cache, batch)
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_copies_have_their_own_addresses(how):
+    """What a pool and a batch keep of their tensors beside them is that of the copy's tensors."""
+    import copy
+    import pickle
+
+    import pika_h3_flex_amd as pk
+
+    record = pk.PagedKV(1, 1, device="cpu").record_bytes
+    pool = pk.PagedKV(3, 2, data=torch.arange(3 * 2 * record, dtype=torch.int64).to(torch.uint8).view(3, 2, record))
+    batch = pk.PagedBatch.build([1, 2], [5, 70], [[2], [0, 1]], device="cpu")
+    again = copy.deepcopy((pool, batch)) if how == "deepcopy" else pickle.loads(pickle.dumps((pool, batch)))
+    assert torch.equal(again[0].data, pool.data) and (again[0].pages, again[0].heads, again[0].fp8) == (3, 2, False)
+    assert again[0]._head == (again[0].data.data_ptr(), 3) and again[0]._head != pool._head
+    assert again[1].rows == 3 and torch.equal(again[1].table, batch.table)
+    assert again[1]._arrays == (again[1].starts.data_ptr(), again[1].lengths.data_ptr(), again[1].table.data_ptr(), 2)
+    assert again[1]._arrays[:3] != batch._arrays[:3]
