@@ -96,7 +96,8 @@ int pkh3_paged_write(const pkh3_paged_args* a, void* stream);
 /* Keys and values of the call's rows out of the pages, as the values they stand for. */
 int pkh3_paged_read(const pkh3_paged_args* a, void* stream);
 
-/* Scratch of pkh3_paged_attn for these shapes (0 on invalid arguments); does not depend on what the batch's arrays hold. */
+/* Scratch of pkh3_paged_attn for these sizes (B, table_pages, rows, heads, kv_heads) and flags, 0 on invalid ones; does not
+   depend on what the batch's arrays hold.  103 MB are enough for any call. */
 size_t pkh3_paged_workspace_bytes(const pkh3_paged_args* a);
 
 /* Attention of the call's rows over their sequences' keys.  A row that sees no key gets zeros.  Results depend on the

@@ -343,3 +343,14 @@ def test_copies_have_their_own_addresses(how):
     assert again[1].rows == 3 and torch.equal(again[1].table, batch.table)
     assert again[1]._arrays == (again[1].starts.data_ptr(), again[1].lengths.data_ptr(), again[1].table.data_ptr(), 2)
     assert again[1]._arrays[:3] != batch._arrays[:3]
+
+
+def test_workspace_of_any_call_has_the_stated_bound(lib):
+    """Sizes from a single row to the largest call, both kinds of pages: never nothing, never more than the header says."""
+    for rows in (0, 1, 17, 40, 1000, 1 << 20):
+        for B in (1, 7, 1024):
+            for kv, heads in ((1, 1), (4, 32), (24, 24)):
+                for pages in (1, 16, 17, 2000, 1 << 20):
+                    for flags in (0, _lib.PAGED_FP8, _lib.PAGED_FP8 | _lib.PAGED_CAUSAL):
+                        a = _lib.PagedArgs(n_pages=1, B=B, table_pages=pages, rows=rows, kv_heads=kv, heads=heads, D=128, flags=flags)
+                        assert 0 < lib.pkh3_paged_workspace_bytes(C.byref(a)) <= 103_000_000
