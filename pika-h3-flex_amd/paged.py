@@ -219,7 +219,7 @@ def paged_read(cache: PagedKV, batch: PagedBatch, rows: Optional[int] = None, *,
     if rows is None:
         raise ValueError("the batch does not know its rows: say how many")
     if out is None:
-        out = torch.empty((2, rows, H, HEAD_DIM), dtype=torch.bfloat16, device=cache.device).unbind(0)
+        out = [torch.empty(rows, H, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2)]
     k, v = out
     k_ss, k_sh, k_rows = _rows_of("k", k, H, index)
     v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
@@ -245,10 +245,12 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     if heads == 0 or heads % cache.heads:
         raise ValueError(f"{heads} query heads are no multiple of the cache's {cache.heads}")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=cache.device)
-    o_ss, o_sh, o_rows = _rows_of("out", out, heads, index)
-    if o_rows != rows:
-        raise ValueError(f"out has {o_rows} rows, q {rows}")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        o_ss, o_sh = heads * HEAD_DIM, HEAD_DIM
+    else:
+        o_ss, o_sh, o_rows = _rows_of("out", out, heads, index)
+        if o_rows != rows:
+            raise ValueError(f"out has {o_rows} rows, q {rows}")
     _check_batch(cache, batch, rows)
     prep = _norm_rope(q_norm_weight, rope_mode, rope_q, rows, index)
     if not rows:
