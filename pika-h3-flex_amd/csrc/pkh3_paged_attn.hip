@@ -97,7 +97,9 @@ __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t*
   int64_t rest = pos - cum[at.b];
   at.h = __builtin_amdgcn_readfirstlane((int)divided(rest, per_head));
   rest -= at.h * per_head;
-  if (!p.causal) {
+  if (blocks == 1) {
+    at.j = 0;
+  } else if (!p.causal) {
     at.j = __builtin_amdgcn_readfirstlane(min((int)divided(rest, unit_cost(p, s, rb, 0)), blocks - 1));
     rest -= at.j * unit_cost(p, s, rb, 0);
   } else {
@@ -358,15 +360,17 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
         for (int kb = 0; kb < 2; ++kb) ke[kb] = ((const unsigned char*)r)[kScaleOff + 32 * half + 16 * kb + c16];
       }
     };
+    Rows16 q;
+    NormLanes norm;
+    if (wave < QB) {                                           // (on their way before the page is known)
+      ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
+      load_norm_lanes(norm, p.norm_w, lane);
+    }
     if (first < end) {
       id = uniform_page(p, at.b, first >> 1);
       ask_k(id, first & 1);
     }
     if (wave < QB) {
-      Rows16 q;
-      ask_queries(p, s, at.h, at.j * RB + 16 * wave, q, lane);
-      NormLanes norm;
-      load_norm_lanes(norm, p.norm_w, lane);
       float x[32];
       queries_moved(p, s, at.j * RB + 16 * wave, q, norm, part + wave * 4096, lane, 1.0f, x);
 #pragma unroll
