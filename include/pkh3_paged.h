@@ -34,7 +34,10 @@
  *   - a table entry outside [0, n_pages) is a page that is not there: its keys are seen by nobody, writes to it are dropped,
  *     reads of it give zeros;
  *   - a row in front of position 0 (more new rows than keys) is not written, reads as zeros, and sees no key under
- *     PKH3_PAGED_CAUSAL (without it, it sees them all).
+ *     PKH3_PAGED_CAUSAL (without it, it sees them all);
+ *   - pkh3_paged_write takes starts and lengths as they are, so that no row comes to another's place: row r of the call stands at
+ *     lengths[b] - starts[b+1] + r, and is written if it is one of the call's rows and that place is in the table.  A sequence that has grown past
+ *     its table loses the rows behind it and keeps what is stored.
  * Rows that belong to no sequence are neither read nor written.  starts must not decrease, and no two places that one call
  * writes may be the same.
  */

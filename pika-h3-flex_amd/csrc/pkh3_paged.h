@@ -52,6 +52,15 @@ __device__ __forceinline__ int uniform_int(const int* p, int64_t i) { return ((c
 __device__ __forceinline__ Sequence uniform_sequence(const PagedParams& p, int b) {
   return make_sequence(uniform_int(p.starts, b), uniform_int(p.starts, b + 1), uniform_int(p.lengths, b), p.rows, p.table_pages);
 }
+// .. and both as a write takes them
+template <bool WRITES>
+__device__ __forceinline__ Sequence moved_sequence(const PagedParams& p, int b) {
+  return WRITES ? make_written(p.starts[b], p.starts[b + 1], p.lengths[b], p.rows, p.table_pages) : sequence(p, b);
+}
+template <bool WRITES>
+__device__ __forceinline__ Sequence uniform_moved_sequence(const PagedParams& p, int b) {
+  return WRITES ? make_written(uniform_int(p.starts, b), uniform_int(p.starts, b + 1), uniform_int(p.lengths, b), p.rows, p.table_pages) : uniform_sequence(p, b);
+}
 __device__ __forceinline__ int uniform_page(const PagedParams& p, int b, int tile) {
   if (tile < 0 || tile >= p.table_pages) return -1;
   return page_in_pool(uniform_int(p.table, (int64_t)b * p.table_stride + tile), p.n_pages);

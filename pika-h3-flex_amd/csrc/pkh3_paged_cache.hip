@@ -17,12 +17,13 @@ struct Item {
   int b;
   TileRows t;
 };
+template <bool WRITES>
 __device__ __forceinline__ bool find_tile(const PagedParams& p, int64_t* cum, int nth, Item& it) {
-  for (int b = threadIdx.x; b < p.B; b += blockDim.x) cum[b + 1] = tiles_of_rows(sequence(p, b));
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) cum[b + 1] = tiles_of_rows(moved_sequence<WRITES>(p, b));
   prefix_sums(cum, p.B);
   if (nth >= cum[p.B]) return false;
   it.b = find_sequence(cum, p.B, nth);
-  it.t = tile_rows(uniform_sequence(p, it.b), __builtin_amdgcn_readfirstlane((int)(nth - cum[it.b])));
+  it.t = tile_rows(uniform_moved_sequence<WRITES>(p, it.b), __builtin_amdgcn_readfirstlane((int)(nth - cum[it.b])));
   return true;
 }
 
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256, 3) void paged_write_kernel(PagedParams p) {
   static_assert((kMaxSequences + 1) * sizeof(int64_t) <= sizeof(lds), "the sums lie where the rows are turned around afterwards");
   const int side = blockIdx.x & 1, group = (blockIdx.x >> 1) % p.groups, nth = (blockIdx.x >> 1) / p.groups;
   Item it;
-  if (!find_tile(p, (int64_t*)lds, nth, it)) return;
+  if (!find_tile<true>(p, (int64_t*)lds, nth, it)) return;
   __syncthreads();
   const TileRows& t = it.t;
   const int64_t id = uniform_page(p, it.b, t.tile);
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256, 3) void paged_read_kernel(PagedParams p) {
   __shared__ __attribute__((aligned(16))) char lds[4 * 8192];
   const int side = blockIdx.x & 1, group = (blockIdx.x >> 1) % p.groups, nth = (blockIdx.x >> 1) / p.groups;
   Item it;
-  if (!find_tile(p, (int64_t*)lds, nth, it)) return;
+  if (!find_tile<false>(p, (int64_t*)lds, nth, it)) return;
   __syncthreads();
   const TileRows& t = it.t;
   const int64_t id = uniform_page(p, it.b, t.tile);

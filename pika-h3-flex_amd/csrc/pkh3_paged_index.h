@@ -19,6 +19,14 @@ constexpr Sequence make_sequence(int start, int end, int length, int rows, int t
   const int at = at_most(at_least(start, 0), rows), to = at_most(at_least(end, 0), rows);
   return {at, at_least(to - at, 0), at_most(at_least(length, 0), table_pages * kPageKeys)};
 }
+// The same for writing, by the values as they are: brought into range, a row would come to another's place and take it.  Row r of the call stands at
+// length - end + r; what is written are the rows whose place is in the table.  Their positions are from 0 on.
+constexpr Sequence make_written(int start, int end, int length, int rows, int table_pages) {
+  const int64_t row0 = (int64_t)end - length, behind = row0 + (int64_t)table_pages * kPageKeys;   // rows whose places would be 0 and the one past the table
+  const int from = at_least(start, 0), until = at_most(end, rows);
+  const int64_t at = row0 > from ? row0 : from, to = behind < until ? behind : until;
+  return to > at ? Sequence{(int)at, (int)(to - at), (int)(to - row0)} : Sequence{0, 0, 0};
+}
 constexpr int page_in_pool(int id, int64_t n_pages) { return id >= 0 && id < n_pages ? id : -1; }
 
 // ---- writing and reading: the tiles that a sequence's rows lie in, in front of position 0 too ----

@@ -428,6 +428,35 @@ def test_arrays_out_of_range_are_brought_into_it():
     assert bool((c == 7.0).all())
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_write_past_the_table_leaves_what_is_stored(fp8):
+    """Tokens behind the last place of their table, and sequences that say they have rows the call does not: no stored byte changes but those of rows in
+    their own place."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([128, 64], 2, fp8, seed=6)
+    table = held.batch([0, 0]).table.clone()
+    table[1, 1] = table[0, 0]                                              # a page that both hold
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    gen = torch.Generator().manual_seed(2)
+    k, v = (_rows(gen, 6, 2).cuda() for _ in range(2))
+    before = held.cache.data.clone()
+    for starts, lengths in (([0, 1, 2], [129, 129]), ([0, 3, 6], [10 ** 9, 2 ** 31 - 1]), ([0, 0, 99], [0, -3]), ([2, 6, 6], [132, 0]),
+                            ([-9, 0, 6], [128, -2 ** 31]), ([0, 2 ** 31 - 1, 6], [-5, 0])):
+        pk.paged_write(held.cache, pk.PagedBatch(as_int(starts), as_int(lengths), table), k, v)
+        assert torch.equal(held.cache.data, before), (starts, lengths)
+    # four rows up to one behind the table: three in their place; eight rows of which the call has six, and of these one is in front of position 0
+    for starts, lengths, where in (([1, 5, 5], [129, 0], (0, 1, 4, 125)), ([0, 0, 8], [0, 7], (1, 1, 6, 0))):
+        pk.paged_write(held.cache, pk.PagedBatch(as_int(starts), as_int(lengths), table), k, v)
+        b, lo, hi, first = where
+        twin = pk.PagedKV(held.cache.pages, 2, fp8=fp8, data=before.clone())
+        keys = [0, 0]
+        keys[b] = first + hi - lo
+        pk.paged_write(twin, pk.PagedBatch(as_int([0, 0 if b else hi - lo, hi - lo]), as_int(keys), table), k[lo:hi], v[lo:hi])
+        assert torch.equal(held.cache.data, twin.data) and not torch.equal(twin.data, before)
+        held.cache.data.copy_(before)
+
+
 def test_strides_order_and_the_output_in_the_queries_place():
     import pika_h3_flex_amd as pk
 

@@ -306,6 +306,37 @@ def test_runs_cover_every_tile_of_every_unit_once(tmp_path):
   CHECK(divided(7, 2) == 3 && divided(1ll << 40, 3) == (1ll << 40) / 3 && divided(5, 1ll << 33) == 0 && divided(4294967295ll, 7) == 4294967295ll / 7, "division");""")
 
 
+def test_rows_are_written_in_their_own_place_or_not_at_all(tmp_path):
+    """Whatever starts and lengths hold, a row that a write stores stands at length - end + row of the values as they are: no other key's place is taken."""
+    _run(tmp_path, """
+  const int wild[] = {0, 1, 5, 63, 64, 65, 129, 192, 193, 1000, -1, -7, 2147483647, -2147483647 - 1, 16777216, 1 << 30};
+  const int n_wild = sizeof(wild) / sizeof(int);
+  for (int a = 0; a < n_wild; ++a) for (int b = 0; b < n_wild; ++b) for (int c = 0; c < n_wild; ++c)
+    for (int rows : {0, 1, 70, 200}) for (int pages : {1, 3, 16777216}) {
+      const Sequence s = make_written(wild[a], wild[b], wild[c], rows, pages);
+      CHECK(s.n >= 0 && s.first >= 0 && s.first + s.n <= rows && s.keys >= 0 && s.keys <= pages * 64, "%d %d %d", wild[a], wild[b], wild[c]);
+      std::vector<int64_t> place(rows, -1);
+      CHECK(tiles_of_rows(s) <= s.n / 64 + 2, "tiles");
+      for (int i = 0; i < tiles_of_rows(s); ++i) {
+        const TileRows t = tile_rows(s, i);
+        for (int at = t.p0; at < t.p1; ++at) {
+          CHECK(t.row0 + at >= 0 && t.row0 + at < rows && place[t.row0 + at] < 0, "row %d", t.row0 + at);
+          place[t.row0 + at] = (int64_t)t.tile * 64 + at;
+        }
+      }
+      for (int r = 0; r < rows; ++r) {
+        const int64_t own = (int64_t)wild[c] - wild[b] + r;
+        CHECK(place[r] == (r >= wild[a] && r < wild[b] && own >= 0 && own < (int64_t)pages * 64 ? own : -1), "row %d of %d %d %d at %lld", r, wild[a], wild[b], wild[c], (long long)place[r]);
+      }
+    }
+  for (int go = 0; go < 3000; ++go) {   // values in range: the same rows as everywhere, those in front of the first key aside
+    const int start = any(0, 50), n = any(0, 300), keys = any(0, 640), rows = start + n + any(0, 3);
+    const Sequence s = make_sequence(start, start + n, keys, rows, 10), w = make_written(start, start + n, keys, rows, 10);
+    CHECK(w.n == std::min(n, keys), "%d of %d rows", w.n, n);
+    if (w.n) CHECK(w.first - w.position() == s.first - s.position() && w.keys == s.keys && tiles_of_rows(w) <= tiles_of_rows(s), "place");
+  }""")
+
+
 def test_the_processor_refuses_what_does_not_go_with_pages():
     proc = pk.PikaH3AttnProcessor()
     cache = pk.PagedKV(2, 1, device="cpu")
