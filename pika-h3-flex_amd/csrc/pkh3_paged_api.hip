@@ -30,12 +30,28 @@ int done(hipError_t e, const char* what) {
 
 bool misaligned(const void* p, unsigned to) { return ((uintptr_t)p & (to - 1)) != 0; }
 
-int check_rows(const char* name, const void* ptr, int64_t ss, int64_t sh, int heads, bool out) {
+// Whether two of rows x heads pieces of 128 elements share an element, strides of 128 at least.  Where the outer stride passes over all of the inner pieces
+// they do not (every slice of a tensor); otherwise each distance along the inner one is held against the two multiples of the outer one beside it.
+bool overlaps(int64_t ss, int64_t sh, int rows, int heads) {
+  if (rows < 2 || heads < 2) return false;
+  const int64_t outer = ss > sh ? ss : sh, inner = ss > sh ? sh : ss;
+  const int n_outer = ss > sh ? rows : heads, n_inner = ss > sh ? heads : rows;
+  if ((outer - kD) / inner >= n_inner - 1) return false;
+  for (int i = 1; i < n_inner; ++i) {
+    const __int128 d = (__int128)inner * i, j = d / outer;
+    if (j >= n_outer) return false;                        // (and all further ones are past the last of the outer)
+    if (j >= 1 && d - j * outer < kD) return true;
+    if (j + 1 < n_outer && (j + 1) * outer - d < kD) return true;
+  }
+  return false;
+}
+
+int check_rows(const char* name, const void* ptr, int64_t ss, int64_t sh, int rows, int heads, bool out) {
   if (!ptr) return fail(PKH3_ENULL, "%s is NULL", name);
   if (misaligned(ptr, 16)) return fail(PKH3_EALIGN, "%s is not 16-byte aligned", name);
   if (ss < 0 || sh < 0) return fail(PKH3_ESTRIDE, "%s: negative stride", name);
   if ((ss % 8) || (sh % 8)) return fail(PKH3_ESTRIDE, "%s: strides must be multiples of 8 elements, got (%lld, %lld)", name, (long long)ss, (long long)sh);
-  if (out && (ss < kD || (heads > 1 && sh < kD)))
+  if (out && (ss < kD || (heads > 1 && sh < kD) || overlaps(ss, sh, rows, heads)))
     return fail(PKH3_ESTRIDE, "%s: rows or heads that are written overlap (strides %lld, %lld)", name, (long long)ss, (long long)sh);
   return PKH3_OK;
 }
@@ -74,11 +90,11 @@ int check(const pkh3_paged_args* a, Call call) {
   if (!a->starts || !a->lengths || !a->table) return fail(PKH3_ENULL, "starts, lengths and table must not be NULL");
   if (misaligned(a->starts, 4) || misaligned(a->lengths, 4) || misaligned(a->table, 4)) return fail(PKH3_EALIGN, "starts, lengths and table must be 4-byte aligned");
   if (call == kAttn) {
-    if ((rc = check_rows("q", a->q, a->q_ss, a->q_sh, a->heads, false))) return rc;
-    if ((rc = check_rows("o", a->o, a->o_ss, a->o_sh, a->heads, true))) return rc;
+    if ((rc = check_rows("q", a->q, a->q_ss, a->q_sh, a->rows, a->heads, false))) return rc;
+    if ((rc = check_rows("o", a->o, a->o_ss, a->o_sh, a->rows, a->heads, true))) return rc;
   } else {
-    if ((rc = check_rows("k", a->k, a->k_ss, a->k_sh, a->kv_heads, call == kRead))) return rc;
-    if ((rc = check_rows("v", a->v, a->v_ss, a->v_sh, a->kv_heads, call == kRead))) return rc;
+    if ((rc = check_rows("k", a->k, a->k_ss, a->k_sh, a->rows, a->kv_heads, call == kRead))) return rc;
+    if ((rc = check_rows("v", a->v, a->v_ss, a->v_sh, a->rows, a->kv_heads, call == kRead))) return rc;
   }
   if (call != kRead) {
     if (a->rope_mode != PKH3_ROPE_NONE) {

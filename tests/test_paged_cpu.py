@@ -95,6 +95,27 @@ def test_read_refuses(lib, mutate, code):
     _refuses(lib, "pkh3_paged_read", mutate, code)
 
 
+def test_outputs_that_overlap_themselves_are_refused(lib):
+    """Strides that give two rows, or two heads of different rows, one address, whichever is the outer one; strides that interleave without overlapping are not."""
+    import itertools
+
+    for ss, sh, rows, heads in itertools.product((128, 136, 256, 384, 512, 640, 1024), (128, 136, 256, 384, 512, 640, 1024), (1, 2, 5), (1, 2, 4)):
+        at = sorted(r * ss + h * sh for r in range(rows) for h in range(heads))
+        overlap = any(b - a < 128 for a, b in zip(at, at[1:]))
+        # where the strides pass, a refusal behind theirs: nothing is launched
+        for entry, name, behind in (("pkh3_paged_attn", "o", dict(workspace=0)), ("pkh3_paged_read", "k", dict(v=0)), ("pkh3_paged_read", "v", None)):
+            if behind is None and not overlap:
+                continue
+            a = _args()
+            a.rows, a.heads, a.kv_heads = rows, heads, heads
+            for n, x in dict(behind or {}, k_ss=heads * 128, v_ss=heads * 128).items():
+                setattr(a, n, x)
+            setattr(a, name + "_ss", ss)
+            setattr(a, name + "_sh", sh)
+            want = _lib.PKH3_ESTRIDE if overlap else _lib.PKH3_EWORKSPACE if name == "o" else _lib.PKH3_ENULL
+            assert getattr(lib, entry)(C.byref(a), None) == want, (entry, name, ss, sh, rows, heads)
+
+
 def test_no_rows_is_no_launch(lib):
     a = _args()
     a.rows = 0
