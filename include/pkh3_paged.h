@@ -67,8 +67,8 @@ typedef struct pkh3_paged_args {
   const int32_t* table;    /* [B][table_stride], table_pages entries of each used */
   int64_t table_stride;
   /* bf16 rows, [rows, heads, 128], addressed as base + row*ss + head*sh + d; 16-byte aligned, strides multiples of 8
-     elements.  write: k and v in; read: k and v out; attn: q in, o out (`o` may be `q` with q's strides, and must not
-     overlap it otherwise).  What a call does not use is not looked at */
+     elements.  write: k and v in; read: k and v out, which must not overlap each other; attn: q in, o out (`o` may be `q`
+     with q's strides, and must not overlap it otherwise).  What a call does not use is not looked at */
   const void* q;
   void* k;
   void* v;

@@ -103,6 +103,7 @@ int check(const pkh3_paged_args* a, Call call) {
     }
     if (a->norm_w && misaligned(a->norm_w, 16)) return fail(PKH3_EALIGN, "norm weights must be 16-byte aligned");
   }
+  if (call == kRead && a->rows > 0 && a->k == a->v) return fail(PKH3_EARG, "k and v are written to one place");
   return PKH3_OK;
 }
 

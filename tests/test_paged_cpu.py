@@ -116,6 +116,12 @@ def test_outputs_that_overlap_themselves_are_refused(lib):
             assert getattr(lib, entry)(C.byref(a), None) == want, (entry, name, ss, sh, rows, heads)
 
 
+def test_reading_both_sides_into_one_place_is_refused(lib):
+    a = _args()
+    assert a.k == a.v and lib.pkh3_paged_read(C.byref(a), None) == _lib.PKH3_EARG
+    assert b"k and v" in lib.pkh3_last_error()
+
+
 def test_no_rows_is_no_launch(lib):
     a = _args()
     a.rows = 0
