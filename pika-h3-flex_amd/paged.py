@@ -22,6 +22,17 @@ PAGE_KEYS = _lib.PAGE_KEYS
 _F32 = C.c_float
 
 
+# Where the elements of a pool's or a batch's tensors lie: what resizing one of them, setting it or giving it other data changes.  (A type of another width
+# changes the shape over the same memory, another device the address.)
+
+def _pool_state(t: torch.Tensor) -> tuple:
+    return t.data_ptr(), t.shape, t.stride()
+
+
+def _batch_state(s: torch.Tensor, n: torch.Tensor, t: torch.Tensor) -> tuple:
+    return s.data_ptr(), s.shape, s.stride(), n.data_ptr(), n.shape, n.stride(), t.data_ptr(), t.shape, t.stride()
+
+
 class PagedKV:
     """A pool of pages: 64 keys and values of ``heads`` heads each, head dim 128, in bf16 or (``fp8``) in e4m3 with a power-of-two
     scale per key, head and side.  ``data`` is uint8 ``[pages, heads, record]`` in the layout of the attention kernel;
@@ -33,14 +44,21 @@ class PagedKV:
             raise ValueError(f"a pool has at least one page and one head, got {pages} and {heads}")
         self.flags = _lib.PAGED_FP8 if self.fp8 else 0
         self.record_bytes = int(_lib.load().pkh3_paged_record_bytes(self.flags))
-        shape = (self.pages, self.heads, self.record_bytes)
         if data is None:
+            shape = (self.pages, self.heads, self.record_bytes)
             data = torch.empty(shape, dtype=torch.uint8, device=device if device is not None else "cuda")
-        elif data.dtype != torch.uint8 or not data.is_contiguous() or data.shape != shape:
-            raise ValueError(f"data must be contiguous uint8 {shape}, got {data.dtype} {tuple(data.shape)}")
         self._data = data
+        self._take()
+
+    def _take(self) -> None:
+        """Checks the tensor and keeps what a call needs of it."""
+        data, shape = self._data, (self.pages, self.heads, self.record_bytes)
+        state = _pool_state(data)
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.shape != shape:
+            raise ValueError(f"data must be contiguous uint8 {shape}, got {data.dtype} {tuple(data.shape)}")
         self._head = (data.data_ptr(), self.pages)
         self._index = data.get_device()
+        self._seen = state
 
     def __reduce__(self):
         # copies and pickles are made anew: what is kept beside the tensor holds its address
@@ -64,7 +82,7 @@ class PagedBatch:
     """The sequences of a call: int32 device tensors ``starts [B + 1]`` (sequence b owns the call's rows ``starts[b] ..
     starts[b+1]-1``, its newest), ``lengths [B]`` (its keys, these rows among them where they are written) and ``table [B, P]``
     (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows them.  What the tensors hold may be
-    changed in place between calls, replays of a captured graph among them, the tensors themselves stay where they are;
+    changed in place between calls, replays of a captured graph among them (a graph goes on with the memory it was captured with);
     include/pkh3_paged.h says what out-of-range values do."""
 
     starts: torch.Tensor
@@ -74,9 +92,11 @@ class PagedBatch:
     _arrays: tuple = field(init=False, repr=False, compare=False)
     _sizes: tuple = field(init=False, repr=False, compare=False)
     _index: int = field(init=False, repr=False, compare=False)
+    _seen: tuple = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
-        # checked once: small calls wait for the host, and a batch is the handle of many
+        # checked here, and again by the call that finds a tensor moved: small calls wait for the host, and a batch is the handle of many
+        seen = _batch_state(self.starts, self.lengths, self.table)
         index = self.table.get_device()
         for name, t, dim in (("starts", self.starts, 1), ("lengths", self.lengths, 1), ("table", self.table, 2)):
             if t.dtype != torch.int32 or t.dim() != dim or (t.stride(dim - 1) != 1 and t.shape[dim - 1] > 1):
@@ -89,6 +109,7 @@ class PagedBatch:
         object.__setattr__(self, "_arrays", (self.starts.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(), self.table.stride(0)))
         object.__setattr__(self, "_sizes", (B, self.table.shape[1]))
         object.__setattr__(self, "_index", index)
+        object.__setattr__(self, "_seen", seen)
 
     def __reduce__(self):
         return PagedBatch, (self.starts, self.lengths, self.table, self.rows)
@@ -153,9 +174,18 @@ def _norm_rope(norm_w, rope_mode, rope, rows: int, index: int) -> tuple:
     return w, _f32("rope cos", rope[0], shape, index), _f32("rope sin", rope[1], shape, index), rope_mode
 
 
-def _check_batch(cache: PagedKV, batch: PagedBatch, rows: int) -> None:
+def _place(cache: PagedKV, batch: PagedBatch) -> int:
+    """The device of a call: that of the cache and the batch, whose tensors are looked for first where they were at their last check."""
+    if _batch_state(batch.starts, batch.lengths, batch.table) != batch._seen:
+        batch.__post_init__()
+    if _pool_state(cache._data) != cache._seen:
+        cache._take()
     if batch._index != cache._index:
         raise ValueError(f"the batch must live with the cache on {cache.device} (got {batch.table.device})")
+    return cache._index
+
+
+def _check_rows(batch: PagedBatch, rows: int) -> None:
     if batch.rows is not None and batch.rows != rows:
         raise ValueError(f"the batch has {batch.rows} rows, the call {rows}")
 
@@ -197,12 +227,12 @@ def paged_write(cache: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Ten
                 norm_eps: float = 1e-6, rope_mode: int = _lib.ROPE_NONE, rope_k=None) -> None:
     """Keys (through RMSNorm and rotation, as given) and values of the call's rows, bf16 ``[rows, heads, 128]``, into their pages.
     ``rope_k``: cos/sin tables ``[rows, 64]``, a row per row of the call.  Runs asynchronously on the current stream."""
-    index, H = cache._index, cache.heads
+    index, H = _place(cache, batch), cache.heads
     k_ss, k_sh, rows = _rows_of("k", k, H, index)
     v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
     if rows != v_rows:
         raise ValueError(f"k has {rows} rows, v {v_rows}")
-    _check_batch(cache, batch, rows)
+    _check_rows(batch, rows)
     prep = _norm_rope(k_norm_weight, rope_mode, rope_k, rows, index)
     if rows:
         _call("pkh3_paged_write", _pack(*cache._head, *batch._arrays, 0, k.data_ptr(), v.data_ptr(), 0, 0, 0, k_ss, k_sh, v_ss, v_sh, 0, 0,
@@ -213,7 +243,7 @@ def paged_read(cache: PagedKV, batch: PagedBatch, rows: Optional[int] = None, *,
     """Keys and values of the call's rows as the cache holds them: ``[k, v]``, bf16 ``[rows, heads, 128]`` (``out``: two tensors
     to put them in).  ``rows``: as ``batch.rows`` where the batch does not know.  Rows of no sequence, in given tensors, stay as they are;
     in new ones they hold anything."""
-    index, H = cache._index, cache.heads
+    index, H = _place(cache, batch), cache.heads
     if rows is None:
         rows = batch.rows if out is None else out[0].shape[0]
     if rows is None:
@@ -225,7 +255,7 @@ def paged_read(cache: PagedKV, batch: PagedBatch, rows: Optional[int] = None, *,
     v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
     if k_rows != rows or v_rows != rows:
         raise ValueError(f"out has {k_rows} and {v_rows} rows, the call {rows}")
-    _check_batch(cache, batch, rows)
+    _check_rows(batch, rows)
     if rows:
         _call("pkh3_paged_read", _pack(*cache._head, *batch._arrays, 0, k.data_ptr(), v.data_ptr(), 0, 0, 0, k_ss, k_sh, v_ss, v_sh, 0, 0,
                                        *batch._sizes, rows, H, 0, HEAD_DIM, 0.0, 0.0, 0, 0, 0, 0, cache.flags, 0, 0), index)
@@ -239,7 +269,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     cache's, over all keys of their sequence, or with ``causal`` over those up to their own position.  A row that sees no key gets
     zeros.  ``workspace``: a uint8 device tensor, or a callable ``(device, nbytes) -> tensor``, as :func:`.ops.attention` takes it; two calls
     that may overlap need one each.  Returns ``out`` (may be ``q``)."""
-    index = cache._index
+    index = _place(cache, batch)
     q_ss, q_sh, rows = _rows_of("q", q, 0, index)
     heads = q.shape[1]
     if heads == 0 or heads % cache.heads:
@@ -251,7 +281,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
         o_ss, o_sh, o_rows = _rows_of("out", out, heads, index)
         if o_rows != rows:
             raise ValueError(f"out has {o_rows} rows, q {rows}")
-    _check_batch(cache, batch, rows)
+    _check_rows(batch, rows)
     prep = _norm_rope(q_norm_weight, rope_mode, rope_q, rows, index)
     if not rows:
         return out

@@ -492,6 +492,38 @@ def test_one_page_in_two_sequences():
     assert bool(((got[1:] - ref).abs() <= BF16 * ref.abs() + (BF16 + 2.0 ** -12) * size).all())
 
 
+def test_calls_follow_tensors_that_moved():
+    """Lengths, table and pool given other memory, other sizes and other strides between two calls: the next one is that of a batch made of them anew."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([100, 63], 2, False, seed=1)
+    batch, cache = held.batch([3, 2]), held.cache
+    q = _rows(torch.Generator().manual_seed(1), 5, 4).cuda()
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+
+    def same():
+        fresh = pk.PagedBatch(*(t.clone() for t in (batch.starts, batch.lengths, batch.table)), batch.rows)
+        pool = pk.PagedKV(cache.pages, 2, data=cache.data.clone())
+        got, want = (pk.paged_attention(q, c, b, causal=True) for c, b in ((cache, batch), (pool, fresh)))
+        return torch.equal(got, want) and bool(torch.isfinite(got).all()) and bool(got.any())
+
+    assert same()
+    batch.lengths.data = as_int([50, 13])
+    assert same()
+    batch.table.set_(torch.cat([batch.table, torch.full((2, 7), -1, dtype=torch.int32, device="cuda")], 1)[:, :4])
+    assert same()
+    before = cache.data.detach()
+    cache.data.data = before.clone()
+    before.zero_()
+    assert same()
+    batch.lengths.resize_(1)
+    with pytest.raises(ValueError, match="starts"):
+        pk.paged_attention(q, cache, batch, causal=True)
+    batch.starts.resize_(2), batch.table.set_(batch.table[:1].clone())
+    batch.starts.copy_(as_int([0, 5]))
+    assert same()
+
+
 def test_a_captured_step_replays_with_changed_batches():
     """A token step in a graph: rows, lengths, pages and inputs change in place between the replays, and every replay equals the eager calls."""
     import pika_h3_flex_amd as pk

@@ -412,3 +412,36 @@ def test_workspace_of_any_call_has_the_stated_bound(lib):
                     for flags in (0, _lib.PAGED_FP8, _lib.PAGED_FP8 | _lib.PAGED_CAUSAL):
                         a = _lib.PagedArgs(n_pages=1, B=B, table_pages=pages, rows=rows, kv_heads=kv, heads=heads, D=128, flags=flags)
                         assert 0 < lib.pkh3_paged_workspace_bytes(C.byref(a)) <= 103_000_000
+
+
+def test_tensors_that_moved_are_taken_where_they_are():
+    """A batch's or a pool's tensor that was resized, set or given other data since the last call: its checks are made again, and the call gets the new address."""
+    from pika_h3_flex_amd import paged
+
+    cache = pk.PagedKV(3, 2, device="cpu")
+    batch = pk.PagedBatch.build([1, 2], [5, 70], [[2], [0, 1]], device="cpu")
+    look = lambda: paged._place(cache, batch)   # noqa: E731
+    look()
+    batch.lengths.data = torch.tensor([7, 71], dtype=torch.int32)
+    look()
+    assert batch._arrays[1] == batch.lengths.data_ptr()
+    wide = torch.full((2, 9), -1, dtype=torch.int32)
+    batch.table.set_(wide[:, :5])
+    look()
+    assert batch._arrays[2:] == (wide.data_ptr(), 9) and batch._sizes == (2, 5)
+    cache.data.data = torch.zeros_like(cache.data)
+    look()
+    assert cache._head == (cache.data.data_ptr(), 3)
+    for change, back in ((lambda: batch.lengths.resize_(1), lambda: batch.lengths.resize_(2)), (lambda: batch.starts.resize_(400), lambda: batch.starts.resize_(3)),
+                         (lambda: batch.table.resize_(3, 5), lambda: batch.table.resize_(2, 5)), (lambda: cache.data.resize_(2, 2, 32768), lambda: cache.data.resize_(3, 2, 32768)),
+                         (lambda: batch.lengths.set_(torch.zeros(4, dtype=torch.int32)[::2]), lambda: batch.lengths.set_(torch.zeros(2, dtype=torch.int32)))):
+        change()
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                look()
+        back()
+        look()
+    assert batch._arrays[:2] == (batch.starts.data_ptr(), batch.lengths.data_ptr()) and cache._head[0] == cache.data.data_ptr()
+    batch.lengths.data = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="int32"):
+        look()
