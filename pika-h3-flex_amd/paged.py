@@ -81,7 +81,8 @@ def _pool_of(pages: int, heads: int, fp8: bool, data: torch.Tensor) -> PagedKV:
 class PagedBatch:
     """The sequences of a call: int32 device tensors ``starts [B + 1]`` (sequence b owns the call's rows ``starts[b] ..
     starts[b+1]-1``, its newest), ``lengths [B]`` (its keys, these rows among them where they are written) and ``table [B, P]``
-    (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows them.  What the tensors hold may be
+    (key j lies in page ``table[b, j // 64]``).  ``rows``: the rows of the call where the host knows that they all are
+    the sequences'; without it rows in front of the first sequence and behind the last may be nobody's, and are zeros in new outputs.  What the tensors hold may be
     changed in place between calls, replays of a captured graph among them (a graph goes on with the memory it was captured with);
     include/pkh3_paged.h says what out-of-range values do."""
 
@@ -241,15 +242,16 @@ def paged_write(cache: PagedKV, batch: PagedBatch, k: torch.Tensor, v: torch.Ten
 
 def paged_read(cache: PagedKV, batch: PagedBatch, rows: Optional[int] = None, *, out=None) -> List[torch.Tensor]:
     """Keys and values of the call's rows as the cache holds them: ``[k, v]``, bf16 ``[rows, heads, 128]`` (``out``: two tensors
-    to put them in).  ``rows``: as ``batch.rows`` where the batch does not know.  Rows of no sequence, in given tensors, stay as they are;
-    in new ones they hold anything."""
+    to put them in, apart from each other).  ``rows``: as ``batch.rows`` where the batch does not know.  Rows of no sequence stay as
+    they are in given tensors; in new ones they are zeros, or where ``batch.rows`` says that there are none may hold anything."""
     index, H = _place(cache, batch), cache.heads
     if rows is None:
         rows = batch.rows if out is None else out[0].shape[0]
     if rows is None:
         raise ValueError("the batch does not know its rows: say how many")
     if out is None:
-        out = [torch.empty(rows, H, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2)]
+        make = torch.zeros if batch.rows is None else torch.empty             # (the kernels leave rows of no sequence alone)
+        out = [make(rows, H, HEAD_DIM, dtype=torch.bfloat16, device=cache.device) for _ in range(2)]
     k, v = out
     k_ss, k_sh, k_rows = _rows_of("k", k, H, index)
     v_ss, v_sh, v_rows = _rows_of("v", v, H, index)
@@ -268,14 +270,15 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     """softmax(norm_rope(q) K^T * scale) V of the call's rows ``q``, bf16 ``[rows, heads, 128]`` with ``heads`` a multiple of the
     cache's, over all keys of their sequence, or with ``causal`` over those up to their own position.  A row that sees no key gets
     zeros.  ``workspace``: a uint8 device tensor, or a callable ``(device, nbytes) -> tensor``, as :func:`.ops.attention` takes it; two calls
-    that may overlap need one each.  Returns ``out`` (may be ``q``)."""
+    that may overlap need one each.  Returns ``out`` (may be ``q``, and must not overlap it otherwise); rows of no sequence are as those of :func:`paged_read`.
+    For inference: gradients do not flow through it, as through none of the package's calls."""
     index = _place(cache, batch)
     q_ss, q_sh, rows = _rows_of("q", q, 0, index)
     heads = q.shape[1]
     if heads == 0 or heads % cache.heads:
         raise ValueError(f"{heads} query heads are no multiple of the cache's {cache.heads}")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = (torch.zeros_like if batch.rows is None else torch.empty_like)(q, memory_format=torch.contiguous_format)
         o_ss, o_sh = heads * HEAD_DIM, HEAD_DIM
     else:
         o_ss, o_sh, o_rows = _rows_of("out", out, heads, index)

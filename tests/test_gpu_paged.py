@@ -492,6 +492,50 @@ def test_one_page_in_two_sequences():
     assert bool(((got[1:] - ref).abs() <= BF16 * ref.abs() + (BF16 + 2.0 ** -12) * size).all())
 
 
+def test_rows_of_no_sequence_are_zeros_in_new_outputs():
+    """A padded batch (rows in front of the first sequence and behind the last, their number not known to the host): new outputs hold zeros there, given ones
+    what they held, eager, captured and through the processor."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([300, 64, 5], 2, False, seed=3)
+    made = held.batch([4, 0, 2])
+    batch = pk.PagedBatch(made.starts + 3, made.lengths, made.table)       # rows 3 .. 8 of 40
+    q = _rows(torch.Generator().manual_seed(1), 40, 4).cuda()
+    ours, rest = slice(3, 9), [i for i in range(40) if not 3 <= i < 9]
+
+    def used():   # memory of the sizes that the calls will ask for has been used before
+        for n in (4, 2, 2):
+            torch.full((40, n, D), 7.0, dtype=torch.bfloat16, device="cuda")
+
+    def calls():
+        return [pk.paged_attention(q, held.cache, batch), *pk.paged_read(held.cache, batch, 40)]
+
+    given = [torch.full((40, n, D), 7.0, dtype=torch.bfloat16, device="cuda") for n in (4, 2, 2)]
+    pk.paged_attention(q, held.cache, batch, out=given[0])
+    pk.paged_read(held.cache, batch, out=given[1:])
+    assert all(bool((t[rest] == 7.0).all()) for t in given)
+    used()
+    for t, want in zip(calls(), given):
+        assert torch.equal(t[ours], want[ours]) and bool((t[rest] == 0).all())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for _ in range(3):
+        for t in got:
+            t.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, want in zip(got, given):
+            assert torch.equal(t[ours], want[ours]) and bool((t[rest] == 0).all())
+    mod = _Module(4, 2, 256, 3).cuda()
+    x = torch.randn((1, 40, 256), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    with torch.no_grad():
+        used()
+        y = pk.PikaH3AttnProcessor()(mod, x, paged_kv=held.cache, paged_batch=batch, paged_write=False)
+    assert bool((y[0, rest] == 0).all()) and bool(y[0, ours].any(-1).all())
+
+
 def test_calls_follow_tensors_that_moved():
     """Lengths, table and pool given other memory, other sizes and other strides between two calls: the next one is that of a batch made of them anew."""
     import pika_h3_flex_amd as pk
