@@ -314,6 +314,8 @@ class PikaH3AttnProcessor:
                                  "fused block's arguments do not go with it")
             return self._paged(attn, hidden_states, paged_kv, paged_batch, write=bool(paged_write), causal=bool(paged_causal),
                                position_ids=position_ids, rope_cos_sin=rope_cos_sin, rope_key=rope_key)
+        if paged_causal or not paged_write:
+            raise ValueError("paged_causal and paged_write are options of a paged call: paged_kv and paged_batch are missing")
         B, S, _ = hidden_states.shape
         H = int(attn.heads)
         mask_given = attention_mask  # the caller's tensor: what the cross-attention key cache recognises

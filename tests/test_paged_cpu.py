@@ -384,6 +384,18 @@ def test_the_processor_refuses_what_does_not_go_with_pages():
         proc.write_paged(Attn(), x[0], cache, batch)
 
 
+@pytest.mark.parametrize("option", [dict(paged_causal=True), dict(paged_write=False)])
+def test_the_processor_refuses_options_of_paged_calls_without_pages(option):
+    """Who forgets the pool does not get attention without the causal limit, or over the call's own keys."""
+    x = torch.zeros((1, 3, 128), dtype=torch.bfloat16)
+
+    class Attn:
+        heads = 1
+
+    with pytest.raises(ValueError, match="paged_kv"):
+        pk.PikaH3AttnProcessor()(Attn(), x, **option)
+
+
 @pytest.mark.parametrize("how", ["deepcopy", "pickle"])
 def test_copies_have_their_own_addresses(how):
     """What a pool and a batch keep of their tensors beside them is that of the copy's tensors."""
