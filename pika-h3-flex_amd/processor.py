@@ -302,7 +302,10 @@ class PikaH3AttnProcessor:
         attention is over the keys that the pool (one per module; its heads may be fewer than the module's, in groups) holds of each of
         them.  The rows' own keys are written first, unless ``paged_write`` is False: cross-attention to states whose keys
         :meth:`write_paged` has put there.  ``paged_causal``: a row sees the keys up to its own.  Positions are those of the rows
-        (``position_ids [T, 3]``).  Masks, block maps, fp8 QK^T and the fused block do not go with it.
+        (``position_ids [T, 3]``).  Masks, block maps, fp8 QK^T and the fused block do not go with it as arguments.  Of the processor's own settings
+        ``fp8_qk``, ``fused_projections``, ``merge_adapters`` and ``cache_cross_kv`` are those of calls without pages: here QK^T runs in bf16 (as under a key
+        mask) and the module's own projections run, adapters as they are.  Rows of no sequence (a padded ``paged_batch`` without ``rows``) attend to
+        nothing and come out as ``to_out`` of zeros.
         """
         if hidden_states.dim() != 3:
             raise ValueError(f"hidden_states must be [B, S, C], got {tuple(hidden_states.shape)}")

@@ -815,3 +815,18 @@ def test_keys_written_by_the_processor_take_their_own_norm():
         mod.norm_k.eps = EPS
         pk.PikaH3AttnProcessor().write_paged(mod, x[None], cache, batch)
         assert not torch.equal(pk.paged_read(cache, batch)[0], pk.paged_read(twin, batch)[0])
+
+
+def test_settings_of_dense_calls_do_not_reach_paged_ones():
+    """fp8 QK^T, fused projections, merged adapters and kept cross-attention keys are settings of calls without pages: a paged call's result is the plain one's."""
+    import pika_h3_flex_amd as pk
+
+    mod = _Module(4, 2, 512, 3).cuda()
+    x = torch.randn((1, 70, 512), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    batch = pk.PagedBatch.build([30, 40], [30, 40], [[2], [0]], device="cuda")
+    got = []
+    with torch.no_grad():
+        for settings in (dict(), dict(fp8_qk=True), dict(fp8_qk="pow2", fused_projections=True, merge_adapters=True), dict(cache_cross_kv=True)):
+            cache = pk.PagedKV(3, 2, device="cuda")
+            got.append(pk.PikaH3AttnProcessor(**settings)(mod, x, paged_kv=cache, paged_batch=batch, paged_causal=True))
+    assert bool(torch.isfinite(got[0]).all()) and all(torch.equal(g, got[0]) for g in got[1:])
