@@ -120,7 +120,11 @@ class PikaH3AttnProcessor:
         """cos/sin tables of a position grid, cached.  With ``rope_key`` (e.g. the caller's geometry key) the cache
         is keyed by it and the grid's identity does not matter.  Without, the key is the grid tensor itself --
         address, length, device and in-place version counter -- and the entry keeps the tensor alive, so its
-        address cannot be handed to another grid while the entry exists."""
+        address cannot be handed to another grid while the entry exists.  Under capture into a graph nothing is taken from the
+        cache and nothing put there: replays make the tables from what the positions hold then (a row of a sequence that grows has
+        another one each time), and a graph's own tables hold nothing before the first of them."""
+        if position_ids.is_cuda and torch.cuda.is_current_stream_capturing():
+            return rope_tables(position_ids, self.rope_axes_dims, self.rope_theta)
         if rope_key is not None:
             key = ("key", rope_key, position_ids.shape[0], str(position_ids.device))
         else:

@@ -830,3 +830,45 @@ def test_settings_of_dense_calls_do_not_reach_paged_ones():
             cache = pk.PagedKV(3, 2, device="cuda")
             got.append(pk.PikaH3AttnProcessor(**settings)(mod, x, paged_kv=cache, paged_batch=batch, paged_causal=True))
     assert bool(torch.isfinite(got[0]).all()) and all(torch.equal(g, got[0]) for g in got[1:])
+
+
+def _grows(proc, mod, cache, batch, x, where):
+    return proc(mod, x, position_ids=where, paged_kv=cache, paged_batch=batch, paged_causal=True)
+
+
+@pytest.mark.parametrize("warm", [True, False])
+def test_a_captured_processor_step_rotates_by_the_positions_of_each_replay(warm):
+    """One token of two documents through the processor in a graph: rows, lengths and positions change in place, and every replay equals an eager step of a
+    processor of its own."""
+    import pika_h3_flex_amd as pk
+
+    mod = _Module(4, 2, 256, 7).cuda()
+    caches = [pk.PagedKV(6, 2, device="cuda") for _ in range(2)]
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    batch = pk.PagedBatch(as_int([0, 1, 2]), as_int([30, 61]), as_int([[3, 0, 5], [1, 4, 2]]))
+    x = torch.zeros((1, 2, 256), dtype=torch.bfloat16, device="cuda")
+    where = torch.ones((2, 3), dtype=torch.float64, device="cuda")
+    proc, gen = pk.PikaH3AttnProcessor(), torch.Generator().manual_seed(8)
+    for cache in caches:                                                   # what came before
+        k, v = (_rows(torch.Generator().manual_seed(s), 89, 2).cuda() for s in (1, 2))
+        pk.paged_write(cache, pk.PagedBatch.build([29, 60], [29, 60], [[3], [1]], device="cuda"), k, v)
+    with torch.no_grad():
+        x.copy_(torch.randn((1, 2, 256), generator=gen))
+        _grows(proc if warm else pk.PikaH3AttnProcessor(), mod, caches[0], batch, x, where)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _grows(proc, mod, caches[0], batch, x, where)
+        # an eager call of the same processor at the same positions, before any replay
+        want = _grows(pk.PikaH3AttnProcessor(), mod, caches[1], batch, x, where)
+        assert torch.equal(_grows(proc, mod, caches[0], batch, x, where), want)
+        for turn in range(6):
+            if turn:
+                batch.lengths.add_(1)
+            x.copy_(torch.randn((1, 2, 256), generator=gen))
+            where.copy_(torch.rand((2, 3), generator=gen, dtype=torch.float64) * 40.0)
+            want = _grows(pk.PikaH3AttnProcessor(), mod, caches[1], batch, x, where)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and bool(torch.isfinite(out).all()), turn
+            assert all(torch.equal(a, b) for a, b in zip(pk.paged_read(caches[0], batch, 2), pk.paged_read(caches[1], batch, 2)))
