@@ -141,6 +141,9 @@ class PikaH3AttnProcessor:
 
     def _workspace(self, device, nbytes: int) -> torch.Tensor:
         with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                # a graph's scratch is the graph's: what is kept here goes when a larger call comes, and replays may run beside eager calls
+                return torch.empty(nbytes, dtype=torch.uint8, device=device)
             key = (str(device), int(torch.cuda.current_stream().cuda_stream))
         ws = self._workspaces.get(key)
         if ws is None or ws.numel() < nbytes:

@@ -872,3 +872,38 @@ def test_a_captured_processor_step_rotates_by_the_positions_of_each_replay(warm)
             torch.cuda.synchronize()
             assert torch.equal(out, want) and bool(torch.isfinite(out).all()), turn
             assert all(torch.equal(a, b) for a, b in zip(pk.paged_read(caches[0], batch, 2), pk.paged_read(caches[1], batch, 2)))
+
+
+def test_a_captured_processor_step_has_scratch_of_its_own():
+    """What the processor keeps for its eager calls is not in the graph: a larger call that replaces it leaves the replays right, and they leave alone what has
+    the memory by then."""
+    import pika_h3_flex_amd as pk
+
+    mod = _Module(4, 2, 256, 7).cuda()
+    held = Held([900, 400], 2, False, seed=2)
+    batch = held.batch([2, 1])
+    x = torch.randn((1, 3, 256), generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+    step = lambda b, rows: proc(mod, rows, paged_kv=held.cache, paged_batch=b, paged_write=False)   # noqa: E731
+    proc = pk.PikaH3AttnProcessor()
+    side = torch.cuda.Stream()
+    with torch.no_grad(), torch.cuda.stream(side):
+        want = step(batch, x)
+        (key, small), = proc._workspaces.items()
+        kept = small.numel()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = step(batch, x)
+        assert list(proc._workspaces) == [key] and proc._workspaces[key] is small
+        rows = torch.randn((1, 700, 256), generator=torch.Generator().manual_seed(8)).to(torch.bfloat16).cuda()
+        wide = held.batch([400, 300])
+        many = pk.PagedBatch(wide.starts, wide.lengths, torch.cat([wide.table, torch.full((2, 9000), -1, dtype=torch.int32, device="cuda")], 1), 700)
+        del small
+        step(many, rows)
+        assert proc._workspaces[key].numel() > kept
+        taken = [torch.full((kept,), 7, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            side.synchronize()
+            assert torch.equal(out, want) and all(bool((t == 7).all()) for t in taken)
