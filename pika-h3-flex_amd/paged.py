@@ -294,8 +294,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *, causa
     own = workspace is None or workspace.numel() * workspace.element_size() < need
     if own:
         workspace = torch.empty(need, dtype=torch.uint8, device=cache.device)
-    elif workspace.get_device() != index:
-        raise ValueError(f"workspace must live on {cache.device} (got {workspace.device})")
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous and live on {cache.device} (got {workspace.device}, strides {workspace.stride()})")
     _call("pkh3_paged_attn", _pack(*cache._head, *batch._arrays, q.data_ptr(), 0, 0, out.data_ptr(), q_ss, q_sh, 0, 0, 0, 0, o_ss, o_sh,
                                    *batch._sizes, rows, cache.heads, heads, HEAD_DIM, 0.0 if softmax_scale is None else _F32(softmax_scale).value,
                                    _F32(norm_eps).value, *prep, cache.flags | (_lib.PAGED_CAUSAL if causal else 0), workspace.data_ptr(),

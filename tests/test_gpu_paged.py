@@ -646,6 +646,20 @@ def test_a_given_workspace_may_hold_anything():
     assert torch.equal(pk.paged_attention(q, held.cache, batch, workspace=small), want)
 
 
+def test_a_workspace_with_gaps_is_refused():
+    """Its elements are not its bytes from the first on: what lies between them is somebody else's."""
+    import pika_h3_flex_amd as pk
+
+    held = Held([4000], 2, False, seed=2)
+    q = _rows(torch.Generator().manual_seed(3), 3, 2).cuda()
+    sizes = []
+    pk.paged_attention(q, held.cache, held.batch([3]), workspace=lambda device, n: sizes.append(n) or torch.empty(n, dtype=torch.uint8, device=device))
+    for gaps in (torch.zeros((sizes[0], 2), dtype=torch.uint8, device="cuda")[:, 0], torch.zeros(1, dtype=torch.uint8, device="cuda").expand(sizes[0])):
+        with pytest.raises(ValueError, match="contiguous"):
+            pk.paged_attention(q, held.cache, held.batch([3]), workspace=gaps)
+        assert not bool(gaps.any())
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("new", [1, 40])
 def test_offsets_past_32_bits(new, fp8):
