@@ -370,6 +370,101 @@ def test_long_units_of_many_rows_are_shared_out(fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+def test_more_than_64_blocks_of_a_causal_sequence(fp8):
+    """Their sums are a wave's work, their places found 64 at a time; tables of more than 16 pages, so that units are cut.  Blocks of 384 rows, of 32 rows, and of
+    16 rows (one long chunk among 200 sequences without rows)."""
+    held = Held([3000], 1, fp8, seed=4)
+    _check_attention(held, [1700], 16, causal=True, on="cuda", norm=True, rope=1)
+    _check_attention(held, [150], 16, causal=True, on="cuda")
+    lengths = [0] * 200
+    lengths[77] = 1500
+    rows = [0] * 200
+    rows[77] = 1100
+    _check_attention(Held(lengths, 1, fp8, seed=4), rows, 1, causal=True, on="cuda")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("wide", [0, 40])
+def test_as_many_sequences_as_a_call_takes(fp8, wide):
+    """1,024 of them, some without rows, some without keys, some without either: read back as written, single tokens, ragged chunks."""
+    import pika_h3_flex_amd as pk
+
+    gen = torch.Generator().manual_seed(11)
+    B = 1024
+    draw = lambda hi: (torch.randint(0, hi, (B,), generator=gen) * (torch.rand(B, generator=gen) < 0.8)).tolist()   # noqa: E731
+    lengths = draw(200)
+    Held.width = wide
+    try:
+        held = Held(lengths, 1, fp8, seed=5)
+        got = pk.paged_read(held.cache, held.batch(lengths))
+        want = [held.stored(b) for b in range(B)]
+        assert all(torch.equal(got[i].cpu().double(), torch.cat([w[i] for w in want])) for i in range(2))
+        _check_attention(held, draw(2), 2, causal=True, on="cuda", repeat=False)
+        _check_attention(held, draw(90), 1, causal=True, on="cuda")
+        _check_attention(held, draw(90), 2, causal=False, on="cuda", norm=True, repeat=False)
+    finally:
+        Held.width = 0
+
+
+@pytest.mark.usefixtures("table_width")
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("side", ["key", "value"])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows", [[3, 5], [60, 30], [500, 450]])
+def test_what_is_not_finite_in_the_cache(rows, what, side, fp8):
+    """One element of one key or value: rows that see it, of heads that read it, show it; no other row, head or sequence does, but where it is a value, and there
+    in its column, rows of its sequence in front of it under the causal limit.  (An infinite key is NaN in 8 bits; in bf16 it gives logits of one sign a row: +inf shows, -inf is
+    a key without weight.)"""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    lengths, at, column = [700, 600], 500, 37                               # key 500 of the first sequence, of kv head 1
+    held = Held(lengths, 2, fp8, seed=21)
+    bad = [torch.cat(x).clone() for x in (held.k, held.v)]
+    bad[0 if side == "key" else 1][at, 1, column] = what
+    pk.paged_write(held.cache, held.batch(lengths), *(t.cuda() for t in bad))
+    q = _rows(torch.Generator().manual_seed(1), sum(rows), 4).cuda()
+    clean = []
+    for b in range(2):
+        k, v = held.stored(b)
+        if b == 0 and fp8:   # what is not finite counts as nothing for its row's scale: the other elements are as if it were zero
+            for t, which in ((k, "key"), (v, "value")):
+                if which == side:
+                    row = (held.k if side == "key" else held.v)[0][at, 1].double().clone()
+                    row[column] = 0.0
+                    t[at, 1] = P.stored(row[None, None], True)[0, 0]
+        clean.append((k.cuda(), v.cuda()))
+    for causal in (False, True):
+        got = pk.paged_attention(q, held.cache, held.batch(rows), causal=causal).double()
+        first = 0
+        for b, n in enumerate(rows):
+            mine = slice(first, first + n)
+            ref, size = P.attend(q[mine], *clean[b], causal=causal)
+            ok = (got[mine] - ref).abs() <= BF16 * ref.abs() + (BF16 + 2.0 ** -14 + math.expm1(2 * 2.0 ** -14)) * size * (1 + BF16)
+            reads = torch.zeros((n, 4, D), dtype=torch.bool, device="cuda")
+            sees = torch.arange(n, device="cuda") + (lengths[b] - n) >= at if causal else torch.ones(n, dtype=torch.bool, device="cuda")
+            if b == 0:
+                reads[sees, 2:] = True                                      # query heads 2 and 3 read kv head 1
+            if side == "value":
+                may = reads.clone()
+                may[:, 2:] |= causal and b == 0
+                others = [c for c in range(D) if c != column]
+                assert bool(ok[..., others].all()) and bool(ok[..., column][~may[..., column]].all())
+                assert not bool(torch.isfinite(got[mine][..., column][reads[..., column]]).any())
+            elif fp8 or math.isnan(what):
+                assert bool(ok[~reads].all()) and bool(torch.isnan(got[mine][reads]).all())
+            else:
+                sign = torch.sign(q[mine, :, column].double() * what)[..., None].expand(n, 4, D)
+                assert bool(ok[~reads].all()) and bool(torch.isnan(got[mine][reads & (sign >= 0)]).all())
+                if b == 0 and not causal:
+                    k, v = (torch.cat([t[:at], t[at + 1:]]) for t in clean[0])
+                    ref, size = P.attend(q[mine], k, v, causal=False)
+                    off = (got[mine] - ref).abs() - (BF16 * ref.abs() + (BF16 + 2.0 ** -14 + math.expm1(2 * 2.0 ** -14)) * size * (1 + BF16))
+                    assert float(off[reads & (sign < 0)].max()) <= 0.0
+            first += n
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_pages_that_are_not_there(fp8):
     """Table entries outside of the pool: their keys are seen by nobody, writes to them dropped, reads of them zero; the rest as without them."""
     import pika_h3_flex_amd as pk
@@ -607,6 +702,49 @@ def test_a_captured_step_replays_with_changed_batches():
             # (bits: the jump of turn 2 brings keys into two of the sequences that nobody wrote, and those hold NaN)
             assert torch.equal(out.view(torch.int16), eager.view(torch.int16)) and bool(torch.isfinite(out[0 if turn >= 2 else slice(None)]).all()), turn
             assert torch.equal(held.cache.data, twin.data)
+
+
+@pytest.mark.parametrize("total,Hq", [(2, 4), (40, 4), (700, 2)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_cuts_move_between_replays(fp8, total, Hq):
+    """A table of many pages and one workspace: which units are cut, where, and how many parts they have follows rows and lengths as they are at each replay; every one
+    against the oracle."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    held = Held([6000, 9000], 2, fp8, seed=13)
+    stored = [tuple(t.cuda() for t in held.stored(b)) for b in range(2)]
+    made = held.batch([0, 0])
+    batch = pk.PagedBatch(made.starts, made.lengths, made.table)
+    q, out = (torch.zeros((total, Hq, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    scratch = []
+
+    def workspace(device, n):
+        if not scratch:
+            scratch.append(torch.full((n,), 0xFF, dtype=torch.uint8, device=device))
+        return scratch[0]
+
+    call = lambda: pk.paged_attention(q, held.cache, batch, causal=True, out=out, workspace=workspace)   # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    gen = torch.Generator().manual_seed(total)
+    for turn, (share, lengths) in enumerate([(0.5, [6000, 9000]), (1.0, [70, 4000]), (0.0, [5999, 8001]), (0.9, [6000, 1]), (0.02, [0, 9000]), (0.5, [64, 65]), (0.5, [6000, 9000])]):
+        n = [round(share * total), total - round(share * total)]
+        batch.starts.copy_(torch.tensor([0, n[0], total], dtype=torch.int32))
+        batch.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        q.copy_(_rows(gen, total, Hq))
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        at = 0
+        for b in range(2):
+            ref, size = P.attend(q[at:at + n[b]], stored[b][0][:lengths[b]], stored[b][1][:lengths[b]], causal=True)
+            off = (out[at:at + n[b]].double() - ref).abs() - (BF16 * ref.abs() + (BF16 + 2.0 ** -14 + math.expm1(2 * 2.0 ** -14)) * size * (1 + BF16))
+            assert float(off.max() if off.numel() else 0.0) <= 0.0, (turn, b)
+            at += n[b]
 
 
 def test_two_streams_with_a_workspace_each():
