@@ -195,7 +195,7 @@ __host__ __device__ constexpr int part_floats(int rb) { return rb * (kD + 2); }
 // bf16 as well, and its products with K are added to S^T; under the bytes of 16 rows that is free (the error of a result against 64 bits falls from 0.0029 of
 // it to 0.0024, where the rounding of P and of the result is left), with 32 rows, whose keys come out of L2, calls took up to 1.8 times as long.
 
-template <bool FP8, int QB>
+template <int QB>
 struct SplitState {
   bf16x8 qf[QB][4];
   f32x4 o[8][QB];
@@ -204,7 +204,7 @@ struct SplitState {
 
 // The weights of one half tile, the running maximum and the row sums.  ve: exponents of the values' scales.
 template <bool FP8, int QB>
-__device__ __forceinline__ void split_softmax(SplitState<FP8, QB>& w, const f32x4 (&s)[2][QB], bf16x8 (&pf)[QB], const unsigned (&ve)[2], float c) {
+__device__ __forceinline__ void split_softmax(SplitState<QB>& w, const f32x4 (&s)[2][QB], bf16x8 (&pf)[QB], const unsigned (&ve)[2], float c) {
   float alpha[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
   while (left > 0) {
     const int nt = block_tiles(p, s, RB, at.j), take = tiles_left(left, at.t, nt, 1);
     __syncthreads();                                           // the sums, or the results of the unit before, are read
-    SplitState<FP8, QB> w;
+    SplitState<QB> w;
     int sees[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) sees[qb] = row_keys(p, s, at.j * RB + 16 * qb + c16);
@@ -537,7 +537,6 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
 }
 
 // ---- the tile form: many query rows, all waves of a workgroup share every key tile ----
-//
 // A unit is 384 query rows, 32 a wave; twelve waves are three a SIMD, one workgroup a CU.  The loop is that of the dense calls: K/V tiles in an LDS ring
 // of three, two tiles ahead of the products, one barrier a tile.  The page of a tile is looked up a step before its copy.  (Units of 128 rows
 // in four waves, three workgroups a CU, in halves of tiles, were behind on all but some calls of a few dozen rows, and there by 2 %: 1,560 rows over
