@@ -104,7 +104,10 @@ int pkh3_paged_read(const pkh3_paged_args* a, void* stream);
 size_t pkh3_paged_workspace_bytes(const pkh3_paged_args* a);
 
 /* Attention of the call's rows over their sequences' keys.  A row that sees no key gets zeros.  Results depend on the
-   arguments and on what the batch's arrays hold, never on timing. */
+   arguments and on what the batch's arrays hold, never on timing.  How the work is cut into blocks of rows goes by the sizes of the call (rows, B, heads,
+   table_pages), for the whole of it: blocks of 16 rows keep what the rounding of q to bf16 after norm or rotation leaves, larger ones do not, and the
+   rounded weights differ, so the last bits of a sequence's result may depend on the batch that it is in.  A chunk over a long context among many sequences
+   without rows is slow: B is best the number of sequences that have some. */
 int pkh3_paged_attn(const pkh3_paged_args* a, void* stream);
 
 #ifdef __cplusplus
