@@ -35,9 +35,10 @@
  *     reads of it give zeros;
  *   - a row in front of position 0 (more new rows than keys) is not written, reads as zeros, and sees no key under
  *     PKH3_PAGED_CAUSAL (without it, it sees them all);
- *   - pkh3_paged_write takes starts and lengths as they are, so that no row comes to another's place: row r of the call stands at
- *     lengths[b] - starts[b+1] + r, and is written if it is one of the call's rows and that place is in the table.  A sequence that has grown past
- *     its table loses the rows behind it and keeps what is stored.
+ *   - a row's place goes by starts and lengths as they are, so that none comes to another's: row r of the call stands at
+ *     lengths[b] - starts[b+1] + r.  pkh3_paged_write writes the rows of the call whose place is in the table, and under PKH3_PAGED_CAUSAL a row sees what
+ *     is stored up to its own place.  A sequence that has grown past its table loses the rows behind it and keeps what is stored.  (pkh3_paged_read
+ *     alone goes by the values brought into range: of such a sequence it gives the last rows of the table.)
  * Rows that belong to no sequence are neither read nor written.  starts must not decrease, and no two places that one call
  * writes may be the same.
  */

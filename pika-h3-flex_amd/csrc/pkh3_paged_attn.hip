@@ -36,8 +36,15 @@ __device__ __forceinline__ int lane_here() {
 
 // ---- the tile space ----
 
+__device__ __forceinline__ Sequence attended(const PagedParams& p, int b) {
+  return make_attended(p.starts[b], p.starts[b + 1], p.lengths[b], p.rows, p.table_pages, p.causal);
+}
+__device__ __forceinline__ Sequence uniform_attended(const PagedParams& p, int b) {
+  return make_attended(uniform_int(p.starts, b), uniform_int(p.starts, b + 1), uniform_int(p.lengths, b), p.rows, p.table_pages, p.causal);
+}
+
 __device__ __forceinline__ int blocks_of(const PagedParams& p, const Sequence& s, int rb) { return blocks_of(s, p.G, rb); }
-__device__ __forceinline__ int block_tiles(const PagedParams& p, const Sequence& s, int rb, int j) { return block_tiles(s, p.G, p.causal, rb, j); }
+__device__ __forceinline__ int block_tiles(const PagedParams& p, const Sequence& s, int rb, int j) { return block_tiles(s, p.G, p.causal, rb, j, p.table_pages); }
 __device__ __forceinline__ int row_keys(const PagedParams& p, const Sequence& s, int r) { return row_keys(s, p.G, p.causal, r); }
 __device__ __forceinline__ int block_cost(const PagedParams& p, const Sequence& s, int rb, int j) { return block_cost(s, p.G, rb, j); }
 __device__ __forceinline__ int64_t unit_cost(const PagedParams& p, const Sequence& s, int rb, int j) {
@@ -60,7 +67,7 @@ __device__ __forceinline__ void sum_tiles(const PagedParams& p, int64_t* cum, in
     int64_t mine = 0;
     bool many = false;
     if (b < p.B) {
-      const Sequence s = sequence(p, b);
+      const Sequence s = attended(p, b);
       const int blocks = blocks_of(p, s, rb);
       many = p.causal && blocks > kAlone;
       if (!p.causal) mine = blocks ? (blocks - 1) * unit_cost(p, s, rb, 0) + unit_cost(p, s, rb, blocks - 1) : 0;
@@ -69,7 +76,7 @@ __device__ __forceinline__ void sum_tiles(const PagedParams& p, int64_t* cum, in
     }
     for (unsigned long long left = __ballot(many); left; left &= left - 1) {
       const int l = __ffsll((unsigned long long)left) - 1;
-      const Sequence s = uniform_sequence(p, __builtin_amdgcn_readfirstlane(at + l));
+      const Sequence s = uniform_attended(p, __builtin_amdgcn_readfirstlane(at + l));
       const int blocks = blocks_of(p, s, rb);
       int64_t sum = 0;
       for (int j = lane; j < blocks; j += 64) sum += unit_cost(p, s, rb, j);
@@ -91,7 +98,7 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
 __device__ __forceinline__ Place find_place(const PagedParams& p, const int64_t* cum, int rb, const Shares& sh, int64_t pos) {
   Place at;
   at.b = find_sequence(cum, p.B, pos);
-  const Sequence s = uniform_sequence(p, at.b);
+  const Sequence s = uniform_attended(p, at.b);
   const int blocks = blocks_of(p, s, rb);
   const int64_t per_head = divided(cum[at.b + 1] - cum[at.b], p.H);
   int64_t rest = pos - cum[at.b];
@@ -147,7 +154,7 @@ __device__ __forceinline__ bool find_run(const PagedParams& p, const int64_t* cu
       found[1] = (int64_t)(uint32_t)x.j << 32 | (uint32_t)x.t;
       found[2] = x.pos;
       if (run.rank > 0) {
-        const Sequence s = uniform_sequence(p, x.b);
+        const Sequence s = uniform_attended(p, x.b);
         const int nt = block_tiles(p, s, rb, x.j);
         p.cuts[run.rank] = i32x4{x.b, x.h, x.j, parts_at(sh, run.rank, x.unit, x.t, nt, block_cost(p, s, rb, x.j))};
       }
@@ -173,7 +180,7 @@ __device__ __forceinline__ bool next_unit(const PagedParams& p, Place& at, Seque
   at.h = 0;
   do {
     if (++at.b >= p.B) return false;
-    s = uniform_sequence(p, at.b);
+    s = uniform_attended(p, at.b);
   } while (s.n == 0);
   blocks = blocks_of(p, s, rb);
   return true;
@@ -322,7 +329,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, 2) void paged_split_kernel(PagedP
   Place at;
   if (!find_run(p, cum, found, RB, run, at)) return;
   int64_t left = run.left;
-  Sequence s = uniform_sequence(p, at.b);
+  Sequence s = uniform_attended(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
     at.t = 0;
@@ -748,7 +755,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
   Place at;
   if (!find_run(p, cum, found, RB, run, at)) return;
   int64_t left = run.left;
-  Sequence s = uniform_sequence(p, at.b);
+  Sequence s = uniform_attended(p, at.b);
   int blocks = blocks_of(p, s, RB);
   if (at.t == block_tiles(p, s, RB, at.j)) {
     at.t = 0;
@@ -808,7 +815,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 1) void paged_tile_kernel(PagedPar
     if (next_unit(p, at, s, blocks, RB, left)) return true;
     if (later.b < 0) return false;
     at.b = later.b, at.h = later.h, at.j = later.j, at.t = later.t, left = later.left;
-    s = uniform_sequence(p, at.b);
+    s = uniform_attended(p, at.b);
     blocks = blocks_of(p, s, RB);
     later.b = -1;
     return true;
@@ -1034,7 +1041,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedParams p) {
   const int run = (int)blockIdx.x + 1;
   const i32x4 cut = p.cuts[run];
   if (run >= p.cuts[0][0] || cut[3] == 0) return;
-  const Sequence s = uniform_sequence(p, cut[0]);
+  const Sequence s = uniform_attended(p, cut[0]);
   const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)blockIdx.y * kRows;
   if (row0 >= rows) return;
   const int here = min(kRows, rows - row0), groups = here > 2 ? 2 : 8 / here;   // groups of 32 threads a row
@@ -1089,7 +1096,7 @@ __global__ __launch_bounds__(256) void paged_merge_tile_kernel(PagedParams p) {
   const int run = (int)blockIdx.x + 1;
   const i32x4 cut = p.cuts[run];
   if (run >= p.cuts[0][0] || cut[3] == 0) return;
-  const Sequence s = uniform_sequence(p, cut[0]);
+  const Sequence s = uniform_attended(p, cut[0]);
   const int rows = min(RB, s.n * p.G.n - cut[2] * RB), row0 = (int)(blockIdx.y >> 1) * 16, half = blockIdx.y & 1;
   if (row0 >= rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;

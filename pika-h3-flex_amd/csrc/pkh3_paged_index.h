@@ -27,6 +27,14 @@ constexpr Sequence make_written(int start, int end, int length, int rows, int ta
   const int64_t at = row0 > from ? row0 : from, to = behind < until ? behind : until;
   return to > at ? Sequence{(int)at, (int)(to - at), (int)(to - row0)} : Sequence{0, 0, 0};
 }
+// .. and for attention: under the causal limit row r sees the keys up to length - end + r, those of its sequence that lie behind the table not among them, as
+// if the table went on with pages that are not there.  `keys` is then the end of the call's last row, which nobody sees past (up to n past the table: the
+// tiles end there).
+constexpr Sequence make_attended(int start, int end, int length, int rows, int table_pages, int causal) {
+  const int at = at_most(at_least(start, 0), rows), to = at_most(at_least(end, 0), rows), n = at_least(to - at, 0);
+  const int last = at_least(length, 0) - (causal ? at_least(end, 0) - to : 0);
+  return {at, n, at_most(at_least(last, 0), table_pages * kPageKeys + (causal ? n : 0))};
+}
 constexpr int page_in_pool(int id, int64_t n_pages) { return id >= 0 && id < n_pages ? id : -1; }
 
 // ---- writing and reading: the tiles that a sequence's rows lie in, in front of position 0 too ----
@@ -72,6 +80,9 @@ constexpr int row_keys(const Sequence& s, const Group& G, int causal, int r) {
 // tiles of block j: of its last row.  One at least: a block without keys writes zeros
 constexpr int block_tiles(const Sequence& s, const Group& G, int causal, int rb, int j) {
   return at_least((row_keys(s, G, causal, (j + 1) * rb - 1) + kPageKeys - 1) >> 6, 1);
+}
+constexpr int block_tiles(const Sequence& s, const Group& G, int causal, int rb, int j, int table_pages) {
+  return at_most(block_tiles(s, G, causal, rb, j), table_pages);
 }
 
 // What a tile of block j costs, by the waves of a workgroup that have rows of it: in the form of 384 rows (12 waves, three a SIMD) 4, or where there

@@ -552,6 +552,30 @@ def test_a_write_past_the_table_leaves_what_is_stored(fp8):
         held.cache.data.copy_(before)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("rows,wide", [(4, 0), (30, 0), (130, 0), (130, 8000)])
+def test_a_causal_chunk_over_the_end_of_its_table(rows, wide, fp8):
+    """Rows whose places are behind the table, or that the call does not have, move no other row: each sees what is stored up to its own place."""
+    import pika_h3_flex_amd as pk
+
+    P = _oracle()
+    held = Held([320, 64], 2, fp8, seed=6)
+    table = held.batch([0, 0]).table
+    stored = [t.cuda() for t in held.stored(0)]
+    table = torch.cat([table, table.new_full((2, wide), -1)], 1)                         # (another form over a wide table, whose pages are not there)
+    q = _rows(torch.Generator().manual_seed(1), rows, 4).cuda()
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")                 # noqa: E731
+    for end, length in ((rows, 320 + rows // 2), (rows, 320 + 2 * rows), (rows + 3, 300), (rows + 40, 350), (rows, 10 ** 9), (rows, rows // 2)):
+        batch = pk.PagedBatch(as_int([0, end, end]), as_int([length, 0]), table)
+        got = pk.paged_attention(q, held.cache, batch, causal=True).double()
+        own = length - end + torch.arange(rows)                                          # the rows' places
+        for r in {0, 1, rows // 2, rows - 1}:
+            m = max(0, min(320, length, int(own[r]) + 1))
+            ref, size = P.attend(q[r:r + 1], stored[0][:m], stored[1][:m], causal=False)
+            bound = BF16 * ref.abs() + (BF16 + 2.0 ** -14 + math.expm1(2 * 2.0 ** -14)) * size * (1 + BF16)
+            assert bool(((got[r:r + 1] - ref).abs() <= bound).all()), (end, length, r)
+
+
 def test_strides_order_and_the_output_in_the_queries_place():
     import pika_h3_flex_amd as pk
 

@@ -364,6 +364,30 @@ def test_rows_are_written_in_their_own_place_or_not_at_all(tmp_path):
   }""")
 
 
+def test_rows_see_the_keys_up_to_their_own_place(tmp_path):
+    """Whatever starts and lengths hold: under the causal limit a row sees what is stored up to length - end + row of the values as they are, otherwise all of it."""
+    _run(tmp_path, """
+  const int wild[] = {0, 1, 5, 63, 64, 65, 129, 192, 193, 1000, -1, -7, 2147483647, -2147483647 - 1, 16777216, 1 << 30};
+  const int n_wild = sizeof(wild) / sizeof(int);
+  for (int a = 0; a < n_wild; ++a) for (int b = 0; b < n_wild; ++b) for (int c = 0; c < n_wild; ++c)
+    for (int rows : {0, 1, 70, 200}) for (int pages : {1, 3, 16777216}) for (int causal : {0, 1}) {
+      const Sequence s = make_attended(wild[a], wild[b], wild[c], rows, pages, causal);
+      CHECK(s.n >= 0 && s.first >= 0 && s.first + s.n <= rows, "%d %d %d", wild[a], wild[b], wild[c]);
+      CHECK(s.n == std::max<int64_t>(0, (int64_t)std::min(wild[b], rows) - std::max(wild[a], 0)), "%d rows", s.n);
+      const int64_t held = std::max<int64_t>(0, std::min<int64_t>(wild[c], (int64_t)pages * 64));
+      for (int g : {1, 6}) for (int rb : {16, 32, 384}) {
+        const Group G = make_group(g);
+        for (int r = 0; r < s.n * g; ++r) {
+          const int64_t own = (int64_t)wild[c] - wild[b] + s.first + r / g, sees = causal ? std::max<int64_t>(0, std::min(held, own + 1)) : held;
+          const int t = block_tiles(s, G, causal, rb, r / rb, pages), k = row_keys(s, G, causal, r);
+          CHECK(t >= 1 && t <= pages && sees <= 64ll * t, "%d tiles", t);
+          CHECK(std::min<int64_t>(k, pages * 64ll) == sees, "row %d of %d %d %d sees %d", r, wild[a], wild[b], wild[c], k);
+          CHECK(std::min<int64_t>(s.keys, pages * 64ll) >= sees && k >= row_keys(s, G, causal, r / rb * rb), "keys");
+        }
+      }
+    }""")
+
+
 def test_the_processor_refuses_what_does_not_go_with_pages():
     proc = pk.PikaH3AttnProcessor()
     cache = pk.PagedKV(2, 1, device="cpu")
