@@ -12,6 +12,7 @@ from .layout import (
 )
 from . import packing
 from . import projections
+from .feed_forward import feed_forward, feed_forward_backward, layer_norm, layer_norm_backward, linear, linear_backward
 from .ops import BlockMask, PreparedKV, attention, attention_prepared, prepare_kv, rope_tables, time_attention_kernel
 from .paged import PagedBatch, PagedKV, paged_attention, paged_read, paged_write
 from .processor import PikaH3AttnProcessor
@@ -19,6 +20,7 @@ from .processor import PikaH3AttnProcessor
 __all__ = [
     "BlockMask", "PikaH3AttnProcessor", "Pkh3Error", "ROPE_HALF", "ROPE_INTERLEAVED", "ROPE_NONE",
     "PagedBatch", "PagedKV", "paged_attention", "paged_read", "paged_write",
+    "feed_forward", "feed_forward_backward", "layer_norm", "layer_norm_backward", "linear", "linear_backward",
     "PreparedKV", "attention", "attention_prepared", "audio_position_ids", "local_window_tile_map", "packing", "prepare_kv", "projections", "rope_tables", "time_attention_kernel",
     "video_position_ids",
 ]

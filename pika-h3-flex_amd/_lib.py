@@ -54,6 +54,13 @@ EXPORTS = (
     "pkh3_paged_read",
     "pkh3_paged_workspace_bytes",
     "pkh3_paged_attn",
+    "pkh3_layer_norm",
+    "pkh3_layer_norm_backward",
+    "pkh3_norm_workspace_bytes",
+    "pkh3_product",
+    "pkh3_product_workspace_bytes",
+    "pkh3_activation_grad",
+    "pkh3_activation_grad_workspace_bytes",
 )
 
 
@@ -144,6 +151,44 @@ class PagedArgs(C.Structure):
 PAGED_ARGS_FORMAT = struct.Struct("@Pq3Pq4P8q6i2f3PiIPN")
 assert PAGED_ARGS_FORMAT.size == C.sizeof(PagedArgs)
 
+# include/pkh3_rows.h
+LAYER_NORM_F32, LAYER_NORM_TABLES_BF16 = 1, 2
+LAYER_NORM_MAX_WIDTH, LAYER_NORM_MAX_TABLES = 16384, 64
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
+PRODUCT_A_ACROSS, PRODUCT_B_ACROSS, PRODUCT_GATED, PRODUCT_GRAD, PRODUCT_BIAS_BF16 = 1, 2, 4, 8, 16
+
+
+class NormArgs(C.Structure):
+    """Mirror of ``struct pkh3_norm_args``."""
+
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("row_index", C.c_void_p), ("out", C.c_void_p),
+        ("dy", C.c_void_p), ("dx", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("x_stride", C.c_int64), ("out_stride", C.c_int64), ("dy_stride", C.c_int64), ("dx_stride", C.c_int64),
+        ("rows", C.c_int32), ("width", C.c_int32), ("tables", C.c_int32), ("eps", C.c_float), ("flags", C.c_uint32),
+    ]
+
+
+NORM_ARGS_FORMAT = struct.Struct("@10PQ4q3ifI4x")
+assert NORM_ARGS_FORMAT.size == C.sizeof(NormArgs)
+
+
+class ProductArgs(C.Structure):
+    """Mirror of ``struct pkh3_product_args``."""
+
+    _fields_ = [
+        ("a", C.c_void_p), ("b", C.c_void_p), ("bias", C.c_void_p), ("gate", C.c_void_p), ("gate_index", C.c_void_p), ("residual", C.c_void_p),
+        ("pre", C.c_void_p), ("out", C.c_void_p), ("sums", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("a_stride", C.c_int64), ("b_stride", C.c_int64), ("gate_stride", C.c_int64), ("residual_stride", C.c_int64), ("pre_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("gate_rows", C.c_int32), ("activation", C.c_int32), ("flags", C.c_uint32),
+    ]
+
+
+PRODUCT_ARGS_FORMAT = struct.Struct("@10PQ6q5iI")
+assert PRODUCT_ARGS_FORMAT.size == C.sizeof(ProductArgs)
+
 
 class Pkh3Error(RuntimeError):
     def __init__(self, code: int, message: str):
@@ -198,6 +243,17 @@ def load() -> C.CDLL:
     for call in (lib.pkh3_paged_write, lib.pkh3_paged_read, lib.pkh3_paged_attn):
         call.argtypes = [C.POINTER(PagedArgs), C.c_void_p]
         call.restype = C.c_int
+    for call in (lib.pkh3_layer_norm, lib.pkh3_layer_norm_backward):
+        call.argtypes = [C.POINTER(NormArgs), C.c_void_p]
+        call.restype = C.c_int
+    for call in (lib.pkh3_product, lib.pkh3_activation_grad):
+        call.argtypes = [C.POINTER(ProductArgs), C.c_void_p]
+        call.restype = C.c_int
+    lib.pkh3_norm_workspace_bytes.argtypes = [C.POINTER(NormArgs)]
+    lib.pkh3_norm_workspace_bytes.restype = C.c_size_t
+    for call in (lib.pkh3_product_workspace_bytes, lib.pkh3_activation_grad_workspace_bytes):
+        call.argtypes = [C.POINTER(ProductArgs)]
+        call.restype = C.c_size_t
     lib.pkh3_version.argtypes = []
     lib.pkh3_version.restype = C.c_int
     lib.pkh3_strerror.argtypes = [C.c_int]

@@ -1,0 +1,219 @@
+// Parameters of the kernels behind include/pkh3_rows.h, and how a product finishes its results.
+#pragma once
+#include "pkh3_common.h"
+
+namespace pkh3 {
+
+// ---- layer norm ----
+
+struct NormParams {
+  const char *x, *dy;
+  char *out, *dx;
+  const char *weight, *bias;     // [tables][width], or null
+  const int* row_index;          // or null
+  float* part;                   // backward: partial sums of the workgroups (norm_slices)
+  uint64_t* touched;             // ... and which tables each of them holds
+  float *dweight, *dbias;
+  int64_t x_stride, out_stride, dy_stride, dx_stride;   // bytes
+  int rows, width, tables, groups;
+  float eps;
+};
+
+int norm_groups(int rows, int tables);              // workgroups of the backward pass, each with sums of its own
+size_t norm_scratch_bytes(int rows, int width, int tables);
+hipError_t launch_norm(const NormParams& p, bool f32, bool tables_bf16, hipStream_t s);
+hipError_t launch_norm_backward(NormParams p, bool f32, bool tables_bf16, char* workspace, hipStream_t s);
+
+// ---- products ----
+
+enum ProductMode { kPlain = 0, kGated = 1, kGrad = 2, kGatedGrad = 3 };
+
+struct ProductParams {
+  const char *a, *b;             // [M, K] and [N, K], or across
+  int64_t a_stride, b_stride;    // bytes
+  const char* bias;
+  const char* gate;
+  const int* gate_index;
+  const char* residual;
+  char* pre;
+  char* out;
+  float* sums;                   // partial sums of out's columns, [rows of partial sums][columns], or null
+  float* part;                   // partial results of a contraction that is cut: [cut][M][columns]
+  int64_t gate_stride, residual_stride, pre_stride, out_stride;   // bytes
+  int M, N, K, gate_rows;
+  int act, bias_bf16;
+};
+
+// How a call is carried out, by its sizes alone.
+struct ProductPlan {
+  int sum_rows;                  // rows of partial column sums
+  size_t sums_off, total;        // bytes of the workspace
+};
+ProductPlan plan_product(int M, int N, int K, bool a_across, bool b_across, int mode, bool sums);
+hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_across, bool b_across, int mode, void* sums, char* workspace, hipStream_t s);
+
+int activation_grad_rows(int M);                    // rows of partial column sums of an activation's gradient
+hipError_t launch_activation_grad(ProductParams p, void* sums, char* workspace, hipStream_t s);
+
+// ---- activations ----
+
+// exp(x); one instruction's error of 2^x (about 1 ulp) and the rounding of x log2(e)
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
+
+// The normal distribution: (1 + erf(v / sqrt 2)) / 2 = erfc(z) / 2 or 1 - erfc(z) / 2, z = |v| / sqrt 2, with erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2).
+// p is a polynomial fitted to log(erfc(z) / t) + z^2 at Chebyshev points of t in [1/8, 1] (z up to 14): 8e-7 of the value everywhere, small tails among it.
+__device__ __forceinline__ float normal_cdf(float v) {
+  const float z = fabsf(v) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.5f * z);
+  float p = -0.190482009f;
+  p = p * t + 0.762907712f;
+  p = p * t - 1.02066945f;
+  p = p * t + 0.367882395f;
+  p = p * t - 0.0490815249f;
+  p = p * t + 0.396733912f;
+  p = p * t + 0.99815875f;
+  p = p * t - 1.26545055f;
+  const float half = 0.5f * t * exp_of(p - z * z);
+  return v < 0.f ? half : 1.0f - half;
+}
+
+constexpr float kTanhScale = 0.79788456080286536f;   // sqrt(2 / pi)
+constexpr float kTanhCube = 0.044715f;
+
+// act(v): 0 none, 1 silu, 2 gelu, 3 gelu through tanh (as v sigmoid(2 u), which keeps its small tail exact)
+template <int ACT>
+__device__ __forceinline__ float act_of(float v) {
+  if constexpr (ACT == 1) return v * sigmoid_of(v);
+  if constexpr (ACT == 2) return v * normal_cdf(v);
+  if constexpr (ACT == 3) return v * sigmoid_of(2.0f * kTanhScale * v * (1.0f + kTanhCube * v * v));
+  return v;
+}
+// act(v) and act'(v)
+template <int ACT>
+__device__ __forceinline__ void act_and_slope(float v, float& value, float& slope) {
+  if constexpr (ACT == 1) {
+    const float q = sigmoid_of(v);
+    value = v * q;
+    slope = q + value * (1.0f - q);
+  } else if constexpr (ACT == 2) {
+    const float q = normal_cdf(v);
+    value = v * q;
+    slope = q + v * 0.39894228040143268f * exp_of(-0.5f * v * v);
+  } else if constexpr (ACT == 3) {
+    const float q = sigmoid_of(2.0f * kTanhScale * v * (1.0f + kTanhCube * v * v));
+    value = v * q;
+    slope = q + value * (1.0f - q) * (2.0f * kTanhScale) * (1.0f + 3.0f * kTanhCube * v * v);
+  } else {
+    value = v;
+    slope = 1.0f;
+  }
+}
+
+// f(activation as a constant)
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  if (act == 0) f(std::integral_constant<int, 0>{});
+  else if (act == 1) f(std::integral_constant<int, 1>{});
+  else if (act == 2) f(std::integral_constant<int, 2>{});
+  else f(std::integral_constant<int, 3>{});
+}
+
+// ---- eight results of a row: columns n .. n + 7 of row m ----
+
+struct Piece {
+  float v[8];
+};
+__device__ __forceinline__ Piece load_piece(const char* at) {
+  const bf16x8 raw = *(const bf16x8*)at;
+  Piece p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p.v[j] = (float)raw[j];
+  return p;
+}
+__device__ __forceinline__ void store_piece(char* at, const Piece& p) {
+  bf16x8 raw;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) raw[j] = (__bf16)p.v[j];
+  *(bf16x8*)at = raw;
+}
+__device__ __forceinline__ Piece load_piece_f32(const char* at) {
+  const f32x4 lo = *(const f32x4*)at, hi = *(const f32x4*)(at + 16);
+  return Piece{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+}
+__device__ __forceinline__ Piece load_table(const char* table, int64_t at, bool bf16) {
+  return bf16 ? load_piece(table + at * 2) : load_piece_f32(table + at * 4);
+}
+
+// The bias of columns n .. n + 7, and of the gates' (mode kGated)
+struct Bias {
+  Piece a, b;
+};
+template <int MODE>
+__device__ __forceinline__ Bias load_bias(const ProductParams& p, int n) {
+  Bias bias{};
+  if (MODE <= kGated && p.bias) {
+    bias.a = load_table(p.bias, n, p.bias_bf16);
+    if (MODE == kGated) bias.b = load_table(p.bias, p.N + n, p.bias_bf16);
+  }
+  return bias;
+}
+
+// From sums to results (see pkh3_product in the header).  a: the sums of columns n .. n + 7, b: of the gates'.  On return what out got, for the sums of columns.
+template <int MODE, int ACT>
+__device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Piece& a, Piece& b, const Bias& bias) {
+  if constexpr (MODE <= kGated) {
+    char* pre = p.pre ? p.pre + m * p.pre_stride + (int64_t)n * 2 : nullptr;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a.v[j] += bias.a.v[j];
+    if (pre) store_piece(pre, a);
+    if constexpr (MODE == kGated) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b.v[j] += bias.b.v[j];
+      if (pre) store_piece(pre + (int64_t)p.N * 2, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a.v[j] *= act_of<ACT>(b.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a.v[j] = act_of<ACT>(a.v[j]);
+    }
+    if (p.gate) {
+      const int row = p.gate_index ? min(max(p.gate_index[m], 0), p.gate_rows - 1) : 0;
+      const Piece g = load_piece(p.gate + row * p.gate_stride + (int64_t)n * 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a.v[j] *= g.v[j];
+    }
+    if (p.residual) {
+      const Piece r = load_piece(p.residual + m * p.residual_stride + (int64_t)n * 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a.v[j] += r.v[j];
+    }
+    store_piece(p.out + m * p.out_stride + (int64_t)n * 2, a);
+  } else if constexpr (MODE == kGrad) {
+    if (ACT != 0) {
+      const Piece z = load_piece(p.pre + m * p.pre_stride + (int64_t)n * 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float value, slope;
+        act_and_slope<ACT>(z.v[j], value, slope);
+        a.v[j] *= slope;
+      }
+    }
+    store_piece(p.out + m * p.out_stride + (int64_t)n * 2, a);
+  } else {
+    const char* pre = p.pre + m * p.pre_stride + (int64_t)n * 2;
+    const Piece va = load_piece(pre), vb = load_piece(pre + (int64_t)p.N * 2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float value, slope;
+      act_and_slope<ACT>(vb.v[j], value, slope);
+      b.v[j] = a.v[j] * va.v[j] * slope;
+      a.v[j] *= value;
+    }
+    char* out = p.out + m * p.out_stride + (int64_t)n * 2;
+    store_piece(out, a);
+    store_piece(out + (int64_t)p.N * 2, b);
+  }
+}
+
+}  // namespace pkh3
