@@ -60,12 +60,13 @@ size_t pkh3_norm_workspace_bytes(const pkh3_norm_args* args);
  * dy W is (dy, W across), its weight's gradient dy^T x is (dy across, x across).  K alone may be any number: rows of a matrix that is stored
  * across need not come in eights.
  *
- *   plain    v = sum + bias[n]; pre[m, n] = v, if given; out = residual[m, n] + gate[index[m], n] * act(v), as far as given
+ *   plain    v = sum + bias[n]; pre[m, n] = v in float32, if given; out = residual[m, n] + gate[index[m], n] * act(v), as far as given
  *   GATED    B has 2 N rows, bias 2 N entries: a = row n, b = row N + n.  pre [M, 2 N] = (a | b), if given; out = a * act(b), then as above
  *   GRAD     sum is the gradient of act(pre) and out [M, N] that of pre: out = sum * act'(pre[m, n])
  *   GRAD and GATED   pre [M, 2 N] = (a | b), out [M, 2 N]: out[m, n] = sum * act(b), out[m, N + n] = sum * a * act'(b)
  *
- * With GRAD, `sums`, if given, gets the sums of out's columns before they were rounded (bfloat16, N or 2 N entries). */
+ * Offered are A and B along (plain, GATED), A along and B across (plain, GRAD, GRAD and GATED), and both across (plain); of others
+ * PKH3_EUNSUPPORTED.  With GRAD, `sums`, if given, gets the sums of out's columns before they were rounded (bfloat16, N or 2 N entries). */
 
 enum {
   PKH3_ACT_NONE = 0,
@@ -87,7 +88,7 @@ typedef struct pkh3_product_args {
   const void* gate;             /* bfloat16 [gate_rows, N] */
   const int32_t* gate_index;    /* [M], brought into [0, gate_rows); NULL: 0 */
   const void* residual;         /* bfloat16 [M, N] */
-  void* pre;                    /* bfloat16: written, with GRAD read */
+  void* pre;                    /* float32 [M, N or 2 N]: written, with GRAD read */
   void* out;
   void* sums;
   void* workspace;              /* 256-byte aligned, pkh3_product_workspace_bytes(); NULL where that is 0 */

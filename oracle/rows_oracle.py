@@ -93,7 +93,7 @@ def finish(z, bound, name, gate=None, index=None, residual=None):
     return rounded(y, bound)
 
 
-def _first(x, w, b):
+def first_product(x, w, b):
     z, e = product(x, w)
     if b is not None:
         z = z + b.double()
@@ -103,12 +103,12 @@ def _first(x, w, b):
 
 def linear(x, w, b=None, name="none", gate=None, index=None, residual=None):
     """(result, bound)"""
-    return finish(*_first(x, w, b), name, gate, index, residual)
+    return finish(*first_product(x, w, b), name, gate, index, residual)
 
 
 def middle(x, w_in, b_in, name, gated):
     """(h, its bound, the first product, its bound), h rounded to bfloat16."""
-    z, e = _first(x, w_in, b_in)
+    z, e = first_product(x, w_in, b_in)
     if not gated:
         h, eh = finish(z, e, name)
         return h, eh, z, e
@@ -122,16 +122,16 @@ def middle(x, w_in, b_in, name, gated):
 
 def feed_forward(x, w_in, w_out, b_in=None, b_out=None, name="silu", gated=True, gate=None, index=None, residual=None):
     h, eh, _, _ = middle(x, w_in, b_in, name, gated)
-    y, _ = _first(h, w_out, b_out)
+    y, _ = first_product(h, w_out, b_out)
     w = w_out.double().abs()
     e = eh @ w.t() + (h.shape[1] + 2) * 2 * HALF_F32 * ((h.abs() + eh) @ w.t()) + 2 * HALF_F32 * y.abs()
     return finish(y, e, "none", gate, index, residual)
 
 
 def _grad(sum_, e, z, ez, name):
-    """sum * act'(z) from a saved z that is rounded to bfloat16: (value, bound) before its own rounding."""
+    """sum * act'(z) from a saved z: (value, bound) before its own rounding."""
     slope = act_slope(name, z)
-    es = CURVATURE[name] * (ez + HALF_BF16 * (z.abs() + ez)) + (4e-6 * (1 + z.abs()) if name != "none" else 0.0)
+    es = CURVATURE[name] * ez + (4e-6 * (1 + z.abs()) if name != "none" else 0.0)
     v = sum_ * slope
     return v, e * (slope.abs() + es) + sum_.abs() * es + 2 * HALF_F32 * v.abs()
 
@@ -152,7 +152,7 @@ def _sums(v, e):
 
 def linear_backward(dy, x, w, b=None, name="none"):
     """[(dx, bound), (dw, bound), (db, bound)]"""
-    z, ez = _first(x, w, b)
+    z, ez = first_product(x, w, b)
     dz, e = _grad(dy.double(), torch.zeros_like(z), z, ez, name)
     db = _sums(dz, e)
     if name != "none":
@@ -170,8 +170,6 @@ def feed_forward_backward(dy, x, w_in, w_out, b_in=None, b_out=None, name="silu"
     if gated:
         a, b = z.chunk(2, 1)
         ea, eb = ez.chunk(2, 1)
-        eb = eb + HALF_BF16 * (b.abs() + eb)              # of the saved values
-        ea = ea + HALF_BF16 * (a.abs() + ea)
         f = act(name, b)
         ef = SLOPE[name] * eb + 4e-6 * f.abs() + 1e-37
         da, e_da = dh * f, e * (f.abs() + ef) + dh.abs() * ef + 2 * HALF_F32 * (dh * f).abs()

@@ -35,22 +35,26 @@ struct ProductParams {
   const char* gate;
   const int* gate_index;
   const char* residual;
-  char* pre;
+  char* pre;                     // float32
   char* out;
   float* sums;                   // partial sums of out's columns, [rows of partial sums][columns], or null
   float* part;                   // partial results of a contraction that is cut: [cut][M][columns]
   int64_t gate_stride, residual_stride, pre_stride, out_stride;   // bytes
   int M, N, K, gate_rows;
   int act, bias_bf16;
+  int cuts;                      // parts of the contraction, with `part`
 };
 
 // How a call is carried out, by its sizes alone.
 struct ProductPlan {
+  int tb;                        // 16-row blocks of A a wave: tiles of 32 * tb rows of A and 256 of B
+  int cuts;                      // parts of the contraction, each with workgroups of its own
   int sum_rows;                  // rows of partial column sums
-  size_t sums_off, total;        // bytes of the workspace
+  size_t part_off, sums_off, total;   // bytes of the workspace
 };
-ProductPlan plan_product(int M, int N, int K, bool a_across, bool b_across, int mode, bool sums);
+ProductPlan plan_product(int M, int N, int K, int mode, bool sums);
 hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_across, bool b_across, int mode, void* sums, char* workspace, hipStream_t s);
+bool product_offered(bool a_across, bool b_across, int mode);
 
 int activation_grad_rows(int M);                    // rows of partial column sums of an activation's gradient
 hipError_t launch_activation_grad(ProductParams p, void* sums, char* workspace, hipStream_t s);
@@ -141,6 +145,10 @@ __device__ __forceinline__ Piece load_piece_f32(const char* at) {
   const f32x4 lo = *(const f32x4*)at, hi = *(const f32x4*)(at + 16);
   return Piece{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
 }
+__device__ __forceinline__ void store_piece_f32(char* at, const Piece& p) {
+  *(f32x4*)at = f32x4{p.v[0], p.v[1], p.v[2], p.v[3]};
+  *(f32x4*)(at + 16) = f32x4{p.v[4], p.v[5], p.v[6], p.v[7]};
+}
 __device__ __forceinline__ Piece load_table(const char* table, int64_t at, bool bf16) {
   return bf16 ? load_piece(table + at * 2) : load_piece_f32(table + at * 4);
 }
@@ -159,18 +167,50 @@ __device__ __forceinline__ Bias load_bias(const ProductParams& p, int n) {
   return bias;
 }
 
+// What else a piece's results need, asked for ahead of them: the gate and the residual, or the saved sums.
+template <int MODE>
+struct Extra {
+  bf16x8 gate, residual;
+};
+template <>
+struct Extra<kGrad> {
+  Piece z;
+};
+template <>
+struct Extra<kGatedGrad> {
+  Piece a, b;
+};
+template <int MODE>
+__device__ __forceinline__ void fetch(const ProductParams& p, int m, int n, Extra<MODE>& e) {
+  if constexpr (MODE == kGrad) {
+    if (p.act) e.z = load_piece_f32(p.pre + m * p.pre_stride + (int64_t)n * 4);
+  } else if constexpr (MODE == kGatedGrad) {
+    const char* pre = p.pre + m * p.pre_stride + (int64_t)n * 4;
+    e.a = load_piece_f32(pre);
+    e.b = load_piece_f32(pre + (int64_t)p.N * 4);
+  } else {
+    if (p.gate) {
+      const int row = p.gate_index ? min(max(p.gate_index[m], 0), p.gate_rows - 1) : 0;
+      e.gate = *(const bf16x8*)(p.gate + row * p.gate_stride + (int64_t)n * 2);
+    }
+    if (p.residual) e.residual = *(const bf16x8*)(p.residual + m * p.residual_stride + (int64_t)n * 2);
+  }
+}
+
 // From sums to results (see pkh3_product in the header).  a: the sums of columns n .. n + 7, b: of the gates'.  On return what out got, for the sums of columns.
+// Sums that are saved for the backward pass stay in float32: rounded to bfloat16 they cost its gradients half as much again as their own rounding does.
 template <int MODE, int ACT>
-__device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Piece& a, Piece& b, const Bias& bias) {
+__device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Piece& a, Piece& b, const Bias& bias, const Extra<MODE>& e) {
+  char* out = p.out + m * p.out_stride + (int64_t)n * 2;
   if constexpr (MODE <= kGated) {
-    char* pre = p.pre ? p.pre + m * p.pre_stride + (int64_t)n * 2 : nullptr;
+    char* pre = p.pre ? p.pre + m * p.pre_stride + (int64_t)n * 4 : nullptr;
 #pragma unroll
     for (int j = 0; j < 8; ++j) a.v[j] += bias.a.v[j];
-    if (pre) store_piece(pre, a);
+    if (pre) store_piece_f32(pre, a);
     if constexpr (MODE == kGated) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) b.v[j] += bias.b.v[j];
-      if (pre) store_piece(pre + (int64_t)p.N * 2, b);
+      if (pre) store_piece_f32(pre + (int64_t)p.N * 4, b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) a.v[j] *= act_of<ACT>(b.v[j]);
     } else {
@@ -178,39 +218,32 @@ __device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Pie
       for (int j = 0; j < 8; ++j) a.v[j] = act_of<ACT>(a.v[j]);
     }
     if (p.gate) {
-      const int row = p.gate_index ? min(max(p.gate_index[m], 0), p.gate_rows - 1) : 0;
-      const Piece g = load_piece(p.gate + row * p.gate_stride + (int64_t)n * 2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] *= g.v[j];
+      for (int j = 0; j < 8; ++j) a.v[j] *= (float)e.gate[j];
     }
     if (p.residual) {
-      const Piece r = load_piece(p.residual + m * p.residual_stride + (int64_t)n * 2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] += r.v[j];
+      for (int j = 0; j < 8; ++j) a.v[j] += (float)e.residual[j];
     }
-    store_piece(p.out + m * p.out_stride + (int64_t)n * 2, a);
+    store_piece(out, a);
   } else if constexpr (MODE == kGrad) {
-    if (ACT != 0) {
-      const Piece z = load_piece(p.pre + m * p.pre_stride + (int64_t)n * 2);
+    if constexpr (ACT != 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float value, slope;
-        act_and_slope<ACT>(z.v[j], value, slope);
+        act_and_slope<ACT>(e.z.v[j], value, slope);
         a.v[j] *= slope;
       }
     }
-    store_piece(p.out + m * p.out_stride + (int64_t)n * 2, a);
+    store_piece(out, a);
   } else {
-    const char* pre = p.pre + m * p.pre_stride + (int64_t)n * 2;
-    const Piece va = load_piece(pre), vb = load_piece(pre + (int64_t)p.N * 2);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float value, slope;
-      act_and_slope<ACT>(vb.v[j], value, slope);
-      b.v[j] = a.v[j] * va.v[j] * slope;
+      act_and_slope<ACT>(e.b.v[j], value, slope);
+      b.v[j] = a.v[j] * e.a.v[j] * slope;
       a.v[j] *= value;
     }
-    char* out = p.out + m * p.out_stride + (int64_t)n * 2;
     store_piece(out, a);
     store_piece(out + (int64_t)p.N * 2, b);
   }

@@ -135,8 +135,9 @@ int check_product_sizes(const pkh3_product_args* a) {
   if (a->K < 1 || a->K > kMostRows) return fail(PKH3_ESHAPE, "K must be in [1, 2^21], got %d", a->K);
   if (a->activation < PKH3_ACT_NONE || a->activation > PKH3_ACT_GELU_TANH) return fail(PKH3_EARG, "unknown activation %d", a->activation);
   const bool a_across = a->flags & PKH3_PRODUCT_A_ACROSS, b_across = a->flags & PKH3_PRODUCT_B_ACROSS;
+  if (!product_offered(a_across, b_across, mode_of(a->flags))) return fail(PKH3_EUNSUPPORTED, "no product of these operands with flags 0x%x", a->flags);
   if (a_across && a->M % 8) return fail(PKH3_ESHAPE, "M must be a multiple of 8 where A is stored across, got %d", a->M);
-  if (!(a_across && b_across) && a->K % 8) return fail(PKH3_ESHAPE, "K must be a multiple of 8 unless both operands are stored across, got %d", a->K);
+  if (!a_across && a->K % 8) return fail(PKH3_ESHAPE, "K must be a multiple of 8 unless both operands are stored across, got %d", a->K);
   return PKH3_OK;
 }
 
@@ -150,7 +151,7 @@ int check_product(const pkh3_product_args* a) {
   const int wide = gated ? 2 * N : N, b_rows = mode == kGated ? 2 * N : N;
   const Matrix A = a->flags & PKH3_PRODUCT_A_ACROSS ? Matrix{"a", a->a, a->a_stride, K, M, 2} : Matrix{"a", a->a, a->a_stride, M, K, 2};
   const Matrix B = a->flags & PKH3_PRODUCT_B_ACROSS ? Matrix{"b", a->b, a->b_stride, K, b_rows, 2} : Matrix{"b", a->b, a->b_stride, b_rows, K, 2};
-  const Matrix out{"out", a->out, a->out_stride, M, mode == kGatedGrad ? wide : N, 2}, pre{"pre", a->pre, a->pre_stride, M, wide, 2};
+  const Matrix out{"out", a->out, a->out_stride, M, mode == kGatedGrad ? wide : N, 2}, pre{"pre", a->pre, a->pre_stride, M, wide, 4};
   const Matrix residual{"residual", a->residual, a->residual_stride, M, N, 2}, gate{"gate", a->gate, a->gate_stride, a->gate_rows, N, 2};
   const Matrix bias{"bias", a->bias, wide, 1, wide, a->flags & PKH3_PRODUCT_BIAS_BF16 ? 2 : 4};
   const Matrix index{"gate_index", a->gate_index, 1, 1, a->gate_index ? M : 0, 4}, sums{"sums", a->sums, wide, 1, wide, 2};
@@ -182,14 +183,14 @@ ProductParams product_params(const pkh3_product_args* a) {
   p.a = (const char*)a->a; p.b = (const char*)a->b; p.a_stride = a->a_stride * 2; p.b_stride = a->b_stride * 2;
   p.bias = (const char*)a->bias; p.gate = (const char*)a->gate; p.gate_index = a->gate_index; p.residual = (const char*)a->residual;
   p.pre = (char*)a->pre; p.out = (char*)a->out;
-  p.gate_stride = a->gate_stride * 2; p.residual_stride = a->residual_stride * 2; p.pre_stride = a->pre_stride * 2; p.out_stride = a->out_stride * 2;
+  p.gate_stride = a->gate_stride * 2; p.residual_stride = a->residual_stride * 2; p.pre_stride = a->pre_stride * 4; p.out_stride = a->out_stride * 2;
   p.M = a->M; p.N = a->N; p.K = a->K; p.gate_rows = a->gate_rows;
   p.act = a->activation; p.bias_bf16 = a->flags & PKH3_PRODUCT_BIAS_BF16 ? 1 : 0;
   return p;
 }
 
 ProductPlan product_plan(const pkh3_product_args* a) {
-  return plan_product(a->M, a->N, a->K, a->flags & PKH3_PRODUCT_A_ACROSS, a->flags & PKH3_PRODUCT_B_ACROSS, mode_of(a->flags), a->sums != nullptr);
+  return plan_product(a->M, a->N, a->K, mode_of(a->flags), a->sums != nullptr);
 }
 
 int check_activation_sizes(const pkh3_product_args* a) {
@@ -263,7 +264,7 @@ int pkh3_activation_grad(const pkh3_product_args* a, void* stream) {
   int rc = check_activation_sizes(a);
   if (rc) return rc;
   const bool act = a->activation != PKH3_ACT_NONE;
-  const Matrix in{"a", a->a, a->a_stride, a->M, a->N, 2}, out{"out", a->out, a->out_stride, a->M, a->N, 2}, pre{"pre", a->pre, a->pre_stride, a->M, a->N, 2};
+  const Matrix in{"a", a->a, a->a_stride, a->M, a->N, 2}, out{"out", a->out, a->out_stride, a->M, a->N, 2}, pre{"pre", a->pre, a->pre_stride, a->M, a->N, 4};
   const Matrix sums{"sums", a->sums, a->N, 1, a->N, 2};
   if (a->M) {
     if ((rc = check_matrix(in))) return rc;

@@ -41,8 +41,7 @@ __device__ __forceinline__ Piece load_row_piece(const char* row, int n) {
 template <bool F32>
 __device__ __forceinline__ void store_row_piece(char* row, int n, const Piece& p) {
   if constexpr (F32) {
-    *(f32x4*)(row + (int64_t)n * 4) = f32x4{p.v[0], p.v[1], p.v[2], p.v[3]};
-    *(f32x4*)(row + (int64_t)n * 4 + 16) = f32x4{p.v[4], p.v[5], p.v[6], p.v[7]};
+    store_piece_f32(row + (int64_t)n * 4, p);
   } else {
     store_piece(row + (int64_t)n * 2, p);
   }

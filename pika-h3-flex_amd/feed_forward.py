@@ -243,7 +243,7 @@ def _linear(x, weight, bias, activation, gate, row_index, residual, out, save):
     o = _matrix("out", out, rows, N, index)
     pre, p = None, (0, 0)
     if save and act:
-        pre = torch.empty(rows, N, dtype=_BF16, device=x.device)
+        pre = torch.empty(rows, N, dtype=_F32, device=x.device)
         p = (pre.data_ptr(), N)
     _product(a, b, o, rows, N, K, flags, index, bias=bias_at, gate=g, residual=r, pre=p, act=act)
     return out, pre
@@ -254,7 +254,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``residual + gate[row_index] * act(x weight^T + bias)``, as far as given, in one pass: ``x`` bfloat16 ``[rows, K]``, ``weight`` ``[N, K]`` as a
     ``torch.nn.Linear`` has it, ``bias`` float32 or bfloat16, ``activation`` one of :data:`ACTIVATIONS`, ``gate`` bfloat16 ``[table rows, N]`` with
     ``row_index`` int32 ``[rows]`` (as :func:`.projections.out_proj` takes them), ``residual`` bfloat16 ``[rows, N]``; ``out`` may be ``residual``.
-    ``save``: also returns what :func:`linear_backward` takes as ``pre`` (``x weight^T + bias`` rounded to bfloat16; None without an activation)."""
+    ``save``: also returns what :func:`linear_backward` takes as ``pre`` (``x weight^T + bias`` in float32; None without an activation)."""
     if _wants_grad(x, weight, bias, gate, residual):
         if out is not None or save or gate is not None:
             raise ValueError("out, save and gate cannot be given where gradients are recorded")
@@ -310,7 +310,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     if act:
         if pre is None:
             raise ValueError(f"activation {activation!r} needs pre")
-        p = _matrix("pre", pre, rows, N, index)
+        p = _matrix("pre", pre, rows, N, index, _F32)
     dev = x.device
     if not rows:
         return (torch.empty_like(x) if x_grad else None, _zeros(dev, N, K) if weight_grad else None, _zeros(dev, N) if bias_grad else None)
@@ -331,8 +331,8 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
 # ---- the two products of a block ----
 
 class Saved(NamedTuple):
-    """What the backward pass of :func:`feed_forward` takes of the forward one, bfloat16: the first product with its bias (``[rows, 2 inner]`` gated: values
-    and gates), and what the second product took."""
+    """What the backward pass of :func:`feed_forward` takes of the forward one: the first product with its bias, float32 (``[rows, 2 inner]`` gated: values
+    and gates), and what the second product took, bfloat16."""
 
     pre: torch.Tensor
     hidden: torch.Tensor
@@ -372,7 +372,7 @@ def _feed_forward(x, w_in, w_out, b_in, b_out, activation, gated, gate, row_inde
     h = (hidden.data_ptr(), inner)
     pre, p = None, (0, 0)
     if save:
-        pre = torch.empty(rows, first, dtype=_BF16, device=x.device)
+        pre = torch.empty(rows, first, dtype=_F32, device=x.device)
         p = (pre.data_ptr(), first)
     _product(a, w1, h, rows, inner, K, f1, index, bias=b1, pre=p, act=act)
     _product(h, w2, o, rows, N, inner, f2, index, bias=b2, gate=g, residual=r)
@@ -401,7 +401,7 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor,
     act = _activation(activation)
     a, w1, w2, rows, K, inner, first, N = _block(x, w_in, w_out, gated, index)
     at = _matrix("dy", dy, rows, N, index)
-    p = _matrix("saved.pre", saved.pre, rows, first, index)
+    p = _matrix("saved.pre", saved.pre, rows, first, index, _F32)
     h = _matrix("saved.hidden", saved.hidden, rows, inner, index)
     dev = x.device
     if not rows:

@@ -183,7 +183,8 @@ def test_linear(rows, K, N):
         if name == "none":
             assert pre is None
         else:
-            _within(pre, O.linear(x, w, b), "pre")
+            assert pre.dtype is F32
+            _within(pre, O.first_product(x, w, b), "pre")
         assert torch.equal(pk.linear(x, w, b, activation=name), got)
         got = pk.linear(x, w, activation=name, gate=gate, row_index=index, residual=residual)
         _within(got, O.linear(x, w, None, name, gate, index, residual), (name, "gate, residual"))
