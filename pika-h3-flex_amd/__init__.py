@@ -12,7 +12,7 @@ from .layout import (
 )
 from . import packing
 from . import projections
-from .feed_forward import feed_forward, feed_forward_backward, layer_norm, layer_norm_backward, linear, linear_backward
+from .rows import feed_forward, feed_forward_backward, layer_norm, layer_norm_backward, linear, linear_backward
 from .ops import BlockMask, PreparedKV, attention, attention_prepared, prepare_kv, rope_tables, time_attention_kernel
 from .paged import PagedBatch, PagedKV, paged_attention, paged_read, paged_write
 from .processor import PikaH3AttnProcessor

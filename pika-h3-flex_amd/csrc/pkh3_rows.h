@@ -1,6 +1,7 @@
 // Parameters of the kernels behind include/pkh3_rows.h, and how a product finishes its results.
 #pragma once
 #include "pkh3_common.h"
+#include "pkh3_rows_index.h"
 
 namespace pkh3 {
 
@@ -26,8 +27,6 @@ hipError_t launch_norm_backward(NormParams p, bool f32, bool tables_bf16, char* 
 
 // ---- products ----
 
-enum ProductMode { kPlain = 0, kGated = 1, kGrad = 2, kGatedGrad = 3 };
-
 struct ProductParams {
   const char *a, *b;             // [M, K] and [N, K], or across
   int64_t a_stride, b_stride;    // bytes
@@ -38,23 +37,16 @@ struct ProductParams {
   char* pre;                     // float32
   char* out;
   float* sums;                   // partial sums of out's columns, [rows of partial sums][columns], or null
-  float* part;                   // partial results of a contraction that is cut: [cut][M][columns]
+  float* part;                   // parts of the tiles that are shared: [2 * run + which][rows of a tile][256]
   int64_t gate_stride, residual_stride, pre_stride, out_stride;   // bytes
   int M, N, K, gate_rows;
   int act, bias_bf16;
-  int cuts;                      // parts of the contraction, with `part`
 };
 
-// How a call is carried out, by its sizes alone.
-struct ProductPlan {
-  int tb;                        // 16-row blocks of A a wave: tiles of 32 * tb rows of A and 256 of B
-  int cuts;                      // parts of the contraction, each with workgroups of its own
-  int sum_rows;                  // rows of partial column sums
-  size_t part_off, sums_off, total;   // bytes of the workspace
-};
-ProductPlan plan_product(int M, int N, int K, int mode, bool sums);
 hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_across, bool b_across, int mode, void* sums, char* workspace, hipStream_t s);
-bool product_offered(bool a_across, bool b_across, int mode);
+hipError_t launch_tiles_8(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
+hipError_t launch_tiles_4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
+hipError_t launch_tiles_2(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
 
 int activation_grad_rows(int M);                    // rows of partial column sums of an activation's gradient
 hipError_t launch_activation_grad(ProductParams p, void* sums, char* workspace, hipStream_t s);
@@ -167,6 +159,17 @@ __device__ __forceinline__ Bias load_bias(const ProductParams& p, int n) {
   return bias;
 }
 
+// The same with row 0 at `first`: the functions below take rows behind it, whose offsets then are 32 bits (rows of a tile, and strides up to 2^24 bytes).
+__device__ __forceinline__ ProductParams from_row(ProductParams p, int first) {
+  p.out += first * p.out_stride;
+  p.pre = p.pre ? p.pre + first * p.pre_stride : nullptr;
+  p.residual = p.residual ? p.residual + first * p.residual_stride : nullptr;
+  p.gate_index = p.gate_index ? p.gate_index + first : nullptr;
+  p.M -= first;
+  return p;
+}
+__device__ __forceinline__ unsigned place(int row, int64_t stride, int n, int size) { return (unsigned)row * (unsigned)stride + (unsigned)(n * size); }
+
 // What else a piece's results need, asked for ahead of them: the gate and the residual, or the saved sums.
 template <int MODE>
 struct Extra {
@@ -183,17 +186,17 @@ struct Extra<kGatedGrad> {
 template <int MODE>
 __device__ __forceinline__ void fetch(const ProductParams& p, int m, int n, Extra<MODE>& e) {
   if constexpr (MODE == kGrad) {
-    if (p.act) e.z = load_piece_f32(p.pre + m * p.pre_stride + (int64_t)n * 4);
+    if (p.act) e.z = load_piece_f32(p.pre + place(m, p.pre_stride, n, 4));
   } else if constexpr (MODE == kGatedGrad) {
-    const char* pre = p.pre + m * p.pre_stride + (int64_t)n * 4;
-    e.a = load_piece_f32(pre);
-    e.b = load_piece_f32(pre + (int64_t)p.N * 4);
+    const char* gates = p.pre + (int64_t)p.N * 4;
+    e.a = load_piece_f32(p.pre + place(m, p.pre_stride, n, 4));
+    e.b = load_piece_f32(gates + place(m, p.pre_stride, n, 4));
   } else {
     if (p.gate) {
       const int row = p.gate_index ? min(max(p.gate_index[m], 0), p.gate_rows - 1) : 0;
       e.gate = *(const bf16x8*)(p.gate + row * p.gate_stride + (int64_t)n * 2);
     }
-    if (p.residual) e.residual = *(const bf16x8*)(p.residual + m * p.residual_stride + (int64_t)n * 2);
+    if (p.residual) e.residual = *(const bf16x8*)(p.residual + place(m, p.residual_stride, n, 2));
   }
 }
 
@@ -201,16 +204,16 @@ __device__ __forceinline__ void fetch(const ProductParams& p, int m, int n, Extr
 // Sums that are saved for the backward pass stay in float32: rounded to bfloat16 they cost its gradients half as much again as their own rounding does.
 template <int MODE, int ACT>
 __device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Piece& a, Piece& b, const Bias& bias, const Extra<MODE>& e) {
-  char* out = p.out + m * p.out_stride + (int64_t)n * 2;
+  const unsigned at = place(m, p.out_stride, n, 2);
   if constexpr (MODE <= kGated) {
-    char* pre = p.pre ? p.pre + m * p.pre_stride + (int64_t)n * 4 : nullptr;
+    const unsigned pre_at = place(m, p.pre_stride, n, 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j) a.v[j] += bias.a.v[j];
-    if (pre) store_piece_f32(pre, a);
+    if (p.pre) store_piece_f32(p.pre + pre_at, a);
     if constexpr (MODE == kGated) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) b.v[j] += bias.b.v[j];
-      if (pre) store_piece_f32(pre + (int64_t)p.N * 4, b);
+      if (p.pre) store_piece_f32(p.pre + (int64_t)p.N * 4 + pre_at, b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) a.v[j] *= act_of<ACT>(b.v[j]);
     } else {
@@ -225,7 +228,7 @@ __device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Pie
 #pragma unroll
       for (int j = 0; j < 8; ++j) a.v[j] += (float)e.residual[j];
     }
-    store_piece(out, a);
+    store_piece(p.out + at, a);
   } else if constexpr (MODE == kGrad) {
     if constexpr (ACT != 0) {
 #pragma unroll
@@ -235,7 +238,7 @@ __device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Pie
         a.v[j] *= slope;
       }
     }
-    store_piece(out, a);
+    store_piece(p.out + at, a);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -244,8 +247,8 @@ __device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Pie
       b.v[j] = a.v[j] * e.a.v[j] * slope;
       a.v[j] *= value;
     }
-    store_piece(out, a);
-    store_piece(out + (int64_t)p.N * 2, b);
+    store_piece(p.out + at, a);
+    store_piece(p.out + (int64_t)p.N * 2 + at, b);
   }
 }
 

@@ -1,0 +1,450 @@
+// Matrix products on plain row-major matrices that finish their own results (include/pkh3_rows.h): out[m, n] = finish(sum over k of A(m, k) B(n, k)).
+//
+// Operands.  MFMA 16x16x32: lane (c = l % 16, g = l / 16) supplies elements 8*g .. +7 of row c of an operand, so a block of 16 rows x 32 contraction elements is 16
+// bytes a lane ("image"), of A and of B alike.  B goes down the result's registers: a lane then holds four consecutive columns of out for one row.  Chunks of 64 contraction
+// elements are copied memory -> LDS as they lie in memory, 128 bytes of a row at a time (what an L2 line holds), without passing through registers, and cut
+// into images on the way from LDS:
+//   along  (rows of K): 128 bytes a row; the 16-byte piece q of row r lies at place q ^ (r % 8), so that eight lanes that read piece q of eight rows meet no bank twice
+//   across (K rows): units of 64 contraction elements x 64 rows, 128 bytes an element; the 32-byte piece b of element k lies at place b ^ s(k), s of the bits 1 and 3 of k,
+//          so that the eight elements that half a wave reads meet no bank twice; a 16-lane transposing read takes four elements of 16 rows and gives each lane those of one row (ds_read_b64_tr_b16), two of them an image
+// A copy's LDS target is linear in the lane, so the places are chosen through the lanes' source addresses.
+//
+// Work split.  Workgroup = 4 waves, one per SIMD = 256 rows of B x 32*TB rows of A; wave (fh, th) = 128 rows of B x 16*TB of A.  Two chunks in LDS: while the products of a
+// chunk's second half run, its place is filled with the chunk after the next, and the first half of the next chunk is read into registers.
+#pragma once
+#include <type_traits>
+
+#include "pkh3_rows.h"
+
+namespace pkh3 {
+
+// The two halves of a direct-to-LDS copy: wave-uniform target and base address, per-lane byte offset.  `lanes`: all or none.
+__device__ __forceinline__ void copy_to(unsigned lds_addr) { asm volatile("s_mov_b32 m0, %0" ::"s"(lds_addr) : "m0"); }
+__device__ __forceinline__ void copy_from(const char* g, unsigned lane_off, unsigned long long lanes) {
+  asm volatile("s_mov_b64 exec, %2\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
+               :
+               : "v"(lane_off), "s"(g), "s"(lanes)
+               : "memory");
+}
+
+// c += a b, as an instruction: the compiler, left to place 256 accumulator registers itself, moves them between the halves of the register file inside the loop.
+// AGPR: they lie in the accumulator half.
+template <bool AGPR>
+__device__ __forceinline__ void mfma_acc(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  if constexpr (AGPR) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(8))) short i16x8;
+__device__ __forceinline__ bf16x8 read_across(const char* at) {
+  using P = __attribute__((address_space(3))) i16x4*;
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)at);
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(at + 4 * 128));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ int across_swizzle(int k) { return ((k >> 1) & 1) | ((k >> 2) & 2); }
+
+// The lane, in a way that keeps what is worked out from it where it is used: along the tiles' loop there are no registers for it.
+__device__ __forceinline__ int lane_here() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// How one operand's tile of ROWS rows comes to LDS (COPIES 1 KiB copies of this wave) and from there to registers.
+template <bool ACROSS, int ROWS, bool PAIRS>
+struct Operand {
+  static constexpr int kCopies = ROWS / 8 / 4;
+  const char* next;              // of the chunk to copy next
+  const char* next_pair;         // ... of the gates' rows (PAIRS)
+  unsigned off[kCopies];
+  int64_t advance;               // bytes from chunk to chunk
+
+  // first: the tile's first row (column of out).  rows: of the matrix; pair: rows from values to gates.  left: contraction elements of the chunk.
+  __device__ __forceinline__ void init(const char* src, int64_t stride, int first, int64_t pair, int64_t k0) {
+    if constexpr (ACROSS) next = src + k0 * stride, advance = kChunk * stride;
+    else next = src + first * stride + k0 * 2, next_pair = next + pair * stride, advance = kChunk * 2;
+  }
+  __device__ __forceinline__ void offsets(int64_t stride, int first, int rows, int wave, int left) {
+    const int lane = lane_here();
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int piece = wave * kCopies + i;
+      if constexpr (ACROSS) {
+        const int k = 8 * (piece & 7) + (lane >> 3), place = lane & 7;
+        const int col = (piece >> 3) * 64 + (((place >> 1) ^ across_swizzle(k)) * 2 + (place & 1)) * 8;
+        off[i] = (unsigned)(min(k, left - 1) * (unsigned)stride) + (unsigned)min(first + col, rows - 8) * 2u;
+      } else {
+        const int r = 8 * piece + (lane >> 3), q = (lane & 7) ^ (r & 7);
+        const int row = PAIRS ? (r >> 5) * 16 + (r & 15) : r;   // (the gates' rows: from their own base)
+        off[i] = (unsigned)min(row, rows - 1 - first) * (unsigned)stride + (unsigned)(q * 8 < left ? q * 16 : 0);
+      }
+    }
+  }
+  template <int I>
+  __device__ __forceinline__ const char* base() const {
+    // a wave's copies are 8 rows each, two of values and two of gates in turn
+    if constexpr (PAIRS) return I & 2 ? next_pair : next;
+    else return next;
+  }
+  __device__ __forceinline__ void step() {
+    next += advance;
+    if constexpr (PAIRS) next_pair += advance;
+  }
+};
+
+// Where this lane finds image (block of 16 rows rb, half ks of a chunk) of a tile in LDS: a base per ... and constant offsets.
+template <bool ACROSS>
+struct Images {
+  const char* at[ACROSS ? 4 : 2];
+  __device__ __forceinline__ void init(const char* lds, int lane, int first_block) {
+    const int c = lane & 15, g = lane >> 4;
+    if constexpr (ACROSS) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        at[b] = lds + (8 * g + (c >> 2)) * 128 + (((b + first_block) & 3) ^ across_swizzle(8 * g + (c >> 2))) * 32 + (c & 3) * 8 + (first_block >> 2) * 8192;
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) at[ks] = lds + (first_block * 16 + c) * 128 + (((4 * ks + g) ^ (c & 7)) * 16);
+    }
+  }
+  // RB: block behind the first one (whose number is a multiple of 4, or the blocks do not leave its unit)
+  template <int RB>
+  __device__ __forceinline__ bf16x8 read(int ks, int slot_bytes) const {
+    if constexpr (ACROSS) return read_across(at[RB & 3] + (RB >> 2) * 8192 + ks * 4096 + slot_bytes);
+    else return *(const bf16x8*)(at[ks] + RB * 2048 + slot_bytes);
+  }
+};
+
+struct ProductCall {
+  ProductParams p;
+  ProductShare s;
+};
+// The kernel's argument, read anew where it is used: along the loop there are no scalar registers for it.
+__device__ __forceinline__ ProductCall call_again() {
+  typedef __attribute__((may_alias)) uint64_t Word;
+  auto at = (const __attribute__((address_space(4))) uint64_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  ProductCall call;
+  static_assert(sizeof(call) % 8 == 0, "copied by words");
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(call) / 8; ++i) ((Word*)&call)[i] = at[i];
+  return call;
+}
+
+// A workgroup's way through its tiles.  start() sets out for chunks first .. first + count - 1 of a tile and copies the first two; run() forms the sums.
+template <bool A_ACROSS, bool B_ACROSS, bool PAIRS, int TB>
+struct Walk {
+  static constexpr int kTileA = 32 * TB, kBytesB = kTileB * 128, kSlot = kBytesB + kTileA * 128;
+  static constexpr bool kAgpr = TB > 2;
+  static constexpr int CB = Operand<B_ACROSS, kTileB, PAIRS>::kCopies, CA = Operand<A_ACROSS, kTileA, false>::kCopies, PP = CA + CB;
+  static constexpr int kReads = 8 + TB;
+  int lane, wave, m0, n0, chunks, left, to_copy;
+  unsigned lds0;
+  unsigned long long lanes;                          // all lanes while chunks are left to copy, then none
+  Operand<B_ACROSS, kTileB, PAIRS> ob;
+  Operand<A_ACROSS, kTileA, false> oa;
+  Images<B_ACROSS> ib;
+  Images<A_ACROSS> ia;
+
+  __device__ __forceinline__ explicit Walk(char* lds_raw) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds_raw;
+    ib.init(lds_raw, lane, (wave & 1) * 8);
+    ia.init(lds_raw + kBytesB, lane, (wave >> 1) * TB);
+  }
+  __device__ __forceinline__ void offsets(int k_left) {
+    const ProductParams p = call_again().p;
+    ob.offsets(p.b_stride, n0, p.N, wave, k_left);
+    oa.offsets(p.a_stride, m0, p.M, wave, k_left);
+  }
+  template <int I>
+  __device__ __forceinline__ void piece_to(int slot) {
+    copy_to(lds0 + slot * kSlot + (I < CB ? (wave * CB + I) * 1024 : kBytesB + (wave * CA + I - CB) * 1024));
+  }
+  template <int I>
+  __device__ __forceinline__ void piece_from() {
+    if constexpr (I < CB) copy_from(ob.template base<I>(), ob.off[I], lanes);
+    else copy_from(oa.template base<I - CB>(), oa.off[I - CB], lanes);
+    if constexpr (I == PP - 1) {
+      ob.step();
+      oa.step();
+      --to_copy;
+      asm volatile("s_cmp_gt_i32 %1, 0\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(to_copy) : "scc");
+      if (to_copy == 1 && left < kChunk) offsets(left);
+    }
+  }
+  template <int I>
+  __device__ __forceinline__ void copy_piece(int slot) {
+    piece_to<I>(slot);
+    asm volatile("s_nop 0");
+    piece_from<I>();
+  }
+  __device__ __forceinline__ void start(int m_first, int n_first, int first, int count) {
+    const ProductParams p = call_again().p;
+    m0 = m_first, n0 = n_first, chunks = to_copy = count;
+    const int64_t k0 = (int64_t)first * kChunk;
+    const int64_t k_left = p.K - k0 - (int64_t)(count - 1) * kChunk;
+    left = k_left < kChunk ? (int)k_left : kChunk;   // contraction elements of the last chunk
+    ob.init(p.b, p.b_stride, n0, p.N, k0);
+    oa.init(p.a, p.a_stride, m0, 0, k0);
+    offsets(count == 1 ? left : kChunk);
+    lanes = ~0ull;
+    static_for<PP>([&](auto ic) { copy_piece<decltype(ic)::value>(0); });
+    static_for<PP>([&](auto ic) { copy_piece<decltype(ic)::value>(1); });
+  }
+  template <int I>
+  __device__ __forceinline__ void read_image(int ks, int slot_bytes, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
+    if constexpr (I < TB) x[I] = ia.template read<I>(ks, slot_bytes);
+    else w[I - TB] = ib.template read<I - TB>(ks, slot_bytes);
+  }
+  // what lies behind the contraction's end is taken for zeros (both operands: it may be anything)
+  __device__ __forceinline__ void clear_rest(int from, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
+    i32x4 keep;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const int k = from + 8 * (lane >> 4) + 2 * d;
+      keep[d] = (k < left ? 0xffff : 0) | (k + 1 < left ? (int)0xffff0000 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, w[i]) & keep);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) x[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, x[i]) & keep);
+    asm volatile("s_nop 1" ::: "memory");            // (an MFMA may not take a register right behind the instruction that wrote it)
+  }
+  // The sums of the tile that start() set out for, whose first two chunks have landed for every wave.
+  __device__ __forceinline__ void run(f32x4 (&acc)[TB][8]) {
+    static_for<TB>([&](auto tc) {
+      static_for<8>([&](auto fc) { acc[decltype(tc)::value][decltype(fc)::value] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+    });
+    bf16x8 wa[8], wb[8], xa[TB], xb[TB];             // images of a chunk's first and second half
+    static_for<kReads>([&](auto ic) { read_image<decltype(ic)::value>(0, 0, wa, xa); });
+#pragma unroll 1
+    for (int kc = 0; kc < chunks; ++kc) {
+      const int slot = kc & 1, here = slot * kSlot, there = kSlot - here;
+      const bool rest = kc == chunks - 1 && left < kChunk;
+      if (rest) clear_rest(0, wa, xa);
+      // first half; the second half's images meanwhile.  (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
+      static_for<8 * TB>([&](auto kk) {
+        constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
+        mfma_acc<kAgpr>(acc[t][fb], wa[fb], xa[t]);
+        if constexpr (TB > 2) {
+          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(1, here, wb, xb);
+        } else {
+          if constexpr (k < kReads) read_image<k>(1, here, wb, xb);
+        }
+      });
+      if (rest) clear_rest(32, wb, xb);
+      // every wave holds the chunk in registers, and the next one is in LDS
+      if (kc) __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));
+      else __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      static_for<8 * TB>([&](auto kk) {
+        constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
+        mfma_acc<kAgpr>(acc[t][fb], wb[fb], xb[t]);
+        if constexpr (TB > 4) {
+          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(0, there, wa, xa);
+          if constexpr (k % 4 == 1 && k / 4 < PP) piece_to<k / 4>(slot);
+          if constexpr (k % 4 == 3 && k / 4 < PP) piece_from<k / 4>();
+        } else if constexpr (TB > 2) {
+          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(0, there, wa, xa);
+          if constexpr (k % 2 == 1 && k / 2 < PP) copy_piece<k / 2>(slot);
+        } else {
+          if constexpr (k < PP) copy_piece<k>(slot);
+          if constexpr (k < kReads) read_image<k>(0, there, wa, xa);
+        }
+      });
+    }
+    // the compiler does not know the instructions above for MFMAs: let the last one retire before anything reads the accumulators
+    static_for<TB>([&](auto tc) {
+      f32x4(&a)[8] = acc[decltype(tc)::value];
+      if constexpr (kAgpr)
+        asm volatile("s_nop 15\n\ts_nop 15" : "+a"(a[0]), "+a"(a[1]), "+a"(a[2]), "+a"(a[3]), "+a"(a[4]), "+a"(a[5]), "+a"(a[6]), "+a"(a[7])::"memory");
+      else
+        asm volatile("s_nop 15\n\ts_nop 15" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7])::"memory");
+    });
+  }
+};
+
+constexpr int kStageBytes = 16 * 128 * 4;            // staged results of a wave: 16 rows of 128 floats, 16-byte pieces at place q ^ row
+
+// A wave's results: 16 rows at a time through LDS (its own part), so that a row's columns leave in 16-byte pieces beside each other, 256 bytes a row.
+// What else the results need is asked for a block of rows ahead.  part: where the sums of a part of a contraction go, as they are.
+template <int MODE, int TB>
+__device__ __forceinline__ void product_epilogue(const ProductParams& all, float* part, int m0, int n0, int sum_row, char* lds, const f32x4 (&acc)[TB][8]) {
+  const ProductParams p = from_row(all, m0);          // (rows are counted from the wave's first)
+  constexpr bool kPairs = MODE == kGated;
+  constexpr int kPieces = kPairs ? 8 : 16;            // pieces of a row of the wave
+  constexpr int kRows = 64 / kPieces, kPasses = 16 / kRows;
+  const int lane = lane_here(), g = lane >> 4, c = lane & 15;
+  const int piece = lane % kPieces, n = n0 + piece * 8, n_at = min(n, p.N - 8);
+  const bool live = n < p.N;
+  auto staged = [&](int row, int q) { return lds + row * 512 + ((q ^ row) * 16); };
+  constexpr int kAsked = MODE == kGatedGrad ? (TB > 2 ? 2 : 1) : kPasses;   // passes whose extras are on their way (what the registers allow)
+  Extra<MODE> extra[kAsked];
+  auto ask = [&](int pass, int i) { fetch<MODE>(p, min(pass * kRows + lane / kPieces, p.M - 1), n_at, extra[i]); };
+  Bias bias{};
+  if (!part && p.M > 0) {
+    bias = load_bias<MODE>(p, n_at);
+#pragma unroll
+    for (int i = 0; i < kAsked; ++i) ask(i, i);
+  }
+  Piece sum_a{}, sum_b{};
+#pragma unroll 1
+  for (int t = 0; t < TB; ++t) {
+    if (16 * t >= p.M) break;
+    __builtin_amdgcn_wave_barrier();
+    static_for<TB>([&](auto tc) {
+      if (t == decltype(tc)::value) {
+#pragma unroll
+        for (int f = 0; f < 8; ++f) *(f32x4*)staged(c, 4 * f + g) = acc[decltype(tc)::value][f];
+      }
+    });
+    __builtin_amdgcn_wave_barrier();
+    auto each = [&](auto&& use) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + lane / kPieces, m = 16 * t + r;
+        auto load = [&](int q) {
+          const f32x4 lo = *(const f32x4*)staged(r, q), hi = *(const f32x4*)staged(r, q + 1);
+          return Piece{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+        };
+        const int q = kPairs ? (piece >> 1) * 8 + (piece & 1) * 2 : piece * 2;
+        Piece a = load(q), b{};
+        if constexpr (kPairs) b = load(q + 4);
+        use(i, m, live && m < p.M, a, b);
+        if constexpr (MODE == kGatedGrad) __builtin_amdgcn_sched_barrier(0);   // (one after the other: all at once they would not fit the registers)
+      }
+    };
+    if (part) {
+      each([&](int i, int, bool there, Piece& a, Piece& b) {
+        if (!there) return;
+        char* to = (char*)(part + (16 * t + i * kRows + lane / kPieces) * kTileB + piece * 8);
+        store_piece_f32(to, a);
+        if constexpr (kPairs) store_piece_f32(to + 128 * 4, b);
+      });
+      continue;
+    }
+    with_activation(p.act, [&](auto act) {
+      each([&](int i, int m, bool there, Piece& a, Piece& b) {
+        if (there) {
+          finish<MODE, decltype(act)::value>(p, m, n, a, b, bias, extra[i % kAsked]);
+          if constexpr (MODE >= kGrad) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              sum_a.v[j] += a.v[j];
+              if constexpr (MODE == kGatedGrad) sum_b.v[j] += b.v[j];
+            }
+          }
+        }
+        ask(kPasses * t + i + kAsked, i % kAsked);    // (past the last block: rows that nobody uses)
+      });
+    });
+  }
+  if constexpr (MODE >= kGrad) {
+    if (p.sums && !part) {
+      const int columns = MODE == kGatedGrad ? 2 * p.N : p.N;
+      float* at = p.sums + (int64_t)sum_row * columns + n;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int over = kPieces; over < 64; over *= 2) {
+          sum_a.v[j] += __shfl_xor(sum_a.v[j], over, 64);
+          if constexpr (MODE == kGatedGrad) sum_b.v[j] += __shfl_xor(sum_b.v[j], over, 64);
+        }
+      }
+      if (live && lane < kPieces) {
+        store_piece_f32((char*)at, sum_a);
+        if constexpr (MODE == kGatedGrad) store_piece_f32((char*)(at + p.N), sum_b);
+      }
+    }
+  }
+}
+
+template <bool A_ACROSS, bool B_ACROSS, int MODE, int TB>
+__global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCall) {
+  constexpr bool kPairs = MODE == kGated;
+  using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB>;
+  // With room for staged results beside the chunks, the next tile's first chunks are on their way while this one's results leave.
+  constexpr bool kAhead = TB > 2;
+  constexpr int kRing = 2 * W::kSlot;
+  __shared__ __attribute__((aligned(1024))) char lds_raw[kRing + (kAhead ? 4 * kStageBytes : 0)];
+  // Workgroups go to the 8 XCDs round-robin: rank is their order by XCD, so that those behind one L2 work on tiles beside each other.
+  const int per_xcd = gridDim.x >> 3, rank = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  const ProductShare shares = call_again().s;
+  const int run_first = run_begin(shares, rank), run_end = run_begin(shares, rank + 1);   // of the chunks of the tiles behind the whole ones
+  int round = 0, at = run_first;                       // whole tiles first, then the run
+  int m_tile = 0, n_tile = 0, first = 0, count = 0, slot = 0, chunks = 0;
+  // The next tile or part of one; false: none.  (Values chosen, not branches taken: the compiler keeps what either branch writes in memory.)
+  auto advance = [&]() __attribute__((always_inline)) {
+    const ProductShare s = call_again().s;
+    chunks = s.chunks;
+    const bool whole = round < s.rounds;
+    const int tile = at / s.chunks;
+    const int lin = whole ? ((blockIdx.x & 7) * s.rounds + round) * per_xcd + (blockIdx.x >> 3) : s.rounds * (int)gridDim.x + tile;
+    first = whole ? 0 : at - tile * s.chunks;
+    count = whole ? s.chunks : min(run_end - at, s.chunks - first);
+    slot = part_slot(s, rank, tile * s.chunks);
+    const TilePlace place = tile_of(s, lin);
+    const bool more = whole || at < run_end;
+    round += whole ? 1 : 0;
+    at += whole ? 0 : count;
+    // (uniform, which the compiler loses sight of on the way)
+    m_tile = __builtin_amdgcn_readfirstlane(place.m), n_tile = __builtin_amdgcn_readfirstlane(place.n);
+    first = __builtin_amdgcn_readfirstlane(first), count = __builtin_amdgcn_readfirstlane(count);
+    return __builtin_amdgcn_readfirstlane(more);
+  };
+  if (!advance()) return;
+  W walk(lds_raw);
+  auto set_out = [&]() __attribute__((always_inline)) { walk.start(m_tile * 32 * TB, n_tile * (kPairs ? kTileB / 2 : kTileB), first, count); };
+  set_out();
+  __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+#pragma unroll 1
+  for (;;) {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    f32x4 acc[TB][8];
+    walk.run(acc);
+    const int wave = walk.wave, wm = (wave >> 1) * 16 * TB, wn = (wave & 1) * (kPairs ? 64 : 128);
+    const int m0 = m_tile * 32 * TB + wm, n0 = n_tile * (kPairs ? kTileB / 2 : kTileB) + wn, sum_row = m_tile * 2 + (wave >> 1);
+    const ProductParams p = call_again().p;
+    float* part = count == chunks ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
+    const bool filled = m0 + 16 * TB <= p.M && n0 < p.N;   // every block of rows has results that leave
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+    __builtin_amdgcn_s_barrier();                      // (no wave reads chunks any more)
+    asm volatile("" ::: "memory");
+    const bool more = advance();
+    if (kAhead && more) set_out();
+    product_epilogue<MODE, TB>(call_again().p, part, m0, n0, sum_row, lds_raw + (kAhead ? kRing : 0) + wave * kStageBytes, acc);
+    if (!more) break;
+    if constexpr (!kAhead) {
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      set_out();
+      __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+    } else {
+      // The copies are older than the epilogue's stores, of which there were at least so many, and both complete in their order.
+      constexpr int kStores = TB * (kPairs ? 2 : 4);
+      if (filled) __builtin_amdgcn_s_waitcnt((kStores & 15) | ((kStores >> 4) << 14) | (7 << 4) | (15 << 8));
+      else __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+    }
+  }
+}
+
+template <int TB>
+hipError_t launch_tiles_of(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s) {
+  const dim3 grid(plan.share.groups);
+  if (a_across) product_kernel<true, true, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (!b_across && mode == kPlain) product_kernel<false, false, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (!b_across) product_kernel<false, false, kGated, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (mode == kPlain) product_kernel<false, true, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (mode == kGrad) product_kernel<false, true, kGrad, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  else product_kernel<false, true, kGatedGrad, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  return hipGetLastError();
+}
+
+}  // namespace pkh3
