@@ -122,6 +122,11 @@ struct ProductCall {
   ProductParams p;
   ProductShare s;
 };
+// Memory behind a pointer that comes out of memory: device memory.  (Taken for anywhere, its accesses would wait for each other.)
+template <class T>
+__device__ __forceinline__ T* in_memory(T* p) {
+  return (T*)(__attribute__((address_space(1))) T*)(uintptr_t)p;
+}
 // The kernel's argument, read anew where it is used: along the loop there are no scalar registers for it.
 __device__ __forceinline__ ProductCall call_again() {
   typedef __attribute__((may_alias)) uint64_t Word;
@@ -131,6 +136,9 @@ __device__ __forceinline__ ProductCall call_again() {
   static_assert(sizeof(call) % 8 == 0, "copied by words");
 #pragma unroll
   for (int i = 0; i < (int)sizeof(call) / 8; ++i) ((Word*)&call)[i] = at[i];
+  ProductParams& p = call.p;
+  p.bias = in_memory(p.bias), p.gate = in_memory(p.gate), p.gate_index = in_memory(p.gate_index), p.residual = in_memory(p.residual);
+  p.pre = in_memory(p.pre), p.out = in_memory(p.out), p.sums = in_memory(p.sums), p.part = in_memory(p.part);
   return call;
 }
 
