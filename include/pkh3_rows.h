@@ -61,12 +61,12 @@ size_t pkh3_norm_workspace_bytes(const pkh3_norm_args* args);
  * across need not come in eights.
  *
  *   plain    v = sum + bias[n]; pre[m, n] = v in float32, if given; out = residual[m, n] + gate[index[m], n] * act(v), as far as given
- *   GATED    B has 2 N rows, bias 2 N entries: a = row n, b = row N + n.  pre [M, 2 N] = (a | b), if given; out = a * act(b), then as above
+ *   GATED    B has 2 N rows, bias 2 N entries: a = row n, b = row N + n.  pre [M, 2 N] = (a | b), if given; out = a * act(b); no gate or residual
  *   GRAD     sum is the gradient of act(pre) and out [M, N] that of pre: out = sum * act'(pre[m, n])
  *   GRAD and GATED   pre [M, 2 N] = (a | b), out [M, 2 N]: out[m, n] = sum * act(b), out[m, N + n] = sum * a * act'(b)
  *
- * Offered are A and B along (plain, GATED), A along and B across (plain, GRAD, GRAD and GATED), and both across (plain); of others
- * PKH3_EUNSUPPORTED.  With GRAD, `sums`, if given, gets the sums of out's columns before they were rounded (bfloat16, N or 2 N entries). */
+ * Offered are A and B along (plain, GATED), A along and B across (plain without anything besides, GRAD, GRAD and GATED), and both
+ * across (plain without anything besides); of others PKH3_EUNSUPPORTED.  With GRAD, `sums`, if given, gets the sums of out's columns before they were rounded (bfloat16, N or 2 N entries). */
 
 enum {
   PKH3_ACT_NONE = 0,

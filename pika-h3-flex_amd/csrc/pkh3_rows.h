@@ -106,15 +106,6 @@ __device__ __forceinline__ void act_and_slope(float v, float& value, float& slop
   }
 }
 
-// f(activation as a constant)
-template <class F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
-  if (act == 0) f(std::integral_constant<int, 0>{});
-  else if (act == 1) f(std::integral_constant<int, 1>{});
-  else if (act == 2) f(std::integral_constant<int, 2>{});
-  else f(std::integral_constant<int, 3>{});
-}
-
 // ---- eight results of a row: columns n .. n + 7 of row m ----
 
 struct Piece {
@@ -159,97 +150,158 @@ __device__ __forceinline__ Bias load_bias(const ProductParams& p, int n) {
   return bias;
 }
 
-// The same with row 0 at `first`: the functions below take rows behind it, whose offsets then are 32 bits (rows of a tile, and strides up to 2^24 bytes).
-__device__ __forceinline__ ProductParams from_row(ProductParams p, int first) {
-  p.out += first * p.out_stride;
-  p.pre = p.pre ? p.pre + first * p.pre_stride : nullptr;
-  p.residual = p.residual ? p.residual + first * p.residual_stride : nullptr;
-  p.gate_index = p.gate_index ? p.gate_index + first : nullptr;
-  p.M -= first;
-  return p;
-}
-__device__ __forceinline__ unsigned place(int row, int64_t stride, int n, int size) { return (unsigned)row * (unsigned)stride + (unsigned)(n * size); }
+// ---- from sums to results (see pkh3_product in the header) ----
+// What a call has besides is a matter of constants, not of branches: behind a branch around a load the compiler waits for all accesses before it, stores
+// among them, whether the load was made or not (a tile's results took 25,000 cycles that way).  Accesses past the last row or column are dropped by
+// the hardware's range check for the same reason.
 
-// What else a piece's results need, asked for ahead of them: the gate and the residual, or the saved sums.
-template <int MODE>
-struct Extra {
-  bf16x8 gate, residual;
-};
-template <>
-struct Extra<kGrad> {
-  Piece z;
-};
-template <>
-struct Extra<kGatedGrad> {
-  Piece a, b;
-};
-template <int MODE>
-__device__ __forceinline__ void fetch(const ProductParams& p, int m, int n, Extra<MODE>& e) {
-  if constexpr (MODE == kGrad) {
-    if (p.act) e.z = load_piece_f32(p.pre + place(m, p.pre_stride, n, 4));
-  } else if constexpr (MODE == kGatedGrad) {
-    const char* gates = p.pre + (int64_t)p.N * 4;
-    e.a = load_piece_f32(p.pre + place(m, p.pre_stride, n, 4));
-    e.b = load_piece_f32(gates + place(m, p.pre_stride, n, 4));
+constexpr int kWithResidual = 1, kWithGate = 2;
+
+// f(activation, what is there besides: as constants).  SUMS: a gradient's product, whose sums are its results.
+template <int MODE, bool SUMS, class F>
+__device__ __forceinline__ void with_form(const ProductParams& p, F&& f) {
+  if constexpr (SUMS) return f(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+  auto by_act = [&](auto besides) {
+    if (p.act == 0) f(std::integral_constant<int, 0>{}, besides);
+    else if (p.act == 1) f(std::integral_constant<int, 1>{}, besides);
+    else if (p.act == 2) f(std::integral_constant<int, 2>{}, besides);
+    else f(std::integral_constant<int, 3>{}, besides);
+  };
+  if constexpr (MODE == kPlain) {
+    if (p.gate && p.residual) by_act(std::integral_constant<int, kWithGate | kWithResidual>{});
+    else if (p.gate) by_act(std::integral_constant<int, kWithGate>{});
+    else if (p.residual) by_act(std::integral_constant<int, kWithResidual>{});
+    else by_act(std::integral_constant<int, 0>{});
   } else {
-    if (p.gate) {
-      const int row = p.gate_index ? min(max(p.gate_index[m], 0), p.gate_rows - 1) : 0;
-      e.gate = *(const bf16x8*)(p.gate + row * p.gate_stride + (int64_t)n * 2);
-    }
-    if (p.residual) e.residual = *(const bf16x8*)(p.residual + place(m, p.residual_stride, n, 2));
+    by_act(std::integral_constant<int, 0>{});
   }
 }
 
-// From sums to results (see pkh3_product in the header).  a: the sums of columns n .. n + 7, b: of the gates'.  On return what out got, for the sums of columns.
-// Sums that are saved for the backward pass stay in float32: rounded to bfloat16 they cost its gradients half as much again as their own rounding does.
-template <int MODE, int ACT>
-__device__ __forceinline__ void finish(const ProductParams& p, int m, int n, Piece& a, Piece& b, const Bias& bias, const Extra<MODE>& e) {
-  const unsigned at = place(m, p.out_stride, n, 2);
-  if constexpr (MODE <= kGated) {
-    const unsigned pre_at = place(m, p.pre_stride, n, 4);
+// Rows of a matrix from one row on: up to 128 of them, whose offsets are 32 bits (strides up to 2^24 bytes).
+constexpr unsigned kNowhere = 0x80000000u;          // an offset that the range check drops
+struct RowsOf {
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned stride;
+  __device__ __forceinline__ RowsOf(char* base, int64_t row_stride, int first)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(base + first * row_stride, 0, (int)kNowhere, 0x00020000)), stride((unsigned)row_stride) {}
+  __device__ __forceinline__ i32x4 load(unsigned at) const { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)); }
+  __device__ __forceinline__ void store(unsigned at, i32x4 v) const {
+    typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc, at, 0, 0);
+  }
+  __device__ __forceinline__ void store_bf16(unsigned at, const Piece& p) const {
+    bf16x8 raw;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a.v[j] += bias.a.v[j];
-    if (p.pre) store_piece_f32(p.pre + pre_at, a);
-    if constexpr (MODE == kGated) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b.v[j] += bias.b.v[j];
-      if (p.pre) store_piece_f32(p.pre + (int64_t)p.N * 4 + pre_at, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] *= act_of<ACT>(b.v[j]);
+    for (int j = 0; j < 8; ++j) raw[j] = (__bf16)p.v[j];
+    store(at, __builtin_bit_cast(i32x4, raw));
+  }
+  __device__ __forceinline__ void store_f32(unsigned at, const Piece& p) const {
+    store(at, __builtin_bit_cast(i32x4, f32x4{p.v[0], p.v[1], p.v[2], p.v[3]}));
+    store(at + 16, __builtin_bit_cast(i32x4, f32x4{p.v[4], p.v[5], p.v[6], p.v[7]}));
+  }
+  __device__ __forceinline__ Piece load_f32(unsigned at) const {
+    const f32x4 lo = __builtin_bit_cast(f32x4, load(at)), hi = __builtin_bit_cast(f32x4, load(at + 16));
+    return Piece{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+  }
+};
+
+// The results' rows from one on; rows counted from there.
+template <int MODE>
+struct Results {
+  const ProductParams& p;
+  RowsOf out, pre, residual;
+  int rows, first;
+  __device__ __forceinline__ Results(const ProductParams& params, int first_row)
+      : p(params), out(params.out, params.out_stride, first_row), pre(params.pre, params.pre_stride, first_row),
+        residual((char*)params.residual, params.residual_stride, first_row), rows(params.M - first_row), first(first_row) {}
+
+  // What else a piece's results need, asked for ahead of them: the gate and the residual, or the saved sums.
+  struct Plain {
+    i32x4 gate, residual;
+  };
+  struct Grad {
+    Piece z;
+  };
+  struct GatedGrad {
+    Piece a, b;
+  };
+  using Extra = std::conditional_t<MODE == kGatedGrad, GatedGrad, std::conditional_t<MODE == kGrad, Grad, Plain>>;
+  __device__ __forceinline__ unsigned at(const RowsOf& m, int row, int n, int size) const {
+    return row < rows && n < p.N ? (unsigned)row * m.stride + (unsigned)(n * size) : kNowhere;
+  }
+  template <int ACT, int BESIDES>
+  __device__ __forceinline__ void fetch(int row, int n, Extra& e) const {
+    if constexpr (MODE == kGrad) {
+      if constexpr (ACT != 0) e.z = pre.load_f32(at(pre, row, n, 4));
+    } else if constexpr (MODE == kGatedGrad) {
+      const unsigned where = at(pre, row, n, 4);
+      e.a = pre.load_f32(where);
+      e.b = pre.load_f32(where == kNowhere ? where : where + (unsigned)p.N * 4);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] = act_of<ACT>(a.v[j]);
+      if constexpr (BESIDES & kWithGate) {
+        int of = 0;
+        if (p.gate_index) of = min(max(p.gate_index[first + min(row, rows - 1)], 0), p.gate_rows - 1);
+        e.gate = *(const i32x4*)(p.gate + of * p.gate_stride + (int64_t)min(n, p.N - 8) * 2);
+      }
+      if constexpr (BESIDES & kWithResidual) e.residual = residual.load(at(residual, row, n, 2));
     }
-    if (p.gate) {
+  }
+  // a: the sums of columns n .. n + 7, b: of the gates'.  On return what out got, for the sums of columns.  Sums that are saved for the
+  // backward pass stay in float32: rounded to bfloat16 they cost its gradients half as much again as their own rounding does.
+  template <int ACT, int BESIDES>
+  __device__ __forceinline__ void finish(int row, int n, Piece& a, Piece& b, const Bias& bias, const Extra& e) const {
+    const unsigned to = at(out, row, n, 2);
+    const unsigned to_b = to == kNowhere ? to : to + (unsigned)p.N * 2;
+    if constexpr (MODE <= kGated) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] *= (float)e.gate[j];
-    }
-    if (p.residual) {
+      for (int j = 0; j < 8; ++j) a.v[j] += bias.a.v[j];
+      if constexpr (MODE == kGated) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] += (float)e.residual[j];
-    }
-    store_piece(p.out + at, a);
-  } else if constexpr (MODE == kGrad) {
-    if constexpr (ACT != 0) {
+        for (int j = 0; j < 8; ++j) b.v[j] += bias.b.v[j];
+      }
+      if (p.pre) {
+        const unsigned keep = at(pre, row, n, 4);
+        pre.store_f32(keep, a);
+        if constexpr (MODE == kGated) pre.store_f32(keep == kNowhere ? keep : keep + (unsigned)p.N * 4, b);
+      }
+      if constexpr (MODE == kGated) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a.v[j] *= act_of<ACT>(b.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a.v[j] = act_of<ACT>(a.v[j]);
+        if constexpr (BESIDES & kWithGate) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a.v[j] *= (float)__builtin_bit_cast(bf16x8, e.gate)[j];
+        }
+        if constexpr (BESIDES & kWithResidual) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a.v[j] += (float)__builtin_bit_cast(bf16x8, e.residual)[j];
+        }
+      }
+      out.store_bf16(to, a);
+    } else if constexpr (MODE == kGrad) {
+      if constexpr (ACT != 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float value, slope;
+          act_and_slope<ACT>(e.z.v[j], value, slope);
+          a.v[j] *= slope;
+        }
+      }
+      out.store_bf16(to, a);
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float value, slope;
-        act_and_slope<ACT>(e.z.v[j], value, slope);
-        a.v[j] *= slope;
+        act_and_slope<ACT>(e.b.v[j], value, slope);
+        b.v[j] = a.v[j] * e.a.v[j] * slope;
+        a.v[j] *= value;
       }
+      out.store_bf16(to, a);
+      out.store_bf16(to_b, b);
     }
-    store_piece(p.out + at, a);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float value, slope;
-      act_and_slope<ACT>(e.b.v[j], value, slope);
-      b.v[j] = a.v[j] * e.a.v[j] * slope;
-      a.v[j] *= value;
-    }
-    store_piece(p.out + at, a);
-    store_piece(p.out + (int64_t)p.N * 2 + at, b);
   }
-}
+};
 
 }  // namespace pkh3

@@ -146,8 +146,11 @@ int check_product(const pkh3_product_args* a) {
   if (rc) return rc;
   const int mode = mode_of(a->flags), M = a->M, N = a->N, K = a->K;
   const bool gated = a->flags & PKH3_PRODUCT_GATED, grad = a->flags & PKH3_PRODUCT_GRAD;
-  if (grad && (a->bias || a->gate || a->residual)) return fail(PKH3_EARG, "bias, gate and residual do not go with PKH3_PRODUCT_GRAD");
+  if (grad && a->bias) return fail(PKH3_EARG, "bias does not go with PKH3_PRODUCT_GRAD");
+  if ((grad || gated) && (a->gate || a->residual)) return fail(PKH3_EARG, "gate and residual do not go with PKH3_PRODUCT_GRAD or PKH3_PRODUCT_GATED");
   if (!grad && a->sums) return fail(PKH3_EARG, "sums go with PKH3_PRODUCT_GRAD");
+  if (mode == kPlain && (a->flags & PKH3_PRODUCT_B_ACROSS) && (a->bias || a->gate || a->residual || a->pre || a->activation))
+    return fail(PKH3_EARG, "bias, activation, gate, residual and pre do not go with operands stored across");
   const int wide = gated ? 2 * N : N, b_rows = mode == kGated ? 2 * N : N;
   const Matrix A = a->flags & PKH3_PRODUCT_A_ACROSS ? Matrix{"a", a->a, a->a_stride, K, M, 2} : Matrix{"a", a->a, a->a_stride, M, K, 2};
   const Matrix B = a->flags & PKH3_PRODUCT_B_ACROSS ? Matrix{"b", a->b, a->b_stride, K, b_rows, 2} : Matrix{"b", a->b, a->b_stride, b_rows, K, 2};

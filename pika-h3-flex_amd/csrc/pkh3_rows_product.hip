@@ -6,40 +6,42 @@ namespace pkh3 {
 // The parts of the tiles that several workgroups share, added up in the order of the contraction, and finished: a workgroup is 8 pieces of 8 columns times 32 rows; with
 // sums of columns it takes as many rows as a wave of product_kernel has, whose place in the sums it fills.
 template <int MODE>
-__global__ __launch_bounds__(256) void product_join_kernel(ProductParams all, ProductShare s, int tb) {
+__global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, ProductShare s, int tb) {
   constexpr bool kPairs = MODE == kGated;
   constexpr int kCols = kPairs ? kTileB / 2 : kTileB;
   __shared__ __attribute__((aligned(16))) Piece staged[MODE >= kGrad ? 2 * 256 : 1];
   const int rows = MODE >= kGrad ? 16 * tb : 32;
   const auto [m_tile, n_tile] = tile_of(s, s.rounds * s.groups + blockIdx.x);
-  const ProductParams p = from_row(all, m_tile * 32 * tb + blockIdx.y * rows);
+  const Results<MODE> res(p, m_tile * 32 * tb + blockIdx.y * rows);
   const int q0 = blockIdx.x * s.chunks;
   const int first = run_of(s, q0), last = run_of(s, q0 + s.chunks - 1);
   if (first == last) return;                           // (one workgroup had all of it and finished it)
   const int col = (blockIdx.z * 8 + (threadIdx.x & 7)) * 8, n = n_tile * kCols + col;
   Piece sum_a{}, sum_b{};
-  for (int r = threadIdx.x >> 3; r < rows; r += 32) {
-    if (n >= p.N || r >= p.M) break;
-    Extra<MODE> extra;
-    fetch<MODE>(p, r, n, extra);
-    const Bias bias = load_bias<MODE>(p, n);
-    Piece a{}, b{};
-    for (int rank = first; rank <= last; ++rank) {
-      const int slot = part_slot(s, rank, q0);
-      const char* from = (const char*)(p.part + ((int64_t)slot * 32 * tb + blockIdx.y * rows + r) * kTileB + col);
-      const Piece va = load_piece_f32(from);
+  with_form<MODE, false>(p, [&](auto act, auto besides) {
+    for (int r = threadIdx.x >> 3; r < rows; r += 32) {
+      if (n >= p.N || r >= res.rows) break;
+      typename Results<MODE>::Extra extra;
+      res.template fetch<decltype(act)::value, decltype(besides)::value>(r, n, extra);
+      const Bias bias = load_bias<MODE>(p, n);
+      Piece a{}, b{};
+      for (int rank = first; rank <= last; ++rank) {
+        const int slot = part_slot(s, rank, q0);
+        const char* from = (const char*)(p.part + ((int64_t)slot * 32 * tb + blockIdx.y * rows + r) * kTileB + col);
+        const Piece va = load_piece_f32(from);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a.v[j] += va.v[j];
-      if constexpr (kPairs) {
-        const Piece vb = load_piece_f32(from + 128 * 4);
+        for (int j = 0; j < 8; ++j) a.v[j] += va.v[j];
+        if constexpr (kPairs) {
+          const Piece vb = load_piece_f32(from + 128 * 4);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b.v[j] += vb.v[j];
+          for (int j = 0; j < 8; ++j) b.v[j] += vb.v[j];
+        }
       }
-    }
-    with_activation(p.act, [&](auto act) { finish<MODE, decltype(act)::value>(p, r, n, a, b, bias, extra); });
+      res.template finish<decltype(act)::value, decltype(besides)::value>(r, n, a, b, bias, extra);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum_a.v[j] += a.v[j], sum_b.v[j] += b.v[j];
-  }
+      for (int j = 0; j < 8; ++j) sum_a.v[j] += a.v[j], sum_b.v[j] += b.v[j];
+    }
+  });
   if constexpr (MODE >= kGrad) {
     if (!p.sums) return;
     staged[threadIdx.x] = sum_a;
@@ -112,21 +114,18 @@ hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_acros
 constexpr int kGradRows = 64;     // rows of a workgroup: 8 at a time, 32 pieces of 8 columns
 
 template <int ACT>
-__global__ __launch_bounds__(256) void activation_grad_kernel(ProductParams all) {
-  const int first = blockIdx.y * kGradRows;
-  ProductParams p = all;
-  if (all.out) p = from_row(all, first);
+__global__ __launch_bounds__(256) void activation_grad_kernel(ProductParams p) {
   __shared__ Piece staged[256];
-  const int n = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
+  const int n = (blockIdx.x * 32 + (threadIdx.x & 31)) * 8, first = blockIdx.y * kGradRows;
+  const Results<kGrad> res(p, first);
   Piece sum{};
   if (n < p.N)
-    for (int i = threadIdx.x >> 5; i < kGradRows; i += 8) {
-      if (first + i >= all.M) break;
+    for (int i = threadIdx.x >> 5; i < kGradRows && i < res.rows; i += 8) {
       Piece a = load_piece(p.a + (first + i) * p.a_stride + (int64_t)n * 2), b{};
       if (p.out) {
-        Extra<kGrad> extra;
-        fetch(p, i, n, extra);
-        finish<kGrad, ACT>(p, i, n, a, b, Bias{}, extra);
+        Results<kGrad>::Extra extra;
+        res.fetch<ACT, 0>(i, n, extra);
+        res.finish<ACT, 0>(i, n, a, b, Bias{}, extra);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum.v[j] += a.v[j];

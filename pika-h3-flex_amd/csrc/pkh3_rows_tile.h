@@ -29,6 +29,12 @@ __device__ __forceinline__ void copy_from(const char* g, unsigned lane_off, unsi
 
 // c += a b, as an instruction: the compiler, left to place 256 accumulator registers itself, moves them between the halves of the register file inside the loop.
 // AGPR: they lie in the accumulator half.
+// FIRST: onto zeros.
+template <bool AGPR>
+__device__ __forceinline__ void mfma_first(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  if constexpr (AGPR) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=v"(c) : "v"(a), "v"(b));
+}
 template <bool AGPR>
 __device__ __forceinline__ void mfma_acc(f32x4& c, const bf16x8& a, const bf16x8& b) {
   if constexpr (AGPR) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
@@ -225,26 +231,28 @@ struct Walk {
   }
   // The sums of the tile that start() set out for, whose first two chunks have landed for every wave.
   __device__ __forceinline__ void run(f32x4 (&acc)[TB][8]) {
-    static_for<TB>([&](auto tc) {
-      static_for<8>([&](auto fc) { acc[decltype(tc)::value][decltype(fc)::value] = f32x4{0.f, 0.f, 0.f, 0.f}; });
-    });
     bf16x8 wa[8], wb[8], xa[TB], xb[TB];             // images of a chunk's first and second half
     static_for<kReads>([&](auto ic) { read_image<decltype(ic)::value>(0, 0, wa, xa); });
-#pragma unroll 1
-    for (int kc = 0; kc < chunks; ++kc) {
-      const int slot = kc & 1, here = slot * kSlot, there = kSlot - here;
-      const bool rest = kc == chunks - 1 && left < kChunk;
-      if (rest) clear_rest(0, wa, xa);
-      // first half; the second half's images meanwhile.  (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
+    // a chunk's first half; the second half's images meanwhile.  (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
+    auto first_half = [&](auto onto_zeros, int here) __attribute__((always_inline)) {
       static_for<8 * TB>([&](auto kk) {
         constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
-        mfma_acc<kAgpr>(acc[t][fb], wa[fb], xa[t]);
+        if constexpr (decltype(onto_zeros)::value) mfma_first<kAgpr>(acc[t][fb], wa[fb], xa[t]);
+        else mfma_acc<kAgpr>(acc[t][fb], wa[fb], xa[t]);
         if constexpr (TB > 2) {
           if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(1, here, wb, xb);
         } else {
           if constexpr (k < kReads) read_image<k>(1, here, wb, xb);
         }
       });
+    };
+#pragma unroll 1
+    for (int kc = 0; kc < chunks; ++kc) {
+      const int slot = kc & 1, here = slot * kSlot, there = kSlot - here;
+      const bool rest = kc == chunks - 1 && left < kChunk;
+      if (rest) clear_rest(0, wa, xa);
+      if (kc) first_half(std::false_type{}, here);
+      else first_half(std::true_type{}, here);
       if (rest) clear_rest(32, wb, xb);
       // every wave holds the chunk in registers, and the next one is in LDS
       if (kc) __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));
@@ -278,98 +286,124 @@ struct Walk {
   }
 };
 
-constexpr int kStageBytes = 16 * 128 * 4;            // staged results of a wave: 16 rows of 128 floats, 16-byte pieces at place q ^ row
-
-// A wave's results: 16 rows at a time through LDS (its own part), so that a row's columns leave in 16-byte pieces beside each other, 256 bytes a row.
-// What else the results need is asked for a block of rows ahead.  part: where the sums of a part of a contraction go, as they are.
-template <int MODE, int TB>
-__device__ __forceinline__ void product_epilogue(const ProductParams& all, float* part, int m0, int n0, int sum_row, char* lds, const f32x4 (&acc)[TB][8]) {
-  const ProductParams p = from_row(all, m0);          // (rows are counted from the wave's first)
-  constexpr bool kPairs = MODE == kGated;
-  constexpr int kPieces = kPairs ? 8 : 16;            // pieces of a row of the wave
-  constexpr int kRows = 64 / kPieces, kPasses = 16 / kRows;
-  const int lane = lane_here(), g = lane >> 4, c = lane & 15;
-  const int piece = lane % kPieces, n = n0 + piece * 8, n_at = min(n, p.N - 8);
-  const bool live = n < p.N;
-  auto staged = [&](int row, int q) { return lds + row * 512 + ((q ^ row) * 16); };
-  constexpr int kAsked = MODE == kGatedGrad ? (TB > 2 ? 2 : 1) : kPasses;   // passes whose extras are on their way (what the registers allow)
-  Extra<MODE> extra[kAsked];
-  auto ask = [&](int pass, int i) { fetch<MODE>(p, min(pass * kRows + lane / kPieces, p.M - 1), n_at, extra[i]); };
-  Bias bias{};
-  if (!part && p.M > 0) {
-    bias = load_bias<MODE>(p, n_at);
+// Two blocks of 16 columns a lane holds four of each (4*g .. +3): after the exchange of rows of 16 lanes it holds eight columns beside each other, from
+// eight_of(g) of the 32 on.
+__device__ __forceinline__ int eight_of(int g) { return (g & 1) * 16 + (g >> 1) * 8; }
+__device__ __forceinline__ Piece eight_columns(const f32x4& first, const f32x4& second) {
+  Piece p;
 #pragma unroll
-    for (int i = 0; i < kAsked; ++i) ask(i, i);
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(first[i]), __float_as_uint(second[i]), false, false);
+    p.v[i] = __uint_as_float(r[0]);
+    p.v[4 + i] = __uint_as_float(r[1]);
   }
-  Piece sum_a{}, sum_b{};
+  return p;
+}
+
+// A wave's results: 16 rows at a time, a lane 16 bytes of a row four times (twice with gates).  What else the results need is asked for a block of rows ahead.
+// The accumulators of block t, which is known when the kernel runs: a branch, not an index.
+template <int TB>
+__device__ __forceinline__ void block_of(int t, const f32x4 (&acc)[TB][8], f32x4 (&block)[8]) {
+  static_for<TB>([&](auto tc) {
+    if (t == decltype(tc)::value) {
+#pragma unroll
+      for (int f = 0; f < 8; ++f) block[f] = acc[decltype(tc)::value][f];
+    }
+  });
+}
+template <bool PAIRS, int F>
+__device__ __forceinline__ void pieces_of(const f32x4 (&block)[8], Piece& a, Piece& b) {
+  if constexpr (PAIRS) {
+    a = eight_columns(block[4 * F], block[4 * F + 2]);
+    b = eight_columns(block[4 * F + 1], block[4 * F + 3]);
+  } else {
+    a = eight_columns(block[2 * F], block[2 * F + 1]);
+  }
+}
+
+template <int MODE, int ACT, int BESIDES, int TB>
+__device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int n0, int sum_row, const Bias (&bias)[MODE == kGated ? 2 : 4], const f32x4 (&acc)[TB][8]) {
+  constexpr bool kPairs = MODE == kGated;
+  constexpr int kPieces = kPairs ? 2 : 4;             // pieces of a row that a lane holds
+  const Results<MODE> res(p, m0);
+  const int lane = lane_here(), g = lane >> 4, c = lane & 15, n = n0 + eight_of(g);
+  constexpr int kAsked = MODE == kGatedGrad ? (TB > 2 ? 2 : 1) : kPieces;   // pieces whose extras are on their way (what the registers allow)
+  typename Results<MODE>::Extra extra[kAsked];
+#pragma unroll
+  for (int i = 0; i < kAsked; ++i) res.template fetch<ACT, BESIDES>(c, n + 32 * i, extra[i]);
+  Piece sum_a[MODE >= kGrad ? kPieces : 1], sum_b[MODE == kGatedGrad ? kPieces : 1];
+  if constexpr (MODE >= kGrad) {
+#pragma unroll
+    for (int f = 0; f < kPieces; ++f) {
+      sum_a[f] = Piece{};
+      if constexpr (MODE == kGatedGrad) sum_b[f] = Piece{};
+    }
+  }
 #pragma unroll 1
   for (int t = 0; t < TB; ++t) {
-    if (16 * t >= p.M) break;
-    __builtin_amdgcn_wave_barrier();
-    static_for<TB>([&](auto tc) {
-      if (t == decltype(tc)::value) {
+    f32x4 block[8];
+    block_of<TB>(t, acc, block);
+    const int row = 16 * t + c;
+    static_for<kPieces>([&](auto fc) {
+      constexpr int f = decltype(fc)::value;
+      Piece a, b{};
+      pieces_of<kPairs, f>(block, a, b);
+      res.template finish<ACT, BESIDES>(row, n + 32 * f, a, b, bias[f], extra[f % kAsked]);
+      if constexpr (MODE >= kGrad) {
+        const bool there = row < res.rows;
 #pragma unroll
-        for (int f = 0; f < 8; ++f) *(f32x4*)staged(c, 4 * f + g) = acc[decltype(tc)::value][f];
-      }
-    });
-    __builtin_amdgcn_wave_barrier();
-    auto each = [&](auto&& use) {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int r = i * kRows + lane / kPieces, m = 16 * t + r;
-        auto load = [&](int q) {
-          const f32x4 lo = *(const f32x4*)staged(r, q), hi = *(const f32x4*)staged(r, q + 1);
-          return Piece{{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
-        };
-        const int q = kPairs ? (piece >> 1) * 8 + (piece & 1) * 2 : piece * 2;
-        Piece a = load(q), b{};
-        if constexpr (kPairs) b = load(q + 4);
-        use(i, m, live && m < p.M, a, b);
-        if constexpr (MODE == kGatedGrad) __builtin_amdgcn_sched_barrier(0);   // (one after the other: all at once they would not fit the registers)
-      }
-    };
-    if (part) {
-      each([&](int i, int, bool there, Piece& a, Piece& b) {
-        if (!there) return;
-        char* to = (char*)(part + (16 * t + i * kRows + lane / kPieces) * kTileB + piece * 8);
-        store_piece_f32(to, a);
-        if constexpr (kPairs) store_piece_f32(to + 128 * 4, b);
-      });
-      continue;
-    }
-    with_activation(p.act, [&](auto act) {
-      each([&](int i, int m, bool there, Piece& a, Piece& b) {
-        if (there) {
-          finish<MODE, decltype(act)::value>(p, m, n, a, b, bias, extra[i % kAsked]);
-          if constexpr (MODE >= kGrad) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              sum_a.v[j] += a.v[j];
-              if constexpr (MODE == kGatedGrad) sum_b.v[j] += b.v[j];
-            }
-          }
+        for (int j = 0; j < 8; ++j) {
+          sum_a[f].v[j] += there ? a.v[j] : 0.f;
+          if constexpr (MODE == kGatedGrad) sum_b[f].v[j] += there ? b.v[j] : 0.f;
         }
-        ask(kPasses * t + i + kAsked, i % kAsked);    // (past the last block: rows that nobody uses)
-      });
+      }
+      constexpr int ahead = f + kAsked;               // (past the last block: rows that nobody uses)
+      res.template fetch<ACT, BESIDES>(16 * (t + ahead / kPieces) + c, n + ahead % kPieces * 32, extra[f % kAsked]);
+      if constexpr (MODE == kGatedGrad) __builtin_amdgcn_sched_barrier(0);   // (one after the other: all at once they would not fit the registers)
     });
   }
   if constexpr (MODE >= kGrad) {
-    if (p.sums && !part) {
+    if (p.sums) {
+      // over the 16 rows that the lanes of a group hold
       const int columns = MODE == kGatedGrad ? 2 * p.N : p.N;
-      float* at = p.sums + (int64_t)sum_row * columns + n;
+      float* to = p.sums + (int64_t)sum_row * columns;
+      auto put = [&](Piece& v, int at) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int over = kPieces; over < 64; over *= 2) {
-          sum_a.v[j] += __shfl_xor(sum_a.v[j], over, 64);
-          if constexpr (MODE == kGatedGrad) sum_b.v[j] += __shfl_xor(sum_b.v[j], over, 64);
+        for (int j = 0; j < 8; ++j) {
+          float x = v.v[j];
+          x = sum_with<0xB1>(x);
+          x = sum_with<0x4E>(x);
+          x = sum_with<0x141>(x);
+          v.v[j] = sum_with<0x140>(x);
         }
-      }
-      if (live && lane < kPieces) {
-        store_piece_f32((char*)at, sum_a);
-        if constexpr (MODE == kGatedGrad) store_piece_f32((char*)(at + p.N), sum_b);
+        if (c == 0) store_piece_f32((char*)(to + at), v);
+      };
+#pragma unroll
+      for (int f = 0; f < kPieces; ++f) {
+        if (n + 32 * f >= p.N) continue;
+        put(sum_a[f], n + 32 * f);
+        if constexpr (MODE == kGatedGrad) put(sum_b[f], p.N + n + 32 * f);
       }
     }
+  }
+}
+
+// The sums of a part of a contraction, as they are: rows of 256 (values and gates: 128 each).
+template <bool PAIRS, int TB>
+__device__ __forceinline__ void leave_part(float* part, int rows, const f32x4 (&acc)[TB][8]) {
+  const int lane = lane_here(), g = lane >> 4, c = lane & 15;
+#pragma unroll 1
+  for (int t = 0; t < TB; ++t) {
+    if (16 * t >= rows) break;
+    f32x4 block[8];
+    block_of<TB>(t, acc, block);
+    static_for<PAIRS ? 2 : 4>([&](auto fc) {
+      Piece a, b{};
+      pieces_of<PAIRS, decltype(fc)::value>(block, a, b);
+      char* to = (char*)(part + (16 * t + c) * kTileB + eight_of(g) + 32 * decltype(fc)::value);
+      store_piece_f32(to, a);
+      if constexpr (PAIRS) store_piece_f32(to + 128 * 4, b);
+    });
   }
 }
 
@@ -377,10 +411,7 @@ template <bool A_ACROSS, bool B_ACROSS, int MODE, int TB>
 __global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCall) {
   constexpr bool kPairs = MODE == kGated;
   using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB>;
-  // With room for staged results beside the chunks, the next tile's first chunks are on their way while this one's results leave.
-  constexpr bool kAhead = TB > 2;
-  constexpr int kRing = 2 * W::kSlot;
-  __shared__ __attribute__((aligned(1024))) char lds_raw[kRing + (kAhead ? 4 * kStageBytes : 0)];
+  __shared__ __attribute__((aligned(1024))) char lds_raw[2 * W::kSlot];
   // Workgroups go to the 8 XCDs round-robin: rank is their order by XCD, so that those behind one L2 work on tiles beside each other.
   const int per_xcd = gridDim.x >> 3, rank = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   const ProductShare shares = call_again().s;
@@ -416,30 +447,39 @@ __global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCal
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     f32x4 acc[TB][8];
-    walk.run(acc);
     const int wave = walk.wave, wm = (wave >> 1) * 16 * TB, wn = (wave & 1) * (kPairs ? 64 : 128);
     const int m0 = m_tile * 32 * TB + wm, n0 = n_tile * (kPairs ? kTileB / 2 : kTileB) + wn, sum_row = m_tile * 2 + (wave >> 1);
+    constexpr int kPieces = kPairs ? 2 : 4;
+    Bias bias[kPieces];                                // (asked for here, it is there when the sums are)
+    {
+      const ProductParams p = call_again().p;
+      const int n = n0 + eight_of(lane_here() >> 4);
+#pragma unroll
+      for (int f = 0; f < kPieces; ++f) bias[f] = B_ACROSS ? Bias{} : load_bias<MODE>(p, min(n + 32 * f, p.N - 8));
+    }
+    walk.run(acc);
     const ProductParams p = call_again().p;
     float* part = count == chunks ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
-    const bool filled = m0 + 16 * TB <= p.M && n0 < p.N;   // every block of rows has results that leave
+    const bool filled = p.M > m0;                      // the wave has rows: then at least so many of its stores were issued as results have pieces
     __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
     __builtin_amdgcn_s_barrier();                      // (no wave reads chunks any more)
     asm volatile("" ::: "memory");
     const bool more = advance();
-    if (kAhead && more) set_out();
-    product_epilogue<MODE, TB>(call_again().p, part, m0, n0, sum_row, lds_raw + (kAhead ? kRing : 0) + wave * kStageBytes, acc);
-    if (!more) break;
-    if constexpr (!kAhead) {
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      set_out();
-      __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
-    } else {
-      // The copies are older than the epilogue's stores, of which there were at least so many, and both complete in their order.
-      constexpr int kStores = TB * (kPairs ? 2 : 4);
-      if (filled) __builtin_amdgcn_s_waitcnt((kStores & 15) | ((kStores >> 4) << 14) | (7 << 4) | (15 << 8));
-      else __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+    if (more) set_out();                               // (the next tile's first chunks are on their way while this one's results leave)
+    const bool whole = !part;
+    if (part) {
+      leave_part<kPairs, TB>(part, p.M - m0, acc);
+    } else if (p.M > m0 || MODE >= kGrad) {
+      const ProductParams q = call_again().p;
+      with_form<MODE, MODE == kPlain && B_ACROSS>(q, [&](auto act, auto besides) {
+        finish_tile<MODE, decltype(act)::value, decltype(besides)::value, TB>(q, m0, n0, sum_row, bias, acc);
+      });
     }
+    if (!more) break;
+    // The copies are older than the epilogue's stores, of which there were at least so many, and both complete in their order.
+    constexpr int kStores = TB * (kPairs ? 2 : 4);
+    if (whole && filled) __builtin_amdgcn_s_waitcnt((kStores & 15) | ((kStores >> 4) << 14) | (7 << 4) | (15 << 8));
+    else __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
   }
 }
 

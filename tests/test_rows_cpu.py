@@ -125,6 +125,16 @@ def test_product_refuses(lib, i):
     assert lib.pkh3_product(None, None) == _lib.PKH3_ENULL
 
 
+def test_products_of_operands_across_refuse_what_goes_with_others(lib):
+    for flags, b_stride in ((_lib.PRODUCT_B_ACROSS, 136), (_lib.PRODUCT_A_ACROSS | _lib.PRODUCT_B_ACROSS, 136)):
+        good = dict(flags=flags, b_stride=b_stride, M=24, a_stride=72)
+        for kw in (dict(bias=0x6000000), dict(activation=1), dict(residual=0x6000000, residual_stride=136), dict(gate=0x6000000, gate_rows=1, gate_stride=136),
+                   dict(pre=0x8000000, pre_stride=136)):
+            assert lib.pkh3_product(C.byref(_product_args(**good, **kw)), None) == _lib.PKH3_EARG, kw
+    for kw in (dict(residual=0x6000000, residual_stride=136), dict(gate=0x6000000, gate_rows=1, gate_stride=136)):
+        assert lib.pkh3_product(C.byref(_product_args(flags=_lib.PRODUCT_GATED, **kw)), None) == _lib.PKH3_EARG, kw
+
+
 def test_product_of_gradients_refuses(lib):
     flags = _lib.PRODUCT_B_ACROSS | _lib.PRODUCT_GRAD
     good = dict(flags=flags, b_stride=136, pre=0x8000000, pre_stride=136, activation=1, sums=0x5000000)
