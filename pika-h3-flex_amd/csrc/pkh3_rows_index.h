@@ -64,7 +64,7 @@ constexpr ProductPlan plan_product(int M, int N, int K, int mode, bool sums) {
   s.m_tiles = (M + 32 * plan.tb - 1) / (32 * plan.tb), s.n_tiles = (N + columns - 1) / columns;
   s.chunks = (K + kChunk - 1) / kChunk;
   const int tiles = s.m_tiles * s.n_tiles;
-  s.groups = plan.tb > 2 ? 256 : 512;                // a workgroup or two on every CU
+  s.groups = 256;                                    // one on every CU
   s.rounds = tiles / s.groups;
   s.rest = tiles - s.rounds * s.groups;
   // tiles behind the whole rounds: shared out where that saves more than it costs

@@ -9,8 +9,8 @@
 //          so that the eight elements that half a wave reads meet no bank twice; a 16-lane transposing read takes four elements of 16 rows and gives each lane those of one row (ds_read_b64_tr_b16), two of them an image
 // A copy's LDS target is linear in the lane, so the places are chosen through the lanes' source addresses.
 //
-// Work split.  Workgroup = 4 waves, one per SIMD = 256 rows of B x 32*TB rows of A; wave (fh, th) = 128 rows of B x 16*TB of A.  Two chunks in LDS: while the products of a
-// chunk's second half run, its place is filled with the chunk after the next, and the first half of the next chunk is read into registers.
+// Work split.  Workgroup = 4 waves, one per SIMD = 256 rows of B x 32*TB rows of A; wave (fh, th) = 128 rows of B x 16*TB of A.  Two to four chunks in LDS: while the
+// products of a chunk's second half run, its place is filled with the chunk that many ahead, and the first half of the next chunk is read into registers.
 #pragma once
 #include <type_traits>
 
@@ -18,22 +18,27 @@
 
 namespace pkh3 {
 
-// The two halves of a direct-to-LDS copy: wave-uniform target and base address, per-lane byte offset.  `lanes`: all or none.
-__device__ __forceinline__ void copy_to(unsigned lds_addr) { asm volatile("s_mov_b32 m0, %0" ::"s"(lds_addr) : "m0"); }
-__device__ __forceinline__ void copy_from(const char* g, unsigned lane_off, unsigned long long lanes) {
-  asm volatile("s_mov_b64 exec, %2\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
-               :
-               : "v"(lane_off), "s"(g), "s"(lanes)
-               : "memory");
+// The two halves of a direct-to-LDS copy: wave-uniform target and base address, per-lane byte offset.
+template <int OFFSET>
+__device__ __forceinline__ void copy_to(unsigned lds_addr) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(lds_addr), "n"(OFFSET) : "m0", "scc"); }
+__device__ __forceinline__ void copy_from(const char* g, unsigned lane_off) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(g) : "memory");
 }
+// The same by all lanes or none: it counts in the waits either way.  (Longer to issue: where it may not be due.)
+__device__ __forceinline__ void copy_from_if(const char* g, unsigned lane_off, unsigned long long lanes) {
+  asm volatile("s_mov_b64 exec, %2\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" : : "v"(lane_off), "s"(g), "s"(lanes) : "memory");
+}
+enum Copying { kNoCopies, kCopies, kCopiesIf };
+// operand of s_waitcnt: at most `vm` copies and `lgkm` LDS reads still on their way
+constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
 
 // c += a b, as an instruction: the compiler, left to place 256 accumulator registers itself, moves them between the halves of the register file inside the loop.
 // AGPR: they lie in the accumulator half.
 // FIRST: onto zeros.
 template <bool AGPR>
 __device__ __forceinline__ void mfma_first(f32x4& c, const bf16x8& a, const bf16x8& b) {
-  if constexpr (AGPR) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));
-  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=v"(c) : "v"(a), "v"(b));
+  if constexpr (AGPR) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
 }
 template <bool AGPR>
 __device__ __forceinline__ void mfma_acc(f32x4& c, const bf16x8& a, const bf16x8& b) {
@@ -59,25 +64,29 @@ __device__ __forceinline__ int lane_here() {
   return lane;
 }
 
-// How one operand's tile of ROWS rows comes to LDS (COPIES 1 KiB copies of this wave) and from there to registers.
-template <bool ACROSS, int ROWS, bool PAIRS>
+// How one operand's tile of ROWS rows comes to LDS, chunk after chunk into SLOTS places: kPieces copies of 1 KiB a chunk and wave.
+template <bool ACROSS, int ROWS, bool PAIRS, int SLOTS>
 struct Operand {
-  static constexpr int kCopies = ROWS / 8 / 4;
+  static constexpr int kPieces = ROWS / 8 / 4, kSlot = ROWS * 128;
   const char* next;              // of the chunk to copy next
   const char* next_pair;         // ... of the gates' rows (PAIRS)
-  unsigned off[kCopies];
+  unsigned off[kPieces];
   int64_t advance;               // bytes from chunk to chunk
+  unsigned fill, ring;           // where this wave's part of that chunk goes, and where it goes in the first place
+  int to_copy;                   // chunks left to copy
 
-  // first: the tile's first row (column of out).  rows: of the matrix; pair: rows from values to gates.  left: contraction elements of the chunk.
-  __device__ __forceinline__ void init(const char* src, int64_t stride, int first, int64_t pair, int64_t k0) {
+  // first: the tile's first row (column of out).  pair: rows from values to gates.
+  __device__ __forceinline__ void init(const char* src, int64_t stride, int first, int64_t pair, int64_t k0, int count) {
     if constexpr (ACROSS) next = src + k0 * stride, advance = kChunk * stride;
     else next = src + first * stride + k0 * 2, next_pair = next + pair * stride, advance = kChunk * 2;
+    fill = ring, to_copy = count;
   }
+  // rows: of the matrix; left: contraction elements of the chunk.
   __device__ __forceinline__ void offsets(int64_t stride, int first, int rows, int wave, int left) {
     const int lane = lane_here();
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int piece = wave * kCopies + i;
+    for (int i = 0; i < kPieces; ++i) {
+      const int piece = wave * kPieces + i;
       if constexpr (ACROSS) {
         const int k = 8 * (piece & 7) + (lane >> 3), place = lane & 7;
         const int col = (piece >> 3) * 64 + (((place >> 1) ^ across_swizzle(k)) * 2 + (place & 1)) * 8;
@@ -89,15 +98,23 @@ struct Operand {
       }
     }
   }
+  // The two halves of copy I; the last one of a chunk moves on.
   template <int I>
-  __device__ __forceinline__ const char* base() const {
-    // a wave's copies are 8 rows each, two of values and two of gates in turn
-    if constexpr (PAIRS) return I & 2 ? next_pair : next;
-    else return next;
+  __device__ __forceinline__ void to() const {
+    copy_to<I * 1024>(fill);
   }
-  __device__ __forceinline__ void step() {
-    next += advance;
-    if constexpr (PAIRS) next_pair += advance;
+  template <int I, Copying C>
+  __device__ __forceinline__ void from(unsigned long long lanes) {
+    // (with pairs a wave's copies are 8 rows each, two of values and two of gates in turn)
+    const char* at = PAIRS && (I & 2) ? next_pair : next;
+    if constexpr (C == kCopiesIf) copy_from_if(at, off[I], lanes);
+    else copy_from(at, off[I]);
+    if constexpr (I == kPieces - 1) {
+      next += advance;
+      if constexpr (PAIRS) next_pair += advance;
+      --to_copy;
+      fill = fill == ring + (SLOTS - 1) * kSlot ? ring : fill + kSlot;
+    }
   }
 };
 
@@ -148,72 +165,105 @@ __device__ __forceinline__ ProductCall call_again() {
   return call;
 }
 
-// A workgroup's way through its tiles.  start() sets out for chunks first .. first + count - 1 of a tile and copies the first two; run() forms the sums.
+// A workgroup's way through its tiles.  start() sets out for chunks first .. first + count - 1 of a tile and copies the first few; run() forms the sums.
+//
+// Copies.  All of a workgroup's copies together take the CU's 64 bytes a clock for half as long as the 256 x 256 products of a chunk take (for longer than
+// those of 64 rows), and have to be on their way for about a microsecond.  So the copies of a chunk are issued over the whole of a chunk's time, each half
+// in the half chunk behind whose barrier the places they go to are free: `late` ones follow the barrier in the middle of a chunk, `soon` ones the half chunk after.
+// Which copies these are and how many places an operand has follows from what fits LDS; the operands' places are counted apart.
 template <bool A_ACROSS, bool B_ACROSS, bool PAIRS, int TB>
 struct Walk {
-  static constexpr int kTileA = 32 * TB, kBytesB = kTileB * 128, kSlot = kBytesB + kTileA * 128;
+  static constexpr int kTileA = 32 * TB;
+  static constexpr int kSlotsB = TB > 2 ? 3 : 4, kSlotsA = TB > 4 ? 2 : 4;
   static constexpr bool kAgpr = TB > 2;
-  static constexpr int CB = Operand<B_ACROSS, kTileB, PAIRS>::kCopies, CA = Operand<A_ACROSS, kTileA, false>::kCopies, PP = CA + CB;
+  using OB = Operand<B_ACROSS, kTileB, PAIRS, kSlotsB>;
+  using OA = Operand<A_ACROSS, kTileA, false, kSlotsA>;
+  static constexpr int CB = OB::kPieces, CA = OA::kPieces, PP = CA + CB;
+  static constexpr int kBytesB = kSlotsB * OB::kSlot, kLds = kBytesB + kSlotsA * OA::kSlot;
   static constexpr int kReads = 8 + TB;
-  int lane, wave, m0, n0, chunks, left, to_copy;
-  unsigned lds0;
-  unsigned long long lanes;                          // all lanes while chunks are left to copy, then none
-  Operand<B_ACROSS, kTileB, PAIRS> ob;
-  Operand<A_ACROSS, kTileA, false> oa;
+  // copies: 0 .. CB - 1 of B, then of A.  TB 8: A's behind the barrier, B's after; 4: the other way round; 2: half of them all
+  static constexpr int kLateFrom = TB > 4 ? CB : 0, kLate = TB > 4 ? CA : TB > 2 ? CB : PP / 2;
+  static constexpr int kSoonFrom = TB > 4 ? 0 : kLate, kSoon = PP - kLate;
+  // copies on their way at the middle of a chunk when the next chunk has landed, and the chunks that start() brings on their way whole
+  static constexpr int kOnTheirWay = TB > 4 ? kSoon : TB > 2 ? 2 * kSoon + kLate : 2 * PP;
+  static constexpr int kStarted = TB > 4 ? 2 : 3;
+  static constexpr int kLateAhead = TB > 4 ? 2 : TB > 2 ? 3 : 4;   // chunks from the one whose middle they follow to that of the late copies (the soon ones': kStarted)
+  int lane, wave, m0, n0, chunks, left;
+  OB ob;
+  OA oa;
   Images<B_ACROSS> ib;
   Images<A_ACROSS> ia;
 
   __device__ __forceinline__ explicit Walk(char* lds_raw) {
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds_raw;
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds_raw;
+    ob.ring = lds0 + wave * CB * 1024;
+    oa.ring = lds0 + kBytesB + wave * CA * 1024;
     ib.init(lds_raw, lane, (wave & 1) * 8);
     ia.init(lds_raw + kBytesB, lane, (wave >> 1) * TB);
   }
-  __device__ __forceinline__ void offsets(int k_left) {
+  __device__ __forceinline__ void offsets_b(int k_left) {
     const ProductParams p = call_again().p;
     ob.offsets(p.b_stride, n0, p.N, wave, k_left);
+  }
+  __device__ __forceinline__ void offsets_a(int k_left) {
+    const ProductParams p = call_again().p;
     oa.offsets(p.a_stride, m0, p.M, wave, k_left);
   }
   template <int I>
-  __device__ __forceinline__ void piece_to(int slot) {
-    copy_to(lds0 + slot * kSlot + (I < CB ? (wave * CB + I) * 1024 : kBytesB + (wave * CA + I - CB) * 1024));
+  __device__ __forceinline__ void piece_to() const {
+    if constexpr (I < CB) ob.template to<I>();
+    else oa.template to<I - CB>();
   }
-  template <int I>
-  __device__ __forceinline__ void piece_from() {
-    if constexpr (I < CB) copy_from(ob.template base<I>(), ob.off[I], lanes);
-    else copy_from(oa.template base<I - CB>(), oa.off[I - CB], lanes);
-    if constexpr (I == PP - 1) {
-      ob.step();
-      oa.step();
-      --to_copy;
-      asm volatile("s_cmp_gt_i32 %1, 0\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(to_copy) : "scc");
-      if (to_copy == 1 && left < kChunk) offsets(left);
+  template <int I, Copying C>
+  __device__ __forceinline__ void piece_from(unsigned long long lanes) {
+    if constexpr (I < CB) {
+      ob.template from<I, C>(lanes);
+      if constexpr (I == CB - 1) {
+        if (ob.to_copy == 1 && left < kChunk) offsets_b(left);
+      }
+    } else {
+      oa.template from<I - CB, C>(lanes);
+      if constexpr (I == PP - 1) {
+        if (oa.to_copy == 1 && left < kChunk) offsets_a(left);
+      }
     }
   }
-  template <int I>
-  __device__ __forceinline__ void copy_piece(int slot) {
-    piece_to<I>(slot);
+  template <int I, Copying C = kCopies>
+  __device__ __forceinline__ void copy_piece(unsigned long long lanes = 0) {
+    piece_to<I>();
     asm volatile("s_nop 0");
-    piece_from<I>();
+    piece_from<I, C>(lanes);
   }
   __device__ __forceinline__ void start(int m_first, int n_first, int first, int count) {
     const ProductParams p = call_again().p;
-    m0 = m_first, n0 = n_first, chunks = to_copy = count;
+    m0 = m_first, n0 = n_first, chunks = count;
     const int64_t k0 = (int64_t)first * kChunk;
     const int64_t k_left = p.K - k0 - (int64_t)(count - 1) * kChunk;
     left = k_left < kChunk ? (int)k_left : kChunk;   // contraction elements of the last chunk
-    ob.init(p.b, p.b_stride, n0, p.N, k0);
-    oa.init(p.a, p.a_stride, m0, 0, k0);
-    offsets(count == 1 ? left : kChunk);
-    lanes = ~0ull;
-    static_for<PP>([&](auto ic) { copy_piece<decltype(ic)::value>(0); });
-    static_for<PP>([&](auto ic) { copy_piece<decltype(ic)::value>(1); });
+    ob.init(p.b, p.b_stride, n0, p.N, k0, count);
+    oa.init(p.a, p.a_stride, m0, 0, k0, count);
+    offsets_b(count == 1 ? left : kChunk);
+    offsets_a(count == 1 ? left : kChunk);
+    // what the halves of the chunks before the first would have copied
+#pragma unroll 1
+    for (int i = 0; i < min(kStarted, count); ++i) static_for<PP>([&](auto ic) { copy_piece<decltype(ic)::value>(); });
+    if constexpr (kLateAhead > kStarted) {
+      if (count > kStarted) static_for<kLate>([&](auto ic) { copy_piece<kLateFrom + decltype(ic)::value>(); });
+    }
   }
+  // the first chunk that start() copied has landed (of this wave's copies)
+  __device__ __forceinline__ void wait_for_first() const {
+    constexpr int kBehind = (kStarted - 1) * PP + (kLateAhead > kStarted ? kLate : 0);
+    if (chunks > kStarted) __builtin_amdgcn_s_waitcnt(wait_for(kBehind, 15));
+    else __builtin_amdgcn_s_waitcnt(wait_for(0, 15));
+  }
+
   template <int I>
-  __device__ __forceinline__ void read_image(int ks, int slot_bytes, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
-    if constexpr (I < TB) x[I] = ia.template read<I>(ks, slot_bytes);
-    else w[I - TB] = ib.template read<I - TB>(ks, slot_bytes);
+  __device__ __forceinline__ void read_image(int ks, int b_bytes, int a_bytes, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
+    if constexpr (I < TB) x[I] = ia.template read<I>(ks, a_bytes);
+    else w[I - TB] = ib.template read<I - TB>(ks, b_bytes);
   }
   // what lies behind the contraction's end is taken for zeros (both operands: it may be anything)
   __device__ __forceinline__ void clear_rest(int from, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
@@ -229,52 +279,73 @@ struct Walk {
     for (int i = 0; i < TB; ++i) x[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, x[i]) & keep);
     asm volatile("s_nop 1" ::: "memory");            // (an MFMA may not take a register right behind the instruction that wrote it)
   }
-  // The sums of the tile that start() set out for, whose first two chunks have landed for every wave.
-  __device__ __forceinline__ void run(f32x4 (&acc)[TB][8]) {
+  // Half a chunk (due: whether copies are, positive if so): the products of w and x with, between them, the reads of the next half's images and the copies FROM .. FROM + COUNT - 1.  At most one such thing follows an
+  // MFMA where there are enough of them: a wave is alone on its SIMD, and the pipe idles whenever the rest takes longer to issue than the MFMA leaves free.
+  // (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
+  template <bool FIRST, Copying C, int FROM, int COUNT>
+  __device__ __forceinline__ void half(f32x4 (&acc)[TB][8], bf16x8 (&w)[8], bf16x8 (&x)[TB], int ks, int b_bytes, int a_bytes, bf16x8 (&w2)[8], bf16x8 (&x2)[TB],
+                                       int due) {
+    unsigned long long lanes = 0;
+    if constexpr (C == kCopiesIf) asm volatile("s_cmp_gt_i32 %1, 0\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(due) : "scc");
+    if constexpr (FIRST) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 1" ::: "memory");          // (registers that only now become sums)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    static_for<8 * TB>([&](auto kk) {
+      constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
+      if constexpr (FIRST) mfma_first<kAgpr>(acc[t][fb], w[fb], x[t]);
+      else mfma_acc<kAgpr>(acc[t][fb], w[fb], x[t]);
+      constexpr int kEvery = 8 * TB / COUNT;         // MFMAs from copy to copy
+      if constexpr (TB > 2) {
+        static_assert(kEvery >= 4, "a copy's halves follow different MFMAs");
+        if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(ks, b_bytes, a_bytes, w2, x2);
+        if constexpr (C != kNoCopies && k % kEvery == 1 && k / kEvery < COUNT) piece_to<FROM + k / kEvery>();
+        if constexpr (C != kNoCopies && k % kEvery == 3 && k / kEvery < COUNT) piece_from<FROM + k / kEvery, C>(lanes);
+      } else {
+        if constexpr (k < kReads) read_image<k>(ks, b_bytes, a_bytes, w2, x2);
+        if constexpr (C != kNoCopies && k % kEvery == 1 && k / kEvery < COUNT) copy_piece<FROM + k / kEvery, C>(lanes);
+      }
+    });
+  }
+  // The sums of the tile that start() set out for, whose first chunk has landed for every wave; `landed`: all that start() copied has.
+  __device__ __forceinline__ void run(f32x4 (&acc)[TB][8], bool landed) {
     bf16x8 wa[8], wb[8], xa[TB], xb[TB];             // images of a chunk's first and second half
-    static_for<kReads>([&](auto ic) { read_image<decltype(ic)::value>(0, 0, wa, xa); });
-    // a chunk's first half; the second half's images meanwhile.  (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
-    auto first_half = [&](auto onto_zeros, int here) __attribute__((always_inline)) {
-      static_for<8 * TB>([&](auto kk) {
-        constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
-        if constexpr (decltype(onto_zeros)::value) mfma_first<kAgpr>(acc[t][fb], wa[fb], xa[t]);
-        else mfma_acc<kAgpr>(acc[t][fb], wa[fb], xa[t]);
-        if constexpr (TB > 2) {
-          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(1, here, wb, xb);
-        } else {
-          if constexpr (k < kReads) read_image<k>(1, here, wb, xb);
-        }
-      });
-    };
-#pragma unroll 1
-    for (int kc = 0; kc < chunks; ++kc) {
-      const int slot = kc & 1, here = slot * kSlot, there = kSlot - here;
+    static_for<kReads>([&](auto ic) { read_image<decltype(ic)::value>(0, 0, 0, wa, xa); });
+    int b_here = 0, a_here = 0, kc = 0;              // the chunk's places in LDS, and the chunk
+    auto chunk = [&](auto first, auto copying, auto&& wait) __attribute__((always_inline)) {
+      constexpr Copying C = decltype(copying)::value;
+      const int b_there = b_here == (kSlotsB - 1) * OB::kSlot ? 0 : b_here + OB::kSlot;
+      const int a_there = a_here == (kSlotsA - 1) * OA::kSlot ? 0 : a_here + OA::kSlot;
       const bool rest = kc == chunks - 1 && left < kChunk;
       if (rest) clear_rest(0, wa, xa);
-      if (kc) first_half(std::false_type{}, here);
-      else first_half(std::true_type{}, here);
+      half<decltype(first)::value, C, kSoonFrom, kSoon>(acc, wa, xa, 1, b_here, a_here, wb, xb, chunks - kc - kStarted);
       if (rest) clear_rest(32, wb, xb);
       // every wave holds the chunk in registers, and the next one is in LDS
-      if (kc) __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));
-      else __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+      wait();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      static_for<8 * TB>([&](auto kk) {
-        constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
-        mfma_acc<kAgpr>(acc[t][fb], wb[fb], xb[t]);
-        if constexpr (TB > 4) {
-          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(0, there, wa, xa);
-          if constexpr (k % 4 == 1 && k / 4 < PP) piece_to<k / 4>(slot);
-          if constexpr (k % 4 == 3 && k / 4 < PP) piece_from<k / 4>();
-        } else if constexpr (TB > 2) {
-          if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(0, there, wa, xa);
-          if constexpr (k % 2 == 1 && k / 2 < PP) copy_piece<k / 2>(slot);
-        } else {
-          if constexpr (k < PP) copy_piece<k>(slot);
-          if constexpr (k < kReads) read_image<k>(0, there, wa, xa);
-        }
+      half<false, C, kLateFrom, kLate>(acc, wb, xb, 0, b_there, a_there, wa, xa, chunks - kc - kLateAhead);
+      b_here = b_there, a_here = a_there;
+    };
+    using No = std::integral_constant<Copying, kNoCopies>;
+    using Yes = std::integral_constant<Copying, kCopies>;
+    using If = std::integral_constant<Copying, kCopiesIf>;
+    chunk(std::true_type{}, If{}, [&]() {
+      if (landed) __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
+      else if (chunks > kStarted) __builtin_amdgcn_s_waitcnt(wait_for(kOnTheirWay, 0));
+      else __builtin_amdgcn_s_waitcnt(wait_for(0, 0));
+    });
+#pragma unroll 1
+    for (kc = 1; kc + kLateAhead < chunks; ++kc)
+      chunk(std::false_type{}, Yes{}, [&]() {
+        if (kStarted > 2 && landed && kc < kStarted - 1) __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
+        else __builtin_amdgcn_s_waitcnt(wait_for(kOnTheirWay, 0));
       });
-    }
+    // (where the soon copies go less far than the late ones, one of these chunks still has some)
+#pragma unroll 1
+    for (; kc < chunks; ++kc)
+      chunk(std::false_type{}, std::conditional_t<(kLateAhead > kStarted), If, No>{}, [&]() { __builtin_amdgcn_s_waitcnt(wait_for(0, 0)); });
     // the compiler does not know the instructions above for MFMAs: let the last one retire before anything reads the accumulators
     static_for<TB>([&](auto tc) {
       f32x4(&a)[8] = acc[decltype(tc)::value];
@@ -327,7 +398,7 @@ __device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int 
   constexpr int kPieces = kPairs ? 2 : 4;             // pieces of a row that a lane holds
   const Results<MODE> res(p, m0);
   const int lane = lane_here(), g = lane >> 4, c = lane & 15, n = n0 + eight_of(g);
-  constexpr int kAsked = MODE == kGatedGrad ? (TB > 2 ? 2 : 1) : kPieces;   // pieces whose extras are on their way (what the registers allow)
+  constexpr int kAsked = MODE == kGatedGrad ? 2 : kPieces;   // pieces whose extras are on their way (what the registers allow)
   typename Results<MODE>::Extra extra[kAsked];
 #pragma unroll
   for (int i = 0; i < kAsked; ++i) res.template fetch<ACT, BESIDES>(c, n + 32 * i, extra[i]);
@@ -408,10 +479,10 @@ __device__ __forceinline__ void leave_part(float* part, int rows, const f32x4 (&
 }
 
 template <bool A_ACROSS, bool B_ACROSS, int MODE, int TB>
-__global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCall) {
+__global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
   constexpr bool kPairs = MODE == kGated;
   using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB>;
-  __shared__ __attribute__((aligned(1024))) char lds_raw[2 * W::kSlot];
+  __shared__ __attribute__((aligned(1024))) char lds_raw[W::kLds];
   // Workgroups go to the 8 XCDs round-robin: rank is their order by XCD, so that those behind one L2 work on tiles beside each other.
   const int per_xcd = gridDim.x >> 3, rank = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   const ProductShare shares = call_again().s;
@@ -441,7 +512,8 @@ __global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCal
   W walk(lds_raw);
   auto set_out = [&]() __attribute__((always_inline)) { walk.start(m_tile * 32 * TB, n_tile * (kPairs ? kTileB / 2 : kTileB), first, count); };
   set_out();
-  __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+  walk.wait_for_first();
+  bool landed = false;
 #pragma unroll 1
   for (;;) {
     __builtin_amdgcn_s_barrier();
@@ -457,11 +529,11 @@ __global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCal
 #pragma unroll
       for (int f = 0; f < kPieces; ++f) bias[f] = B_ACROSS ? Bias{} : load_bias<MODE>(p, min(n + 32 * f, p.N - 8));
     }
-    walk.run(acc);
+    walk.run(acc, landed);
     const ProductParams p = call_again().p;
     float* part = count == chunks ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
     const bool filled = p.M > m0;                      // the wave has rows: then at least so many of its stores were issued as results have pieces
-    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+    __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
     __builtin_amdgcn_s_barrier();                      // (no wave reads chunks any more)
     asm volatile("" ::: "memory");
     const bool more = advance();
@@ -478,8 +550,9 @@ __global__ __launch_bounds__(256, TB > 2 ? 1 : 2) void product_kernel(ProductCal
     if (!more) break;
     // The copies are older than the epilogue's stores, of which there were at least so many, and both complete in their order.
     constexpr int kStores = TB * (kPairs ? 2 : 4);
-    if (whole && filled) __builtin_amdgcn_s_waitcnt((kStores & 15) | ((kStores >> 4) << 14) | (7 << 4) | (15 << 8));
-    else __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+    if (whole && filled) __builtin_amdgcn_s_waitcnt(wait_for(kStores, 15));
+    else __builtin_amdgcn_s_waitcnt(wait_for(0, 15));
+    landed = true;
   }
 }
 
