@@ -10,35 +10,39 @@ enum ProductMode { kPlain = 0, kGated = 1, kGrad = 2, kGatedGrad = 3 };
 constexpr int kTileB = 256;       // rows of B of a tile
 constexpr int kChunk = 64;        // contraction elements of a chunk
 
-// How a product's tiles are shared out.  Every workgroup takes `rounds` whole tiles; the chunks of the `rest` tiles behind them lie end to end and are cut into
-// `runs` runs, one a workgroup (as many runs as tiles: whole tiles), the first `longer` of them of run_chunks + 1 chunks, the others of run_chunks.  A run covers parts of at
-// most two tiles, since there are at least as many runs as tiles.
+// How a product's tiles are shared out.  Every workgroup takes `rounds` whole tiles.  The contraction of each of the `rest` tiles behind them is cut into `cuts` parts of as
+// many chunks (or one more); the parts are units of their own, those of the same part of all tiles beside each other: workgroups that run together then read the same part
+// of the matrices they share.
 struct ProductShare {
-  int m_tiles, n_tiles, chunks, groups, rounds, rest, runs, run_chunks, longer, unused;
+  int m_tiles, n_tiles, chunks, groups, rounds, rest, cuts, blocks;
 };
-// first chunk of a run
-constexpr int run_begin(const ProductShare& s, int run) {
-  const int r = run < s.runs ? run : s.runs;
-  return r * s.run_chunks + (r < s.longer ? r : s.longer);
-}
-// the run that holds a chunk
-constexpr int run_of(const ProductShare& s, int chunk) {
-  const int behind = s.longer * (s.run_chunks + 1);
-  return chunk < behind ? chunk / (s.run_chunks + 1) : s.longer + (chunk - behind) / s.run_chunks;
-}
-// where a run's part of the tile whose first chunk is tile_begin lies among the parts: the one that the run begins in comes first
-constexpr int part_slot(const ProductShare& s, int run, int tile_begin) { return 2 * run + (run_begin(s, run) < tile_begin ? 1 : 0); }
+constexpr int units_of(const ProductShare& s) { return s.rest * s.cuts; }
+// first chunk of a part
+constexpr int part_begin(const ProductShare& s, int part) { return (int)((int64_t)s.chunks * part / s.cuts); }
 
-// Where a tile lies: blocks of 8 tiles of B walk down the tiles of A, so that the workgroups that run behind one L2 at a time share 8 tiles of B and 4 of A.
+// What a workgroup does in its turn: unit `at` of the rounds' tiles or of the parts.  The workgroups come to the 8 XCDs round-robin; those of one XCD take units beside each other.
+constexpr int unit_of(int turns, int turn, int group, int groups) { return ((group & 7) * turns + turn) * (groups >> 3) + (group >> 3); }
+constexpr int part_turns(const ProductShare& s) { return (units_of(s) + s.groups - 1) / s.groups; }
+
+// Where a tile lies: the tiles of B in `blocks` blocks as wide as each other, or one tile wider, each of which walks down the tiles of A.  The workgroups that run behind
+// one L2 at a time take tiles that follow each other, and read from memory once what they share, so a block is about as wide as it is high in rows.
 struct TilePlace {
   int m, n;
 };
 constexpr TilePlace tile_of(const ProductShare& s, int lin) {
-  constexpr int kBlockN = 8;
-  const int full = s.n_tiles / kBlockN * kBlockN;
-  if (lin < full * s.m_tiles) return {lin % (kBlockN * s.m_tiles) / kBlockN, lin / (kBlockN * s.m_tiles) * kBlockN + lin % kBlockN};
-  const int over = lin - full * s.m_tiles, width = s.n_tiles - full;
-  return {over / width, full + over % width};
+  const int width = s.n_tiles / s.blocks, wider = s.n_tiles - width * s.blocks, in_wider = wider * (width + 1) * s.m_tiles;
+  if (lin < in_wider) {
+    const int block = lin / ((width + 1) * s.m_tiles), rem = lin - block * (width + 1) * s.m_tiles;
+    return {rem / (width + 1), block * (width + 1) + rem % (width + 1)};
+  }
+  const int block = (lin - in_wider) / (width * s.m_tiles), rem = lin - in_wider - block * width * s.m_tiles;
+  return {rem / width, wider * (width + 1) + block * width + rem % width};
+}
+// The blocks for `together` tiles behind an L2, of `height` rows of A to 256 of B: width^2 * 256 = together * height, no narrower than fills them.
+constexpr int tile_blocks(int together, int height, int m_tiles, int n_tiles) {
+  int width = 1;
+  while (width < n_tiles && (width * width * kTileB < together * height || width * m_tiles < together)) ++width;
+  return (2 * n_tiles + width) / (2 * width) < 1 ? 1 : (2 * n_tiles + width) / (2 * width);
 }
 
 // How a call is carried out, by its sizes alone.
@@ -56,26 +60,43 @@ constexpr bool product_offered(bool a_across, bool b_across, int mode) {
 
 constexpr size_t whole_256(size_t n) { return (n + 255) / 256 * 256; }
 
-constexpr ProductPlan plan_product(int M, int N, int K, int mode, bool sums) {
-  ProductPlan plan{};
-  plan.tb = M > 1024 ? 8 : M > 256 ? 4 : 2;
-  const int columns = mode == kGated ? kTileB / 2 : kTileB;
-  ProductShare& s = plan.share;
-  s.m_tiles = (M + 32 * plan.tb - 1) / (32 * plan.tb), s.n_tiles = (N + columns - 1) / columns;
-  s.chunks = (K + kChunk - 1) / kChunk;
-  const int tiles = s.m_tiles * s.n_tiles;
-  s.groups = 256;                                    // one on every CU
-  s.rounds = tiles / s.groups;
-  s.rest = tiles - s.rounds * s.groups;
-  // tiles behind the whole rounds: shared out where that saves more than it costs
-  s.runs = s.rest;
-  if (s.rest && s.rest * 3 < s.groups * 2) {
-    const int64_t runs = (int64_t)s.rest * s.chunks / 4;
-    s.runs = runs < s.rest ? s.rest : runs > s.groups ? s.groups : (int)runs;
+// The time that a plan takes, in tenths of a microsecond, from what was measured: a chunk of a tile of 256, 128 and 64 rows 1.2, 0.68 and 0.48 us, what a tile takes besides 5, 3.5 and 2.5;
+// parts go to memory and come back at 4 TB/s, and are joined by a launch of its own, 5 us.
+constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
+  const int64_t chunk = tb > 4 ? 120 : tb > 2 ? 68 : 48, tile = tb > 4 ? 500 : tb > 2 ? 350 : 250;   // hundredths
+  int64_t time = s.rounds * (s.chunks * chunk + tile);
+  if (s.rest) time += part_turns(s) * ((int64_t)((s.chunks + s.cuts - 1) / s.cuts) * chunk + tile);
+  if (s.cuts > 1) {
+    const int64_t rows = (int64_t)s.m_tiles * 32 * tb, bytes = (int64_t)units_of(s) * 32 * tb * kTileB * 4 * M / rows * 2;
+    time += 500 + bytes / 40000;
   }
-  if (s.rest) s.run_chunks = s.rest * s.chunks / s.runs, s.longer = s.rest * s.chunks % s.runs;
+  return time;
+}
+
+constexpr ProductPlan plan_product(int M, int N, int K, int mode, bool sums) {
+  const int columns = mode == kGated ? kTileB / 2 : kTileB;
+  ProductPlan plan{};
+  int64_t best = 0;
+  for (int tb = 8; tb >= 2; tb /= 2) {
+    ProductShare s{};
+    s.m_tiles = (M + 32 * tb - 1) / (32 * tb), s.n_tiles = (N + columns - 1) / columns;
+    s.chunks = (K + kChunk - 1) / kChunk;
+    s.groups = 256;                                  // one on every CU
+    const int64_t tiles = (int64_t)s.m_tiles * s.n_tiles;
+    s.rounds = (int)(tiles / s.groups);
+    s.rest = (int)(tiles - (int64_t)s.rounds * s.groups);
+    const int together = tiles < 256 ? (int)(tiles + 7) / 8 : 32;
+    s.blocks = tile_blocks(together, 32 * tb, s.m_tiles, s.n_tiles);
+    const int most = s.rest == 0 || s.chunks < 4 ? 1 : s.chunks / 2 < 64 ? s.chunks / 2 : 64;
+    for (int cuts = 1; cuts <= most && (cuts == 1 || s.rest * cuts <= 4 * s.groups); ++cuts) {
+      s.cuts = cuts;
+      const int64_t time = plan_time(s, tb, M);
+      if (plan.tb == 0 || time < best) plan.tb = tb, plan.share = s, best = time;
+    }
+  }
+  const ProductShare& s = plan.share;
   plan.sum_rows = sums ? s.m_tiles * 2 : 0;
-  plan.sums_off = s.runs > s.rest ? whole_256((size_t)2 * s.runs * 32 * plan.tb * kTileB * sizeof(float)) : 0;
+  plan.sums_off = s.cuts > 1 ? whole_256((size_t)units_of(s) * 32 * plan.tb * kTileB * sizeof(float)) : 0;
   plan.total = plan.sums_off + whole_256((size_t)plan.sum_rows * (mode == kGatedGrad ? 2 : 1) * N * sizeof(float));
   return plan;
 }

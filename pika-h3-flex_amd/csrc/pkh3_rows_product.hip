@@ -3,7 +3,7 @@
 
 namespace pkh3 {
 
-// The parts of the tiles that several workgroups share, added up in the order of the contraction, and finished: a workgroup is 8 pieces of 8 columns times 32 rows; with
+// The parts of the tiles whose contraction was cut, added up in their order, and finished: a workgroup is 8 pieces of 8 columns times 32 rows; with
 // sums of columns it takes as many rows as a wave of product_kernel has, whose place in the sums it fills.
 template <int MODE>
 __global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, ProductShare s, int tb) {
@@ -13,9 +13,6 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, Prod
   const int rows = MODE >= kGrad ? 16 * tb : 32;
   const auto [m_tile, n_tile] = tile_of(s, s.rounds * s.groups + blockIdx.x);
   const Results<MODE> res(p, m_tile * 32 * tb + blockIdx.y * rows);
-  const int q0 = blockIdx.x * s.chunks;
-  const int first = run_of(s, q0), last = run_of(s, q0 + s.chunks - 1);
-  if (first == last) return;                           // (one workgroup had all of it and finished it)
   const int col = (blockIdx.z * 8 + (threadIdx.x & 7)) * 8, n = n_tile * kCols + col;
   Piece sum_a{}, sum_b{};
   with_form<MODE, false>(p, [&](auto act, auto besides) {
@@ -25,9 +22,9 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, Prod
       res.template fetch<decltype(act)::value, decltype(besides)::value>(r, n, extra);
       const Bias bias = load_bias<MODE>(p, n);
       Piece a{}, b{};
-      for (int rank = first; rank <= last; ++rank) {
-        const int slot = part_slot(s, rank, q0);
-        const char* from = (const char*)(p.part + ((int64_t)slot * 32 * tb + blockIdx.y * rows + r) * kTileB + col);
+      for (int part = 0; part < s.cuts; ++part) {
+        const int64_t slot = (int64_t)part * s.rest + blockIdx.x;
+        const char* from = (const char*)(p.part + (slot * 32 * tb + blockIdx.y * rows + r) * kTileB + col);
         const Piece va = load_piece_f32(from);
 #pragma unroll
         for (int j = 0; j < 8; ++j) a.v[j] += va.v[j];
@@ -90,7 +87,7 @@ static hipError_t launch_column_sums(const float* part, int rows, int columns, v
 
 hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_across, bool b_across, int mode, void* sums, char* workspace, hipStream_t s) {
   p.sums = sums ? (float*)(workspace + plan.sums_off) : nullptr;
-  const bool cut = plan.share.runs > plan.share.rest;
+  const bool cut = plan.share.cuts > 1;
   p.part = cut ? (float*)(workspace + plan.part_off) : nullptr;
   hipError_t e;
   if (plan.tb == 8) e = launch_tiles_8(p, plan, a_across, b_across, mode, s);

@@ -483,29 +483,21 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
   constexpr bool kPairs = MODE == kGated;
   using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB>;
   __shared__ __attribute__((aligned(1024))) char lds_raw[W::kLds];
-  // Workgroups go to the 8 XCDs round-robin: rank is their order by XCD, so that those behind one L2 work on tiles beside each other.
-  const int per_xcd = gridDim.x >> 3, rank = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  const ProductShare shares = call_again().s;
-  const int run_first = run_begin(shares, rank), run_end = run_begin(shares, rank + 1);   // of the chunks of the tiles behind the whole ones
-  int round = 0, at = run_first;                       // whole tiles first, then the run
-  int m_tile = 0, n_tile = 0, first = 0, count = 0, slot = 0, chunks = 0;
+  int turn = 0, m_tile = 0, n_tile = 0, first = 0, count = 0, slot = 0;
   // The next tile or part of one; false: none.  (Values chosen, not branches taken: the compiler keeps what either branch writes in memory.)
   auto advance = [&]() __attribute__((always_inline)) {
     const ProductShare s = call_again().s;
-    chunks = s.chunks;
-    const bool whole = round < s.rounds;
-    const int tile = at / s.chunks;
-    const int lin = whole ? ((blockIdx.x & 7) * s.rounds + round) * per_xcd + (blockIdx.x >> 3) : s.rounds * (int)gridDim.x + tile;
-    first = whole ? 0 : at - tile * s.chunks;
-    count = whole ? s.chunks : min(run_end - at, s.chunks - first);
-    slot = part_slot(s, rank, tile * s.chunks);
-    const TilePlace place = tile_of(s, lin);
-    const bool more = whole || at < run_end;
-    round += whole ? 1 : 0;
-    at += whole ? 0 : count;
+    const bool whole = turn < s.rounds;
+    const int turns = whole ? s.rounds : part_turns(s), unit = unit_of(turns, whole ? turn : turn - s.rounds, blockIdx.x, s.groups);
+    const bool more = whole || (turn - s.rounds < turns && unit < units_of(s));
+    const int part = whole || !more ? 0 : unit / s.rest;
+    const TilePlace place = tile_of(s, whole ? unit : s.rounds * s.groups + unit - part * s.rest);
+    const int from = part_begin(s, part), to = whole ? s.chunks : part_begin(s, part + 1);
+    ++turn;
     // (uniform, which the compiler loses sight of on the way)
     m_tile = __builtin_amdgcn_readfirstlane(place.m), n_tile = __builtin_amdgcn_readfirstlane(place.n);
-    first = __builtin_amdgcn_readfirstlane(first), count = __builtin_amdgcn_readfirstlane(count);
+    first = __builtin_amdgcn_readfirstlane(from), count = __builtin_amdgcn_readfirstlane(to - from);
+    slot = __builtin_amdgcn_readfirstlane(whole || s.cuts == 1 ? -1 : unit);
     return __builtin_amdgcn_readfirstlane(more);
   };
   if (!advance()) return;
@@ -531,7 +523,7 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
     }
     walk.run(acc, landed);
     const ProductParams p = call_again().p;
-    float* part = count == chunks ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
+    float* part = slot < 0 ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
     const bool filled = p.M > m0;                      // the wave has rows: then at least so many of its stores were issued as results have pieces
     __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
     __builtin_amdgcn_s_barrier();                      // (no wave reads chunks any more)

@@ -270,49 +270,38 @@ int main() {
     ProductPlan plan = plan_product(M, N, K, mode, mode >= kGrad);
     const ProductShare& s = plan.share;
     const int columns = mode == kGated ? 128 : 256, tiles = s.m_tiles * s.n_tiles;
-    CHECK(s.groups % 8 == 0 && s.groups * s.rounds + s.rest == tiles && s.runs >= s.rest && s.runs <= s.groups);
+    CHECK(s.groups % 8 == 0 && s.groups * s.rounds + s.rest == tiles && s.rest < s.groups && s.cuts >= 1 && (s.cuts == 1 || s.cuts * 2 <= s.chunks));
     CHECK((int64_t)s.m_tiles * 32 * plan.tb >= M && (int64_t)s.n_tiles * columns >= N && (int64_t)s.chunks * kChunk >= K && (int64_t)(s.chunks - 1) * kChunk < K);
+    CHECK(s.blocks >= 1 && s.blocks <= s.n_tiles);
     std::set<std::pair<int, int>> places;
     for (int i = 0; i < tiles; ++i) {
       TilePlace at = tile_of(s, i);
       CHECK(at.m >= 0 && at.m < s.m_tiles && at.n >= 0 && at.n < s.n_tiles);
       CHECK(places.insert({at.m, at.n}).second);
     }
-    // whole rounds: as the kernel's workgroups take them
-    const int per_xcd = s.groups / 8;
-    std::vector<char> taken(tiles, 0);
-    for (int block = 0; block < s.groups; ++block)
-      for (int round = 0; round < s.rounds; ++round) {
-        const int lin = ((block & 7) * s.rounds + round) * per_xcd + (block >> 3);
-        CHECK(lin >= 0 && lin < s.rounds * s.groups && !taken[lin]);
-        taken[lin] = 1;
+    // as the kernel's workgroups take them: whole tiles, then parts, each once
+    std::vector<char> taken(tiles, 0), used(s.rest * s.cuts + 1, 0);
+    for (int group = 0; group < s.groups; ++group) {
+      for (int turn = 0; turn < s.rounds; ++turn) {
+        const int unit = unit_of(s.rounds, turn, group, s.groups);
+        CHECK(unit >= 0 && unit < s.rounds * s.groups && !taken[unit]);
+        taken[unit] = 1;
       }
-    // runs: every chunk of the other tiles once, at most two tiles a run, and the parts where the joining looks for them
-    if (s.rest == 0) { CHECK(run_begin(s, 0) == 0 && run_begin(s, s.groups) == 0); continue; }
-    CHECK(run_begin(s, 0) == 0 && run_begin(s, s.runs) == s.rest * s.chunks && run_begin(s, s.groups) == s.rest * s.chunks);
-    std::vector<std::vector<int>> parts(s.rest);
-    std::vector<char> used(2 * s.runs, 0);
-    for (int run = 0; run < s.groups; ++run) {
-      int at = run_begin(s, run), end = run_begin(s, run + 1), seen = 0;
-      while (at < end) {
-        const int tile = at / s.chunks, first = at - tile * s.chunks, count = end - at < s.chunks - first ? end - at : s.chunks - first;
-        CHECK(run_of(s, at) == run && run_of(s, at + count - 1) == run && ++seen <= 2);
-        if (count < s.chunks) {
-          const int slot = part_slot(s, run, tile * s.chunks);
-          CHECK(slot < 2 * s.runs && !used[slot]);
-          used[slot] = 1;
-          CHECK((size_t)(slot + 1) * 32 * plan.tb * kTileB * 4 <= (plan.sums_off ? plan.sums_off : 0));
-          parts[tile].push_back(slot);
-        }
-        at += count;
+      for (int turn = 0; turn < part_turns(s); ++turn) {
+        const int unit = unit_of(part_turns(s), turn, group, s.groups);
+        CHECK(unit >= 0);
+        if (unit >= units_of(s)) break;                // (and so are all that follow)
+        CHECK(!used[unit]);
+        used[unit] = 1;
       }
     }
-    for (int tile = 0; tile < s.rest; ++tile) {
-      const int q0 = tile * s.chunks, first = run_of(s, q0), last = run_of(s, q0 + s.chunks - 1);
-      if (first == last) { CHECK(parts[tile].empty()); continue; }
-      CHECK((int)parts[tile].size() == last - first + 1);
-      for (int run = first; run <= last; ++run) CHECK(parts[tile][run - first] == part_slot(s, run, q0));
+    for (int i = 0; i < s.rounds * s.groups; ++i) CHECK(taken[i]);
+    for (int i = 0; i < units_of(s); ++i) CHECK(used[i]);
+    if (s.rest) {
+      CHECK(part_begin(s, 0) == 0 && part_begin(s, s.cuts) == s.chunks);
+      for (int part = 0; part < s.cuts; ++part) CHECK(part_begin(s, part + 1) > part_begin(s, part));
     }
+    CHECK(s.cuts == 1 || (size_t)units_of(s) * 32 * plan.tb * kTileB * 4 <= plan.sums_off);
   }
   printf("ok\n");
   return 0;
