@@ -48,8 +48,21 @@ hipError_t launch_tiles_8(const ProductParams& p, const ProductPlan& plan, bool 
 hipError_t launch_tiles_4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
 hipError_t launch_tiles_2(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
 
+hipError_t launch_thin(const ProductParams& p, int mode, hipStream_t s);
+
 int activation_grad_rows(int M);                    // rows of partial column sums of an activation's gradient
 hipError_t launch_activation_grad(ProductParams p, void* sums, char* workspace, hipStream_t s);
+
+// ---- copies ----
+
+// The two halves of a direct-to-LDS copy: wave-uniform target and base address, per-lane byte offset.
+template <int OFFSET>
+__device__ __forceinline__ void copy_to(unsigned lds_addr) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(lds_addr), "n"(OFFSET) : "m0", "scc"); }
+__device__ __forceinline__ void copy_from(const char* g, unsigned lane_off) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(g) : "memory");
+}
+// operand of s_waitcnt: at most `vm` copies and `lgkm` LDS reads still on their way
+constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
 
 // ---- activations ----
 
@@ -148,6 +161,20 @@ __device__ __forceinline__ Bias load_bias(const ProductParams& p, int n) {
     if (MODE == kGated) bias.b = load_table(p.bias, p.N + n, p.bias_bf16);
   }
   return bias;
+}
+
+// Two blocks of 16 columns a lane holds four of each (4*g .. +3): after the exchange of rows of 16 lanes it holds eight columns beside each other, from
+// eight_of(g) of the 32 on.
+__device__ __forceinline__ int eight_of(int g) { return (g & 1) * 16 + (g >> 1) * 8; }
+__device__ __forceinline__ Piece eight_columns(const f32x4& first, const f32x4& second) {
+  Piece p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(first[i]), __float_as_uint(second[i]), false, false);
+    p.v[i] = __uint_as_float(r[0]);
+    p.v[4 + i] = __uint_as_float(r[1]);
+  }
+  return p;
 }
 
 // ---- from sums to results (see pkh3_product in the header) ----

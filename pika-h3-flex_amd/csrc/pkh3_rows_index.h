@@ -47,6 +47,7 @@ constexpr int tile_blocks(int together, int height, int m_tiles, int n_tiles) {
 
 // How a call is carried out, by its sizes alone.
 struct ProductPlan {
+  bool thin;                     // the form for few rows
   int tb;                        // 16-row blocks of A a wave: tiles of 32 * tb rows of A and 256 of B
   ProductShare share;
   int sum_rows;                  // rows of partial column sums
@@ -59,6 +60,10 @@ constexpr bool product_offered(bool a_across, bool b_across, int mode) {
 }
 
 constexpr size_t whole_256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Few rows of operands along: the form of pkh3_rows_thin.hip, in 16 columns a workgroup where 32 would leave CUs without one.
+constexpr bool is_thin(int M, bool along) { return along && M <= 64; }
+constexpr bool thin_narrow(int N) { return N <= 32 * 192; }
 
 // The time that a plan takes, in tenths of a microsecond, from what was measured: a chunk of a tile of 256, 128 and 64 rows 1.2, 0.68 and 0.48 us, what a tile takes besides 5, 3.5 and 2.5;
 // parts go to memory and come back at 4 TB/s, and are joined by a launch of its own, 5 us.
@@ -73,9 +78,13 @@ constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
   return time;
 }
 
-constexpr ProductPlan plan_product(int M, int N, int K, int mode, bool sums) {
+constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bool sums) {
   const int columns = mode == kGated ? kTileB / 2 : kTileB;
   ProductPlan plan{};
+  if (is_thin(M, along)) {
+    plan.thin = true;
+    return plan;
+  }
   int64_t best = 0;
   for (int tb = 8; tb >= 2; tb /= 2) {
     ProductShare s{};

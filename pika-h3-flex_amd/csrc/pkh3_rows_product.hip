@@ -89,6 +89,7 @@ hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_acros
   p.sums = sums ? (float*)(workspace + plan.sums_off) : nullptr;
   const bool cut = plan.share.cuts > 1;
   p.part = cut ? (float*)(workspace + plan.part_off) : nullptr;
+  if (plan.thin) return launch_thin(p, mode, s);
   hipError_t e;
   if (plan.tb == 8) e = launch_tiles_8(p, plan, a_across, b_across, mode, s);
   else if (plan.tb == 4) e = launch_tiles_4(p, plan, a_across, b_across, mode, s);

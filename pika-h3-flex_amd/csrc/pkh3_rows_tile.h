@@ -18,20 +18,11 @@
 
 namespace pkh3 {
 
-// The two halves of a direct-to-LDS copy: wave-uniform target and base address, per-lane byte offset.
-template <int OFFSET>
-__device__ __forceinline__ void copy_to(unsigned lds_addr) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(lds_addr), "n"(OFFSET) : "m0", "scc"); }
-__device__ __forceinline__ void copy_from(const char* g, unsigned lane_off) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(lane_off), "s"(g) : "memory");
-}
-// The same by all lanes or none: it counts in the waits either way.  (Longer to issue: where it may not be due.)
+// The second half of a copy by all lanes or none: it counts in the waits either way.  (Longer to issue: where it may not be due.)
 __device__ __forceinline__ void copy_from_if(const char* g, unsigned lane_off, unsigned long long lanes) {
   asm volatile("s_mov_b64 exec, %2\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" : : "v"(lane_off), "s"(g), "s"(lanes) : "memory");
 }
 enum Copying { kNoCopies, kCopies, kCopiesIf };
-// operand of s_waitcnt: at most `vm` copies and `lgkm` LDS reads still on their way
-constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8); }
-
 // c += a b, as an instruction: the compiler, left to place 256 accumulator registers itself, moves them between the halves of the register file inside the loop.
 // AGPR: they lie in the accumulator half.
 // FIRST: onto zeros.
@@ -356,20 +347,6 @@ struct Walk {
     });
   }
 };
-
-// Two blocks of 16 columns a lane holds four of each (4*g .. +3): after the exchange of rows of 16 lanes it holds eight columns beside each other, from
-// eight_of(g) of the 32 on.
-__device__ __forceinline__ int eight_of(int g) { return (g & 1) * 16 + (g >> 1) * 8; }
-__device__ __forceinline__ Piece eight_columns(const f32x4& first, const f32x4& second) {
-  Piece p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(first[i]), __float_as_uint(second[i]), false, false);
-    p.v[i] = __uint_as_float(r[0]);
-    p.v[4 + i] = __uint_as_float(r[1]);
-  }
-  return p;
-}
 
 // A wave's results: 16 rows at a time, a lane 16 bytes of a row four times (twice with gates).  What else the results need is asked for a block of rows ahead.
 // The accumulators of block t, which is known when the kernel runs: a branch, not an index.

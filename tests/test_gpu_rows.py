@@ -171,7 +171,7 @@ def _linear_inputs(rows, K, N, seed, table_type=F32):
 
 LINEAR_SHAPES = [(1, 8, 8), (1, 1024, 264), (2, 40, 24), (3, 72, 1000), (15, 136, 520), (16, 512, 256), (17, 2048, 128), (33, 264, 648), (64, 1000, 512),
                  (65, 96, 136), (100, 4096, 64), (127, 328, 248), (129, 1032, 264), (255, 64, 2056), (257, 520, 512), (300, 11008, 96), (1085, 768, 776),
-                 (2003, 200, 1288)]
+                 (2003, 200, 1288), (3, 72, 6200), (20, 2056, 6152), (50, 264, 6408)]
 
 
 @pytest.mark.parametrize("rows,K,N", LINEAR_SHAPES)

@@ -267,7 +267,7 @@ int main() {
     auto log_size = [](int most) { int bits = 1 + rand() % 21; int v = 1 + rand() % (1 << bits); return v < most ? v : most; };
     int M = log_size(60000), N = (log_size(20000) + 7) / 8 * 8, K = log_size(60000), mode = rand() % 4;
     if ((int64_t)M * N > 400000000ll) continue;
-    ProductPlan plan = plan_product(M, N, K, mode, mode >= kGrad);
+    ProductPlan plan = plan_product(M, N, K, false, mode, mode >= kGrad);
     const ProductShare& s = plan.share;
     const int columns = mode == kGated ? 128 : 256, tiles = s.m_tiles * s.n_tiles;
     CHECK(s.groups % 8 == 0 && s.groups * s.rounds + s.rest == tiles && s.rest < s.groups && s.cuts >= 1 && (s.cuts == 1 || s.cuts * 2 <= s.chunks));
