@@ -61,19 +61,25 @@ constexpr bool product_offered(bool a_across, bool b_across, int mode) {
 
 constexpr size_t whole_256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Few rows of operands along: the form of pkh3_rows_thin.hip, in 16 columns a workgroup where 32 would leave CUs without one.
-constexpr bool is_thin(int M, bool along) { return along && M <= 64; }
-constexpr bool thin_narrow(int N) { return N <= 32 * 192; }
+// The form of pkh3_rows_thin.hip, for few rows of operands along: workgroups of up to 64 rows times 32 columns, or of 16 where 32 would leave CUs without one (and with gates).
+constexpr int thin_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+constexpr bool thin_narrow(int M, int N) { return (int64_t)((N + 31) / 32) * ((M + thin_rows(M) - 1) / thin_rows(M)) < 192; }
+// Its time as plan_time() has it: a workgroup's rows and weights at the 90 GB/s a CU that calls of one workgroup a CU reach, 60 where there are more.
+constexpr int64_t thin_time(int M, int N, int K, int mode) {
+  const int columns = mode == kGated || thin_narrow(M, N) ? 16 : 32, blocks = thin_rows(M) + (mode == kGated ? 32 : columns);
+  const int64_t groups = (int64_t)((N + columns - 1) / columns) * ((M + thin_rows(M) - 1) / thin_rows(M)), bytes = (int64_t)blocks * K * 2;
+  return groups <= 256 ? bytes / 900 : bytes * groups / 256 / 600;
+}
 
-// The time that a plan takes, in tenths of a microsecond, from what was measured: a chunk of a tile of 256, 128 and 64 rows 1.2, 0.68 and 0.48 us, what a tile takes besides 5, 3.5 and 2.5;
-// parts go to memory and come back at 4 TB/s, and are joined by a launch of its own, 5 us.
+// The time that a plan takes, in hundredths of a microsecond besides the launch, from what was measured: a chunk of a tile of 256, 128 and 64 rows 1.2, 0.68 and 0.48 us, what a tile takes besides 5, 3.5 and 2.5;
+// parts go to memory and come back at 4 TB/s, and are joined by a launch of its own, 8 us.
 constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
   const int64_t chunk = tb > 4 ? 120 : tb > 2 ? 68 : 48, tile = tb > 4 ? 500 : tb > 2 ? 350 : 250;   // hundredths
   int64_t time = s.rounds * (s.chunks * chunk + tile);
   if (s.rest) time += part_turns(s) * ((int64_t)((s.chunks + s.cuts - 1) / s.cuts) * chunk + tile);
   if (s.cuts > 1) {
     const int64_t rows = (int64_t)s.m_tiles * 32 * tb, bytes = (int64_t)units_of(s) * 32 * tb * kTileB * 4 * M / rows * 2;
-    time += 500 + bytes / 40000;
+    time += 800 + bytes / 40000;
   }
   return time;
 }
@@ -81,10 +87,6 @@ constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
 constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bool sums) {
   const int columns = mode == kGated ? kTileB / 2 : kTileB;
   ProductPlan plan{};
-  if (is_thin(M, along)) {
-    plan.thin = true;
-    return plan;
-  }
   int64_t best = 0;
   for (int tb = 8; tb >= 2; tb /= 2) {
     ProductShare s{};
@@ -102,6 +104,10 @@ constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bo
       const int64_t time = plan_time(s, tb, M);
       if (plan.tb == 0 || time < best) plan.tb = tb, plan.share = s, best = time;
     }
+  }
+  if (along && thin_time(M, N, K, mode) < best) {
+    plan.thin = true;
+    return plan;
   }
   const ProductShare& s = plan.share;
   plan.sum_rows = sums ? s.m_tiles * 2 : 0;

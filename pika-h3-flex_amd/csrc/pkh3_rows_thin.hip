@@ -144,7 +144,7 @@ static void launch_rows(const ProductParams& p, hipStream_t s) {
 
 hipError_t launch_thin(const ProductParams& p, int mode, hipStream_t s) {
   if (mode == kGated) launch_rows<kGated, 2>(p, s);
-  else if (thin_narrow(p.N)) launch_rows<kPlain, 1>(p, s);
+  else if (thin_narrow(p.M, p.N)) launch_rows<kPlain, 1>(p, s);
   else launch_rows<kPlain, 2>(p, s);
   return hipGetLastError();
 }
