@@ -22,7 +22,7 @@ struct NormParams {
 
 int norm_groups(int rows, int tables);              // workgroups of the backward pass, each with sums of its own
 size_t norm_scratch_bytes(int rows, int width, int tables);
-hipError_t launch_norm(const NormParams& p, bool f32, bool tables_bf16, hipStream_t s);
+hipError_t launch_norm(NormParams p, bool f32, bool tables_bf16, hipStream_t s);
 hipError_t launch_norm_backward(NormParams p, bool f32, bool tables_bf16, char* workspace, hipStream_t s);
 
 // ---- products ----

@@ -3,9 +3,10 @@
 //   forward    y = xh w[r] + b[r], xh = (x - mean) rstd
 //   backward   g = dy w[r]:  dx = rstd (g - mean(g) - xh mean(g xh)),  dw[r] = sum of dy xh, db[r] = sum of dy over the rows of table row r
 //
-// A row lies in the registers of the lanes that share it (a wave up to 2,048 elements, a workgroup above), 8 elements a piece, so memory is read once
-// and the variance is taken about the mean.  The backward pass forms the statistics again from the row, which it needs anyway, instead of keeping them.  Both
-// are bound by memory.
+// A row lies in the registers of the lanes that share it (a wave or a workgroup), 8 elements a piece, and the next row is on its way while one is worked on, so memory is
+// read once and the variance is taken about the mean.  The backward pass forms the statistics again from the row, which it needs anyway, instead of keeping them.  Both
+// are bound by memory: 48,360 rows of 2,048 in bfloat16 take 84 us forward (4.7 TB/s; a copy of as many bytes takes 75) and 157 us backward
+// (3.8 TB/s), 15,342 rows of 1,536 in float32 30 us (6.2 TB/s; a copy 27) and 55 us (5.1 TB/s).
 //
 // Sums for the tables: every workgroup takes one run of rows and keeps the sums of the table row that it is at in registers (its rows come
 // in runs of one table row, so they rarely change); when the table row changes, and at the end, the workgroup's lanes add up in LDS and the sums go to the
@@ -16,12 +17,12 @@ namespace pkh3 {
 
 constexpr int kNormThreads = 256;
 
-// `count` values summed over the LANES lanes that share a row
+// COUNT values summed over the LANES lanes that share a row (lds: COUNT floats a wave)
 template <int LANES, int COUNT>
 __device__ __forceinline__ void row_sums(float (&x)[COUNT], float* lds) {
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) x[i] = wave_sum(x[i]);
-  if constexpr (LANES == 256) {
+  if constexpr (LANES > 64) {
     const int wave = threadIdx.x >> 6;
     __syncthreads();                                  // (what the sums before these were read from)
     if ((threadIdx.x & 63) == 0) {
@@ -30,87 +31,127 @@ __device__ __forceinline__ void row_sums(float (&x)[COUNT], float* lds) {
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) x[i] = (lds[i] + lds[COUNT + i]) + (lds[2 * COUNT + i] + lds[3 * COUNT + i]);
+    for (int i = 0; i < COUNT; ++i) {
+      x[i] = lds[i];
+      for (int w = 1; w < LANES / 64; ++w) x[i] += lds[w * COUNT + i];
+    }
   }
 }
 
-template <bool F32>
-__device__ __forceinline__ Piece load_row_piece(const char* row, int n) {
-  return F32 ? load_piece_f32(row + (int64_t)n * 4) : load_piece(row + (int64_t)n * 2);
-}
 template <bool F32>
 __device__ __forceinline__ void store_row_piece(char* row, int n, const Piece& p) {
-  if constexpr (F32) {
-    store_piece_f32(row + (int64_t)n * 4, p);
-  } else {
-    store_piece(row + (int64_t)n * 2, p);
-  }
+  if constexpr (F32) store_piece_f32(row + (int64_t)n * 4, p);
+  else store_piece(row + (int64_t)n * 2, p);
 }
 
-// A row of NP pieces a lane: loaded (zeros past its end), its mean taken off, and 1 / sqrt(variance + eps) returned.
+// A row of NP pieces a lane as it lies in memory (zeros past its end): on its way while the row before it is worked on.
 template <bool F32, int LANES, int NP>
-struct Row {
-  Piece x[NP];
+struct Raw {
+  i32x4 v[NP][F32 ? 2 : 1];
   __device__ __forceinline__ void load(const char* row, int lane, int width) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int n = (i * LANES + lane) * 8;
-      x[i] = n < width ? load_row_piece<F32>(row, n) : Piece{};
-    }
-  }
-  __device__ __forceinline__ float centre(int lane, int width, float eps, float* lds) {
-    float s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] += x[i].v[j];
-    row_sums<LANES>(s, lds);
-    const float mean = s[0] / (float)width;
-    s[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const bool live = (i * LANES + lane) * 8 < width;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[i].v[j] = live ? x[i].v[j] - mean : 0.f;
-        s[0] += x[i].v[j] * x[i].v[j];
+      for (int h = 0; h < (F32 ? 2 : 1); ++h) {
+        v[i][h] = i32x4{0, 0, 0, 0};
+        if (n < width) v[i][h] = *(const i32x4*)(row + (int64_t)n * (F32 ? 4 : 2) + h * 16);
       }
     }
-    row_sums<LANES>(s, lds);
-    return 1.0f / sqrtf(s[0] / (float)width + eps);
+  }
+  __device__ __forceinline__ Piece piece(int i) const {
+    Piece p;
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p.v[j] = __int_as_float(v[i][j >> 2][j & 3]);
+    } else {
+      const bf16x8 raw = __builtin_bit_cast(bf16x8, v[i][0]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p.v[j] = (float)raw[j];
+    }
+    return p;
   }
 };
 
+// The row with its mean taken off, and 1 / sqrt(variance + eps).
+template <bool F32, int LANES, int NP>
+__device__ __forceinline__ float centre(Piece (&x)[NP], const Raw<F32, LANES, NP>& raw, int lane, int width, float eps, float* lds) {
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    x[i] = raw.piece(i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[0] += x[i].v[j];
+  }
+  row_sums<LANES>(s, lds);
+  const float mean = s[0] / (float)width;
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const bool live = i < NP / 2 || (i * LANES + lane) * 8 < width;   // (wider than the next smaller form, so the first half is full)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[i].v[j] = live ? x[i].v[j] - mean : 0.f;
+      s[0] += x[i].v[j] * x[i].v[j];
+    }
+  }
+  row_sums<LANES>(s, lds);
+  return 1.0f / sqrtf(s[0] / (float)width + eps);
+}
+
 __device__ __forceinline__ int table_of(const NormParams& p, int row) { return p.row_index ? min(max(p.row_index[row], 0), p.tables - 1) : 0; }
 
-template <bool F32, bool TB16, int LANES, int NP>
-__global__ __launch_bounds__(kNormThreads) void norm_kernel(NormParams p) {
-  __shared__ float lds[4];
-  const int lane = threadIdx.x % LANES;
-  const int row = blockIdx.x * (kNormThreads / LANES) + threadIdx.x / LANES;
-  if (row >= p.rows) return;                          // (whole waves, and with LANES == 256 none)
-  Row<F32, LANES, NP> r;
-  r.load(p.x + row * p.x_stride, lane, p.width);
-  const int64_t table = (int64_t)table_of(p, row) * p.width;
-  const float rstd = r.centre(lane, p.width, p.eps, lds);
+template <bool TB16, int LANES, int NP>
+__device__ __forceinline__ void load_table_row(Piece (&to)[NP], const char* table, int t, int lane, int width, float without) {
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int n = (i * LANES + lane) * 8;
-    if (n >= p.width) break;
-    Piece y;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y.v[j] = r.x[i].v[j] * rstd;
-    if (p.weight) {
-      const Piece w = load_table(p.weight, table + n, TB16);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y.v[j] *= w.v[j];
+    for (int j = 0; j < 8; ++j) to[i].v[j] = without;
+    if (table && n < width) to[i] = load_table(table, (int64_t)t * width + n, TB16);
+  }
+}
+
+// rows of a workgroup: one run, dealt to its waves (or taken by all of them) in turn
+struct Run {
+  int first, end;
+};
+__device__ __forceinline__ Run run_of_rows(const NormParams& p) {
+  return {(int)((int64_t)p.rows * blockIdx.x / p.groups), (int)((int64_t)p.rows * (blockIdx.x + 1) / p.groups)};
+}
+
+template <bool F32, bool TB16, int LANES, int NP>
+__global__ __launch_bounds__(kNormThreads) void norm_kernel(NormParams p) {
+  constexpr int kRows = kNormThreads / LANES;         // rows at a time
+  __shared__ float lds[4];
+  const int lane = threadIdx.x % LANES, which = __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+  const Run run = run_of_rows(p);
+  int row = run.first + which, held = -1;
+  if (row >= run.end) return;                         // (whole waves, and with LANES == 256 all of them)
+  Raw<F32, LANES, NP> raw;
+  raw.load(p.x + row * p.x_stride, lane, p.width);
+  Piece w[NP], b[NP];
+#pragma unroll 1
+  for (; row < run.end; row += kRows) {
+    const int t = __builtin_amdgcn_readfirstlane(table_of(p, row));
+    if (t != held) {
+      load_table_row<TB16, LANES>(w, p.weight, t, lane, p.width, 1.f);
+      load_table_row<TB16, LANES>(b, p.bias, t, lane, p.width, 0.f);
+      held = t;
     }
-    if (p.bias) {
-      const Piece b = load_table(p.bias, table + n, TB16);
+    const Raw<F32, LANES, NP> now = raw;
+    raw.load(p.x + min(row + kRows, run.end - 1) * p.x_stride, lane, p.width);
+    Piece x[NP];
+    const float rstd = centre<F32, LANES, NP>(x, now, lane, p.width, p.eps, lds);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y.v[j] += b.v[j];
+    for (int i = 0; i < NP; ++i) {
+      const int n = (i * LANES + lane) * 8;
+      if (n >= p.width) break;
+      Piece y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y.v[j] = x[i].v[j] * rstd * w[i].v[j] + b[i].v[j];
+      store_row_piece<F32>(p.out + row * p.out_stride, n, y);
     }
-    store_row_piece<F32>(p.out + row * p.out_stride, n, y);
   }
 }
 
@@ -118,12 +159,12 @@ __global__ __launch_bounds__(kNormThreads) void norm_kernel(NormParams p) {
 __host__ __device__ inline int64_t slice_floats(int tables, int width) { return (int64_t)tables * 2 * width; }
 
 template <bool F32, bool TB16, int LANES, int NP>
-__global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormParams p) {
-  constexpr int kRows = kNormThreads / LANES;         // rows at a time
-  __shared__ float lds[8];
+__global__ __launch_bounds__(LANES > kNormThreads ? LANES : kNormThreads) void norm_backward_kernel(NormParams p) {
+  constexpr int kRows = LANES > kNormThreads ? 1 : kNormThreads / LANES;   // rows at a time
+  __shared__ float lds[2 * 16];
   __shared__ __attribute__((aligned(16))) float staged[LANES == 64 ? 3 * 64 * 8 : 1];
-  const int lane = threadIdx.x % LANES, which = threadIdx.x / LANES;
-  const int first = (int)((int64_t)p.rows * blockIdx.x / p.groups), end = (int)((int64_t)p.rows * (blockIdx.x + 1) / p.groups);
+  const int lane = threadIdx.x % LANES, which = __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
+  const auto [first, end] = run_of_rows(p);
   float* slice = p.part + (int64_t)blockIdx.x * slice_floats(p.tables, p.width);
   const bool sums = p.part != nullptr;
   uint64_t touched = 0;
@@ -144,31 +185,41 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormParams 
       }
     }
     Piece w[NP], dw[NP], db[NP];
+    load_table_row<TB16, LANES>(w, p.weight, t, lane, p.width, 1.f);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int n = (i * LANES + lane) * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[i].v[j] = 1.f, dw[i].v[j] = 0.f, db[i].v[j] = 0.f;
-      if (p.weight && n < p.width) w[i] = load_table(p.weight, (int64_t)t * p.width + n, TB16);
-    }
+    for (int i = 0; i < NP; ++i) dw[i] = Piece{}, db[i] = Piece{};
+    // The next row on its way where the registers allow it: 48,360 rows of 2,048 in bfloat16 take 157 us so and 196 without. Four pieces of float32
+    // a lane lose more by the registers (15,342 rows of 1,536: 72 us so, 55 without), and where a row has several waves others fill the gap
+    // (48,360 rows of 4,096: 294 us so, 261 without; 15,342 of 8,192: 203 and 172).
+    constexpr bool kAhead = LANES == 64 && (NP < 4 || !F32);
+    Raw<F32, LANES, NP> raw_x, raw_dy;
+    auto ask = [&](int row) {
+      raw_x.load(p.x + row * p.x_stride, lane, p.width);
+      raw_dy.load(p.dy + row * p.dy_stride, lane, p.width);
+    };
+    if (kAhead) ask(min(at + which, to - 1));
+#pragma unroll 1
     for (int row = at + which; row < to; row += kRows) {
-      Row<F32, LANES, NP> r, d;
-      r.load(p.x + row * p.x_stride, lane, p.width);
-      d.load(p.dy + row * p.dy_stride, lane, p.width);
-      const float rstd = r.centre(lane, p.width, p.eps, lds);
+      if (!kAhead) ask(row);
+      const Raw<F32, LANES, NP> x_now = raw_x, dy_now = raw_dy;
+      if (kAhead) ask(min(row + kRows, to - 1));
+      Piece x[NP], d[NP];
+      const float rstd = centre<F32, LANES, NP>(x, x_now, lane, p.width, p.eps, lds);
       float s[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
+      for (int i = 0; i < NP; ++i) {
+        d[i] = dy_now.piece(i);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float xh = r.x[i].v[j] * rstd, g = d.x[i].v[j] * w[i].v[j];
-          r.x[i].v[j] = xh;
-          dw[i].v[j] += d.x[i].v[j] * xh;
-          db[i].v[j] += d.x[i].v[j];
-          d.x[i].v[j] = g;
+          const float xh = x[i].v[j] * rstd, g = d[i].v[j] * w[i].v[j];
+          x[i].v[j] = xh;
+          dw[i].v[j] += d[i].v[j] * xh;
+          db[i].v[j] += d[i].v[j];
+          d[i].v[j] = g;
           s[0] += g;
           s[1] += g * xh;
         }
+      }
       row_sums<LANES>(s, lds);
       const float mean_g = s[0] / (float)p.width, mean_gx = s[1] / (float)p.width;
 #pragma unroll
@@ -177,7 +228,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormParams 
         if (n >= p.width) break;
         Piece y;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y.v[j] = rstd * (d.x[i].v[j] - mean_g - r.x[i].v[j] * mean_gx);
+        for (int j = 0; j < 8; ++j) y.v[j] = rstd * (d[i].v[j] - mean_g - x[i].v[j] * mean_gx);
         store_row_piece<F32>(p.dx + row * p.dx_stride, n, y);
       }
     }
@@ -218,21 +269,35 @@ __global__ __launch_bounds__(kNormThreads) void norm_backward_kernel(NormParams 
   if (sums && threadIdx.x == 0) p.touched[blockIdx.x] = touched;
 }
 
-// dweight and dbias from the slices: a workgroup is 32 columns of one table row (8 lanes of 4), 32 slices at a time
-__global__ __launch_bounds__(256) void norm_sums_kernel(NormParams p) {
-  __shared__ f32x4 staged[256];
+// dweight and dbias from the slices: a workgroup is 32 columns of one table row (8 lanes of 4), 128 slices at a time, four times that asked for together
+constexpr int kSumThreads = 1024;
+
+__global__ __launch_bounds__(kSumThreads) void norm_sums_kernel(NormParams p) {
+  __shared__ f32x4 staged[kSumThreads];
   const int t = blockIdx.y, half = blockIdx.z;
   float* out = half ? p.dbias : p.dweight;
   if (!out) return;
   const int col = blockIdx.x * 32 + (threadIdx.x & 7) * 4;
+  const int64_t slice = slice_floats(p.tables, p.width);
+  const float* at = p.part + ((int64_t)t * 2 + half) * p.width + min(col, p.width - 4);
+  constexpr int kAt = kSumThreads / 8;
   f32x4 sum{0.f, 0.f, 0.f, 0.f};
-  if (col < p.width) {
-    const float* at = p.part + ((int64_t)t * 2 + half) * p.width + col;
-    for (int g = threadIdx.x >> 3; g < p.groups; g += 32)
-      if ((p.touched[g] >> t) & 1) sum += *(const f32x4*)(at + (int64_t)g * slice_floats(p.tables, p.width));
+  for (int g = threadIdx.x >> 3; g < p.groups; g += 4 * kAt) {
+    f32x4 v[4];
+    bool there[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int from = min(g + i * kAt, p.groups - 1);
+      there[i] = g + i * kAt < p.groups && ((p.touched[from] >> t) & 1);
+      v[i] = *(const f32x4*)(at + from * slice);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += there[i] ? v[i][j] : 0.f;   // (what nobody wrote may be anything)
   }
   staged[threadIdx.x] = sum;
-  for (int over = 128; over >= 8; over /= 2) {
+  for (int over = kSumThreads / 2; over >= 8; over /= 2) {
     __syncthreads();
     if ((int)threadIdx.x < over) staged[threadIdx.x] += staged[threadIdx.x + over];
   }
@@ -254,18 +319,21 @@ static void with_form(bool f32, bool tb16, int width, F&& f) {
   else tb16 ? by_width(std::false_type{}, std::true_type{}) : by_width(std::false_type{}, std::false_type{});
 }
 
-hipError_t launch_norm(const NormParams& p, bool f32, bool tables_bf16, hipStream_t s) {
+// Workgroups of the forward pass: as many as there are rows for, up to six a CU, which then have several rows a wave, the next one on its way.
+hipError_t launch_norm(NormParams p, bool f32, bool tables_bf16, hipStream_t s) {
   with_form(f32, tables_bf16, p.width, [&](auto a, auto b, auto lanes, auto np) {
     constexpr int kRows = kNormThreads / decltype(lanes)::value;
-    norm_kernel<decltype(a)::value, decltype(b)::value, decltype(lanes)::value, decltype(np)::value><<<(p.rows + kRows - 1) / kRows, kNormThreads, 0, s>>>(p);
+    p.groups = (p.rows + kRows - 1) / kRows < 1536 ? (p.rows + kRows - 1) / kRows : 1536;
+    norm_kernel<decltype(a)::value, decltype(b)::value, decltype(lanes)::value, decltype(np)::value><<<p.groups, kNormThreads, 0, s>>>(p);
   });
   return hipGetLastError();
 }
 
-// A workgroup for 16 rows while there are few, up to 1,024 of them; with many tables fewer, so that the slices stay small.
+// A workgroup for 8 rows up to 512 of them, for 32 up to 1,024 (their slices are then a sixth of what the rows move); with many tables fewer, so that the slices stay small.
 int norm_groups(int rows, int tables) {
-  const int by_rows = (rows + 15) / 16, most = 8192 / tables < 1024 ? 8192 / tables : 1024;
-  return by_rows < most ? by_rows : most;
+  const int by_8 = (rows + 7) / 8 < 512 ? (rows + 7) / 8 : 512, by_32 = (rows + 31) / 32 < 1024 ? (rows + 31) / 32 : 1024;
+  const int groups = by_8 > by_32 ? by_8 : by_32, most = 8192 / tables;
+  return groups < most ? groups : most;
 }
 
 static size_t touched_bytes(int groups) { return ((size_t)groups * 8 + 255) / 256 * 256; }
@@ -275,17 +343,33 @@ size_t norm_scratch_bytes(int rows, int width, int tables) {
   return touched_bytes(groups) + ((size_t)groups * slice_floats(tables, width) * sizeof(float) + 255) / 256 * 256;
 }
 
+// f(type of the rows, of the tables, lanes a row, pieces a lane) for the backward pass, which holds five times as much of a row a lane
+template <class F>
+static void with_backward_form(bool f32, bool tb16, int width, F&& f) {
+  auto by_width = [&](auto rows32, auto tables16) {
+    if (width <= 512) f(rows32, tables16, std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (width <= 1024) f(rows32, tables16, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else if (width <= 2048) f(rows32, tables16, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else if (width <= 4096) f(rows32, tables16, std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (width <= 8192) f(rows32, tables16, std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else f(rows32, tables16, std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+  };
+  if (f32) tb16 ? by_width(std::true_type{}, std::true_type{}) : by_width(std::true_type{}, std::false_type{});
+  else tb16 ? by_width(std::false_type{}, std::true_type{}) : by_width(std::false_type{}, std::false_type{});
+}
+
 hipError_t launch_norm_backward(NormParams p, bool f32, bool tables_bf16, char* workspace, hipStream_t s) {
   const bool sums = p.dweight || p.dbias;
   p.groups = norm_groups(p.rows, p.tables);
   p.touched = sums ? (uint64_t*)workspace : nullptr;
   p.part = sums ? (float*)(workspace + touched_bytes(p.groups)) : nullptr;
-  with_form(f32, tables_bf16, p.width, [&](auto a, auto b, auto lanes, auto np) {
-    norm_backward_kernel<decltype(a)::value, decltype(b)::value, decltype(lanes)::value, decltype(np)::value><<<p.groups, kNormThreads, 0, s>>>(p);
+  with_backward_form(f32, tables_bf16, p.width, [&](auto a, auto b, auto lanes, auto np) {
+    constexpr int kThreads = decltype(lanes)::value > kNormThreads ? decltype(lanes)::value : kNormThreads;
+    norm_backward_kernel<decltype(a)::value, decltype(b)::value, decltype(lanes)::value, decltype(np)::value><<<p.groups, kThreads, 0, s>>>(p);
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !sums) return e;
-  norm_sums_kernel<<<dim3((p.width + 31) / 32, p.tables, 2), 256, 0, s>>>(p);
+  norm_sums_kernel<<<dim3((p.width + 31) / 32, p.tables, 2), kSumThreads, 0, s>>>(p);
   return hipGetLastError();
 }
 
