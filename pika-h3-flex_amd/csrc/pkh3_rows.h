@@ -112,7 +112,7 @@ __device__ __forceinline__ void act_and_slope(float v, float& value, float& slop
   } else if constexpr (ACT == 3) {
     const float q = sigmoid_of(2.0f * kTanhScale * v * (1.0f + kTanhCube * v * v));
     value = v * q;
-    slope = q + value * (1.0f - q) * (2.0f * kTanhScale) * (1.0f + 3.0f * kTanhCube * v * v);
+    slope = q + value * (1.0f - q) * (2.0f * kTanhScale) * (1.0f + 3.0f * kTanhCube * fminf(v * v, 1e30f));   // (no 0 times infinity far out)
   } else {
     value = v;
     slope = 1.0f;

@@ -6,7 +6,8 @@ The layers are the reference's ``ff.net.0.proj`` and ``ff.net.2`` (src/pika_h3/c
 rows (patches/0001-h3-adaln-fp32.patch:34-40).
 
 Rows are ``[rows, width]`` with unit column stride, other strides and widths multiples of 8 elements, 16-byte aligned.  Where gradients are recorded and an
-input needs them, the three calls take part in torch's differentiation; the ``*_backward`` functions are the same passes by themselves.
+input needs them, the three calls take part in torch's differentiation (not while a stream is captured); the ``*_backward`` functions are the same passes by
+themselves, which a graph may hold.
 """
 from __future__ import annotations
 
@@ -92,7 +93,13 @@ def _activation(name: str) -> int:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call is recorded for torch's differentiation.  Not while a stream is captured: the nodes that add up the leaves' gradients may live already, with the
+    stream of an eager pass, and running them on it inside a capture ends the process."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("gradients are not recorded while a stream is captured: call the forward and the *_backward functions under torch.no_grad()")
+    return True
 
 
 def _scratch_bytes(entry: str, args) -> int:
@@ -160,6 +167,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if _wants_grad(x, weight, bias):
         if out is not None:
             raise ValueError("out cannot be given where gradients are recorded")
+        for t in (weight, bias):
+            if t is not None and t.dim() == 2 and t.shape[0] > _lib.LAYER_NORM_MAX_TABLES:
+                raise ValueError(f"gradients of at most {_lib.LAYER_NORM_MAX_TABLES} table rows, got {t.shape[0]}")
         return _LayerNorm.apply(x, weight, bias, row_index, eps)
     return _layer_norm(x, weight, bias, row_index, eps, out)
 
