@@ -92,12 +92,12 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _wants_grad(*tensors) -> bool:
+def _wants_grad(x, *tensors) -> bool:
     """Whether a call is recorded for torch's differentiation.  Not while a stream is captured: the nodes that add up the leaves' gradients may live already, with the
     stream of an eager pass, and running them on it inside a capture ends the process."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, *tensors)):
         return False
-    if torch.cuda.is_current_stream_capturing():
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("gradients are not recorded while a stream is captured: call the forward and the *_backward functions under torch.no_grad()")
     return True
 
