@@ -50,11 +50,10 @@ def test_nothing_touches_a_product_before_it_is_there(tmp_path):
         f = tmp_path / f"{i}.elf"
         f.write_bytes(image)
         text = subprocess.run([OBJDUMP, "-d", str(f)], check=True, capture_output=True, text=True).stdout
-        for name, listing in re.findall(r"^[0-9a-f]+ <(\S*4pkh3\d+(?:product_kernel|thin_product_kernel)\S*)>:\n(.*?)(?=^[0-9a-f]+ <|\Z)", text, re.M | re.S):
+        for name, listing in re.findall(r"^[0-9a-f]+ <(\S*4pkh3\d+product_kernel\S*)>:\n(.*?)(?=^[0-9a-f]+ <|\Z)", text, re.M | re.S):
             forms[name] = _young(listing)
-            assert listing.count("v_mfma") >= (2 if "thin" in name else 96), name
-    # three heights of tiles times six kinds of product; the form for few rows in nine
-    assert sum("thin" not in n for n in forms) == 18 and sum("thin" in n for n in forms) == 9, sorted(forms)
+            assert listing.count("v_mfma") >= 96, name
+    assert len(forms) == 18, sorted(forms)      # three heights of tiles, six kinds of product
     assert not {n: h[:3] for n, h in forms.items() if h}
 
 
