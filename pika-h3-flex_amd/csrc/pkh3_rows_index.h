@@ -71,15 +71,17 @@ constexpr int64_t thin_time(int M, int N, int K, int mode) {
   return groups <= 256 ? bytes / 900 : bytes * groups / 256 / 600;
 }
 
-// The time that a plan takes, in hundredths of a microsecond besides the launch, from what was measured: a chunk of a tile of 256, 128 and 64 rows 1.2, 0.68 and 0.48 us, what a tile takes besides 5, 3.5 and 2.5;
-// parts go to memory and come back at 4 TB/s, and are joined by a launch of its own, 8 us.
+// The time that a plan takes, in hundredths of a microsecond besides the launch, from what was measured with weights that come from memory: a chunk of a
+// tile of 256, 128 and 64 rows 1.1, 0.8 and 0.62 us, what a tile takes besides 5, 3.5 and 2.5; parts go to memory and come back at 6 TB/s, and are joined by a launch
+// of its own, 8 us.  (Over 42 products of 128 to 9,500 rows the choice takes 0.3 % longer than the best of the forms and cuts; 3 % with the 1.2, 0.68 and
+// 0.48 us that a chunk takes where the weights are in the caches.)
 constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
-  const int64_t chunk = tb > 4 ? 120 : tb > 2 ? 68 : 48, tile = tb > 4 ? 500 : tb > 2 ? 350 : 250;   // hundredths
+  const int64_t chunk = tb > 4 ? 110 : tb > 2 ? 80 : 62, tile = tb > 4 ? 500 : tb > 2 ? 350 : 250;   // hundredths
   int64_t time = s.rounds * (s.chunks * chunk + tile);
   if (s.rest) time += part_turns(s) * ((int64_t)((s.chunks + s.cuts - 1) / s.cuts) * chunk + tile);
   if (s.cuts > 1) {
     const int64_t rows = (int64_t)s.m_tiles * 32 * tb, bytes = (int64_t)units_of(s) * 32 * tb * kTileB * 4 * M / rows * 2;
-    time += 800 + bytes / 40000;
+    time += 800 + bytes / 60000;
   }
   return time;
 }
