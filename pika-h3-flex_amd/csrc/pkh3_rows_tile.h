@@ -445,13 +445,10 @@ __device__ __forceinline__ void leave_part(float* part, int rows, const f32x4 (&
     if (16 * t >= rows) break;
     f32x4 block[8];
     block_of<TB>(t, acc, block);
-    static_for<PAIRS ? 2 : 4>([&](auto fc) {
-      Piece a, b{};
-      pieces_of<PAIRS, decltype(fc)::value>(block, a, b);
-      char* to = (char*)(part + (16 * t + c) * kTileB + eight_of(g) + 32 * decltype(fc)::value);
-      store_piece_f32(to, a);
-      if constexpr (PAIRS) store_piece_f32(to + 128 * 4, b);
-    });
+    // (values and gates: blocks of them in turn)
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+      *(f32x4*)(part + (16 * t + c) * kTileB + 4 * g + (PAIRS ? (f >> 1) * 16 + (f & 1) * 128 : f * 16)) = block[f];
   }
 }
 
