@@ -46,7 +46,9 @@ struct ProductParams {
 hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_across, bool b_across, int mode, void* sums, char* workspace, hipStream_t s);
 hipError_t launch_tiles_8(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
 hipError_t launch_tiles_4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
-hipError_t launch_tiles_2(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
+hipError_t launch_tiles_4x4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
+hipError_t launch_tiles_2x4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
+hipError_t launch_tiles_3x4(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s);
 
 hipError_t launch_thin(const ProductParams& p, int mode, hipStream_t s);
 

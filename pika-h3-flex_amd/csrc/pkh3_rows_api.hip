@@ -193,7 +193,7 @@ ProductParams product_params(const pkh3_product_args* a) {
 }
 
 ProductPlan product_plan(const pkh3_product_args* a) {
-  return plan_product(a->M, a->N, a->K, !(a->flags & (PKH3_PRODUCT_A_ACROSS | PKH3_PRODUCT_B_ACROSS)), mode_of(a->flags), a->sums != nullptr);
+  return plan_product(a->M, a->N, a->K, !(a->flags & (PKH3_PRODUCT_A_ACROSS | PKH3_PRODUCT_B_ACROSS)), mode_of(a->flags), a->sums != nullptr, a->flags & PKH3_PRODUCT_A_ACROSS);
 }
 
 int check_activation_sizes(const pkh3_product_args* a) {

@@ -7,7 +7,6 @@ namespace pkh3 {
 
 enum ProductMode { kPlain = 0, kGated = 1, kGrad = 2, kGatedGrad = 3 };
 
-constexpr int kTileB = 256;       // rows of B of a tile
 constexpr int kChunk = 64;        // contraction elements of a chunk
 
 // How a product's tiles are shared out.  Every workgroup takes `rounds` whole tiles.  The contraction of each of the `rest` tiles behind them is cut into `cuts` parts of as
@@ -38,17 +37,17 @@ constexpr TilePlace tile_of(const ProductShare& s, int lin) {
   const int block = (lin - in_wider) / (width * s.m_tiles), rem = lin - in_wider - block * width * s.m_tiles;
   return {rem / width, wider * (width + 1) + block * width + rem % width};
 }
-// The blocks for `together` tiles behind an L2, of `height` rows of A to 256 of B: width^2 * 256 = together * height, no narrower than fills them.
-constexpr int tile_blocks(int together, int height, int m_tiles, int n_tiles) {
+// The blocks for `together` tiles behind an L2, of `height` rows of A to `wide` of B: width^2 * wide = together * height, no narrower than fills them.
+constexpr int tile_blocks(int together, int height, int wide, int m_tiles, int n_tiles) {
   int width = 1;
-  while (width < n_tiles && (width * width * kTileB < together * height || width * m_tiles < together)) ++width;
+  while (width < n_tiles && (width * width * wide < together * height || width * m_tiles < together)) ++width;
   return (2 * n_tiles + width) / (2 * width) < 1 ? 1 : (2 * n_tiles + width) / (2 * width);
 }
 
 // How a call is carried out, by its sizes alone.
 struct ProductPlan {
   bool thin;                     // the form for few rows
-  int tb;                        // 16-row blocks of A a wave: tiles of 32 * tb rows of A and 256 of B
+  int tb, fb;                    // 16-row blocks of A and of B a wave: tiles of 32 * tb rows of A and 32 * fb of B
   ProductShare share;
   int sum_rows;                  // rows of partial column sums
   size_t part_off, sums_off, total;   // bytes of the workspace
@@ -72,25 +71,31 @@ constexpr int64_t thin_time(int M, int N, int K, int mode) {
 }
 
 // The time that a plan takes, in hundredths of a microsecond besides the launch, from what was measured with weights that come from memory: a chunk of a
-// tile of 256, 128 and 64 rows 1.1, 0.8 and 0.62 us, what a tile takes besides 5, 3.5 and 2.5; parts go to memory and come back at 6 TB/s, and are joined by a launch
-// of its own, 8 us.  (Over 42 products of 128 to 9,500 rows the choice takes 0.3 % longer than the best of the forms and cuts; 3 % with the 1.2, 0.68 and
-// 0.48 us that a chunk takes where the weights are in the caches.)
-constexpr int64_t plan_time(const ProductShare& s, int tb, int M) {
-  const int64_t chunk = tb > 4 ? 110 : tb > 2 ? 80 : 62, tile = tb > 4 ? 500 : tb > 2 ? 350 : 250;   // hundredths
+// tile of 256 x 256, 128 x 256, 128 x 128, 96 x 128 and 64 x 128 rows 1.1, 0.8, 0.52, 0.46 and 0.36 us, what a tile takes besides 5, 3.5, 2.5, 2.2 and 2; parts go to memory and
+// come back at 6 TB/s, and are joined by a launch of its own, 8 us.  (Over 42 products of 128 to 9,500 rows the choice takes 0.6 % longer than the best of the
+// forms and cuts, at worst 15 %.)  What a smaller tile costs in copies for each product it gives back where there are few tiles: 1,085 x 2,048 x 2,048 takes 33.4 us in 72
+// tiles of 128 x 256, 24.7 in 144 of 128 x 128 and 21.9 in 192 of 96 x 128; 1,044 x 1,600 with a contraction of 608 12.5 us in tiles of 128 x 128, 11.6 of 96 x 128 and
+// 10.2 of 64 x 128; 4,000 x 2,048 x 2,048 35 us in 256 tiles of 128 x 256 and 43 of 128 x 128; 3,265 x 9,296 x 2,320 127 us of 256 x 256 and 159 of 128 x 256.
+constexpr int64_t plan_time(const ProductShare& s, int tb, int fb, int M) {
+  const int64_t chunk = tb > 4 ? 110 : fb > 4 ? 80 : tb > 3 ? 52 : tb > 2 ? 46 : 36, tile = tb > 4 ? 500 : fb > 4 ? 350 : tb > 3 ? 250 : tb > 2 ? 220 : 200;
   int64_t time = s.rounds * (s.chunks * chunk + tile);
   if (s.rest) time += part_turns(s) * ((int64_t)((s.chunks + s.cuts - 1) / s.cuts) * chunk + tile);
   if (s.cuts > 1) {
-    const int64_t rows = (int64_t)s.m_tiles * 32 * tb, bytes = (int64_t)units_of(s) * 32 * tb * kTileB * 4 * M / rows * 2;
+    const int64_t rows = (int64_t)s.m_tiles * 32 * tb, bytes = (int64_t)units_of(s) * 32 * tb * 32 * fb * 4 * M / rows * 2;
     time += 800 + bytes / 60000;
   }
   return time;
 }
 
-constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bool sums) {
-  const int columns = mode == kGated ? kTileB / 2 : kTileB;
+// Tiles that there are, in 16-row blocks a wave.  (Those of 96 rows not where A is stored across, whose rows come to LDS in units of 64.)
+constexpr int kForms[5][2] = {{8, 8}, {4, 8}, {4, 4}, {3, 4}, {2, 4}};
+
+constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bool sums, bool a_across = false) {
   ProductPlan plan{};
   int64_t best = 0;
-  for (int tb = 8; tb >= 2; tb /= 2) {
+  for (const auto& form : kForms) {
+    const int tb = form[0], fb = form[1], columns = mode == kGated ? 16 * fb : 32 * fb;
+    if (tb == 3 && a_across) continue;
     ProductShare s{};
     s.m_tiles = (M + 32 * tb - 1) / (32 * tb), s.n_tiles = (N + columns - 1) / columns;
     s.chunks = (K + kChunk - 1) / kChunk;
@@ -99,12 +104,12 @@ constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bo
     s.rounds = (int)(tiles / s.groups);
     s.rest = (int)(tiles - (int64_t)s.rounds * s.groups);
     const int together = tiles < 256 ? (int)(tiles + 7) / 8 : 32;
-    s.blocks = tile_blocks(together, 32 * tb, s.m_tiles, s.n_tiles);
+    s.blocks = tile_blocks(together, 32 * tb, 32 * fb, s.m_tiles, s.n_tiles);
     const int most = s.rest == 0 || s.chunks < 4 ? 1 : s.chunks / 2 < 64 ? s.chunks / 2 : 64;
     for (int cuts = 1; cuts <= most && (cuts == 1 || s.rest * cuts <= 4 * s.groups); ++cuts) {
       s.cuts = cuts;
-      const int64_t time = plan_time(s, tb, M);
-      if (plan.tb == 0 || time < best) plan.tb = tb, plan.share = s, best = time;
+      const int64_t time = plan_time(s, tb, fb, M);
+      if (plan.tb == 0 || time < best) plan.tb = tb, plan.fb = fb, plan.share = s, best = time;
     }
   }
   if (along && thin_time(M, N, K, mode) < best) {
@@ -113,7 +118,7 @@ constexpr ProductPlan plan_product(int M, int N, int K, bool along, int mode, bo
   }
   const ProductShare& s = plan.share;
   plan.sum_rows = sums ? s.m_tiles * 2 : 0;
-  plan.sums_off = s.cuts > 1 ? whole_256((size_t)units_of(s) * 32 * plan.tb * kTileB * sizeof(float)) : 0;
+  plan.sums_off = s.cuts > 1 ? whole_256((size_t)units_of(s) * 32 * plan.tb * 32 * plan.fb * sizeof(float)) : 0;
   plan.total = plan.sums_off + whole_256((size_t)plan.sum_rows * (mode == kGatedGrad ? 2 : 1) * N * sizeof(float));
   return plan;
 }

@@ -6,14 +6,14 @@ namespace pkh3 {
 // The parts of the tiles whose contraction was cut, added up in their order, and finished: a workgroup is 8 pieces of 8 columns times 32 rows; with
 // sums of columns it takes as many rows as a wave of product_kernel has, whose place in the sums it fills.
 template <int MODE>
-__global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, ProductShare s, int tb) {
+__global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, ProductShare s, int tb, int fb) {
   constexpr bool kPairs = MODE == kGated;
-  constexpr int kCols = kPairs ? kTileB / 2 : kTileB;
+  const int wide = 32 * fb, columns = kPairs ? wide / 2 : wide;
   __shared__ __attribute__((aligned(16))) Piece staged[MODE >= kGrad ? 2 * 256 : 1];
   const int rows = MODE >= kGrad ? 16 * tb : 32;
   const auto [m_tile, n_tile] = tile_of(s, s.rounds * s.groups + blockIdx.x);
   const Results<MODE> res(p, m_tile * 32 * tb + blockIdx.y * rows);
-  const int col = (blockIdx.z * 8 + (threadIdx.x & 7)) * 8, n = n_tile * kCols + col;
+  const int col = (blockIdx.z * 8 + (threadIdx.x & 7)) * 8, n = n_tile * columns + col;
   Piece sum_a{}, sum_b{};
   with_form<MODE, false>(p, [&](auto act, auto besides) {
     for (int r = threadIdx.x >> 3; r < rows; r += 32) {
@@ -24,12 +24,12 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, Prod
       Piece a{}, b{};
       for (int part = 0; part < s.cuts; ++part) {
         const int64_t slot = (int64_t)part * s.rest + blockIdx.x;
-        const char* from = (const char*)(p.part + (slot * 32 * tb + blockIdx.y * rows + r) * kTileB + col);
+        const char* from = (const char*)(p.part + (slot * 32 * tb + blockIdx.y * rows + r) * wide + col);
         const Piece va = load_piece_f32(from);
 #pragma unroll
         for (int j = 0; j < 8; ++j) a.v[j] += va.v[j];
         if constexpr (kPairs) {
-          const Piece vb = load_piece_f32(from + 128 * 4);
+          const Piece vb = load_piece_f32(from + columns * 4);
 #pragma unroll
           for (int j = 0; j < 8; ++j) b.v[j] += vb.v[j];
         }
@@ -92,15 +92,17 @@ hipError_t launch_product(ProductParams p, const ProductPlan& plan, bool a_acros
   if (plan.thin) return launch_thin(p, mode, s);
   hipError_t e;
   if (plan.tb == 8) e = launch_tiles_8(p, plan, a_across, b_across, mode, s);
-  else if (plan.tb == 4) e = launch_tiles_4(p, plan, a_across, b_across, mode, s);
-  else e = launch_tiles_2(p, plan, a_across, b_across, mode, s);
+  else if (plan.fb == 8) e = launch_tiles_4(p, plan, a_across, b_across, mode, s);
+  else if (plan.tb == 4) e = launch_tiles_4x4(p, plan, a_across, b_across, mode, s);
+  else if (plan.tb == 3) e = launch_tiles_3x4(p, plan, a_across, b_across, mode, s);
+  else e = launch_tiles_2x4(p, plan, a_across, b_across, mode, s);
   if (e != hipSuccess) return e;
   if (cut) {
-    const dim3 grid(plan.share.rest, mode >= kGrad ? 2 : plan.tb, mode == kGated ? 2 : 4);
-    if (mode == kPlain) product_join_kernel<kPlain><<<grid, 256, 0, s>>>(p, plan.share, plan.tb);
-    else if (mode == kGated) product_join_kernel<kGated><<<grid, 256, 0, s>>>(p, plan.share, plan.tb);
-    else if (mode == kGrad) product_join_kernel<kGrad><<<grid, 256, 0, s>>>(p, plan.share, plan.tb);
-    else product_join_kernel<kGatedGrad><<<grid, 256, 0, s>>>(p, plan.share, plan.tb);
+    const dim3 grid(plan.share.rest, mode >= kGrad ? 2 : plan.tb, plan.fb / (mode == kGated ? 4 : 2));
+    if (mode == kPlain) product_join_kernel<kPlain><<<grid, 256, 0, s>>>(p, plan.share, plan.tb, plan.fb);
+    else if (mode == kGated) product_join_kernel<kGated><<<grid, 256, 0, s>>>(p, plan.share, plan.tb, plan.fb);
+    else if (mode == kGrad) product_join_kernel<kGrad><<<grid, 256, 0, s>>>(p, plan.share, plan.tb, plan.fb);
+    else product_join_kernel<kGatedGrad><<<grid, 256, 0, s>>>(p, plan.share, plan.tb, plan.fb);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (!sums) return e;

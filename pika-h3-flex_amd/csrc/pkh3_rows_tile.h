@@ -9,8 +9,13 @@
 //          so that the eight elements that half a wave reads meet no bank twice; a 16-lane transposing read takes four elements of 16 rows and gives each lane those of one row (ds_read_b64_tr_b16), two of them an image
 // A copy's LDS target is linear in the lane, so the places are chosen through the lanes' source addresses.
 //
-// Work split.  Workgroup = 4 waves, one per SIMD = 256 rows of B x 32*TB rows of A; wave (fh, th) = 128 rows of B x 16*TB of A.  Two to four chunks in LDS: while the
-// products of a chunk's second half run, its place is filled with the chunk that many ahead, and the first half of the next chunk is read into registers.
+// Work split.  Workgroup = 4 waves, one per SIMD = 32*TB rows of A x 32*FB rows of B; wave (fh, th) = 16*TB x 16*FB of them.  256 workgroups, one a CU, take the tiles
+// in turn (pkh3_rows_index.h), and the next tile's first chunks come while one's results leave.  Both operands have rings of two to four chunks in LDS.
+//
+// What bounds it.  256 x 256: the matrix units (2,048 of a chunk's 2,300 cycles), whose clock the board's power holds at 1.7 GHz: 15,342 x 2,048 with a contraction of 5,504
+// takes 242 us, 1.43 PFLOP/s.  Smaller tiles: LDS, which every row of a chunk passes three times (written once, read by two waves: 3 cycles a row, 768 a chunk of 128 x 128, whose
+// products take 512), and with weights from memory what a CU takes in of lines that its L2 does not have, about 40 GB/s.  The results of a tile
+// are not covered by the next one's products: 15,342 x 5,504 gradients of gated halves, which read 675 MB and write 338, take 448 us where the product alone takes 240.
 #pragma once
 #include <type_traits>
 
@@ -162,23 +167,25 @@ __device__ __forceinline__ ProductCall call_again() {
 // those of 64 rows), and have to be on their way for about a microsecond.  So the copies of a chunk are issued over the whole of a chunk's time, each half
 // in the half chunk behind whose barrier the places they go to are free: `late` ones follow the barrier in the middle of a chunk, `soon` ones the half chunk after.
 // Which copies these are and how many places an operand has follows from what fits LDS; the operands' places are counted apart.
-template <bool A_ACROSS, bool B_ACROSS, bool PAIRS, int TB>
+template <bool A_ACROSS, bool B_ACROSS, bool PAIRS, int TB, int FB>
 struct Walk {
-  static constexpr int kTileA = 32 * TB;
-  static constexpr int kSlotsB = TB > 2 ? 3 : 4, kSlotsA = TB > 4 ? 2 : 4;
-  static constexpr bool kAgpr = TB > 2;
+  static constexpr int kTileA = 32 * TB, kTileB = 32 * FB;
+  static constexpr int kAhead = FB < 8 ? 0 : TB > 4 ? 2 : 1;   // which of the three ways of copying ahead
+  static constexpr int kSlotsB = kAhead ? 3 : 4, kSlotsA = kAhead == 2 ? 2 : 4;
+  static constexpr bool kAgpr = TB * FB > 16;
+  static_assert(!A_ACROSS || TB % 2 == 0, "units of 64 rows");
   using OB = Operand<B_ACROSS, kTileB, PAIRS, kSlotsB>;
   using OA = Operand<A_ACROSS, kTileA, false, kSlotsA>;
   static constexpr int CB = OB::kPieces, CA = OA::kPieces, PP = CA + CB;
   static constexpr int kBytesB = kSlotsB * OB::kSlot, kLds = kBytesB + kSlotsA * OA::kSlot;
-  static constexpr int kReads = 8 + TB;
-  // copies: 0 .. CB - 1 of B, then of A.  TB 8: A's behind the barrier, B's after; 4: the other way round; 2: half of them all
-  static constexpr int kLateFrom = TB > 4 ? CB : 0, kLate = TB > 4 ? CA : TB > 2 ? CB : PP / 2;
-  static constexpr int kSoonFrom = TB > 4 ? 0 : kLate, kSoon = PP - kLate;
+  static constexpr int kReads = FB + TB;
+  // copies: 0 .. CB - 1 of B, then of A.  256 x 256: A's behind the barrier, B's after; 128 x 256: the other way round; smaller tiles: half of them all
+  static constexpr int kLateFrom = kAhead == 2 ? CB : 0, kLate = kAhead == 2 ? CA : kAhead ? CB : PP / 2;
+  static constexpr int kSoonFrom = kAhead == 2 ? 0 : kLate, kSoon = PP - kLate;
   // copies on their way at the middle of a chunk when the next chunk has landed, and the chunks that start() brings on their way whole
-  static constexpr int kOnTheirWay = TB > 4 ? kSoon : TB > 2 ? 2 * kSoon + kLate : 2 * PP;
-  static constexpr int kStarted = TB > 4 ? 2 : 3;
-  static constexpr int kLateAhead = TB > 4 ? 2 : TB > 2 ? 3 : 4;   // chunks from the one whose middle they follow to that of the late copies (the soon ones': kStarted)
+  static constexpr int kOnTheirWay = kAhead == 2 ? kSoon : kAhead ? 2 * kSoon + kLate : 2 * PP;
+  static constexpr int kStarted = kAhead == 2 ? 2 : 3;
+  static constexpr int kLateAhead = kAhead == 2 ? 2 : kAhead ? 3 : 4;   // chunks from the one whose middle they follow to that of the late copies (the soon ones': kStarted)
   int lane, wave, m0, n0, chunks, left;
   OB ob;
   OA oa;
@@ -191,7 +198,7 @@ struct Walk {
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds_raw;
     ob.ring = lds0 + wave * CB * 1024;
     oa.ring = lds0 + kBytesB + wave * CA * 1024;
-    ib.init(lds_raw, lane, (wave & 1) * 8);
+    ib.init(lds_raw, lane, (wave & 1) * FB);
     ia.init(lds_raw + kBytesB, lane, (wave >> 1) * TB);
   }
   __device__ __forceinline__ void offsets_b(int k_left) {
@@ -252,12 +259,12 @@ struct Walk {
   }
 
   template <int I>
-  __device__ __forceinline__ void read_image(int ks, int b_bytes, int a_bytes, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
+  __device__ __forceinline__ void read_image(int ks, int b_bytes, int a_bytes, bf16x8 (&w)[FB], bf16x8 (&x)[TB]) const {
     if constexpr (I < TB) x[I] = ia.template read<I>(ks, a_bytes);
     else w[I - TB] = ib.template read<I - TB>(ks, b_bytes);
   }
   // what lies behind the contraction's end is taken for zeros (both operands: it may be anything)
-  __device__ __forceinline__ void clear_rest(int from, bf16x8 (&w)[8], bf16x8 (&x)[TB]) const {
+  __device__ __forceinline__ void clear_rest(int from, bf16x8 (&w)[FB], bf16x8 (&x)[TB]) const {
     i32x4 keep;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
@@ -265,7 +272,7 @@ struct Walk {
       keep[d] = (k < left ? 0xffff : 0) | (k + 1 < left ? (int)0xffff0000 : 0);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, w[i]) & keep);
+    for (int i = 0; i < FB; ++i) w[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, w[i]) & keep);
 #pragma unroll
     for (int i = 0; i < TB; ++i) x[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(i32x4, x[i]) & keep);
     asm volatile("s_nop 1" ::: "memory");            // (an MFMA may not take a register right behind the instruction that wrote it)
@@ -274,7 +281,7 @@ struct Walk {
   // MFMA where there are enough of them: a wave is alone on its SIMD, and the pipe idles whenever the rest takes longer to issue than the MFMA leaves free.
   // (Blocks of A back and forth: from one MFMA to the next only one operand changes.)
   template <bool FIRST, Copying C, int FROM, int COUNT>
-  __device__ __forceinline__ void half(f32x4 (&acc)[TB][8], bf16x8 (&w)[8], bf16x8 (&x)[TB], int ks, int b_bytes, int a_bytes, bf16x8 (&w2)[8], bf16x8 (&x2)[TB],
+  __device__ __forceinline__ void half(f32x4 (&acc)[TB][FB], bf16x8 (&w)[FB], bf16x8 (&x)[TB], int ks, int b_bytes, int a_bytes, bf16x8 (&w2)[FB], bf16x8 (&x2)[TB],
                                        int due) {
     unsigned long long lanes = 0;
     if constexpr (C == kCopiesIf) asm volatile("s_cmp_gt_i32 %1, 0\n\ts_cselect_b64 %0, -1, 0" : "=s"(lanes) : "s"(due) : "scc");
@@ -283,13 +290,13 @@ struct Walk {
       asm volatile("s_nop 1" ::: "memory");          // (registers that only now become sums)
       __builtin_amdgcn_sched_barrier(0);
     }
-    static_for<8 * TB>([&](auto kk) {
+    constexpr bool kRoomy = FB * TB >= 2 * kReads && FB * TB / (kSoon > kLate ? kSoon : kLate) >= 4;
+    static_for<FB * TB>([&](auto kk) {
       constexpr int k = decltype(kk)::value, fb = k / TB, t = fb & 1 ? TB - 1 - k % TB : k % TB;
       if constexpr (FIRST) mfma_first<kAgpr>(acc[t][fb], w[fb], x[t]);
       else mfma_acc<kAgpr>(acc[t][fb], w[fb], x[t]);
-      constexpr int kEvery = 8 * TB / COUNT;         // MFMAs from copy to copy
-      if constexpr (TB > 2) {
-        static_assert(kEvery >= 4, "a copy's halves follow different MFMAs");
+      constexpr int kEvery = FB * TB / COUNT;        // MFMAs from copy to copy
+      if constexpr (kRoomy) {                        // a copy's halves follow different MFMAs
         if constexpr (k % 2 == 0 && k / 2 < kReads) read_image<k / 2>(ks, b_bytes, a_bytes, w2, x2);
         if constexpr (C != kNoCopies && k % kEvery == 1 && k / kEvery < COUNT) piece_to<FROM + k / kEvery>();
         if constexpr (C != kNoCopies && k % kEvery == 3 && k / kEvery < COUNT) piece_from<FROM + k / kEvery, C>(lanes);
@@ -300,8 +307,8 @@ struct Walk {
     });
   }
   // The sums of the tile that start() set out for, whose first chunk has landed for every wave; `landed`: all that start() copied has.
-  __device__ __forceinline__ void run(f32x4 (&acc)[TB][8], bool landed) {
-    bf16x8 wa[8], wb[8], xa[TB], xb[TB];             // images of a chunk's first and second half
+  __device__ __forceinline__ void run(f32x4 (&acc)[TB][FB], bool landed) {
+    bf16x8 wa[FB], wb[FB], xa[TB], xb[TB];             // images of a chunk's first and second half
     static_for<kReads>([&](auto ic) { read_image<decltype(ic)::value>(0, 0, 0, wa, xa); });
     int b_here = 0, a_here = 0, kc = 0;              // the chunk's places in LDS, and the chunk
     auto chunk = [&](auto first, auto copying, auto&& wait) __attribute__((always_inline)) {
@@ -339,8 +346,10 @@ struct Walk {
       chunk(std::false_type{}, std::conditional_t<(kLateAhead > kStarted), If, No>{}, [&]() { __builtin_amdgcn_s_waitcnt(wait_for(0, 0)); });
     // the compiler does not know the instructions above for MFMAs: let the last one retire before anything reads the accumulators
     static_for<TB>([&](auto tc) {
-      f32x4(&a)[8] = acc[decltype(tc)::value];
-      if constexpr (kAgpr)
+      f32x4(&a)[FB] = acc[decltype(tc)::value];
+      if constexpr (FB == 4)
+        asm volatile("s_nop 15\n\ts_nop 15" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3])::"memory");
+      else if constexpr (kAgpr)
         asm volatile("s_nop 15\n\ts_nop 15" : "+a"(a[0]), "+a"(a[1]), "+a"(a[2]), "+a"(a[3]), "+a"(a[4]), "+a"(a[5]), "+a"(a[6]), "+a"(a[7])::"memory");
       else
         asm volatile("s_nop 15\n\ts_nop 15" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7])::"memory");
@@ -350,17 +359,17 @@ struct Walk {
 
 // A wave's results: 16 rows at a time, a lane 16 bytes of a row four times (twice with gates).  What else the results need is asked for a block of rows ahead.
 // The accumulators of block t, which is known when the kernel runs: a branch, not an index.
-template <int TB>
-__device__ __forceinline__ void block_of(int t, const f32x4 (&acc)[TB][8], f32x4 (&block)[8]) {
+template <int TB, int FB>
+__device__ __forceinline__ void block_of(int t, const f32x4 (&acc)[TB][FB], f32x4 (&block)[FB]) {
   static_for<TB>([&](auto tc) {
     if (t == decltype(tc)::value) {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) block[f] = acc[decltype(tc)::value][f];
+      for (int f = 0; f < FB; ++f) block[f] = acc[decltype(tc)::value][f];
     }
   });
 }
-template <bool PAIRS, int F>
-__device__ __forceinline__ void pieces_of(const f32x4 (&block)[8], Piece& a, Piece& b) {
+template <bool PAIRS, int F, int FB>
+__device__ __forceinline__ void pieces_of(const f32x4 (&block)[FB], Piece& a, Piece& b) {
   if constexpr (PAIRS) {
     a = eight_columns(block[4 * F], block[4 * F + 2]);
     b = eight_columns(block[4 * F + 1], block[4 * F + 3]);
@@ -369,10 +378,10 @@ __device__ __forceinline__ void pieces_of(const f32x4 (&block)[8], Piece& a, Pie
   }
 }
 
-template <int MODE, int ACT, int BESIDES, int TB>
-__device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int n0, int sum_row, const Bias (&bias)[MODE == kGated ? 2 : 4], const f32x4 (&acc)[TB][8]) {
+template <int MODE, int ACT, int BESIDES, int TB, int FB>
+__device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int n0, int sum_row, const Bias (&bias)[MODE == kGated ? FB / 4 : FB / 2], const f32x4 (&acc)[TB][FB]) {
   constexpr bool kPairs = MODE == kGated;
-  constexpr int kPieces = kPairs ? 2 : 4;             // pieces of a row that a lane holds
+  constexpr int kPieces = kPairs ? FB / 4 : FB / 2;   // pieces of a row that a lane holds
   const Results<MODE> res(p, m0);
   const int lane = lane_here(), g = lane >> 4, c = lane & 15, n = n0 + eight_of(g);
   constexpr int kAsked = MODE == kGatedGrad ? 2 : kPieces;   // pieces whose extras are on their way (what the registers allow)
@@ -389,13 +398,13 @@ __device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int 
   }
 #pragma unroll 1
   for (int t = 0; t < TB; ++t) {
-    f32x4 block[8];
-    block_of<TB>(t, acc, block);
+    f32x4 block[FB];
+    block_of<TB, FB>(t, acc, block);
     const int row = 16 * t + c;
     static_for<kPieces>([&](auto fc) {
       constexpr int f = decltype(fc)::value;
       Piece a, b{};
-      pieces_of<kPairs, f>(block, a, b);
+      pieces_of<kPairs, f, FB>(block, a, b);
       res.template finish<ACT, BESIDES>(row, n + 32 * f, a, b, bias[f], extra[f % kAsked]);
       if constexpr (MODE >= kGrad) {
         const bool there = row < res.rows;
@@ -436,26 +445,27 @@ __device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int 
   }
 }
 
-// The sums of a part of a contraction, as they are: rows of 256 (values and gates: 128 each).
-template <bool PAIRS, int TB>
-__device__ __forceinline__ void leave_part(float* part, int rows, const f32x4 (&acc)[TB][8]) {
+// The sums of a part of a contraction, as they are: rows as wide as the tile (values and gates: half of it each).
+template <bool PAIRS, int TB, int FB>
+__device__ __forceinline__ void leave_part(float* part, int rows, const f32x4 (&acc)[TB][FB]) {
   const int lane = lane_here(), g = lane >> 4, c = lane & 15;
 #pragma unroll 1
   for (int t = 0; t < TB; ++t) {
     if (16 * t >= rows) break;
-    f32x4 block[8];
-    block_of<TB>(t, acc, block);
+    f32x4 block[FB];
+    block_of<TB, FB>(t, acc, block);
     // (values and gates: blocks of them in turn)
 #pragma unroll
-    for (int f = 0; f < 8; ++f)
-      *(f32x4*)(part + (16 * t + c) * kTileB + 4 * g + (PAIRS ? (f >> 1) * 16 + (f & 1) * 128 : f * 16)) = block[f];
+    for (int f = 0; f < FB; ++f)
+      *(f32x4*)(part + (16 * t + c) * 32 * FB + 4 * g + (PAIRS ? (f >> 1) * 16 + (f & 1) * 16 * FB : f * 16)) = block[f];
   }
 }
 
-template <bool A_ACROSS, bool B_ACROSS, int MODE, int TB>
+template <bool A_ACROSS, bool B_ACROSS, int MODE, int TB, int FB>
 __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
   constexpr bool kPairs = MODE == kGated;
-  using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB>;
+  constexpr int kColumns = kPairs ? 16 * FB : 32 * FB;   // of out, a tile
+  using W = Walk<A_ACROSS, B_ACROSS, kPairs, TB, FB>;
   __shared__ __attribute__((aligned(1024))) char lds_raw[W::kLds];
   int turn = 0, m_tile = 0, n_tile = 0, first = 0, count = 0, slot = 0;
   // The next tile or part of one; false: none.  (Values chosen, not branches taken: the compiler keeps what either branch writes in memory.)
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
   };
   if (!advance()) return;
   W walk(lds_raw);
-  auto set_out = [&]() __attribute__((always_inline)) { walk.start(m_tile * 32 * TB, n_tile * (kPairs ? kTileB / 2 : kTileB), first, count); };
+  auto set_out = [&]() __attribute__((always_inline)) { walk.start(m_tile * 32 * TB, n_tile * kColumns, first, count); };
   set_out();
   walk.wait_for_first();
   bool landed = false;
@@ -484,10 +494,10 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
   for (;;) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    f32x4 acc[TB][8];
-    const int wave = walk.wave, wm = (wave >> 1) * 16 * TB, wn = (wave & 1) * (kPairs ? 64 : 128);
-    const int m0 = m_tile * 32 * TB + wm, n0 = n_tile * (kPairs ? kTileB / 2 : kTileB) + wn, sum_row = m_tile * 2 + (wave >> 1);
-    constexpr int kPieces = kPairs ? 2 : 4;
+    f32x4 acc[TB][FB];
+    const int wave = walk.wave, wm = (wave >> 1) * 16 * TB, wn = (wave & 1) * (kColumns / 2);
+    const int m0 = m_tile * 32 * TB + wm, n0 = n_tile * kColumns + wn, sum_row = m_tile * 2 + (wave >> 1);
+    constexpr int kPieces = kPairs ? FB / 4 : FB / 2;
     Bias bias[kPieces];                                // (asked for here, it is there when the sums are)
     {
       const ProductParams p = call_again().p;
@@ -497,7 +507,7 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
     }
     walk.run(acc, landed);
     const ProductParams p = call_again().p;
-    float* part = slot < 0 ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * kTileB + wn;
+    float* part = slot < 0 ? nullptr : p.part + ((int64_t)slot * 32 * TB + wm) * 32 * FB + wn;
     const bool filled = p.M > m0;                      // the wave has rows: then at least so many of its stores were issued as results have pieces
     __builtin_amdgcn_s_waitcnt(wait_for(63, 0));
     __builtin_amdgcn_s_barrier();                      // (no wave reads chunks any more)
@@ -506,31 +516,32 @@ __global__ __launch_bounds__(256, 1) void product_kernel(ProductCall) {
     if (more) set_out();                               // (the next tile's first chunks are on their way while this one's results leave)
     const bool whole = !part;
     if (part) {
-      leave_part<kPairs, TB>(part, p.M - m0, acc);
+      leave_part<kPairs, TB, FB>(part, p.M - m0, acc);
     } else if (p.M > m0 || MODE >= kGrad) {
       const ProductParams q = call_again().p;
       with_form<MODE, MODE == kPlain && B_ACROSS>(q, [&](auto act, auto besides) {
-        finish_tile<MODE, decltype(act)::value, decltype(besides)::value, TB>(q, m0, n0, sum_row, bias, acc);
+        finish_tile<MODE, decltype(act)::value, decltype(besides)::value, TB, FB>(q, m0, n0, sum_row, bias, acc);
       });
     }
     if (!more) break;
     // The copies are older than the epilogue's stores, of which there were at least so many, and both complete in their order.
-    constexpr int kStores = TB * (kPairs ? 2 : 4);
+    constexpr int kStores = TB * kPieces;
     if (whole && filled) __builtin_amdgcn_s_waitcnt(wait_for(kStores, 15));
     else __builtin_amdgcn_s_waitcnt(wait_for(0, 15));
     landed = true;
   }
 }
 
-template <int TB>
+template <int TB, int FB>
 hipError_t launch_tiles_of(const ProductParams& p, const ProductPlan& plan, bool a_across, bool b_across, int mode, hipStream_t s) {
   const dim3 grid(plan.share.groups);
-  if (a_across) product_kernel<true, true, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
-  else if (!b_across && mode == kPlain) product_kernel<false, false, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
-  else if (!b_across) product_kernel<false, false, kGated, TB><<<grid, 256, 0, s>>>({p, plan.share});
-  else if (mode == kPlain) product_kernel<false, true, kPlain, TB><<<grid, 256, 0, s>>>({p, plan.share});
-  else if (mode == kGrad) product_kernel<false, true, kGrad, TB><<<grid, 256, 0, s>>>({p, plan.share});
-  else product_kernel<false, true, kGatedGrad, TB><<<grid, 256, 0, s>>>({p, plan.share});
+  if (a_across) {
+    if constexpr (TB % 2 == 0) product_kernel<true, true, kPlain, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
+  } else if (!b_across && mode == kPlain) product_kernel<false, false, kPlain, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (!b_across) product_kernel<false, false, kGated, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (mode == kPlain) product_kernel<false, true, kPlain, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
+  else if (mode == kGrad) product_kernel<false, true, kGrad, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
+  else product_kernel<false, true, kGatedGrad, TB, FB><<<grid, 256, 0, s>>>({p, plan.share});
   return hipGetLastError();
 }
 

@@ -267,11 +267,12 @@ int main() {
     auto log_size = [](int most) { int bits = 1 + rand() % 21; int v = 1 + rand() % (1 << bits); return v < most ? v : most; };
     int M = log_size(60000), N = (log_size(20000) + 7) / 8 * 8, K = log_size(60000), mode = rand() % 4;
     if ((int64_t)M * N > 400000000ll) continue;
-    ProductPlan plan = plan_product(M, N, K, false, mode, mode >= kGrad);
+    ProductPlan plan = plan_product(M, N, K, false, mode, mode >= kGrad, trial % 2);
     const ProductShare& s = plan.share;
-    const int columns = mode == kGated ? 128 : 256, tiles = s.m_tiles * s.n_tiles;
+    const int columns = (mode == kGated ? 16 : 32) * plan.fb, tiles = s.m_tiles * s.n_tiles;
     CHECK(s.groups % 8 == 0 && s.groups * s.rounds + s.rest == tiles && s.rest < s.groups && s.cuts >= 1 && (s.cuts == 1 || s.cuts * 2 <= s.chunks));
     CHECK((int64_t)s.m_tiles * 32 * plan.tb >= M && (int64_t)s.n_tiles * columns >= N && (int64_t)s.chunks * kChunk >= K && (int64_t)(s.chunks - 1) * kChunk < K);
+    CHECK(plan.tb != 3 || trial % 2 == 0);
     CHECK(s.blocks >= 1 && s.blocks <= s.n_tiles);
     std::set<std::pair<int, int>> places;
     for (int i = 0; i < tiles; ++i) {
@@ -301,7 +302,7 @@ int main() {
       CHECK(part_begin(s, 0) == 0 && part_begin(s, s.cuts) == s.chunks);
       for (int part = 0; part < s.cuts; ++part) CHECK(part_begin(s, part + 1) > part_begin(s, part));
     }
-    CHECK(s.cuts == 1 || (size_t)units_of(s) * 32 * plan.tb * kTileB * 4 <= plan.sums_off);
+    CHECK(s.cuts == 1 || (size_t)units_of(s) * 32 * plan.tb * 32 * plan.fb * 4 <= plan.sums_off);
   }
   printf("ok\n");
   return 0;
