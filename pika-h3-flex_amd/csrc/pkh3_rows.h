@@ -72,32 +72,37 @@ constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
 
-// The normal distribution: (1 + erf(v / sqrt 2)) / 2 = erfc(z) / 2 or 1 - erfc(z) / 2, z = |v| / sqrt 2, with erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2).
+// The normal distribution's tail beyond |v|: erfc(z) / 2, z = |v| / sqrt 2, with erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2).
 // p is a polynomial fitted to log(erfc(z) / t) + z^2 at Chebyshev points of t in [1/8, 1] (z up to 14): 8e-7 of the value everywhere, small tails among it.
-__device__ __forceinline__ float normal_cdf(float v) {
-  const float z = fabsf(v) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(1.0f + 0.5f * z);
-  float p = -0.190482009f;
-  p = p * t + 0.762907712f;
-  p = p * t - 1.02066945f;
-  p = p * t + 0.367882395f;
-  p = p * t - 0.0490815249f;
-  p = p * t + 0.396733912f;
-  p = p * t + 0.99815875f;
-  p = p * t - 1.26545055f;
-  const float half = 0.5f * t * exp_of(p - z * z);
-  return v < 0.f ? half : 1.0f - half;
+// (Its coefficients are those times log2(e), with -1 for the half in the last one: an activation's instructions are what a tile's results take besides memory, 256 of
+// them a lane at 4 cycles each and 16 for those of exp2 and the reciprocal.)
+__device__ __forceinline__ float normal_tail(float v) {
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.35355339059327376f * fabsf(v));
+  float p = -0.274807450f;
+  p = p * t + 1.10064317f;
+  p = p * t - 1.47251475f;
+  p = p * t + 0.530742107f;
+  p = p * t - 0.0708096726f;
+  p = p * t + 0.572366047f;
+  p = p * t + 1.44003868f;
+  p = p * t - 2.82565923f;
+  return t * __builtin_amdgcn_exp2f(p - 0.5f * kLog2e * (v * v));
 }
 
 constexpr float kTanhScale = 0.79788456080286536f;   // sqrt(2 / pi)
 constexpr float kTanhCube = 0.044715f;
+// sigmoid(2 u), u = sqrt(2 / pi) (v + 0.044715 v^3)
+__device__ __forceinline__ float tanh_gate(float v) {
+  constexpr float kOnce = -2.0f * kTanhScale * kLog2e, kCubed = kOnce * kTanhCube;
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * (kOnce + kCubed * (v * v))));
+}
 
 // act(v): 0 none, 1 silu, 2 gelu, 3 gelu through tanh (as v sigmoid(2 u), which keeps its small tail exact)
 template <int ACT>
 __device__ __forceinline__ float act_of(float v) {
   if constexpr (ACT == 1) return v * sigmoid_of(v);
-  if constexpr (ACT == 2) return v * normal_cdf(v);
-  if constexpr (ACT == 3) return v * sigmoid_of(2.0f * kTanhScale * v * (1.0f + kTanhCube * v * v));
+  if constexpr (ACT == 2) return fmaxf(v, 0.f) - fabsf(v) * normal_tail(v);
+  if constexpr (ACT == 3) return v * tanh_gate(v);
   return v;
 }
 // act(v) and act'(v)
@@ -108,11 +113,11 @@ __device__ __forceinline__ void act_and_slope(float v, float& value, float& slop
     value = v * q;
     slope = q + value * (1.0f - q);
   } else if constexpr (ACT == 2) {
-    const float q = normal_cdf(v);
+    const float tail = normal_tail(v), q = v < 0.f ? tail : 1.0f - tail;
     value = v * q;
     slope = q + v * 0.39894228040143268f * exp_of(-0.5f * v * v);
   } else if constexpr (ACT == 3) {
-    const float q = sigmoid_of(2.0f * kTanhScale * v * (1.0f + kTanhCube * v * v));
+    const float q = tanh_gate(v);
     value = v * q;
     slope = q + value * (1.0f - q) * (2.0f * kTanhScale) * (1.0f + 3.0f * kTanhCube * fminf(v * v, 1e30f));   // (no 0 times infinity far out)
   } else {
