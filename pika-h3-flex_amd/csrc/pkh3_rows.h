@@ -263,8 +263,13 @@ struct Results {
   __device__ __forceinline__ unsigned at(const RowsOf& m, int row, int n, int size) const {
     return row < rows && n < p.N ? (unsigned)row * m.stride + (unsigned)(n * size) : kNowhere;
   }
+  // The row of the gate that a row takes.
+  __device__ __forceinline__ int gate_row(int row) const {
+    return p.gate_index ? min(max(p.gate_index[first + min(row, rows - 1)], 0), p.gate_rows - 1) : 0;
+  }
+  // gate_of: gate_row(row), where there is a gate
   template <int ACT, int BESIDES>
-  __device__ __forceinline__ void fetch(int row, int n, Extra& e) const {
+  __device__ __forceinline__ void fetch(int row, int n, int gate_of, Extra& e) const {
     if constexpr (MODE == kGrad) {
       if constexpr (ACT != 0) e.z = pre.load_f32(at(pre, row, n, 4));
     } else if constexpr (MODE == kGatedGrad) {
@@ -273,9 +278,7 @@ struct Results {
       e.b = pre.load_f32(where == kNowhere ? where : where + (unsigned)p.N * 4);
     } else {
       if constexpr (BESIDES & kWithGate) {
-        int of = 0;
-        if (p.gate_index) of = min(max(p.gate_index[first + min(row, rows - 1)], 0), p.gate_rows - 1);
-        e.gate = *(const i32x4*)(p.gate + of * p.gate_stride + (int64_t)min(n, p.N - 8) * 2);
+        e.gate = *(const i32x4*)(p.gate + gate_of * p.gate_stride + (int64_t)min(n, p.N - 8) * 2);
       }
       if constexpr (BESIDES & kWithResidual) e.residual = residual.load(at(residual, row, n, 2));
     }

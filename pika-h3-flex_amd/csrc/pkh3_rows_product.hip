@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductParams p, Prod
     for (int r = threadIdx.x >> 3; r < rows; r += 32) {
       if (n >= p.N || r >= res.rows) break;
       typename Results<MODE>::Extra extra;
-      res.template fetch<decltype(act)::value, decltype(besides)::value>(r, n, extra);
+      res.template fetch<decltype(act)::value, decltype(besides)::value>(r, n, decltype(besides)::value & kWithGate ? res.gate_row(r) : 0, extra);
       const Bias bias = load_bias<MODE>(p, n);
       Piece a{}, b{};
       for (int part = 0; part < s.cuts; ++part) {
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void activation_grad_kernel(ProductParams p) {
       Piece a = load_piece(p.a + (first + i) * p.a_stride + (int64_t)n * 2), b{};
       if (p.out) {
         Results<kGrad>::Extra extra;
-        res.fetch<ACT, 0>(i, n, extra);
+        res.fetch<ACT, 0>(i, n, 0, extra);
         res.finish<ACT, 0>(i, n, a, b, Bias{}, extra);
       }
 #pragma unroll

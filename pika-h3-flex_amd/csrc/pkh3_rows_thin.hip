@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * NW) void thin_product_kernel(ProductParams p) 
   if (res.rows <= 0) return;
   with_form<MODE, false>(p, [&](auto act, auto besides) {
     typename Results<MODE>::Extra extra;
-    res.template fetch<decltype(act)::value, decltype(besides)::value>(row, n, extra);
+    res.template fetch<decltype(act)::value, decltype(besides)::value>(row, n, decltype(besides)::value & kWithGate ? res.gate_row(row) : 0, extra);
     res.template finish<decltype(act)::value, decltype(besides)::value>(row, n, a, b, bias, extra);
   });
 }
