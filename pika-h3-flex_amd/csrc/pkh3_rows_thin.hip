@@ -130,7 +130,8 @@ __global__ __launch_bounds__(64 * NW) void thin_product_kernel(ProductParams p) 
   });
 }
 
-// Waves and chunks of a wave in LDS: 64 to 144 KiB a workgroup.  Narrow ones have the CU for themselves and share the contraction out among more waves.
+// Chunks of a wave in LDS: 64 to 144 KiB a workgroup.  Of narrow ones there may be more than CUs, and with up to 80 KiB two of them share one (one row, 2,048 to 6,000, weights out
+// of memory: 10.6 us with eight waves and 128 KiB a workgroup, now 8.0; 24 rows, 2,048 to 5,120 12.7 with 144 KiB, now 10; 48 rows 14.8 with 120, now 12.8).
 template <int MODE, int FB>
 static void launch_rows(const ProductParams& p, hipStream_t s) {
   constexpr int kCols = MODE == kGated || FB == 1 ? 16 : 32;
@@ -140,9 +141,9 @@ static void launch_rows(const ProductParams& p, hipStream_t s) {
     thin_product_kernel<MODE, TM, FB, NW, decltype(depth)::value><<<dim3(columns, (p.M + 16 * TM - 1) / (16 * TM)), 64 * NW, 0, s>>>(p);
   };
   using std::integral_constant;
-  if (p.M <= 16) launch(integral_constant<int, 1>{}, integral_constant<int, FB == 1 ? 8 : 4>{}, integral_constant<int, FB == 1 ? 4 : 3>{});
-  else if (p.M <= 32) launch(integral_constant<int, 2>{}, integral_constant<int, FB == 1 ? 8 : 4>{}, integral_constant<int, 3>{});
-  else launch(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
+  if (p.M <= 16) launch(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<int, FB == 1 ? 4 : 3>{});
+  else if (p.M <= 32) launch(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
+  else launch(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, FB == 1 ? 2 : 3>{});
 }
 
 hipError_t launch_thin(const ProductParams& p, int mode, hipStream_t s) {
