@@ -7,22 +7,24 @@
 // different rows (16 rows, 4,096 x 12,288: 34 us that way).
 //
 // Bound by the weights: one row, 2,048 to 8,192, weights out of memory 8.4 us (4 TB/s, 2 us of them the launch) and 4.9 out of L2; 64 rows 12.2; 200 rows, 8,192 to 2,048 25 us, where
-// tiles take 26.  With more than 256 workgroups of a long contraction the last ones run by themselves (10 rows, 4,368 to 8,960, 280 of them: 28 us, tiles 26).
+// tiles take 26.  Where there are some more than 256 workgroups, a few CUs have two (10 rows, 4,368 to 8,960, 280 of them: 28 us, tiles 26).
 #include "pkh3_rows.h"
 
 namespace pkh3 {
 
-template <int MODE, int TM, int FB, int NW, int DEPTH>
-__global__ __launch_bounds__(64 * NW) void thin_product_kernel(ProductParams p) {
+constexpr int kThinWaves = 4;
+
+template <int MODE, int TM, int FB, int DEPTH>
+__global__ __launch_bounds__(64 * kThinWaves) void thin_product_kernel(ProductParams p) {
   constexpr bool kPairs = MODE == kGated;
   static_assert(!kPairs || FB == 2, "values and gates");
   constexpr int kCols = kPairs || FB == 1 ? 16 : 32, kBlocks = FB + TM, kSlot = kBlocks * 2048;
   static_assert(TM * FB * 1024 <= DEPTH * kSlot, "the sums go through the chunks' places");
-  __shared__ __attribute__((aligned(1024))) char lds_raw[NW * DEPTH * kSlot];
+  __shared__ __attribute__((aligned(1024))) char lds_raw[kThinWaves * DEPTH * kSlot];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n0 = blockIdx.x * kCols, m0 = blockIdx.y * 16 * TM;
-  const int chunks = (p.K + kChunk - 1) / kChunk, first = chunks * wave / NW, count = chunks * (wave + 1) / NW - first;
+  const int chunks = (p.K + kChunk - 1) / kChunk, first = chunks * wave / kThinWaves, count = chunks * (wave + 1) / kThinWaves - first;
   const int left = p.K - (chunks - 1) * kChunk;        // contraction elements of the last chunk
   f32x4 acc[TM][FB];
 #pragma unroll
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(64 * NW) void thin_product_kernel(ProductParams p) 
 #pragma unroll
   for (int f = 0; f < FB; ++f) {
     sum[f] = *at(0, wave * FB + f);
-    for (int i = 1; i < NW; ++i) sum[f] += *at(i, wave * FB + f);
+    for (int i = 1; i < kThinWaves; ++i) sum[f] += *at(i, wave * FB + f);
   }
   const Results<MODE> res(p, m0 + 16 * wave);
   // eight columns beside each other: out of two blocks, or of one, then in every other group of lanes
@@ -136,14 +138,14 @@ template <int MODE, int FB>
 static void launch_rows(const ProductParams& p, hipStream_t s) {
   constexpr int kCols = MODE == kGated || FB == 1 ? 16 : 32;
   const int columns = (p.N + kCols - 1) / kCols;
-  auto launch = [&](auto tm, auto nw, auto depth) {
-    constexpr int TM = decltype(tm)::value, NW = decltype(nw)::value;
-    thin_product_kernel<MODE, TM, FB, NW, decltype(depth)::value><<<dim3(columns, (p.M + 16 * TM - 1) / (16 * TM)), 64 * NW, 0, s>>>(p);
+  auto launch = [&](auto tm, auto depth) {
+    constexpr int TM = decltype(tm)::value;
+    thin_product_kernel<MODE, TM, FB, decltype(depth)::value><<<dim3(columns, (p.M + 16 * TM - 1) / (16 * TM)), 64 * kThinWaves, 0, s>>>(p);
   };
   using std::integral_constant;
-  if (p.M <= 16) launch(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<int, FB == 1 ? 4 : 3>{});
-  else if (p.M <= 32) launch(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 3>{});
-  else launch(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, FB == 1 ? 2 : 3>{});
+  if (p.M <= 16) launch(integral_constant<int, 1>{}, integral_constant<int, FB == 1 ? 4 : 3>{});
+  else if (p.M <= 32) launch(integral_constant<int, 2>{}, integral_constant<int, 3>{});
+  else launch(integral_constant<int, 4>{}, integral_constant<int, FB == 1 ? 2 : 3>{});
 }
 
 hipError_t launch_thin(const ProductParams& p, int mode, hipStream_t s) {
