@@ -68,6 +68,7 @@ size_t pkh3_norm_workspace_bytes(const pkh3_norm_args* args);
  * Offered are A and B along (plain, GATED), A along and B across (plain without anything besides, GRAD, GRAD and GATED), and both
  * across (plain without anything besides); of others PKH3_EUNSUPPORTED.  With GRAD, `sums`, if given, gets the sums of out's columns before they were rounded (bfloat16, N or 2 N entries). */
 
+/* Activations.  Of an infinite sum they are what the formulas give: +inf of +inf, NaN (infinity times zero) of -inf, and slopes of NaN. */
 enum {
   PKH3_ACT_NONE = 0,
   PKH3_ACT_SILU = 1,            /* v / (1 + exp(-v)) */

@@ -97,11 +97,12 @@ __device__ __forceinline__ float tanh_gate(float v) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * (kOnce + kCubed * (v * v))));
 }
 
-// act(v): 0 none, 1 silu, 2 gelu, 3 gelu through tanh (as v sigmoid(2 u), which keeps its small tail exact)
+// act(v): 0 none, 1 silu, 2 gelu, 3 gelu through tanh (as v sigmoid(2 u), which keeps its small tail exact).  Of infinities what the formulas give: +inf for +inf, and for
+// -inf their infinity times zero, NaN.
 template <int ACT>
 __device__ __forceinline__ float act_of(float v) {
   if constexpr (ACT == 1) return v * sigmoid_of(v);
-  if constexpr (ACT == 2) return fmaxf(v, 0.f) - fabsf(v) * normal_tail(v);
+  if constexpr (ACT == 2) return fmaxf(v, 0.f) - fabsf(fminf(v, 1e30f)) * normal_tail(v);   // (+inf: not infinity times its tail of 0)
   if constexpr (ACT == 3) return v * tanh_gate(v);
   return v;
 }

@@ -1,0 +1,41 @@
+"""Calls of the feed-forward half that its own documents allow and that went wrong once: see each test."""
+import math
+
+import pytest
+import torch
+
+import pika_h3_flex_amd as pk
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+INF, NAN = math.inf, math.nan
+
+
+def _same(got, want):
+    got, want = got.float().cpu(), torch.as_tensor(want, dtype=torch.float32)
+    return torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0, INF, -INF), want.nan_to_num(0.0, INF, -INF))
+
+
+@pytest.mark.parametrize("rows", [1, 40, 700])
+def test_activations_of_infinities(rows):
+    """An infinite sum: the activation of +inf is +inf; that of -inf is -inf * 0, NaN, and so is NaN's, as the formulas have it.  700 rows by 4,104 columns take tiles."""
+    N = 4104 if rows == 700 else 16
+    eye = torch.eye(8, device=DEV, dtype=BF16)
+    w = torch.cat([eye] * (N // 8))                       # out[:, n] = x[:, n % 8], as far as that is finite: one value a row besides zeros
+    for value, want in ((INF, INF), (-INF, NAN), (NAN, NAN)):
+        x = torch.full((rows, 8), 0.0, device=DEV, dtype=BF16)
+        bias = torch.zeros(N, device=DEV)
+        bias[3] = value
+        for name in ("silu", "gelu", "gelu_tanh"):
+            y = pk.linear(x, w, bias, activation=name)
+            assert _same(y[:, 3], [want] * rows), (name, value, y[0, 3])
+            others = torch.arange(N, device=DEV) != 3
+            assert torch.count_nonzero(y[:, others]) == 0, name
+            # gated: 2 * act(value)
+            both = torch.cat([torch.full((N,), 2.0, device=DEV), bias])
+            _, saved = pk.feed_forward(x, torch.cat([w, w]), torch.zeros(8, N, device=DEV, dtype=BF16), both, activation=name, save=True)
+            assert _same(saved.hidden[:, 3], [want] * rows), (name, value, saved.hidden[0, 3])
+            # the pass back: slopes of an infinite sum are the formulas' 0 times infinity
+            _, _, db = pk.linear_backward(torch.ones(rows, 8, device=DEV, dtype=BF16), x, eye, bias[:8].expand(rows, 8).contiguous(), activation=name)
+            assert db[[0, 1, 2, 4, 5, 6, 7]].isfinite().all() and db[3].isnan(), (name, value)
