@@ -102,6 +102,13 @@ def _wants_grad(x, *tensors) -> bool:
     return True
 
 
+def _written(out: torch.Tensor) -> torch.Tensor:
+    """A caller's ``out`` after the launch that fills it.  The kernels know addresses only; torch's version counter tells whoever holds the tensor's earlier contents (a recorded
+    call that saved it, a cache that goes by it) that they are gone."""
+    torch.autograd.graph.increment_version(out)
+    return out
+
+
 def _scratch_bytes(entry: str, args) -> int:
     lib = _lib.load()
     n = int(getattr(lib, entry)(C.byref(args)))
@@ -152,11 +159,12 @@ def _layer_norm(x, weight, bias, row_index, eps, out=None):
     x_at, x_row = _matrix("x", x, -1, -1, index, x.dtype)
     rows, width = x.shape
     w, b, where, tables, tables_type = _norm_tables(weight, bias, row_index, rows, width, index)
+    given = out
     if out is None:
         out = torch.empty(rows, width, dtype=x.dtype, device=x.device)
     o_at, o_row = _matrix("out", out, rows, width, index, x.dtype)
     _call("pkh3_layer_norm", _pack_norm(x_at, w, b, where, o_at, 0, 0, 0, 0, 0, 0, x_row, o_row, 0, 0, rows, width, tables, eps, flags | tables_type), index)
-    return out
+    return out if given is None else _written(out)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
@@ -164,7 +172,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - mean) / sqrt(var + eps) * weight + bias`` for the rows of ``x``, bfloat16 or float32 ``[rows, width]``, as ``x``'s type.  ``weight`` and
     ``bias``: float32 or bfloat16 ``[width]``, or ``[tables, width]`` with ``row_index`` int32 ``[rows]`` saying which table row a row takes (values are
     brought into range); a modulation ``norm(x) * (1 + scale) + shift`` is the tables ``1 + scale`` and ``shift``.  Width up to 16,384.  ``out`` may be ``x``."""
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(x, weight, bias, out):
         if out is not None:
             raise ValueError("out cannot be given where gradients are recorded")
         for t in (weight, bias):
@@ -248,6 +256,7 @@ def _linear(x, weight, bias, activation, gate, row_index, residual, out, save):
         bias_at, narrow = _vector("bias", bias, N, index)
         flags = _lib.PRODUCT_BIAS_BF16 if narrow else 0
     g, r = _finish(gate, row_index, residual, rows, N, index)
+    given = out
     if out is None:
         out = torch.empty(rows, N, dtype=_BF16, device=x.device)
     o = _matrix("out", out, rows, N, index)
@@ -256,7 +265,7 @@ def _linear(x, weight, bias, activation, gate, row_index, residual, out, save):
         pre = torch.empty(rows, N, dtype=_F32, device=x.device)
         p = (pre.data_ptr(), N)
     _product(a, b, o, rows, N, K, flags, index, bias=bias_at, gate=g, residual=r, pre=p, act=act)
-    return out, pre
+    return out if given is None else _written(out), pre
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "none", gate: Optional[torch.Tensor] = None,
@@ -265,7 +274,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     ``torch.nn.Linear`` has it, ``bias`` float32 or bfloat16, ``activation`` one of :data:`ACTIVATIONS`, ``gate`` bfloat16 ``[table rows, N]`` with
     ``row_index`` int32 ``[rows]`` (as :func:`.projections.out_proj` takes them), ``residual`` bfloat16 ``[rows, N]``; ``out`` may be ``residual``.
     ``save``: also returns what :func:`linear_backward` takes as ``pre`` (``x weight^T + bias`` in float32; None without an activation)."""
-    if _wants_grad(x, weight, bias, gate, residual):
+    if _wants_grad(x, weight, bias, gate, residual, out):
         if out is not None or save or gate is not None:
             raise ValueError("out, save and gate cannot be given where gradients are recorded")
         return _Linear.apply(x, weight, bias, residual, activation)
@@ -375,6 +384,7 @@ def _feed_forward(x, w_in, w_out, b_in, b_out, activation, gated, gate, row_inde
         b2, narrow = _vector("b_out", b_out, N, index)
         f2 |= _lib.PRODUCT_BIAS_BF16 if narrow else 0
     g, r = _finish(gate, row_index, residual, rows, N, index)
+    given = out
     if out is None:
         out = torch.empty(rows, N, dtype=_BF16, device=x.device)
     o = _matrix("out", out, rows, N, index)
@@ -386,7 +396,7 @@ def _feed_forward(x, w_in, w_out, b_in, b_out, activation, gated, gate, row_inde
         p = (pre.data_ptr(), first)
     _product(a, w1, h, rows, inner, K, f1, index, bias=b1, pre=p, act=act)
     _product(h, w2, o, rows, N, inner, f2, index, bias=b2, gate=g, residual=r)
-    return out, Saved(pre, hidden) if save else None
+    return out if given is None else _written(out), Saved(pre, hidden) if save else None
 
 
 def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None, b_out: Optional[torch.Tensor] = None, *,
@@ -395,7 +405,7 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in:
     """``residual + gate[row_index] * (h w_out^T + b_out)`` with ``h = act(x w_in^T + b_in)``, or, ``gated``, ``h = a * act(b)`` where the first half of
     ``w_in``'s rows (and of ``b_in``) makes a and the second b.  ``x`` bfloat16 ``[rows, width]``, ``w_in`` ``[inner or 2 inner, width]``, ``w_out``
     ``[outputs, inner]``; the rest as :func:`linear` takes it.  h is rounded to bfloat16 between the products.  ``save``: also returns :class:`Saved`."""
-    if _wants_grad(x, w_in, w_out, b_in, b_out, gate, residual):
+    if _wants_grad(x, w_in, w_out, b_in, b_out, gate, residual, out):
         if out is not None or save or gate is not None:
             raise ValueError("out, save and gate cannot be given where gradients are recorded")
         return _FeedForward.apply(x, w_in, w_out, b_in, b_out, residual, activation, gated)

@@ -39,3 +39,18 @@ def test_activations_of_infinities(rows):
             # the pass back: slopes of an infinite sum are the formulas' 0 times infinity
             _, _, db = pk.linear_backward(torch.ones(rows, 8, device=DEV, dtype=BF16), x, eye, bias[:8].expand(rows, 8).contiguous(), activation=name)
             assert db[[0, 1, 2, 4, 5, 6, 7]].isfinite().all() and db[3].isnan(), (name, value)
+
+
+def test_a_saved_tensor_that_a_call_overwrote_is_noticed():
+    """A recorded call saves its input; one that writes in place over that input afterwards has torch refuse the stale backward pass."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    make = lambda *s: torch.randn(s, generator=gen, device=DEV).to(BF16)  # noqa: E731
+    w = make(64, 64).requires_grad_()
+    for overwrite in (lambda x: pk.layer_norm(x, out=x), lambda x: pk.linear(make(16, 64), w, residual=x, out=x),
+                      lambda x: pk.feed_forward(make(16, 64), w, w, gated=False, residual=x, out=x)):
+        x = make(16, 64)
+        y = pk.linear(x, w)
+        with torch.no_grad():
+            overwrite(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()

@@ -1,0 +1,57 @@
+"""What the front end of the feed-forward half does around its launches, with the launches left out: tensors of host memory, entries written down in place of being called."""
+import pytest
+import torch
+
+import pika_h3_flex_amd as pk
+from pika_h3_flex_amd import rows as front
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture
+def entries(monkeypatch):
+    """Names of the C entries that calls come to."""
+    names = []
+    monkeypatch.setattr(front, "_place", lambda x: -1)
+    monkeypatch.setattr(front, "_call", lambda name, args, index: names.append(name))
+    return names
+
+
+def _parts(rows=4, width=64, inner=32):
+    x, w_in, w_out = torch.ones(rows, width, dtype=BF16), torch.ones(inner, width, dtype=BF16), torch.ones(width, inner, dtype=BF16)
+    return x, w_in, w_out
+
+
+def _calls(x, w_in, w_out):
+    """The three calls with an ``out`` of their own shape."""
+    return ((x.shape, lambda out: pk.layer_norm(x, out=out)), ((x.shape[0], w_in.shape[0]), lambda out: pk.linear(x, w_in, out=out)),
+            (x.shape, lambda out: pk.feed_forward(x, w_in, w_out, gated=False, out=out)))
+
+
+def test_what_a_call_overwrites_has_another_version(entries):
+    x, w_in, w_out = _parts()
+    for shape, call in _calls(x, w_in, w_out):
+        out = torch.zeros(shape, dtype=BF16)
+        before = out._version
+        assert call(out) is out and out._version > before
+    residual, before = torch.zeros(4, 32, dtype=BF16), x._version
+    pk.linear(x, w_in, residual=residual, out=residual)
+    assert residual._version > 0 and x._version == before
+    buffer = torch.zeros(4, 128, dtype=BF16)                     # a slice shares the counter of its buffer
+    pk.layer_norm(x, out=buffer[:, 64:])
+    assert buffer._version > 0
+    before = x._version
+    pk.layer_norm(x, out=x)
+    assert x._version > before
+
+
+def test_an_output_that_is_differentiated_is_refused(entries):
+    x, w_in, w_out = _parts()
+    for shape, call in _calls(x, w_in, w_out):
+        out = torch.zeros(shape, dtype=BF16, requires_grad=True)
+        with pytest.raises(ValueError, match="out"):
+            call(out)
+        assert not entries
+        with torch.no_grad():
+            call(out)
+        entries.clear()
