@@ -6,7 +6,7 @@ The layers are the reference's ``ff.net.0.proj`` and ``ff.net.2`` (src/pika_h3/c
 rows (patches/0001-h3-adaln-fp32.patch:34-40).
 
 Rows are ``[rows, width]`` with unit column stride, other strides and widths multiples of 8 elements, 16-byte aligned.  Where gradients are recorded and an
-input needs them, the three calls take part in torch's differentiation (not while a stream is captured); the ``*_backward`` functions are the same passes by
+input needs them, the three calls take part in torch's differentiation (backwards; not while a stream is captured); the ``*_backward`` functions are the same passes by
 themselves, which a graph may hold.
 """
 from __future__ import annotations
@@ -16,6 +16,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from .ops import _raw_stream
@@ -92,9 +93,16 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
+def _refuse_tangents(*tensors) -> None:
+    """The passes carry no tangents of forward-mode differentiation (inside a dual level a tensor may have one): raises where one would be lost."""
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("forward-mode tangents are not carried through these calls")
+
+
 def _wants_grad(x, *tensors) -> bool:
     """Whether a call is recorded for torch's differentiation.  Not while a stream is captured: the nodes that add up the leaves' gradients may live already, with the
     stream of an eager pass, and running them on it inside a capture ends the process."""
+    _refuse_tangents(x, *tensors)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, *tensors)):
         return False
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
@@ -186,6 +194,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
                         row_index: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """The backward pass of :func:`layer_norm` from the gradient ``dy`` of its result and the arguments of the call: ``(dx, dweight, dbias)``, ``dx`` as
     ``x``, the others float32 in the shape of ``weight`` and ``bias`` (None where these are).  Up to 64 table rows."""
+    _refuse_tangents(dy, x, weight, bias)
     index = _place(x)
     flags = _rows_type(x)
     x_at, x_row = _matrix("x", x, -1, -1, index, x.dtype)
@@ -318,6 +327,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
                     x_grad: bool = True, weight_grad: bool = True, bias_grad: bool = True):
     """``(dx, dweight, dbias)`` of ``act(x weight^T + bias)`` from the gradient ``dy`` of that (a residual's gradient is ``dy`` itself; that of a gated result
     is multiplied by the gate first), bfloat16 all; None for what is not asked for.  ``pre``: what :func:`linear` returned with ``save``."""
+    _refuse_tangents(dy, x, weight, pre)
     index = _place(x)
     act = _activation(activation)
     xa = _matrix("x", x, -1, -1, index)
@@ -417,6 +427,7 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor,
                           gated: bool = True, x_grad: bool = True, weight_grad: bool = True, bias_grad: bool = True):
     """``(dx, dw_in, dw_out, db_in, db_out)`` of :func:`feed_forward` without its gate and residual (see :func:`linear_backward`), bfloat16; None for what is not
     asked for."""
+    _refuse_tangents(dy, x, w_in, w_out, saved.pre, saved.hidden)
     index = _place(x)
     act = _activation(activation)
     a, w1, w2, rows, K, inner, first, N = _block(x, w_in, w_out, gated, index)

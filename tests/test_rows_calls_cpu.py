@@ -55,3 +55,28 @@ def test_an_output_that_is_differentiated_is_refused(entries):
         with torch.no_grad():
             call(out)
         entries.clear()
+
+
+def test_forward_mode_tangents_are_refused(entries):
+    """A dual tensor does not require gradients: its tangent would be lost without a word."""
+    x, w_in, w_out = _parts()
+    fw = torch.autograd.forward_ad
+    dy, hidden = torch.ones(4, 64, dtype=BF16), torch.ones(4, 32, dtype=BF16)
+    saved = front.Saved(torch.ones(4, 32), hidden)
+    weight = torch.ones(64, dtype=BF16)
+    calls = [lambda a, w: pk.layer_norm(a, weight), lambda a, w: pk.linear(a, w), lambda a, w: pk.feed_forward(a, w, w_out, gated=False),
+             lambda a, w: pk.linear(hidden, w_out, residual=a), lambda a, w: pk.layer_norm_backward(dy, a, weight), lambda a, w: pk.layer_norm_backward(a, dy, weight),
+             lambda a, w: pk.linear_backward(hidden, a, w), lambda a, w: pk.feed_forward_backward(a, dy, w, w_out, saved, gated=False)]
+    with fw.dual_level():
+        dual, dual_w = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(w_in, torch.ones_like(w_in))
+        for i, call in enumerate(calls):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual, w_in)
+        for call in (calls[1], calls[2], calls[6], calls[7]):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(x, dual_w)
+        assert not entries
+        assert calls[1](x, w_in).shape == (4, 32)                # (without tangents a level changes nothing)
+    with pytest.raises(RuntimeError):                            # torch.func's tensors have no address, or a tangent
+        torch.func.jvp(lambda a: pk.linear(a, w_in), (x,), (torch.ones_like(x),))
