@@ -243,6 +243,8 @@ def _finish(gate, row_index, residual, rows: int, N: int, index: int):
     g, r = (0, 0, 0, 0), (0, 0)
     if gate is not None:
         at, stride = _matrix("gate", gate, -1, N, index)
+        if gate.shape[0] < 1:                             # (without rows it has no address either, and would be taken for none)
+            raise ValueError("gate must have a row")
         if gate.shape[0] > 1 and row_index is None:
             raise ValueError(f"{gate.shape[0]} gate rows need a row_index")
         g = (at, 0 if row_index is None else _index("row_index", row_index, rows, index), stride, gate.shape[0])

@@ -80,3 +80,14 @@ def test_forward_mode_tangents_are_refused(entries):
         assert calls[1](x, w_in).shape == (4, 32)                # (without tangents a level changes nothing)
     with pytest.raises(RuntimeError):                            # torch.func's tensors have no address, or a tangent
         torch.func.jvp(lambda a: pk.linear(a, w_in), (x,), (torch.ones_like(x),))
+
+
+def test_a_gate_without_rows_is_refused(entries):
+    """Its address is NULL, which the entry takes for no gate."""
+    x, w_in, w_out = _parts()
+    index = torch.zeros(4, dtype=torch.int32)
+    for call in (lambda g: pk.linear(x, w_in, gate=g, row_index=index), lambda g: pk.linear(x, w_in, gate=g),
+                 lambda g: pk.feed_forward(x, w_in, w_out, gated=False, gate=torch.zeros(g.shape[0], 64, dtype=BF16), row_index=index)):
+        with pytest.raises(ValueError, match="gate"):
+            call(torch.zeros(0, 32, dtype=BF16))
+        call(torch.zeros(1, 32, dtype=BF16))
