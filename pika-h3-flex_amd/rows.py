@@ -286,8 +286,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     ``row_index`` int32 ``[rows]`` (as :func:`.projections.out_proj` takes them), ``residual`` bfloat16 ``[rows, N]``; ``out`` may be ``residual``.
     ``save``: also returns what :func:`linear_backward` takes as ``pre`` (``x weight^T + bias`` in float32; None without an activation)."""
     if _wants_grad(x, weight, bias, gate, residual, out):
-        if out is not None or save or gate is not None:
-            raise ValueError("out, save and gate cannot be given where gradients are recorded")
+        if out is not None or save or gate is not None or row_index is not None:
+            raise ValueError("out, save and gate (and its row_index) cannot be given where gradients are recorded")
         return _Linear.apply(x, weight, bias, residual, activation)
     y, pre = _linear(x, weight, bias, activation, gate, row_index, residual, out, save)
     return (y, pre) if save else y
@@ -418,8 +418,8 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in:
     ``w_in``'s rows (and of ``b_in``) makes a and the second b.  ``x`` bfloat16 ``[rows, width]``, ``w_in`` ``[inner or 2 inner, width]``, ``w_out``
     ``[outputs, inner]``; the rest as :func:`linear` takes it.  h is rounded to bfloat16 between the products.  ``save``: also returns :class:`Saved`."""
     if _wants_grad(x, w_in, w_out, b_in, b_out, gate, residual, out):
-        if out is not None or save or gate is not None:
-            raise ValueError("out, save and gate cannot be given where gradients are recorded")
+        if out is not None or save or gate is not None or row_index is not None:
+            raise ValueError("out, save and gate (and its row_index) cannot be given where gradients are recorded")
         return _FeedForward.apply(x, w_in, w_out, b_in, b_out, residual, activation, gated)
     y, saved = _feed_forward(x, w_in, w_out, b_in, b_out, activation, gated, gate, row_index, residual, out, save)
     return (y, saved) if save else y

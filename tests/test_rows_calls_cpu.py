@@ -91,3 +91,14 @@ def test_a_gate_without_rows_is_refused(entries):
         with pytest.raises(ValueError, match="gate"):
             call(torch.zeros(0, 32, dtype=BF16))
         call(torch.zeros(1, 32, dtype=BF16))
+
+
+def test_a_row_index_without_a_gate_is_refused_where_gradients_are_recorded(entries):
+    """As it is where they are not."""
+    x, w_in, w_out = _parts()
+    index = torch.zeros(4, dtype=torch.int32)
+    for w in (w_in, w_in.clone().requires_grad_()):
+        for call in (lambda: pk.linear(x, w, row_index=index), lambda: pk.feed_forward(x, w, w_out, gated=False, row_index=index)):
+            with pytest.raises(ValueError, match="row_index"):
+                call()
+    assert not entries
