@@ -28,7 +28,7 @@ extern "C" {
 #define PKH3_LAYER_NORM_F32 1u        /* x, out, dy and dx are float32, else bfloat16 */
 #define PKH3_LAYER_NORM_TABLES_BF16 2u /* weight and bias are bfloat16, else float32 */
 #define PKH3_LAYER_NORM_MAX_WIDTH 16384
-#define PKH3_LAYER_NORM_MAX_TABLES 64 /* of the backward pass */
+#define PKH3_LAYER_NORM_MAX_TABLES 64 /* with dweight or dbias; else 65,535 */
 
 typedef struct pkh3_norm_args {
   const void* x;                /* [rows, width] */

@@ -72,18 +72,19 @@ int check_workspace(const void* at, uint64_t have, size_t need) {
 
 // ---- layer norm ----
 
-int check_norm_sizes(const pkh3_norm_args* a, bool backward) {
+// sums: the tables' gradients are asked for
+int check_norm_sizes(const pkh3_norm_args* a, bool sums) {
   if (!a) return fail(PKH3_ENULL, "args is NULL");
   if (a->flags & ~(PKH3_LAYER_NORM_F32 | PKH3_LAYER_NORM_TABLES_BF16)) return fail(PKH3_EARG, "unknown flag bits 0x%x", a->flags);
   if (a->rows < 0 || a->rows > kMostRows) return fail(PKH3_ESHAPE, "rows must be in [0, 2^21], got %d", a->rows);
   if (a->width < 8 || a->width > PKH3_LAYER_NORM_MAX_WIDTH || a->width % 8) return fail(PKH3_ESHAPE, "width must be a multiple of 8 in [8, %d], got %d", PKH3_LAYER_NORM_MAX_WIDTH, a->width);
-  const int most = backward ? PKH3_LAYER_NORM_MAX_TABLES : 65535;
+  const int most = sums ? PKH3_LAYER_NORM_MAX_TABLES : 65535;
   if (a->tables < 1 || a->tables > most) return fail(PKH3_ESHAPE, "tables must be in [1, %d], got %d", most, a->tables);
   return PKH3_OK;
 }
 
 int check_norm(const pkh3_norm_args* a, bool backward) {
-  int rc = check_norm_sizes(a, backward);
+  int rc = check_norm_sizes(a, backward && a && (a->dweight || a->dbias));
   if (rc) return rc;
   if (!(a->eps >= 0.f) || a->eps > 3e38f) return fail(PKH3_EARG, "eps must be finite and >= 0");
   const int size = a->flags & PKH3_LAYER_NORM_F32 ? 4 : 2, tsize = a->flags & PKH3_LAYER_NORM_TABLES_BF16 ? 2 : 4;

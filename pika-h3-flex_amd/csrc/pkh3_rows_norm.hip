@@ -329,7 +329,7 @@ hipError_t launch_norm(NormParams p, bool f32, bool tables_bf16, hipStream_t s) 
   return hipGetLastError();
 }
 
-// A workgroup for 8 rows up to 512 of them, for 32 up to 1,024 (their slices are then a sixth of what the rows move); with many tables fewer, so that the slices stay small.
+// A workgroup for 8 rows up to 512 of them, for 32 up to 1,024 (their slices are then a sixth of what the rows move); with many tables (up to 64 where there are sums) fewer, so that the slices stay small.
 int norm_groups(int rows, int tables) {
   const int by_8 = (rows + 7) / 8 < 512 ? (rows + 7) / 8 : 512, by_32 = (rows + 31) / 32 < 1024 ? (rows + 31) / 32 : 1024;
   const int groups = by_8 > by_32 ? by_8 : by_32, most = 8192 / tables;
@@ -360,7 +360,7 @@ static void with_backward_form(bool f32, bool tb16, int width, F&& f) {
 
 hipError_t launch_norm_backward(NormParams p, bool f32, bool tables_bf16, char* workspace, hipStream_t s) {
   const bool sums = p.dweight || p.dbias;
-  p.groups = norm_groups(p.rows, p.tables);
+  p.groups = norm_groups(p.rows, sums ? p.tables : 1);
   p.touched = sums ? (uint64_t*)workspace : nullptr;
   p.part = sums ? (float*)(workspace + touched_bytes(p.groups)) : nullptr;
   with_backward_form(f32, tables_bf16, p.width, [&](auto a, auto b, auto lanes, auto np) {

@@ -184,16 +184,16 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         if out is not None:
             raise ValueError("out cannot be given where gradients are recorded")
         for t in (weight, bias):
-            if t is not None and t.dim() == 2 and t.shape[0] > _lib.LAYER_NORM_MAX_TABLES:
+            if t is not None and t.requires_grad and t.dim() == 2 and t.shape[0] > _lib.LAYER_NORM_MAX_TABLES:
                 raise ValueError(f"gradients of at most {_lib.LAYER_NORM_MAX_TABLES} table rows, got {t.shape[0]}")
         return _LayerNorm.apply(x, weight, bias, row_index, eps)
     return _layer_norm(x, weight, bias, row_index, eps, out)
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
-                        row_index: Optional[torch.Tensor] = None, eps: float = 1e-6):
+                        row_index: Optional[torch.Tensor] = None, eps: float = 1e-6, weight_grad: bool = True, bias_grad: bool = True):
     """The backward pass of :func:`layer_norm` from the gradient ``dy`` of its result and the arguments of the call: ``(dx, dweight, dbias)``, ``dx`` as
-    ``x``, the others float32 in the shape of ``weight`` and ``bias`` (None where these are).  Up to 64 table rows."""
+    ``x``, the others float32 in the shape of ``weight`` and ``bias`` (None where these are, or are not asked for).  Tables that gradients are asked of have up to 64 rows."""
     _refuse_tangents(dy, x, weight, bias)
     index = _place(x)
     flags = _rows_type(x)
@@ -203,8 +203,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     w, b, where, tables, tables_type = _norm_tables(weight, bias, row_index, rows, width, index)
     dx = torch.empty(rows, width, dtype=x.dtype, device=x.device)
     make = torch.empty if rows else torch.zeros
-    dw = None if weight is None else make(weight.shape, dtype=_F32, device=x.device)
-    db = None if bias is None else make(bias.shape, dtype=_F32, device=x.device)
+    dw = make(weight.shape, dtype=_F32, device=x.device) if weight is not None and weight_grad else None
+    db = make(bias.shape, dtype=_F32, device=x.device) if bias is not None and bias_grad else None
     if not rows:
         return dx, dw, db
     scratch, need = None, 0
@@ -478,8 +478,8 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, row_index = ctx.saved_tensors
-        dx, dw, db = layer_norm_backward(_usable(dy, x.dtype), x, weight, bias, row_index=row_index, eps=ctx.eps)
         need = ctx.needs_input_grad
+        dx, dw, db = layer_norm_backward(_usable(dy, x.dtype), x, weight, bias, row_index=row_index, eps=ctx.eps, weight_grad=need[1], bias_grad=need[2])
         return dx if need[0] else None, _as(dw, weight, need[1]), _as(db, bias, need[2]), None, None
 
 

@@ -5,6 +5,8 @@ import pytest
 import torch
 
 import pika_h3_flex_amd as pk
+from oracle import rows_oracle as O
+from tests.test_gpu_rows import _norm_grad_bounds, _norm_inputs, _within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -54,3 +56,20 @@ def test_a_saved_tensor_that_a_call_overwrote_is_noticed():
             overwrite(x)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+@pytest.mark.parametrize("rows,width,tables", [(5, 64, 65), (3000, 264, 1000), (40, 2056, 8193)])
+def test_gradients_of_rows_under_many_frozen_tables(rows, width, tables):
+    x, w, b, index, dy = _norm_inputs(rows, width, BF16, tables, F32, rows)
+    leaf = x.clone().requires_grad_()
+    pk.layer_norm(leaf, w, b, row_index=index, eps=1e-5).backward(dy)
+    want = O.layer_norm_backward(dy, x, w, b, index, 1e-5)
+    _within(leaf.grad, (want[0], _norm_grad_bounds(dy, x, w, index, want, 1e-5)[0]), "dx")
+    # with the tables' gradients, or one of them, dx has the same bits
+    few = index % 64
+    both = pk.layer_norm_backward(dy, x, w[:64], b[:64], row_index=few)
+    for weight_grad, bias_grad in ((False, False), (True, False), (False, True)):
+        got = pk.layer_norm_backward(dy, x, w[:64], b[:64], row_index=few, weight_grad=weight_grad, bias_grad=bias_grad)
+        assert torch.equal(got[0], both[0])
+        for part, whole, asked in zip(got[1:], both[1:], (weight_grad, bias_grad)):
+            assert torch.equal(part, whole) if asked else part is None

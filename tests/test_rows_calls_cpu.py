@@ -102,3 +102,27 @@ def test_a_row_index_without_a_gate_is_refused_where_gradients_are_recorded(entr
             with pytest.raises(ValueError, match="row_index"):
                 call()
     assert not entries
+
+
+def test_frozen_tables(lib, entries, monkeypatch):
+    """Only the tables' own gradients are bound to 64 rows, and they are formed where they are asked for alone."""
+    calls = []
+    monkeypatch.setattr(front, "_call", lambda name, args, index: calls.append((name, front._lib.NORM_ARGS_FORMAT.unpack(args))))
+    x = torch.ones(4, 64, dtype=BF16, requires_grad=True)
+    index = torch.zeros(4, dtype=torch.int32)
+    for tables in (3, 65, 1000):
+        weight, bias = torch.ones(tables, 64), torch.ones(tables, 64)
+        pk.layer_norm(x, weight, bias, row_index=index).sum().backward()
+        name, args = calls[-1]
+        assert name == "pkh3_layer_norm_backward" and not any(args[i] for i in (7, 8, 9, 10)), tables        # no sums, no workspace
+    weight = torch.ones(3, 64, requires_grad=True)
+    pk.layer_norm(x, weight, torch.ones(3, 64), row_index=index).sum().backward()
+    assert calls[-1][1][7] and not calls[-1][1][8]
+    got = pk.layer_norm_backward(x.detach(), x.detach(), weight.detach(), bias[:3], row_index=index, weight_grad=False)
+    assert got[1] is None and got[2].shape == (3, 64) and not calls[-1][1][7] and calls[-1][1][8]
+    with pytest.raises(pk.Pkh3Error):
+        pk.layer_norm_backward(x.detach(), x.detach(), torch.ones(65, 64), row_index=index)
+    # the entry (no rows, so that nothing is launched)
+    for dweight, code in ((0, front._lib.PKH3_OK), (0x6000000, front._lib.PKH3_ESHAPE)):
+        a = front._lib.NormArgs(dweight=dweight, rows=0, width=264, tables=65535)
+        assert lib.pkh3_layer_norm_backward(a, None) == code
