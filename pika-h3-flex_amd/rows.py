@@ -346,7 +346,7 @@ def linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre
     if not rows:
         return (torch.empty_like(x) if x_grad else None, _zeros(dev, N, K) if weight_grad else None, _zeros(dev, N) if bias_grad else None)
     db = torch.empty(N, dtype=_BF16, device=dev) if bias_grad else None
-    if act:
+    if act and (x_grad or weight_grad or bias_grad):
         dz = torch.empty(rows, N, dtype=_BF16, device=dev)
         z = (dz.data_ptr(), N)
         _activation_grad(at, p, z, db.data_ptr() if bias_grad else 0, rows, N, act, index)
@@ -430,6 +430,11 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor,
     """``(dx, dw_in, dw_out, db_in, db_out)`` of :func:`feed_forward` without its gate and residual (see :func:`linear_backward`), bfloat16; None for what is not
     asked for."""
     _refuse_tangents(dy, x, w_in, w_out, saved.pre, saved.hidden)
+    return _feed_forward_backward(dy, x, w_in, w_out, saved, activation, gated, (x_grad, weight_grad, weight_grad, bias_grad, bias_grad))
+
+
+def _feed_forward_backward(dy, x, w_in, w_out, saved: Saved, activation: str, gated: bool, wanted):
+    """``wanted``: for each of the five gradients whether it is."""
     index = _place(x)
     act = _activation(activation)
     a, w1, w2, rows, K, inner, first, N = _block(x, w_in, w_out, gated, index)
@@ -438,17 +443,19 @@ def feed_forward_backward(dy: torch.Tensor, x: torch.Tensor, w_in: torch.Tensor,
     h = _matrix("saved.hidden", saved.hidden, rows, inner, index)
     dev = x.device
     if not rows:
-        return (torch.empty_like(x) if x_grad else None, *((_zeros(dev, first, K), _zeros(dev, N, inner)) if weight_grad else (None, None)),
-                *((_zeros(dev, first), _zeros(dev, N)) if bias_grad else (None, None)))
-    dz = torch.empty(rows, first, dtype=_BF16, device=dev)
-    z = (dz.data_ptr(), first)
-    db_in = torch.empty(first, dtype=_BF16, device=dev) if bias_grad else None
-    flags = _lib.PRODUCT_B_ACROSS | _lib.PRODUCT_GRAD | (_lib.PRODUCT_GATED if gated else 0)
-    _product(at, w2, z, rows, inner, N, flags, index, pre=p, sums=db_in.data_ptr() if bias_grad else 0, act=act)
-    dx = _input_grad(dz, z, w_in, w1, rows, first, K, index) if x_grad else None
-    dw_in = _weight_grad(z, a, dev, rows, first, K, index) if weight_grad else None
-    dw_out = _weight_grad(at, h, dev, rows, N, inner, index) if weight_grad else None
-    db_out = _column_sums(dy, at, rows, N, index) if bias_grad else None
+        shapes = (first, K), (N, inner), (first,), (N,)
+        return (torch.empty_like(x) if wanted[0] else None, *(_zeros(dev, *shape) if want else None for shape, want in zip(shapes, wanted[1:])))
+    dx = dw_in = db_in = None
+    if wanted[0] or wanted[1] or wanted[3]:
+        dz = torch.empty(rows, first, dtype=_BF16, device=dev)
+        z = (dz.data_ptr(), first)
+        db_in = torch.empty(first, dtype=_BF16, device=dev) if wanted[3] else None
+        flags = _lib.PRODUCT_B_ACROSS | _lib.PRODUCT_GRAD | (_lib.PRODUCT_GATED if gated else 0)
+        _product(at, w2, z, rows, inner, N, flags, index, pre=p, sums=db_in.data_ptr() if wanted[3] else 0, act=act)
+        dx = _input_grad(dz, z, w_in, w1, rows, first, K, index) if wanted[0] else None
+        dw_in = _weight_grad(z, a, dev, rows, first, K, index) if wanted[1] else None
+    dw_out = _weight_grad(at, h, dev, rows, N, inner, index) if wanted[2] else None
+    db_out = _column_sums(dy, at, rows, N, index) if wanted[4] else None
     return dx, dw_in, dw_out, db_in, db_out
 
 
@@ -516,7 +523,5 @@ class _FeedForward(torch.autograd.Function):
         need = ctx.needs_input_grad
         dy = _usable(dy, _BF16)
         activation, gated = ctx.kind
-        dx, dw1, dw2, db1, db2 = feed_forward_backward(dy, x, w_in, w_out, Saved(*saved), activation=activation, gated=gated, x_grad=need[0],
-                                                       weight_grad=need[1] or need[2], bias_grad=need[3] or need[4])
-        return (dx, dw1 if need[1] else None, dw2 if need[2] else None, _as(db1, b_in, need[3]), _as(db2, b_out, need[4]), dy if need[5] else None,
-                None, None)
+        dx, dw1, dw2, db1, db2 = _feed_forward_backward(dy, x, w_in, w_out, Saved(*saved), activation, gated, need[:5])
+        return dx, dw1, dw2, _as(db1, b_in, need[3]), _as(db2, b_out, need[4]), dy if need[5] else None, None, None

@@ -73,3 +73,23 @@ def test_gradients_of_rows_under_many_frozen_tables(rows, width, tables):
         assert torch.equal(got[0], both[0])
         for part, whole, asked in zip(got[1:], both[1:], (weight_grad, bias_grad)):
             assert torch.equal(part, whole) if asked else part is None
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_each_recorded_gradient_of_a_block_by_itself(gated):
+    """With whichever of the others frozen, a gradient has the bits of the whole pass."""
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    make = lambda *s: (torch.randn(s, generator=gen, device=DEV) * 0.3).to(BF16)  # noqa: E731
+    parts = [make(150, 72), make(272 if gated else 136, 72), make(72, 136), make(272 if gated else 136).float(), make(72), make(150, 72)]
+    dy = make(150, 72)
+
+    def grads(wanted):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(parts)]
+        pk.feed_forward(*leaves[:5], activation="gelu", gated=gated, residual=leaves[5]).backward(dy)
+        return [t.grad for t in leaves]
+
+    whole = grads(range(6))
+    for wanted in ([0], [1], [2], [3], [4], [5], [1, 3], [2, 4], [0, 2, 3]):
+        for i, g in enumerate(grads(wanted)):
+            assert (g is None) == (i not in wanted)
+            assert g is None or (torch.equal(g, whole[i]) and g.dtype is parts[i].dtype), (wanted, i)

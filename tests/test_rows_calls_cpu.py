@@ -126,3 +126,31 @@ def test_frozen_tables(lib, entries, monkeypatch):
     for dweight, code in ((0, front._lib.PKH3_OK), (0x6000000, front._lib.PKH3_ESHAPE)):
         a = front._lib.NormArgs(dweight=dweight, rows=0, width=264, tables=65535)
         assert lib.pkh3_layer_norm_backward(a, None) == code
+
+
+def test_recorded_passes_form_what_is_asked_for(entries, monkeypatch):
+    """The products behind each gradient alone: two weights of a block are two gradients, and none at all takes no launch."""
+    monkeypatch.setattr(front, "_product_scratch", lambda *a: 0)
+    monkeypatch.setattr(front, "_activation_scratch", lambda *a: 0)
+    product, sums = "pkh3_product", "pkh3_activation_grad"
+    x, w_in, w_out = _parts()
+    b_in, b_out, residual = torch.ones(32), torch.ones(64), torch.ones(4, 64, dtype=BF16)
+    # x, w_in, w_out, b_in, b_out, residual; launches of the backward pass
+    for wanted, launches in (((1, 0, 0, 0, 0, 0), [product] * 2), ((0, 1, 0, 0, 0, 0), [product] * 2), ((0, 0, 1, 0, 0, 0), [product]), ((0, 0, 0, 1, 0, 0), [product]),
+                             ((0, 0, 0, 0, 1, 0), [sums]), ((0, 0, 0, 0, 0, 1), []), ((1, 1, 1, 1, 1, 1), [product] * 4 + [sums])):
+        leaves = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, w_in, w_out, b_in, b_out, residual), wanted)]
+        y = pk.feed_forward(*leaves[:5], residual=leaves[5], gated=False)
+        entries.clear()
+        y.sum().backward()
+        assert entries == launches, wanted
+        assert [t.grad is not None for t in leaves] == [bool(w) for w in wanted]
+        assert all(t.grad is None or t.grad.dtype is t.dtype for t in leaves)
+    # x, weight, bias, residual
+    for activation, wanted, launches in (("silu", (0, 0, 0, 1), []), ("silu", (1, 0, 0, 0), [sums, product]), ("silu", (0, 0, 1, 0), [sums]), ("silu", (1, 1, 1, 1), [sums, product, product]),
+                                         ("none", (0, 0, 0, 1), []), ("none", (0, 1, 0, 0), [product]), ("none", (0, 0, 1, 0), [sums])):
+        leaves = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, w_in, b_in, torch.ones(4, 32, dtype=BF16)), wanted)]
+        y = pk.linear(*leaves[:3], activation=activation, residual=leaves[3])
+        entries.clear()
+        y.sum().backward()
+        assert entries == launches, (activation, wanted)
+        assert [t.grad is not None for t in leaves] == [bool(w) for w in wanted]
