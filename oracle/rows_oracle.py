@@ -81,10 +81,19 @@ def rounded(y, bound):
     return y, bound + HALF_BF16 * (y.abs() + bound) + 1e-30
 
 
+def act_error(name, v):
+    """How far an activation in float32 is off: 2e-6 of the value and, far out, 1e-37.  On the negative side it is exp(-E) in the main, E = |v|, v^2 / 2 or 2 |u| (u the tanh form's), and
+    an exponent with up to five roundings on its way (constants, squares, products, the difference) is off by 5 * 2^-24 E, and so is the value, relative to itself."""
+    if name == "none":
+        return torch.zeros_like(v)
+    far = {"silu": -v, "gelu": 0.5 * v * v, "gelu_tanh": -2.0 * _TANH * (v + 0.044715 * v ** 3)}[name]
+    return act(name, v).abs() * (2e-6 + 5 * HALF_F32 * torch.where(v < 0, far, torch.zeros_like(v)).clamp(max=90.0)) + 1e-37
+
+
 def finish(z, bound, name, gate=None, index=None, residual=None):
-    """Activation (its own error: 2e-6 of the value and, far out, 1e-37), gate and residual; rounded."""
+    """Activation (its own error: act_error), gate and residual; rounded."""
     y = act(name, z)
-    bound = bound * SLOPE[name] + (2e-6 * y.abs() + 1e-37 if name != "none" else 0.0)
+    bound = bound * SLOPE[name] + act_error(name, z)
     if gate is not None:
         g = take(gate, index, z.shape[0])
         y, bound = y * g, bound * g.abs() + 2 * HALF_F32 * (y * g).abs()
@@ -115,7 +124,7 @@ def middle(x, w_in, b_in, name, gated):
     a, b = z.chunk(2, 1)
     ea, eb = e.chunk(2, 1)
     f = act(name, b)
-    ef = eb * SLOPE[name] + 2e-6 * f.abs() + 1e-37
+    ef = eb * SLOPE[name] + act_error(name, b)
     h, eh = rounded(a * f, ea * f.abs() + (a.abs() + ea) * ef + 2 * HALF_F32 * (a * f).abs())
     return h, eh, z, e
 
@@ -171,7 +180,7 @@ def feed_forward_backward(dy, x, w_in, w_out, b_in=None, b_out=None, name="silu"
         a, b = z.chunk(2, 1)
         ea, eb = ez.chunk(2, 1)
         f = act(name, b)
-        ef = SLOPE[name] * eb + 4e-6 * f.abs() + 1e-37
+        ef = SLOPE[name] * eb + 2 * act_error(name, b)
         da, e_da = dh * f, e * (f.abs() + ef) + dh.abs() * ef + 2 * HALF_F32 * (dh * f).abs()
         p = dh * a
         ep = e * (a.abs() + ea) + dh.abs() * ea

@@ -72,8 +72,10 @@ constexpr int wait_for(int vm, int lgkm) { return (vm & 15) | ((vm >> 4) << 14) 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
 
-// The normal distribution's tail beyond |v|: erfc(z) / 2, z = |v| / sqrt 2, with erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2).
-// p is a polynomial fitted to log(erfc(z) / t) + z^2 at Chebyshev points of t in [1/8, 1] (z up to 14): 8e-7 of the value everywhere, small tails among it.
+// The normal distribution's tail beyond |v|: erfc(z) / 2, z = |v| / sqrt 2, with erfc(z) = t exp(-z^2 + p(t)), t = 1 / (1 + z / 2), the form in which W. H. Press et al.,
+// "Numerical Recipes", give the error function.  p is a polynomial of lower degree, fitted here to log(erfc(z) / t) + z^2 at Chebyshev points of t in [1/8, 1] (z up to 14),
+// to 8e-7 of the value.  In float32 the roundings of the exponent come on top, which grow with it: 1.2e-6 of the value up to |v| of 2, 2.5e-6 up to 6, 1.1e-5 up to 13.  The
+// result's own rounding to bfloat16 is 350 times that.
 // (Its coefficients are those times log2(e), with -1 for the half in the last one: an activation's instructions are what a tile's results take besides memory, 256 of
 // them a lane at 4 cycles each and 16 for those of exp2 and the reciprocal.)
 __device__ __forceinline__ float normal_tail(float v) {

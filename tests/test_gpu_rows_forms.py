@@ -102,8 +102,7 @@ def test_gated(tile, share, M, N, K):
         _, saved = pk.feed_forward(x.view, w.view, w_out, bias, activation=name, save=True)
         _equal(saved.pre, z, "pre")
         f = O.act(name, b)
-        ef = 2e-6 * f.abs() + 1e-37 if name != "none" else 0.0
-        _within(saved.hidden, O.rounded(a * f, a.abs() * ef + 2 * O.HALF_F32 * (a * f).abs()), name)
+        _within(saved.hidden, O.rounded(a * f, a.abs() * O.act_error(name, b) + 2 * O.HALF_F32 * (a * f).abs()), name)
     assert x.frame_is_left() and w.frame_is_left()
 
 
@@ -175,7 +174,7 @@ def test_gated_grad(tile, share, M, N, K):
     for name in ACTIVATIONS[1:]:
         f, slope = O.act(name, b), O.act_slope(name, b)
         da, p = s * f, s * a
-        e_da = s.abs() * (4e-6 * f.abs() + 1e-37) + 2 * O.HALF_F32 * da.abs()
+        e_da = s.abs() * 2 * O.act_error(name, b) + 2 * O.HALF_F32 * da.abs()
         e_db = 4e-6 * (1 + b.abs()) * p.abs() + 4 * O.HALF_F32 * (p * slope).abs()
         v, e = torch.cat([da, p * slope], 1), torch.cat([e_da, e_db], 1)
         got, sums = call(name, z)
