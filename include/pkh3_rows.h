@@ -50,7 +50,8 @@ typedef struct pkh3_norm_args {
 
 int pkh3_layer_norm(const pkh3_norm_args* args, void* stream);
 /* dx = (g - mean(g) - xh * mean(g * xh)) / sqrt(var + eps), g = dy * weight[r], xh the normalised row; dweight[r] and dbias[r] are the sums of
- * dy * xh and of dy over the rows of table row r (zeros where there are none), added up in an order that depends on the sizes and the row index alone. */
+ * dy * xh and of dy over the rows of table row r (zeros where there are none), added up in an order that depends on the sizes and the row index alone.  Meant for rows that
+ * take the same table row for a while: with another one at every row the call takes six times as long. */
 int pkh3_layer_norm_backward(const pkh3_norm_args* args, void* stream);
 size_t pkh3_norm_workspace_bytes(const pkh3_norm_args* args);
 

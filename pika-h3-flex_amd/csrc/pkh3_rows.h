@@ -37,7 +37,7 @@ struct ProductParams {
   char* pre;                     // float32
   char* out;
   float* sums;                   // partial sums of out's columns, [rows of partial sums][columns], or null
-  float* part;                   // parts of the tiles that are cut: [unit][rows of a tile][256]
+  float* part;                   // parts of the tiles that are cut: [unit][rows of a tile][columns of a tile]
   int64_t gate_stride, residual_stride, pre_stride, out_stride;   // bytes
   int M, N, K, gate_rows;
   int act, bias_bf16;

@@ -63,7 +63,11 @@ constexpr size_t whole_256(size_t n) { return (n + 255) / 256 * 256; }
 // The form of pkh3_rows_thin.hip, for few rows of operands along: workgroups of up to 64 rows times 32 columns, or of 16 where 32 would leave CUs without one (and with gates).
 constexpr int thin_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 constexpr bool thin_narrow(int M, int N) { return (int64_t)((N + 31) / 32) * ((M + thin_rows(M) - 1) / thin_rows(M)) < 192; }
-// Its time as plan_time() has it: a workgroup's rows and weights at the 90 GB/s a CU that calls of one workgroup a CU reach, 60 where there are more.
+// Its time as plan_time() has it: a workgroup's rows and weights at the 90 GB/s a CU that calls of one workgroup a CU reach, 60 where there are more.  That knows of no memory behind
+// the CUs and of no results, as plan_time() does not.  Over 55 products of 1 to 6,000 rows, weights out of memory, both forms timed: up to 300 rows the choice takes up to 1.15 times the
+// better form (64 rows, 8,192 to 2,048: 23.9 us, tiles 20.8), where the few rows' form is right up to half of it (128 rows, 2,048 to 2,048: 8.6 us, tiles 19.1).  Above, most choices are right too
+// (424 rows, 912 to 200: 5.9 us, tiles 10.6; 3,255 rows, 224 to 120: 4.7, 7.7), but the form is also taken where tiles take less, by up to 35 %: 693 rows, 408 to 1,560 13.1 us, tiles
+// 9.5; 2,373 rows, 80 to 768 10.4, 7.0; 6,001 rows, 264 to 248 14.7, 9.6.
 constexpr int64_t thin_time(int M, int N, int K, int mode) {
   const int columns = mode == kGated || thin_narrow(M, N) ? 16 : 32, blocks = thin_rows(M) + (mode == kGated ? 32 : columns);
   const int64_t groups = (int64_t)((N + columns - 1) / columns) * ((M + thin_rows(M) - 1) / thin_rows(M)), bytes = (int64_t)blocks * K * 2;

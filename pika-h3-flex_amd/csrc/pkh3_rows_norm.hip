@@ -5,12 +5,15 @@
 //
 // A row lies in the registers of the lanes that share it (a wave or a workgroup), 8 elements a piece, and the next row is on its way while one is worked on, so memory is
 // read once and the variance is taken about the mean.  The backward pass forms the statistics again from the row, which it needs anyway, instead of keeping them.  Both
-// are bound by memory: 48,360 rows of 2,048 in bfloat16 take 84 us forward (4.7 TB/s; a copy of as many bytes takes 75) and 157 us backward
-// (3.8 TB/s), 15,342 rows of 1,536 in float32 30 us (6.2 TB/s; a copy 27) and 55 us (5.1 TB/s).
+// are bound by memory: 48,360 rows of 2,048 in bfloat16 take 84 us forward (4.7 TB/s; a copy of as many bytes takes 75) and 152 us backward
+// (3.8 TB/s; 132 without sums for the tables), 15,342 rows of 1,536 in float32 39 us (4.8 TB/s) and 62 us (4.5 TB/s; 55 without sums).  15,342 rows of 2,048 in bfloat16 take 27 and 57 us (3.3 TB/s
+// backward, 49 without sums): two workgroups a CU, whose registers hold two rows and the next two, and the second launch.
 //
 // Sums for the tables: every workgroup takes one run of rows and keeps the sums of the table row that it is at in registers (its rows come
 // in runs of one table row, so they rarely change); when the table row changes, and at the end, the workgroup's lanes add up in LDS and the sums go to the
-// workgroup's own slice of the workspace.  A second launch adds the slices up in their order: no atomics, the same bits every time.
+// workgroup's own slice of the workspace.  A second launch adds the slices up in their order: no atomics, the same bits every time.  What a change costs: 48,360 rows of 2,048
+// that take three table rows in three runs 163 us, in runs of 64 rows 171, of 8 252, at random 820, and with another table row at every row 1,070 (one of a workgroup's
+// waves has a row at a time then).  Forward: 85, 86, 91, 97 and 103 us.
 #include "pkh3_rows.h"
 
 namespace pkh3 {

@@ -6,8 +6,8 @@
 // lanes beside each other take the CU's vector-memory path a quarter of the time that images straight into the registers take, where such lanes lie in
 // different rows (16 rows, 4,096 x 12,288: 34 us that way).
 //
-// Bound by the weights: one row, 2,048 to 8,192, weights out of memory 8.4 us (4 TB/s, 2 us of them the launch) and 4.9 out of L2; 64 rows 12.2; 200 rows, 8,192 to 2,048 25 us, where
-// tiles take 26.  Where there are some more than 256 workgroups, a few CUs have two (10 rows, 4,368 to 8,960, 280 of them: 28 us, tiles 26).
+// Bound by the weights: one row, 2,048 to 8,192, weights out of memory 8.6 us (3.9 TB/s, 2 us of them the launch) and 4.9 out of L2; 128 rows, 2,048 to 2,048 8.5, where tiles take 19;
+// 200 rows, 8,192 to 2,048 25, tiles 24.  Where there are some more than 256 workgroups, a few CUs have two (10 rows, 4,368 to 8,960, 280 of them: 28.6 us, tiles 25.6).
 #include "pkh3_rows.h"
 
 namespace pkh3 {

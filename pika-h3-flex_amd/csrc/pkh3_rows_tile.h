@@ -13,8 +13,9 @@
 // in turn (pkh3_rows_index.h), and the next tile's first chunks come while one's results leave.  Both operands have rings of two to four chunks in LDS.
 //
 // What bounds it.  256 x 256: the matrix units (2,048 of a chunk's 2,300 cycles), whose clock the board's power holds at 1.7 GHz: 15,342 x 2,048 with a contraction of 5,504
-// takes 242 us, 1.43 PFLOP/s.  Smaller tiles: LDS, which every row of a chunk passes three times (written once, read by two waves: 3 cycles a row, 768 a chunk of 128 x 128, whose
-// products take 512), and with weights from memory what a CU takes in of lines that its L2 does not have, about 40 GB/s.  The results of a tile
+// takes 242 us, 1.43 PFLOP/s.  Smaller tiles: what a CU takes in of lines that its L2 does not have, about 40 GB/s, and waits that a single wave a SIMD leaves uncovered.  No unit is busy: of
+// 1,085 x 2,048 x 2,048 in tiles of 96 x 128 (23 us) the matrix units work 27 % of the time, LDS delivers images 16 % of it, without a conflict, and the waves
+// wait for 45 %; of 4,000 x 2,048 x 2,048 in 128 x 256 (37 us) 48, 18 and 31 %; of 2,003 x 5,160 x 1,400 in 256 x 256 (47 us) 51, 13 and 26 %.  The results of a tile
 // are not covered by the next one's products: 15,342 x 5,504 gradients of gated halves, which read 675 MB and write 338, take 448 us where the product alone takes 240.
 #pragma once
 #include <type_traits>
@@ -357,7 +358,7 @@ struct Walk {
   }
 };
 
-// A wave's results: 16 rows at a time, a lane 16 bytes of a row four times (twice with gates).  What else the results need is asked for a block of rows ahead.
+// A wave's results: 16 rows at a time, a lane 16 bytes of a row FB / 2 times (half as often with gates).  What else the results need is asked for a block of rows ahead.
 // The accumulators of block t, which is known when the kernel runs: a branch, not an index.
 template <int TB, int FB>
 __device__ __forceinline__ void block_of(int t, const f32x4 (&acc)[TB][FB], f32x4 (&block)[FB]) {
@@ -431,7 +432,7 @@ __device__ __forceinline__ void finish_tile(const ProductParams& p, int m0, int 
     }
   };
   // The first block by itself: where it met the others in the loop, the compiler would wait for as few accesses on their way as in the first turn, where no result has left yet,
-  // and so, in every turn, for stores just issued (1,085 x 2,048 x 2,048, gate and residual: 23.4 us so, 22.8 now).  (Gradients take as long either way: memory bounds theirs.)
+  // and so, in every turn, for stores just issued (1,085 x 2,048 x 2,048, gate and residual: 23.4 us so, 22.8 now).  (Gradients take as long either way.)
   constexpr bool kPeel = BESIDES != 0;
   if constexpr (kPeel) rows_of(0);
 #pragma unroll 1
