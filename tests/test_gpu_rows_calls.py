@@ -93,3 +93,23 @@ def test_each_recorded_gradient_of_a_block_by_itself(gated):
         for i, g in enumerate(grads(wanted)):
             assert (g is None) == (i not in wanted)
             assert g is None or (torch.equal(g, whole[i]) and g.dtype is parts[i].dtype), (wanted, i)
+
+
+def test_keys_kept_for_text_states_follow_what_is_written_over_them():
+    """The processor keeps a cross-attention's keys by the text states' version: states that a call wrote over in place give their own keys, not the earlier ones."""
+    from tests.test_gpu_full import _Attn
+
+    torch.manual_seed(3)
+    H, hidden, width = 3, 384, 200
+    attn = _Attn(hidden, H, kv_dim=width).cuda().to(BF16)
+    enc, x = torch.randn((1, 64, width), device=DEV, dtype=BF16), torch.randn((1, 150, hidden), device=DEV, dtype=BF16)
+    w = torch.randn((width, width), device=DEV, dtype=BF16)
+    plain, cached = pk.PikaH3AttnProcessor(), pk.PikaH3AttnProcessor(cache_cross_kv=True)
+    with torch.no_grad():
+        before = cached(attn, x, encoder_hidden_states=enc)
+        for write in (lambda e: pk.linear(e.clone(), w, residual=e, out=e), lambda e: pk.layer_norm(e, out=e),
+                      lambda e: pk.feed_forward(e.clone(), w, w, gated=False, residual=e, out=e)):
+            write(enc[0])
+            got = cached(attn, x, encoder_hidden_states=enc)
+            assert torch.equal(got, plain(attn, x, encoder_hidden_states=enc)) and not torch.equal(got, before)
+            before = got
